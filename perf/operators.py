@@ -1,0 +1,474 @@
+"""Workloads for the gated-recurrence block's operators: the gated linear recurrence over (T, B, N)
+sequences, the norms around a block fused with its gate and residual scale, and the activation
+checkpoints in 8 bits that their backward passes read.
+
+A case is a dict of plain values; ``kind`` names the operator:
+
+  scan   ``gated_scan``: forward, and with ``mode`` 'train' its backward pass
+  norm   ``norm_gate_residual``: the same
+  pack   ``pack8`` and ``unpack8``: a tensor to 8 bits and back
+  step   ``gated_step``: recurrence, norms, gate and residual of one time step (streaming)
+
+``checkpoint`` says that the operator keeps what its backward pass reads in 8 bits. With ``joint``
+the inputs are column slices of one projection's output, as the block makes them.
+"""
+
+import math
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+DTYPES = {'fp32': torch.float32, 'bf16': torch.bfloat16}
+BLOCK = 64       # steps between the states that a checkpointed scan keeps
+GROUP = 64       # channels of a row that share an 8-bit scale
+EPS = 1e-6
+
+
+def _scan(name, T, B, N, dtype, **more):
+    return dict(dict(name=name, kind='scan', mode='train', T=T, B=B, N=N, dtype=dtype, joint=dtype == 'bf16',
+                     masks=False, checkpoint=False), **more)
+
+
+def _norm(name, R, N, dtype, resid, **more):
+    return dict(dict(name=name, kind='norm', mode='train', R=R, N=N, dtype=dtype, resid=resid, checkpoint=False), **more)
+
+
+def listed():
+    return [
+        # streaming inference of a few sessions, one time step: latency
+        dict(name='step_small', kind='step', B=4, N=256, dtype='bf16', resid='fp32'),
+        # the same for many sessions of a wide model
+        dict(name='step_large', kind='step', B=512, N=2048, dtype='bf16', resid='fp32'),
+        # the memorisation task's layer (64 neurons, 32 steps, batch 64): launches and host path count
+        _scan('scan_small', 32, 64, 64, 'fp32'),
+        # speech commands: 250 steps, batch 128, 512 channels, slices of the block's projection
+        _scan('scan_ordinary', 250, 128, 512, 'bf16'),
+        # long sequences of few channels: 700 event channels, batch 2
+        _scan('scan_long', 16384, 2, 700, 'fp32'),
+        # packed and padded streams of an odd width
+        _scan('scan_ragged', 1000, 50, 333, 'bf16', masks=True),
+        # the widest layer's training step, activations kept in 8 bits
+        _scan('scan_8bit', 1024, 64, 2048, 'bf16', checkpoint=True),
+        # norms, gate and residual of the ordinary block: 250 steps of batch 128
+        _norm('norm_ordinary', 32000, 512, 'bf16', 'bf16'),
+        # evaluating a small model of an odd width: forward only
+        _norm('norm_eval', 5000, 700, 'fp32', 'fp32', mode='infer'),
+        # the widest block's, residual stream in 32 bits, activations kept in 8 bits
+        _norm('norm_8bit', 65536, 2048, 'bf16', 'fp32', checkpoint=True),
+        # the saved input of a Linear, event channels in 32 bits
+        dict(name='pack_small', kind='pack', R=8000, N=700, dtype='fp32'),
+        # the same for the widest block
+        dict(name='pack_large', kind='pack', R=65536, N=2048, dtype='bf16'),
+    ]
+
+
+def draw(rng):
+    """A case of the listed ones' ranges: sizes spread over their logarithms, odd ones too."""
+    def size(lo, hi):
+        v = int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+        return min(hi, v if rng.random() < 0.5 else max(lo, v // 20 * 20))
+
+    kind = rng.choice(['scan', 'scan', 'scan', 'norm', 'norm', 'pack', 'step'])
+    dtype = rng.choice(['bf16', 'bf16', 'fp32'])
+    resid = rng.choice(['fp32', dtype])
+    if kind == 'step':
+        return dict(kind=kind, B=size(1, 512), N=size(32, 2048), dtype=dtype, resid=resid)
+    if kind == 'pack':
+        return dict(kind=kind, R=size(200, 65536), N=size(32, 2048), dtype=dtype)
+    mode = rng.choice(['train', 'train', 'infer'])
+    checkpoint = mode == 'train' and rng.random() < 0.4
+    if kind == 'norm':
+        return dict(kind=kind, mode=mode, R=size(200, 65536), N=size(32, 2048), dtype=dtype, resid=resid, checkpoint=checkpoint)
+    N = size(32, 2048)
+    T = size(16, 16384)
+    B = size(1, max(2, min(512, (1 << 26) // (T * N))))
+    return dict(kind=kind, mode=mode, T=T, B=B, N=N, dtype=dtype, joint=rng.random() < 0.5, masks=rng.random() < 0.4,
+                checkpoint=checkpoint)
+
+
+# ---------------------------------------------------------------- inputs --------------------
+
+def _leaf(t):
+    return t.detach().requires_grad_(True)
+
+
+def prepare(case, seed):
+    dev = torch.device('cuda')
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    dt = DTYPES[case['dtype']]
+
+    def normal(*shape, dtype=torch.float32, std=1.0):
+        return (torch.randn(*shape, generator=gen, device=dev, dtype=torch.float32) * std).to(dtype)
+
+    def uniform(*shape, lo=0.0, hi=1.0):
+        return torch.rand(*shape, generator=gen, device=dev) * (hi - lo) + lo
+
+    s = {'case': case}
+    if case['kind'] == 'scan':
+        T, B, N = case['T'], case['B'], case['N']
+        if case['joint']:
+            proj = normal(T, B, 3 * N, dtype=dt)
+            z, f = proj[..., :N], proj[..., N:2 * N]
+        else:
+            z, f = normal(T, B, N, dtype=dt), normal(T, B, N, dtype=dt)
+        # leaks from a step or two to some hundred steps
+        s.update(z=_leaf(z), f=_leaf(f), bias=_leaf(uniform(N, lo=0.0, hi=6.0)), h0=_leaf(normal(B, N)), starts=None,
+                 lengths=None)
+        if case['masks']:
+            s['starts'] = uniform(T, B) < 1.0 / 128
+            lengths = (uniform(B) * (T + 1)).to(torch.int64).clamp_(max=T)
+            lengths[0] = T
+            if B > 1:
+                lengths[-1] = 0
+            s['lengths'] = lengths
+        if case['mode'] == 'train':
+            s.update(dh=normal(T, B, N, dtype=dt), dlast=normal(B, N))
+    elif case['kind'] == 'norm':
+        R, N = case['R'], case['N']
+        rt = DTYPES[case['resid']]
+        s.update(o=_leaf(normal(R, N, dtype=dt, std=0.5)), g=_leaf(normal(R, N, dtype=dt)), x=_leaf(normal(R, N, dtype=rt)),
+                 weight=_leaf(1 + normal(N, std=0.1)), scale=_leaf(uniform(N, lo=0.1, hi=1.0)),
+                 next_weight=_leaf(1 + normal(N, std=0.1)))
+        if case['mode'] == 'train':
+            s.update(dx=normal(R, N, dtype=rt), du=normal(R, N, dtype=dt))
+    elif case['kind'] == 'pack':
+        s['x'] = normal(case['R'], case['N'], dtype=dt) * uniform(case['R'], 1, lo=0.1, hi=4.0).to(dt)
+    else:
+        B, N = case['B'], case['N']
+        proj = normal(B, 3 * N, dtype=dt)
+        s.update(z=proj[:, :N], f=proj[:, N:2 * N], g=proj[:, 2 * N:], x=normal(B, N, dtype=DTYPES[case['resid']]),
+                 h=normal(B, N, std=0.5), bias=uniform(N, lo=0.0, hi=6.0), weight=1 + normal(N, std=0.1),
+                 scale=uniform(N, lo=0.1, hi=1.0), next_weight=1 + normal(N, std=0.1))
+    return s
+
+
+# ---------------------------------------------------------------- the framework's calls -----
+
+def _ops():
+    pkg = str(Path(__file__).resolve().parent.parent / 'snn-delays_amd')
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from delrec import checkpoint8, gated
+    return gated, checkpoint8
+
+
+def _run_own(s):
+    case = s['case']
+    gated, checkpoint8 = _ops()
+    if case['kind'] == 'scan':
+        def call():
+            return gated.gated_scan(s['z'], s['f'], bias=s['bias'], h0=s['h0'], starts=s['starts'], lengths=s['lengths'],
+                                    checkpoint=case['checkpoint'])
+        if case['mode'] == 'infer':
+            with torch.no_grad():
+                h, last = call()
+            return {'h': h, 'last': last}
+        h, last = call()
+        dz, df, db, d0 = torch.autograd.grad((h, last), (s['z'], s['f'], s['bias'], s['h0']), (s['dh'], s['dlast']))
+        return {'h': h, 'last': last, 'dz': dz, 'df': df, 'db': db, 'd0': d0}
+    if case['kind'] == 'norm':
+        def call():
+            return gated.norm_gate_residual(s['o'], s['g'], s['x'], s['weight'], s['scale'], s['next_weight'], eps=EPS,
+                                            checkpoint=case['checkpoint'])
+        if case['mode'] == 'infer':
+            with torch.no_grad():
+                x, u = call()
+            return {'x': x, 'u': u}
+        x, u = call()
+        names = ('o', 'g', 'x', 'weight', 'scale', 'next_weight')
+        grads = torch.autograd.grad((x, u), [s[n] for n in names], (s['dx'], s['du']))
+        return {'x': x, 'u': u, **{'d_' + n: t for n, t in zip(names, grads)}}
+    if case['kind'] == 'pack':
+        return {'x': checkpoint8.unpack8(checkpoint8.pack8(s['x']))}
+    with torch.no_grad():
+        x, u, h = gated.gated_step(s['z'], s['f'], s['g'], s['x'], s['h'], bias=s['bias'], weight=s['weight'],
+                                   scale=s['scale'], next_weight=s['next_weight'], eps=EPS)
+    return {'x': x, 'u': u, 'h': h}
+
+
+# ---------------------------------------------------------------- plain forms ---------------
+
+def _round8(x):
+    """The values that groups of 64 channels of a row stand for in 8 bits."""
+    n = x.shape[-1]
+    p = torch.nn.functional.pad(x, (0, -n % GROUP)).unflatten(-1, (-1, GROUP))
+    scale = (p.abs().amax(-1, keepdim=True) * (1.0 / 127)).clamp(min=2.0 ** -126)
+    return ((p * scale.reciprocal()).round() * scale).flatten(-2)[..., :n]
+
+
+def _affine_scan(a, b, dim):
+    """All prefixes of h <- a h + b along ``dim``, by doubling."""
+    a, b = a.clone(), b.clone()
+    n, s = a.shape[dim], 1
+    while s < n:
+        lo_a, hi_a = a.narrow(dim, 0, n - s), a.narrow(dim, s, n - s)
+        lo_b, hi_b = b.narrow(dim, 0, n - s), b.narrow(dim, s, n - s)
+        hi_b += hi_a * lo_b
+        if 2 * s < n:
+            hi_a.copy_(hi_a * lo_a)
+        s *= 2
+    return b
+
+
+def _gates(z, f, bias, starts, pad):
+    """(a, k z, k, the leak's own a) with the masks: a start forgets the state, padding keeps it."""
+    k = torch.sigmoid(-(f + bias))
+    a = torch.sigmoid(f + bias)
+    decay, inp = a, k * z
+    if starts is not None:
+        decay = torch.where(starts, 0.0, decay)
+        decay, inp = torch.where(pad, 1.0, decay), torch.where(pad, 0.0, inp)
+    return decay, inp, k, a
+
+
+def _plain_scan(s):
+    case = s['case']
+    dt = DTYPES[case['dtype']]
+    z, f, bias, h0 = s['z'].float(), s['f'].float(), s['bias'], s['h0']
+    T = z.shape[0]
+    starts = pad = None
+    if case['masks']:
+        starts = s['starts'][..., None]
+        pad = (torch.arange(T, device=z.device)[:, None] >= s['lengths'])[..., None]
+    decay, inp, k, a = _gates(z, f, bias, starts, pad)
+    inp[0] += decay[0] * h0
+    h = _affine_scan(decay, inp, 0)
+    last = h[-1].clone()
+    out = {'h': (h if pad is None else torch.where(pad, 0.0, h)).to(dt), 'last': last}
+    if case['mode'] == 'infer':
+        return out
+    before = torch.cat([h0[None], h[:-1]])
+    if case['checkpoint']:
+        z, f = _round8(z), _round8(f)
+        decay, inp, k, a = _gates(z, f, bias, starts, pad)
+        blocks = -(-T // BLOCK)
+
+        def blocked(t, fill):
+            t = torch.nn.functional.pad(t, (0, 0, 0, 0, 0, blocks * BLOCK - T), value=fill)
+            return t.unflatten(0, (blocks, BLOCK))
+        d, i = blocked(decay, 1.0), blocked(inp, 0.0)
+        kept = before[::BLOCK]
+        i[:, 0] += d[:, 0] * kept
+        inner = _affine_scan(d, i, 1)
+        before = torch.cat([kept[:, None], inner[:, :-1]], 1).flatten(0, 1)[:T]
+    if starts is not None:
+        before = torch.where(starts, 0.0, before)
+    dh = s['dh'].float()
+    if pad is not None:
+        dh = torch.where(pad, 0.0, dh)
+    # lam_t = dh_t + decay_{t+1} lam_{t+1}, latest step first
+    dh[-1] += s['dlast']
+    back = torch.cat([torch.zeros_like(decay[:1]), decay[1:].flip(0)])
+    lam = _affine_scan(back, dh.flip(0), 0).flip(0)
+    d0 = decay[0] * lam[0]
+    dz, df = lam * k, lam * a * k * (before - z)
+    if pad is not None:
+        dz, df = torch.where(pad, 0.0, dz), torch.where(pad, 0.0, df)
+    out.update(dz=dz.to(dt), df=df.to(dt), db=df.sum((0, 1)), d0=d0)
+    return out
+
+
+def _norm_block(o, g, x, weight, scale):
+    r = (o.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    return r, x + scale * (o * r * weight) * (g * torch.sigmoid(g))
+
+
+def _plain_norm(s):
+    case = s['case']
+    dt, rt = DTYPES[case['dtype']], DTYPES[case['resid']]
+    o, g, x = s['o'].float(), s['g'].float(), s['x'].float()
+    w, sc, w2 = s['weight'], s['scale'], s['next_weight']
+    r, xn = _norm_block(o, g, x, w, sc)
+    r2 = (xn.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    out = {'x': xn.to(rt), 'u': (xn * r2 * w2).to(dt)}
+    if case['mode'] == 'infer':
+        return out
+    if case['checkpoint']:
+        o, g, x = _round8(o), _round8(g), _round8(x)
+        xn = x + sc * (o * r * w) * (g * torch.sigmoid(g))
+    du = s['du'].float()
+    unit2 = xn * r2
+    v2 = w2 * du
+    dx = s['dx'].float() + r2 * (v2 - unit2 * (v2 * unit2).mean(-1, keepdim=True))
+    sig = torch.sigmoid(g)
+    unit = o * r
+    n = unit * w
+    dy = sc * dx
+    dn = dy * (g * sig)
+    v = w * dn
+    out.update(d_o=(r * (v - unit * (v * unit).mean(-1, keepdim=True))).to(dt),
+               d_g=(dy * n * (sig * (1 + g * (1 - sig)))).to(dt), d_x=dx.to(rt), d_weight=(dn * unit).sum(0),
+               d_scale=(dx * n * (g * sig)).sum(0), d_next_weight=(du * unit2).sum(0))
+    return out
+
+
+def _plain_step(s):
+    case = s['case']
+    z, f, g, x = s['z'].float(), s['f'].float(), s['g'].float(), s['x'].float()
+    pre = f + s['bias']
+    h = torch.sigmoid(pre) * s['h'] + torch.sigmoid(-pre) * z
+    _, xn = _norm_block(h, g, x, s['weight'], s['scale'])
+    r2 = (xn.square().mean(-1, keepdim=True) + EPS).rsqrt()
+    return {'x': xn.to(DTYPES[case['resid']]), 'u': (xn * r2 * s['next_weight']).to(DTYPES[case['dtype']]), 'h': h}
+
+
+def run(state):
+    if own:
+        return _run_own(state)
+    with torch.no_grad():
+        kind = state['case']['kind']
+        if kind == 'scan':
+            return _plain_scan(state)
+        if kind == 'norm':
+            return _plain_norm(state)
+        if kind == 'pack':
+            return {'x': _round8(state['x'].float()).to(state['x'].dtype)}
+        return _plain_step(state)
+
+
+# ---------------------------------------------------------------- work ----------------------
+
+def work(case):
+    size = {'fp32': 4, 'bf16': 2}
+    e = size[case['dtype']]
+    train = case.get('mode') == 'train'
+    if case['kind'] == 'scan':
+        rows = case['B'] * case['N']
+        n = case['T'] * rows
+        # z, f, h and, in training, dh, dz, df; the states at both ends and their gradients
+        return {'bytes': n * e * (6 if train else 3) + rows * 4 * (4 if train else 2), 'flops': n * (30 if train else 10)}
+    if case['kind'] == 'norm':
+        n, r = case['R'] * case['N'], size[case['resid']]
+        # o, g, u, x, x' and, in training, du, dx', do, dg, dx
+        return {'bytes': n * ((6 * e + 4 * r) if train else (3 * e + 2 * r)), 'flops': n * (45 if train else 15)}
+    if case['kind'] == 'pack':
+        n = case['R'] * case['N']
+        return {'bytes': 2 * n * e, 'flops': 4 * n}
+    n = case['B'] * case['N']
+    return {'bytes': n * (4 * e + 8 + 2 * size[case['resid']]) + case['N'] * 16, 'flops': 25 * n}
+
+
+# ---------------------------------------------------------------- 64 bits -------------------
+
+def _kept8(x):
+    """8-bit values by their definition, one group of columns at a time."""
+    parts = []
+    for c in range(0, x.shape[-1], GROUP):
+        part = x[..., c:c + GROUP]
+        step = torch.maximum(part.abs().max(-1, keepdim=True).values / 127, torch.full((), 2.0 ** -126, dtype=x.dtype, device=x.device))
+        parts.append(torch.round(part / step) * step)
+    return torch.cat(parts, -1)
+
+
+def _exact_scan(s):
+    case = s['case']
+    T = case['T']
+    z, f = s['z'].detach().double(), s['f'].detach().double()
+    b, h = s['bias'].detach().double(), s['h0'].detach().double()
+    live = torch.ones(T, case['B'], 1, dtype=torch.bool, device=z.device)
+    fresh = torch.zeros_like(live)
+    if case['masks']:
+        live = (torch.arange(T, device=z.device)[:, None] < s['lengths'][None, :])[..., None]
+        fresh = s['starts'][..., None]
+    zero = torch.zeros((), dtype=torch.float64, device=z.device)
+
+    def advance(h, zt, ft, t):
+        leak = 1 / (1 + torch.exp(ft + b))
+        h_in = torch.where(fresh[t], zero, h) if case['masks'] else h
+        new = h_in + leak * (zt - h_in)
+        return (torch.where(live[t], new, h) if case['masks'] else new), h_in, leak
+
+    ys, ins, leaks, states = [], [], [], []
+    for t in range(T):
+        if t % BLOCK == 0:
+            states.append(h)
+        h, h_in, leak = advance(h, z[t], f[t], t)
+        ys.append(torch.where(live[t], h, zero))
+        if case['mode'] == 'train' and not case['checkpoint']:
+            ins.append(h_in)
+            leaks.append(leak)
+    out = {'h': torch.stack(ys), 'last': h}
+    if case['mode'] == 'infer':
+        return out
+    del ys
+    if case['checkpoint']:
+        z, f = _kept8(z), _kept8(f)
+        for t in range(T):
+            if t % BLOCK == 0:
+                h = states[t // BLOCK]
+            h, h_in, leak = advance(h, z[t], f[t], t)
+            ins.append(h_in)
+            leaks.append(leak)
+    carry = s['dlast'].double()
+    dz, df = torch.zeros_like(z), torch.zeros_like(f)
+    for t in reversed(range(T)):
+        lam = s['dh'][t].double() + carry
+        k = leaks[t]
+        dz[t] = torch.where(live[t], lam * k, zero)
+        df[t] = torch.where(live[t], lam * (ins[t] - z[t]) * k * (1 - k), zero)
+        back = lam * (1 - k)
+        if case['masks']:
+            back = torch.where(live[t], torch.where(fresh[t], zero, back), carry)
+        carry = back
+    out.update(dz=dz, df=df, db=df.flatten(0, 1).sum(0), d0=carry)
+    return out
+
+
+def _exact_norm(s):
+    case = s['case']
+    names = ('o', 'g', 'x', 'weight', 'scale', 'next_weight')
+    o, g, x, w, sc, w2 = (s[n].detach().double() for n in names)
+
+    def unit(v):
+        return v / torch.sqrt((v * v).sum(-1, keepdim=True) / v.shape[-1] + EPS)
+
+    def block(o, g, x, w, sc, w2):
+        new = x + sc * unit(o) * w * g / (1 + torch.exp(-g))
+        return new, unit(new) * w2
+
+    if case['mode'] == 'infer':
+        new, u = block(o, g, x, w, sc, w2)
+        return {'x': new, 'u': u}
+    cot = (s['dx'].double(), s['du'].double())
+    if not case['checkpoint']:
+        with torch.enable_grad():
+            args = [t.requires_grad_(True) for t in (o, g, x, w, sc, w2)]
+            res = block(*args)
+            grads = torch.autograd.grad(res, args, cot)
+        return {'x': res[0].detach(), 'u': res[1].detach(), **{'d_' + n: t for n, t in zip(names, grads)}}
+    new, u = block(o, g, x, w, sc, w2)
+    length = torch.sqrt((o * o).mean(-1, keepdim=True) + EPS)
+    length2 = torch.sqrt((new * new).mean(-1, keepdim=True) + EPS)
+    out = {'x': new, 'u': u}
+    o, g, x = _kept8(o), _kept8(g), _kept8(x)
+    swish = g / (1 + torch.exp(-g))
+    e = o / length
+    e2 = (x + sc * w * e * swish) / length2
+    t2 = cot[1] * w2
+    gx = cot[0] + (t2 - e2 * (t2 * e2).mean(-1, keepdim=True)) / length2
+    t1 = gx * sc * swish * w
+    slope = (swish + (1 - swish) / (1 + torch.exp(-g)))
+    out.update(d_o=(t1 - e * (t1 * e).mean(-1, keepdim=True)) / length, d_g=gx * sc * e * w * slope, d_x=gx,
+               d_weight=(gx * sc * swish * e).sum(0), d_scale=(gx * e * w * swish).sum(0), d_next_weight=(cot[1] * e2).sum(0))
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    with torch.no_grad():
+        if case['kind'] == 'scan':
+            # a step of the 64-bit loops is some twenty launches
+            return _exact_scan(s) if case['T'] <= 20000 else None
+        if case['kind'] == 'norm':
+            return _exact_norm(s)
+        if case['kind'] == 'pack':
+            return {'x': _kept8(s['x'].double())}
+        pre = s['f'].double() + s['bias'].double()
+        h = s['h'].double() + (s['z'].double() - s['h'].double()) / (1 + torch.exp(pre))
+        g = s['g'].double()
+        unit = h / torch.sqrt((h * h).mean(-1, keepdim=True) + EPS)
+        new = s['x'].double() + s['scale'].double() * unit * s['weight'].double() * g / (1 + torch.exp(-g))
+        return {'x': new, 'u': new / torch.sqrt((new * new).mean(-1, keepdim=True) + EPS) * s['next_weight'].double(), 'h': h}
