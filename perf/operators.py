@@ -256,7 +256,7 @@ def _plain_scan(s):
         before = torch.cat([kept[:, None], inner[:, :-1]], 1).flatten(0, 1)[:T]
     if starts is not None:
         before = torch.where(starts, 0.0, before)
-    dh = s['dh'].float()
+    dh = s['dh'].to(torch.float32, copy=True)
     if pad is not None:
         dh = torch.where(pad, 0.0, dh)
     # lam_t = dh_t + decay_{t+1} lam_{t+1}, latest step first
