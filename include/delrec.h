@@ -277,6 +277,126 @@ typedef struct {
     size_t workspace_bytes;
 } delrec_readout_ce_args;
 
+/* ---- Gated linear recurrence, norms with gate and residual, 8-bit activation checkpoints ----
+ * No counterpart in the reference: the operators of a residual block
+ *     u = rms(x) w2;  z, f, g = W u;  h = gated scan of z under the gate f;
+ *     x' = x + scale * rms(h) w * silu(g)
+ * on the same time-major (T, B, N) sequences as the delayed-LIF layers. Activations are fp32 or
+ * bf16 (bf16 != 0); gates, states, norms and sums are computed and kept in 32 bits. */
+
+/* A (rows0, rows1, N) tensor: element (i, j, n) at data[i * s0 + j * s1 + n] (strides in
+ * elements, any sign; the last axis is contiguous). */
+typedef struct {
+    void* data;
+    int64_t s0, s1;
+} delrec_rows;
+
+/* A (rows, N) tensor kept in 8 bits: groups of 64 columns of a row (the last one shorter) share
+ * scale = max(amax * fl(1/127), 2^-126) and q = rint(x * fl(1/scale)), which stands for q * scale.
+ * A group that holds an infinity or a NaN has scale NaN (and q 0). */
+enum { DELREC_PACK8_GROUP = 64 };
+typedef struct {
+    int8_t* q;                   /* (rows, N) contiguous                                   */
+    float* scale;                /* (rows, ceil(N / 64)) contiguous                        */
+} delrec_packed8;
+
+/* k_t = sigmoid(-(f_t + bias)); h_t = h_{t-1} + k_t (z_t - h_{t-1}). At a start the state before
+ * the step is 0; from lengths[b] on the state stays and h is written 0 (z, f are not used there).
+ * states[i] is the state before step 64 i, which the backward pass starts from; with z8 / f8 the
+ * call also keeps z and f in 8 bits (over T * B rows). Outputs must not overlap inputs. */
+enum { DELREC_GATED_BLOCK = 64 };
+typedef struct {
+    int32_t T, B, N, bf16;
+    delrec_rows z, f;            /* (T, B, N)                                              */
+    const float* bias;           /* (N) or NULL                                            */
+    const float* h0;             /* (B, N) or NULL: 0                                      */
+    const uint8_t* starts;       /* (T, B) non-zero: a sequence starts here; or NULL       */
+    const int64_t* lengths;      /* (B) steps of each row, in [0, T]; or NULL: T           */
+    delrec_rows h;               /* out (T, B, N)                                          */
+    float* h_last;               /* out (B, N) the state after the last step               */
+    float* states;               /* out (ceil(T / 64), B, N), or NULL                      */
+    delrec_packed8 z8, f8;       /* out, or NULL pointers                                  */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_gated_scan_fwd_args;
+
+/* Gradients of that scan from dh and dlast. z and f are read as given, or, where z8.q is not NULL,
+ * as the 8-bit values that the forward kept; the states between the kept ones are recomputed. */
+typedef struct {
+    int32_t T, B, N, bf16;
+    delrec_rows z, f;            /* (T, B, N), not read with z8 / f8                       */
+    delrec_packed8 z8, f8;
+    const float* bias;
+    const float* states;         /* (ceil(T / 64), B, N) from the forward                  */
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows dh;              /* (T, B, N)                                              */
+    const float* dlast;          /* (B, N) or NULL: 0                                      */
+    delrec_rows dz, df;          /* out (T, B, N)                                          */
+    float* db;                   /* out (N), or NULL                                       */
+    float* dh0;                  /* out (B, N), or NULL                                    */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_gated_scan_bwd_args;
+
+/* x' = x + scale * (o r w) * silu(g), r = 1/sqrt(mean o^2 + eps), and u = x' r2 w2, r2 =
+ * 1/sqrt(mean x'^2 + eps) (of x' before it is rounded), over R0 * R1 rows of N >= 2. w2 NULL: no u.
+ * o.data NULL: no block, u = x r2 w2 alone (x_out not written). stats keeps r and r2 for the
+ * backward pass; o8 / g8 / x8 keep the inputs in 8 bits. */
+typedef struct {
+    int32_t R0, R1, N, bf16, x_bf16;   /* bf16: o, g, u; x_bf16: x, x_out                  */
+    delrec_rows o, g, x;
+    const float* w;              /* (N)                                                    */
+    const float* scale;          /* (N)                                                    */
+    const float* w2;             /* (N) or NULL                                            */
+    float eps;
+    void* x_out;                 /* out (R0, R1, N) contiguous                             */
+    void* u;                     /* out (R0, R1, N) contiguous                             */
+    float* stats;                /* out (R0 * R1, 2), or NULL                              */
+    delrec_packed8 o8, g8, x8;   /* out, or NULL pointers                                  */
+} delrec_norm_gate_fwd_args;
+
+typedef struct {
+    int32_t R0, R1, N, bf16, x_bf16;
+    delrec_rows o, g, x;         /* as the forward's, not read where the 8-bit form is given */
+    delrec_packed8 o8, g8, x8;
+    const float* w;
+    const float* scale;
+    const float* w2;
+    const float* stats;
+    delrec_rows dx_out;          /* gradient of x' (data NULL: 0)                          */
+    delrec_rows du;              /* gradient of u (data NULL: 0)                           */
+    delrec_rows d_o, dg, dx;     /* out                                                    */
+    float* dw;                   /* out (N)                                                */
+    float* dscale;               /* out (N)                                                */
+    float* dw2;                  /* out (N)                                                */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_norm_gate_bwd_args;
+
+/* One time step of the block for B rows: h' = h + k (z - h), then x' and u from o = h' as above
+ * (h' in 32 bits). h_out may be h. */
+typedef struct {
+    int32_t B, N, bf16, x_bf16;
+    delrec_rows z, f, g, x;      /* (1, B, N)                                              */
+    const float* h;              /* (B, N)                                                 */
+    const float* bias;           /* (N) or NULL                                            */
+    const float* w;
+    const float* scale;
+    const float* w2;             /* or NULL                                                */
+    float eps;
+    float* h_out;                /* out (B, N)                                             */
+    void* x_out;                 /* out (B, N)                                             */
+    void* u;                     /* out (B, N) when w2 is given                            */
+} delrec_gated_step_args;
+
+/* A tensor to 8 bits, and the values that it stands for. */
+typedef struct {
+    int32_t R0, R1, N, bf16;
+    delrec_rows x;               /* pack8: in; unpack8: out                                */
+    delrec_packed8 p;            /* pack8: out; unpack8: in                                */
+} delrec_pack8_args;
+
 /* Workspace kinds for delrec_query_workspace; flags bit 0: weights are bf16; synaptic
  * kinds: bit 1: hybrid delays (d == NULL), bits 8..15: ceil(2 * s_max) on the float32 s_max
  * the entry point receives (s_uniform for the hybrid), capped at 255 -- the most lags of
@@ -286,7 +406,9 @@ typedef struct {
 enum { DELREC_WS_AXONAL_FWD = 1, DELREC_WS_AXONAL_BWD = 2, DELREC_WS_SYN_FWD = 3,
        DELREC_WS_SYN_BWD = 4, DELREC_WS_SPIKE_LINEAR = 5 /* N = K inputs, L = M outputs */,
        DELREC_WS_SPIKE_LINEAR_DW = 6 /* N = K inputs, L = M outputs */,
-       DELREC_WS_READOUT_CE = 7 /* N = C classes, L = 1 */ };
+       DELREC_WS_READOUT_CE = 7 /* N = C classes, L = 1 */,
+       DELREC_WS_GATED_FWD = 8, DELREC_WS_GATED_BWD = 9 /* both: L = 1 */,
+       DELREC_WS_NORM_GATE_BWD = 10 /* T = R0, B = R1, L = 1 */ };
 
 int delrec_axonal_fwd(const delrec_axonal_fwd_args* a, void* stream);
 int delrec_axonal_bwd(const delrec_axonal_bwd_args* a, void* stream);
@@ -318,6 +440,13 @@ int delrec_spike_linear_dw(const delrec_spike_linear_dw_args* a, void* stream);
  * in the reference. */
 int delrec_spike_linear_dx_split(const float* g, int64_t rows, int32_t M, void* out, void* stream);
 int delrec_readout_ce(const delrec_readout_ce_args* a, void* stream);
+int delrec_gated_scan_fwd(const delrec_gated_scan_fwd_args* a, void* stream);
+int delrec_gated_scan_bwd(const delrec_gated_scan_bwd_args* a, void* stream);
+int delrec_gated_step(const delrec_gated_step_args* a, void* stream);
+int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream);
+int delrec_norm_gate_bwd(const delrec_norm_gate_bwd_args* a, void* stream);
+int delrec_pack8(const delrec_pack8_args* a, void* stream);
+int delrec_unpack8(const delrec_pack8_args* a, void* stream);
 int delrec_lif_fwd(const delrec_lif_fwd_args* a, void* stream);
 int delrec_lif_bwd(const delrec_lif_bwd_args* a, void* stream);
 
@@ -366,7 +495,7 @@ int delrec_peak_mfma(int32_t kind, int32_t iters, float* sink, size_t sink_bytes
 const char* delrec_strerror(int status);
 /* "delrec-mi355x <DELREC_ABI_VERSION> (gfx950)": a binding checks it before use (the
  * argument structs change between versions). */
-#define DELREC_ABI_VERSION "0.5.0"
+#define DELREC_ABI_VERSION "0.6.0"
 const char* delrec_version(void);
 
 #ifdef __cplusplus

@@ -797,6 +797,9 @@ int delrec_query_workspace(int32_t kind, int32_t T, int32_t B, int32_t N, int32_
         case DELREC_WS_READOUT_CE:
             c.take<float>((size_t)B);
             break;
+        case DELREC_WS_GATED_FWD: c.take<float>(gated_fwd_ws(T, B, N)); break;
+        case DELREC_WS_GATED_BWD: c.take<float>(gated_bwd_ws(T, B, N)); break;
+        case DELREC_WS_NORM_GATE_BWD: c.take<float>(norm_gate_bwd_ws((long long)T * B, N)); break;
         default: return DELREC_ERR_ARG;
     }
     *bytes = c.used;

@@ -577,6 +577,59 @@ const int* lag_bf16_cls(const LagBf16& a);
 // dW = sum_k pw; dd = W/s^2 * sum_k pd; ds[j] = sum_i W[i,j] * sum_k ps[i,j]
 void launch_lag_finish(const LagGemm& a, float* dW, float* dd, float* ds, hipStream_t stream);
 
+// ---- gated-recurrence block (gated.hip, normgate.hip, pack8.hip) ----
+struct GatedScan {               // forward and backward of the gated linear recurrence
+    int T, B, N, bf16;
+    delrec_rows z, f;
+    const float* bias;
+    const float* h0;
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows h;
+    float* h_last;
+    float* states;               // [ceil(T / 64)][B][N]
+    delrec_packed8 z8, f8;
+    delrec_rows dh, dz, df;
+    const float* dlast;
+    float* db;
+    float* dh0;
+    float* ws;                   // workspace, gated_fwd_ws / gated_bwd_ws floats
+};
+size_t gated_fwd_ws(int T, int B, int N);   // floats
+size_t gated_bwd_ws(int T, int B, int N);
+void launch_gated_fwd(const GatedScan& p, hipStream_t stream);
+void launch_gated_bwd(const GatedScan& p, hipStream_t stream);
+struct NormGate {                // norms, gate and residual of R0 * R1 rows; h: one step's form
+    int R0, R1, N, bf16, x_bf16;
+    delrec_rows o, g, x, z, f;
+    const float* h;              // step: the state, o = its update (NULL otherwise)
+    const float* bias;
+    float* h_out;
+    const float* w;              // NULL: no block, only the norm of x
+    const float* scale;
+    const float* w2;
+    float eps;
+    void* x_out;
+    void* u;
+    float* stats;                // [rows][2]: r, r2
+    delrec_packed8 o8, g8, x8;
+    delrec_rows dx_out, du, d_o, dg, dx;
+    float* dw;
+    float* dscale;
+    float* dw2;
+    float* part;                 // workspace of the backward
+};
+size_t norm_gate_bwd_ws(long long rows, int N);   // floats
+void launch_norm_gate(const NormGate& p, bool fwd, hipStream_t stream);
+struct Pack8 {
+    int R0, R1, N, bf16;
+    delrec_rows x;
+    delrec_packed8 p;
+};
+void launch_pack8(const Pack8& p, bool pack, hipStream_t stream);
+// o_k[n] = sum over rows r of part[r * pitch + k * N + n], k < pitch / N <= 3 (NULL: skipped)
+void launch_column_sums(const float* part, int rows, int N, int pitch, float* o0, float* o1, float* o2, hipStream_t stream);
+
 void launch_lif(bool fwd, const delrec_lif_fwd_args* fa, const delrec_lif_bwd_args* ba,
                 const Lif& k, int cus, hipStream_t stream);
 void launch_delay_grad(const float* C, const float* W, const float* d, float sigma, int N,

@@ -19,8 +19,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / 'csrc'
 INCLUDE = PKG.parent.parent / 'include'
 OUT = PKG / 'libdelrec_hip.so'
-SOURCES = ('abi.hip', 'axonal.hip', 'axwide.hip', 'farsparse.hip', 'gemm.hip', 'hybblock.hip', 'hybstep.hip', 'lagmm.hip', 'lagstep.hip', 'peaks.hip',
-           'readout.hip', 'spikelinear.hip', 'synaptic.hip', 'synlin.hip')
+SOURCES = ('abi.hip', 'axonal.hip', 'axwide.hip', 'farsparse.hip', 'gated.hip', 'gated_abi.hip', 'gemm.hip', 'hybblock.hip', 'hybstep.hip', 'lagmm.hip', 'lagstep.hip', 'normgate.hip',
+           'pack8.hip', 'peaks.hip', 'readout.hip', 'spikelinear.hip', 'synaptic.hip', 'synlin.hip')
 ARCH = os.environ.get('DELREC_OFFLOAD_ARCH', 'gfx950')
 
 

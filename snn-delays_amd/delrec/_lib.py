@@ -19,6 +19,7 @@ LIB_PATH = Path(os.environ.get('DELREC_HIP_LIB', _HERE / 'libdelrec_hip.so'))
 
 c_f32 = ctypes.c_float
 c_i32 = ctypes.c_int32
+c_i64 = ctypes.c_int64
 c_vp = ctypes.c_void_p
 c_size = ctypes.c_size_t
 
@@ -28,6 +29,8 @@ DELREC_ERR_WINDOW = 5
 DELREC_ERR_SCRATCH = 9
 WS_AXONAL_FWD, WS_AXONAL_BWD, WS_SYN_FWD, WS_SYN_BWD, WS_SPIKE_LINEAR = 1, 2, 3, 4, 5
 WS_SPIKE_LINEAR_DW, WS_READOUT_CE = 6, 7
+WS_GATED_FWD, WS_GATED_BWD, WS_NORM_GATE_BWD = 8, 9, 10
+GATED_BLOCK, PACK8_GROUP = 64, 64
 READOUT_SUM, READOUT_MEAN, READOUT_MAX = 0, 1, 2
 
 # Every symbol include/delrec.h declares (checked by the CPU test suite).
@@ -36,7 +39,9 @@ EXPORTS = ('delrec_axonal_fwd', 'delrec_axonal_bwd', 'delrec_axonal_bwd_noalloc'
            'delrec_lif_fwd', 'delrec_lif_bwd', 'delrec_delay_grad', 'delrec_query_workspace',
            'delrec_strerror', 'delrec_version', 'delrec_scan_timing', 'delrec_scan_timing_read',
            'delrec_max_post', 'delrec_max_take', 'delrec_peak_mfma', 'delrec_spike_linear_dw',
-           'delrec_spike_linear_dx_split', 'delrec_readout_ce')
+           'delrec_spike_linear_dx_split', 'delrec_readout_ce', 'delrec_gated_scan_fwd',
+           'delrec_gated_scan_bwd', 'delrec_gated_step', 'delrec_norm_gate_fwd', 'delrec_norm_gate_bwd',
+           'delrec_pack8', 'delrec_unpack8')
 
 
 class DelrecError(RuntimeError):
@@ -118,8 +123,55 @@ class LifBwdArgs(ctypes.Structure):
                 ('lif', Lif), ('dx', c_vp)]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [('data', c_vp), ('s0', c_i64), ('s1', c_i64)]
+
+
+class Packed8(ctypes.Structure):
+    _fields_ = [('q', c_vp), ('scale', c_vp)]
+
+
+class GatedScanFwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('bf16', c_i32), ('z', Rows), ('f', Rows),
+                ('bias', c_vp), ('h0', c_vp), ('starts', c_vp), ('lengths', c_vp), ('h', Rows),
+                ('h_last', c_vp), ('states', c_vp), ('z8', Packed8), ('f8', Packed8),
+                ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class GatedScanBwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('bf16', c_i32), ('z', Rows), ('f', Rows),
+                ('z8', Packed8), ('f8', Packed8), ('bias', c_vp), ('states', c_vp), ('starts', c_vp),
+                ('lengths', c_vp), ('dh', Rows), ('dlast', c_vp), ('dz', Rows), ('df', Rows),
+                ('db', c_vp), ('dh0', c_vp), ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class NormGateFwdArgs(ctypes.Structure):
+    _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x_bf16', c_i32),
+                ('o', Rows), ('g', Rows), ('x', Rows), ('w', c_vp), ('scale', c_vp), ('w2', c_vp),
+                ('eps', c_f32), ('x_out', c_vp), ('u', c_vp), ('stats', c_vp), ('o8', Packed8),
+                ('g8', Packed8), ('x8', Packed8)]
+
+
+class NormGateBwdArgs(ctypes.Structure):
+    _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x_bf16', c_i32),
+                ('o', Rows), ('g', Rows), ('x', Rows), ('o8', Packed8), ('g8', Packed8), ('x8', Packed8),
+                ('w', c_vp), ('scale', c_vp), ('w2', c_vp), ('stats', c_vp), ('dx_out', Rows), ('du', Rows),
+                ('d_o', Rows), ('dg', Rows), ('dx', Rows), ('dw', c_vp), ('dscale', c_vp), ('dw2', c_vp),
+                ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class GatedStepArgs(ctypes.Structure):
+    _fields_ = [('B', c_i32), ('N', c_i32), ('bf16', c_i32), ('x_bf16', c_i32), ('z', Rows), ('f', Rows),
+                ('g', Rows), ('x', Rows), ('h', c_vp), ('bias', c_vp), ('w', c_vp), ('scale', c_vp),
+                ('w2', c_vp), ('eps', c_f32), ('h_out', c_vp), ('x_out', c_vp), ('u', c_vp)]
+
+
+class Pack8Args(ctypes.Structure):
+    _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x', Rows), ('p', Packed8)]
+
+
 # the DELREC_ABI_VERSION of include/delrec.h these ctypes structs mirror
-ABI_VERSION = '0.5.0'
+ABI_VERSION = '0.6.0'
 
 _lib = None
 
@@ -135,7 +187,9 @@ def load():
     lib = ctypes.CDLL(str(LIB_PATH))
     for name in ('delrec_axonal_fwd', 'delrec_axonal_bwd', 'delrec_axonal_bwd_noalloc', 'delrec_syn_fwd',
                  'delrec_syn_bwd', 'delrec_spike_linear_fwd', 'delrec_spike_linear_dw', 'delrec_readout_ce',
-                 'delrec_lif_fwd', 'delrec_lif_bwd'):
+                 'delrec_lif_fwd', 'delrec_lif_bwd', 'delrec_gated_scan_fwd', 'delrec_gated_scan_bwd',
+                 'delrec_gated_step', 'delrec_norm_gate_fwd', 'delrec_norm_gate_bwd', 'delrec_pack8',
+                 'delrec_unpack8'):
         getattr(lib, name).restype = c_i32
         getattr(lib, name).argtypes = [c_vp, c_vp]
     lib.delrec_delay_grad.restype = c_i32
