@@ -28,7 +28,7 @@ def close(got, ref, tol, what, mass=None):
     big = (float(ref.abs().max()) if ref.numel() else 0.0) if mass is None else mass
     bound = tol * big + (2.0 ** -8 * ref.abs() if got.dtype == BF16 else 0.0) + 1e-30
     bad = ~((got64 - ref).abs() <= bound)
-    assert not bad.any(), f'{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((got64 - ref).abs().max()):.3e}, largest {ref.abs().max():.3e}'
+    assert int(bad.sum()) == 0, f'{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((got64 - ref).abs().max()):.3e}, largest {ref.abs().max():.3e}'
 
 
 def rnd(gen, *shape, dtype=FP32, std=1.0):
