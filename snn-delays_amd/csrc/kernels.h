@@ -618,6 +618,7 @@ struct NormGate {                // norms, gate and residual of R0 * R1 rows; h:
     float* dscale;
     float* dw2;
     float* part;                 // workspace of the backward
+    int flat;                    // set by the launcher: row r of every tensor is at r * s1
 };
 size_t norm_gate_bwd_ws(long long rows, int N);   // floats
 void launch_norm_gate(const NormGate& p, bool fwd, hipStream_t stream);

@@ -5,12 +5,24 @@
 //     dx = dx' + r2 (v2 - e2 <v2 e2>),  dn = scale dx silu(g),  v = w dn,
 //     do = r (v - e <v e>),  dg = scale dx e w silu'(g),
 //     dw2 = sum du e2,  dscale = sum dx y,  dw = sum dn e       (sums over the rows).
+//
+// Bound by memory: a row stays in registers between its loads and its stores, the two row sums
+// are exchanges between its lanes. A row is 16, 64, 256 or 512 lanes, each with NE vectors of
+// four columns, as few lanes as hold it in at most four vectors (16 lanes: four rows a wave, no
+// LDS). The backward recomputes x', e and the gate from o, g and x (or their 8 bits) and the two
+// kept norms: one residual tensor is read, not two. Its column sums stay in registers over all the
+// rows a workgroup takes; the workgroups' sums are added in a second launch, in a fixed order.
+#include <algorithm>
+#include <initializer_list>
+
 #include "gated.h"
 #include "kernels.h"
 
 namespace delrec {
 
 namespace {
+
+// ---- rows of any width (two or three columns, or past 8192): one workgroup a row ----
 
 constexpr int kNb = 256;
 
@@ -39,7 +51,7 @@ __device__ __forceinline__ float val8(const delrec_rows& x, const delrec_packed8
 
 // the block's output at one position: o (or, in a step, the state's update), gate, residual
 template <class S, class X>
-__global__ void __launch_bounds__(kNb) norm_gate_fwd_kernel(NormGate p) {
+__global__ void __launch_bounds__(kNb) norm_any_fwd_kernel(NormGate p) {
     __shared__ float red[4];
     const long long row = blockIdx.x;
     const int N = p.N;
@@ -85,7 +97,7 @@ __global__ void __launch_bounds__(kNb) norm_gate_fwd_kernel(NormGate p) {
 }
 
 template <class S, class X>
-__global__ void __launch_bounds__(kNb) norm_gate_bwd_kernel(NormGate p) {
+__global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
     __shared__ float red[4];
     const int N = p.N, tid = threadIdx.x;
     const bool block = p.w != nullptr;
@@ -162,27 +174,443 @@ void launch_column_sums(const float* part, int rows, int N, int pitch, float* o0
     hipLaunchKernelGGL(column_sums_kernel, dim3((N + 63) / 64, pitch / N), dim3(1024), 0, stream, part, rows, N, pitch, o0, o1, o2);
 }
 
-static int norm_gate_parts(long long rows) { return (int)(rows < 512 ? rows : 512); }
-size_t norm_gate_bwd_ws(long long rows, int N) { return (size_t)norm_gate_parts(rows) * 3 * N; }
+// ---- rows of 4 to 8192 columns in registers ----
 
-template <class S, class X>
-static void launch_norm_gate_t(const NormGate& p, bool fwd, hipStream_t stream) {
-    const long long rows = (long long)p.R0 * p.R1;
-    if (fwd) hipLaunchKernelGGL((norm_gate_fwd_kernel<S, X>), dim3((unsigned)rows), dim3(kNb), 0, stream, p);
-    else hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X>), dim3(norm_gate_parts(rows)), dim3(kNb), 0, stream, p);
+namespace {
+
+template <int LPR>
+constexpr int kRowBlock = LPR < 256 ? 256 : LPR;
+
+// a sum over the row's lanes; `slot`: this call's LDS words (two sets, used in turn)
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v, float* red, int slot) {
+    v = group_sum_t<LPR < 64 ? LPR : 64>(v);
+    if constexpr (LPR > 64) {
+        constexpr int W = LPR / 64;
+        if ((threadIdx.x & 63) == 0) red[slot * W + (threadIdx.x >> 6)] = v;
+        barrier_lds();
+        v = red[slot * W];
+#pragma unroll
+        for (int q = 1; q < W; ++q) v += red[slot * W + q];
+    }
+    return v;
 }
 
-void launch_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
-    if (!p.bf16) launch_norm_gate_t<float, float>(p, fwd, stream);
-    else if (p.x_bf16) launch_norm_gate_t<__bf16, __bf16>(p, fwd, stream);
-    else launch_norm_gate_t<__bf16, float>(p, fwd, stream);
-    if (fwd) {
-        if (p.o8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.o, p.o8}, true, stream);
-        if (p.g8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.g, p.g8}, true, stream);
-        if (p.x8.q) launch_pack8({p.R0, p.R1, p.N, p.x_bf16, p.x, p.x8}, true, stream);
-    } else {
-        launch_column_sums(p.part, norm_gate_parts((long long)p.R0 * p.R1), p.N, 3 * p.N, p.dw, p.dscale, p.dw2, stream);
+// The lane's columns. The last lane of a row whose width is no multiple of 4 is moved back to end
+// with it; lanes past the row repeat its last columns. Both compute and, where they store, store
+// the values of columns that other lanes hold as well; sums leave the first `skip` out.
+template <int LPR, int NE>
+struct Cols {
+    int n0[NE], skip[NE], group[NE];
+    bool on[NE], first[NE];
+    __device__ __forceinline__ Cols(int lane, int N) {
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            const int i = (e * LPR + lane) * 4;
+            on[e] = i < N;
+            n0[e] = min(i, N - 4);
+            skip[e] = on[e] ? i - n0[e] : 4;
+            group[e] = i / kGroup8;
+            first[e] = on[e] && i % kGroup8 == 0;
+        }
     }
+};
+
+template <class T>
+__device__ __forceinline__ T* row_at(const delrec_rows& x, long long row, const NormGate& p) {
+    if (p.flat) return (T*)x.data + row * x.s1;
+    const unsigned r = (unsigned)row, i = r / (unsigned)p.R1, j = r - i * (unsigned)p.R1;
+    return (T*)x.data + i * x.s0 + j * x.s1;
+}
+
+template <int NE>
+__device__ __forceinline__ void load_cols(float (&v)[NE][4], const float* x, const int (&n0)[NE]) {
+#pragma unroll
+    for (int e = 0; e < NE; ++e) {
+        const auto t = vload<float, 4>(x + n0[e]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[e][j] = t.get(j);
+    }
+}
+
+enum { kNormOnly = 0, kNormBlock = 1, kNormStep = 2 };
+
+}  // namespace
+
+template <class S, class X, int LPR, int NE, int FORM>
+__global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_fwd_kernel(NormGate p) {
+    __shared__ float red[2 * (LPR > 64 ? LPR / 64 : 1)];
+    constexpr int RPW = kRowBlock<LPR> / LPR;
+    const int lane = threadIdx.x % LPR, N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
+    const Cols<LPR, NE> c(lane, N);
+    const long long rows = (long long)p.R0 * p.R1;
+    float w[NE][4], sc[NE][4], w2[NE][4], bias[NE][4];
+    if constexpr (FORM != kNormOnly) {
+        load_cols<NE>(w, p.w, c.n0);
+        load_cols<NE>(sc, p.scale, c.n0);
+    }
+    if (p.w2) load_cols<NE>(w2, p.w2, c.n0);
+    if constexpr (FORM == kNormStep) {
+        if (p.bias) load_cols<NE>(bias, p.bias, c.n0);
+    }
+    const float inv_n = 1.0f / (float)N;
+    // rows past the end repeat the last one and store nothing (its lanes join the exchanges)
+    for (long long r0 = (long long)blockIdx.x * RPW; r0 < rows; r0 += (long long)gridDim.x * RPW) {
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        const bool live = mine < rows;
+        Vec<X, 4> xv[NE];
+        Vec<S, 4> ov[NE], gv[NE];
+        float o[NE][4], x[NE][4], r = 0.0f, r2 = 0.0f, s = 0.0f;
+        const X* xp = row_at<const X>(p.x, row, p);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) xv[e] = vload<X, 4>(xp + c.n0[e]);
+        if constexpr (FORM != kNormOnly) {
+            const S* gp = row_at<const S>(p.g, row, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) gv[e] = vload<S, 4>(gp + c.n0[e]);
+            if constexpr (FORM == kNormBlock) {
+                const S* op = row_at<const S>(p.o, row, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    ov[e] = vload<S, 4>(op + c.n0[e]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[e][j] = ov[e].get(j);
+                }
+            } else {
+                const S* zp = row_at<const S>(p.z, row, p);
+                const S* fp = row_at<const S>(p.f, row, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const auto z = vload<S, 4>(zp + c.n0[e]);
+                    const auto f = vload<S, 4>(fp + c.n0[e]);
+                    const auto h = vload<float, 4>(p.h + row * N + c.n0[e]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float k = gate_in(f.get(j) + (p.bias ? bias[e][j] : 0.0f));
+                        o[e][j] = fmaf(k, z.get(j) - h.get(j), h.get(j));
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s += j >= c.skip[e] ? o[e][j] * o[e][j] : 0.0f;
+            r = 1.0f / sqrtf(lanes_sum<LPR>(s, red, 0) * inv_n + p.eps);
+            s = 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[e][j] = xv[e].get(j);
+                if constexpr (FORM != kNormOnly) {
+                    const float g = gv[e].get(j);
+                    x[e][j] = fmaf(sc[e][j], o[e][j] * r * w[e][j] * (g * sigm(g)), x[e][j]);
+                }
+                s += j >= c.skip[e] ? x[e][j] * x[e][j] : 0.0f;
+            }
+            if constexpr (FORM != kNormOnly) {
+                if (live && c.on[e]) {
+                    vstore<X, 4>((X*)p.x_out + row * N + c.n0[e], x[e]);
+                    // in place: no lane may read a column of h that another has written. Every
+                    // lane of the row has read its own before the first row sum.
+                    if constexpr (FORM == kNormStep) vstore<float, 4>(p.h_out + row * N + c.n0[e], o[e]);
+                }
+            }
+        }
+        if (p.w2) {
+            r2 = 1.0f / sqrtf(lanes_sum<LPR>(s, red, 1) * inv_n + p.eps);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                float u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) u[j] = x[e][j] * r2 * w2[e][j];
+                if (live && c.on[e]) vstore<S, 4>((S*)p.u + row * N + c.n0[e], u);
+            }
+        }
+        // rows with one sum alone: its words are read before the next row's are written
+        if constexpr (LPR > 64) {
+            if (FORM == kNormOnly || !p.w2) barrier_lds();
+        }
+        if constexpr (FORM != kNormStep) {
+            if (p.stats && live && lane == 0) {
+                p.stats[2 * row] = r;
+                p.stats[2 * row + 1] = r2;
+            }
+            if (p.x8.q) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const int skip = live ? c.skip[e] : 4;
+                    const bool first = live && c.first[e];
+                    const size_t q = row * N + c.n0[e], g = row * ng + c.group[e];
+                    float v[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = xv[e].get(j);
+                    store8<4>(v, skip, first, p.x8.q + q, p.x8.scale + g);
+                    if constexpr (FORM == kNormBlock) {
+                        store8<4>(o[e], skip, first, p.o8.q + q, p.o8.scale + g);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = gv[e].get(j);
+                        store8<4>(v, skip, first, p.g8.q + q, p.g8.scale + g);
+                    }
+                }
+            }
+        }
+    }
+}
+
+// PACK: o, g and x from their 8 bits
+template <class S, class X, int LPR, int NE, bool BLOCK, bool PACK>
+__global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate p) {
+    constexpr int RPW = kRowBlock<LPR> / LPR, W = LPR > 64 ? LPR / 64 : 1;
+    __shared__ float red[2 * W];
+    __shared__ float slots[RPW > 1 ? RPW : 1][RPW > 1 ? LPR * NE * 4 : 1];
+    const int lane = threadIdx.x % LPR, N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
+    const Cols<LPR, NE> c(lane, N);
+    const long long rows = (long long)p.R0 * p.R1;
+    float w[NE][4], sc[NE][4], w2[NE][4], acc[3][NE][4];
+    if constexpr (BLOCK) {
+        load_cols<NE>(w, p.w, c.n0);
+        load_cols<NE>(sc, p.scale, c.n0);
+    }
+    if (p.w2) load_cols<NE>(w2, p.w2, c.n0);
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            acc[0][e][j] = acc[1][e][j] = acc[2][e][j] = 0.0f;
+            if (!p.w2) w2[e][j] = 0.0f;
+        }
+    const float inv_n = 1.0f / (float)N;
+    for (long long r0 = (long long)blockIdx.x * RPW; r0 < rows; r0 += (long long)gridDim.x * RPW) {
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        const bool live = mine < rows;
+        float o[NE][4], g[NE][4], x[NE][4], up[NE][4], du[NE][4];
+        auto take = [&](auto tag, const delrec_rows& src, const delrec_packed8& q, float (&v)[NE][4]) {
+            using T = decltype(tag);
+            if constexpr (PACK) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const auto t = load8<4>(q, (size_t)row, c.n0[e], N, ng);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[e][j] = t.get(j);
+                }
+            } else {
+                const T* b = row_at<const T>(src, row, p);
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
+                    const auto t = vload<T, 4>(b + c.n0[e]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[e][j] = t.get(j);
+                }
+            }
+        };
+        auto grad = [&](auto tag, const delrec_rows& src, float (&v)[NE][4]) {
+            using T = decltype(tag);
+            const T* b = src.data ? row_at<const T>(src, row, p) : nullptr;
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                if (b) {
+                    const auto t = vload<T, 4>(b + c.n0[e]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[e][j] = live ? t.get(j) : 0.0f;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[e][j] = 0.0f;
+                }
+            }
+        };
+        if constexpr (BLOCK) {
+            take(S{}, p.o, p.o8, o);
+            take(S{}, p.g, p.g8, g);
+        }
+        take(X{}, p.x, p.x8, x);
+        grad(X{}, p.dx_out, up);
+        grad(S{}, p.du, du);
+        const float r = p.stats[2 * row], r2 = p.stats[2 * row + 1];
+        // o becomes e = o r, x becomes e2 = x' r2
+        float s = 0.0f, si[NE][4], sg[NE][4];
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (BLOCK) {
+                    o[e][j] *= r;
+                    sg[e][j] = sigm(g[e][j]);
+                    si[e][j] = g[e][j] * sg[e][j];
+                    x[e][j] = fmaf(sc[e][j], o[e][j] * w[e][j] * si[e][j], x[e][j]);
+                }
+                x[e][j] *= r2;
+                s += j >= c.skip[e] ? w2[e][j] * du[e][j] * x[e][j] : 0.0f;
+            }
+        const float m2 = lanes_sum<LPR>(s, red, 0) * inv_n;
+        s = 0.0f;
+        X* dxp = row_at<X>(p.dx, row, p);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            float dg[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float dx = fmaf(r2, w2[e][j] * du[e][j] - x[e][j] * m2, up[e][j]);
+                acc[2][e][j] = fmaf(du[e][j], x[e][j], acc[2][e][j]);
+                up[e][j] = dx;
+                if constexpr (BLOCK) {
+                    const float dxs = dx * si[e][j], dn = sc[e][j] * dxs, ew = o[e][j] * w[e][j];
+                    acc[0][e][j] = fmaf(dn, o[e][j], acc[0][e][j]);
+                    acc[1][e][j] = fmaf(dxs, ew, acc[1][e][j]);
+                    dg[j] = sc[e][j] * dx * ew * fmaf(si[e][j], 1.0f - sg[e][j], sg[e][j]);
+                    g[e][j] = w[e][j] * dn;  // v
+                    s += j >= c.skip[e] ? g[e][j] * o[e][j] : 0.0f;
+                }
+            }
+            if (live && c.on[e]) {
+                vstore<X, 4>(dxp + c.n0[e], up[e]);
+                if constexpr (BLOCK) vstore<S, 4>(row_at<S>(p.dg, row, p) + c.n0[e], dg);
+            }
+        }
+        if constexpr (BLOCK) {
+            const float m = lanes_sum<LPR>(s, red, 1) * inv_n;
+            S* dop = row_at<S>(p.d_o, row, p);
+#pragma unroll
+            for (int e = 0; e < NE; ++e) {
+                float d[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[j] = r * (g[e][j] - o[e][j] * m);
+                if (live && c.on[e]) vstore<S, 4>(dop + c.n0[e], d);
+            }
+        } else if constexpr (LPR > 64) {
+            barrier_lds();
+        }
+    }
+    float* part = p.part + (size_t)blockIdx.x * 3 * N;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        if constexpr (RPW > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) slots[threadIdx.x / LPR][(e * LPR + lane) * 4 + j] = acc[k][e][j];
+            __syncthreads();
+            if (threadIdx.x < LPR)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        for (int q = 1; q < RPW; ++q) acc[k][e][j] += slots[q][(e * LPR + lane) * 4 + j];
+        }
+        if (threadIdx.x < LPR)
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+                if (c.on[e]) vstore<float, 4>(part + (size_t)k * N + c.n0[e], acc[k][e]);
+    }
+}
+
+namespace {
+
+bool in_registers(int N) { return N >= 4 && N <= 8192; }
+
+// (lanes of a row, vectors of a lane). The backward holds three more rows and the column sums:
+// two vectors a lane up to 2048 columns.
+struct RowPlan {
+    int lanes, vecs, rpw;
+};
+RowPlan row_plan(int N, bool fwd) {
+    RowPlan q{};
+    if (N <= 64) q = {16, 1};
+    else if (N <= 128) q = {16, 2};
+    else if (N <= 256) q = {64, 1};
+    else if (N <= 512) q = {64, 2};
+    else if (N <= 1024) q = fwd ? RowPlan{64, 4} : RowPlan{256, 1};
+    else if (N <= 2048) q = {256, 2};
+    else if (N <= 4096) q = {256, 4};
+    else q = {512, 4};
+    q.rpw = q.lanes < 256 ? 256 / q.lanes : 1;
+    return q;
+}
+
+// workgroups of the backward, one set of column sums each: enough to fill the GPU, few enough that
+// the sums are small beside the rows
+int norm_gate_parts(long long rows, int N) {
+    const long long wg = in_registers(N) ? (rows + row_plan(N, false).rpw - 1) / row_plan(N, false).rpw : rows;
+    return (int)std::min<long long>(wg, in_registers(N) ? 1024 : 512);
+}
+
+template <class S, class X, int LPR, int NE>
+void run_fwd(const NormGate& p, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    const int rpw = kRowBlock<LPR> / LPR;
+    const dim3 grid((unsigned)std::min<long long>((rows + rpw - 1) / rpw, 4096)), block(kRowBlock<LPR>);
+    if (p.h) hipLaunchKernelGGL((norm_gate_fwd_kernel<S, X, LPR, NE, kNormStep>), grid, block, 0, stream, p);
+    else if (p.w) hipLaunchKernelGGL((norm_gate_fwd_kernel<S, X, LPR, NE, kNormBlock>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((norm_gate_fwd_kernel<S, X, LPR, NE, kNormOnly>), grid, block, 0, stream, p);
+}
+
+template <class S, class X, int LPR, int NE>
+void run_bwd(const NormGate& p, int parts, hipStream_t stream) {
+    const dim3 grid(parts), block(kRowBlock<LPR>);
+    if (p.w) {
+        if (p.x8.q) hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, true, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, true, false>), grid, block, 0, stream, p);
+    } else {
+        if (p.x8.q) hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, false, true>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, false, false>), grid, block, 0, stream, p);
+    }
+}
+
+template <class S, class X>
+void run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    const int parts = norm_gate_parts(rows, p.N);
+    if (!in_registers(p.N)) {
+        if (fwd) {
+            hipLaunchKernelGGL((norm_any_fwd_kernel<S, X>), dim3((unsigned)rows), dim3(kNb), 0, stream, p);
+            if (p.o8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.o, p.o8}, true, stream);
+            if (p.g8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.g, p.g8}, true, stream);
+            if (p.x8.q) launch_pack8({p.R0, p.R1, p.N, p.x_bf16, p.x, p.x8}, true, stream);
+        } else {
+            hipLaunchKernelGGL((norm_any_bwd_kernel<S, X>), dim3(parts), dim3(kNb), 0, stream, p);
+        }
+        return;
+    }
+    const RowPlan q = row_plan(p.N, fwd);
+    if (fwd) {
+        if (q.lanes == 16) q.vecs == 1 ? run_fwd<S, X, 16, 1>(p, stream) : run_fwd<S, X, 16, 2>(p, stream);
+        else if (q.lanes == 64) q.vecs == 1 ? run_fwd<S, X, 64, 1>(p, stream) : q.vecs == 2 ? run_fwd<S, X, 64, 2>(p, stream) : run_fwd<S, X, 64, 4>(p, stream);
+        else if (q.lanes == 256) q.vecs == 2 ? run_fwd<S, X, 256, 2>(p, stream) : run_fwd<S, X, 256, 4>(p, stream);
+        else run_fwd<S, X, 512, 4>(p, stream);
+    } else {
+        if (q.lanes == 16) q.vecs == 1 ? run_bwd<S, X, 16, 1>(p, parts, stream) : run_bwd<S, X, 16, 2>(p, parts, stream);
+        else if (q.lanes == 64) q.vecs == 1 ? run_bwd<S, X, 64, 1>(p, parts, stream) : run_bwd<S, X, 64, 2>(p, parts, stream);
+        else if (q.lanes == 256) q.vecs == 1 ? run_bwd<S, X, 256, 1>(p, parts, stream) : q.vecs == 2 ? run_bwd<S, X, 256, 2>(p, parts, stream) : run_bwd<S, X, 256, 4>(p, parts, stream);
+        else run_bwd<S, X, 512, 4>(p, parts, stream);
+    }
+}
+
+}  // namespace
+
+size_t norm_gate_bwd_ws(long long rows, int N) { return (size_t)norm_gate_parts(rows, N) * 3 * N; }
+
+void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
+    NormGate p = a;
+    // rows one pitch apart in every tensor need no division by R1
+    p.flat = p.R0 == 1;
+    if (!p.flat) {
+        p.flat = 1;
+        for (const delrec_rows* t : {&p.o, &p.g, &p.x, &p.dx_out, &p.du, &p.d_o, &p.dg, &p.dx})
+            if (t->data && t->s0 != t->s1 * p.R1) p.flat = 0;
+        if (p.R1 == 1) {
+            p.flat = 1;
+            for (delrec_rows* t : {&p.o, &p.g, &p.x, &p.dx_out, &p.du, &p.d_o, &p.dg, &p.dx}) t->s1 = t->s0;
+            p.R1 = p.R0;
+            p.R0 = 1;
+        }
+    }
+    if (!p.bf16) run_norm_gate<float, float>(p, fwd, stream);
+    else if (p.x_bf16) run_norm_gate<__bf16, __bf16>(p, fwd, stream);
+    else run_norm_gate<__bf16, float>(p, fwd, stream);
+    if (!fwd)
+        launch_column_sums(p.part, norm_gate_parts((long long)p.R0 * p.R1, p.N), p.N, 3 * p.N, p.dw, p.dscale, p.dw2, stream);
 }
 
 }  // namespace delrec

@@ -1,12 +1,15 @@
 // A (rows, N) tensor to 8 bits and back: groups of 64 columns of a row share one 32-bit scale,
 //     scale = max(amax / 127, 2^-126), q = rint(x / scale), x^ = q scale.
+#include <algorithm>
+
 #include "gated.h"
 #include "kernels.h"
 
 namespace delrec {
 
+// one to three columns: a wave a row
 template <class S>
-__global__ void __launch_bounds__(256) pack8_kernel(Pack8 p) {
+__global__ void __launch_bounds__(256) pack8_any_kernel(Pack8 p) {
     const int lane = threadIdx.x & 63;
     const long long grp = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     const int ng = (p.N + kGroup8 - 1) / kGroup8;
@@ -24,7 +27,7 @@ __global__ void __launch_bounds__(256) pack8_kernel(Pack8 p) {
 }
 
 template <class S>
-__global__ void __launch_bounds__(256) unpack8_kernel(Pack8 p) {
+__global__ void __launch_bounds__(256) unpack8_any_kernel(Pack8 p) {
     const int ng = (p.N + kGroup8 - 1) / kGroup8;
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= (long long)p.R0 * p.R1 * p.N) return;
@@ -34,17 +37,87 @@ __global__ void __launch_bounds__(256) unpack8_kernel(Pack8 p) {
     x[n] = (S)((float)p.p.q[i] * p.p.scale[row * ng + n / kGroup8]);
 }
 
-void launch_pack8(const Pack8& p, bool pack, hipStream_t stream) {
+// Rows of four columns and more: LPR lanes a row, four columns a lane (16 lanes a group), kRows
+// rows at once so that their loads are in flight together. The last lane of a row whose width is
+// no multiple of 4 is moved back to end with it.
+namespace {
+constexpr int kRows = 4;
+
+__device__ __forceinline__ long long row_offset(const Pack8& p, long long row) {
+    if (p.R0 == 1) return row * p.x.s1;
+    if (p.R1 == 1) return row * p.x.s0;
+    const unsigned r = (unsigned)row, i = r / (unsigned)p.R1;
+    return i * p.x.s0 + (r - i * (unsigned)p.R1) * p.x.s1;
+}
+}  // namespace
+
+template <class S, int LPR, bool PACK>
+__global__ void __launch_bounds__(256) pack8_kernel(Pack8 p) {
+    constexpr int RPW = 256 / LPR;
+    const int N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
+    const int i = (blockIdx.x * LPR + threadIdx.x % LPR) * 4, n0 = min(i, N - 4), group = min(i, N - 1) / kGroup8;
+    const bool on = i < N, first = on && i % kGroup8 == 0;
     const long long rows = (long long)p.R0 * p.R1;
-    if (pack) {
-        const unsigned g = (unsigned)((rows * ((p.N + kGroup8 - 1) / kGroup8) + 3) / 4);
-        if (p.bf16) hipLaunchKernelGGL(pack8_kernel<__bf16>, dim3(g), dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL(pack8_kernel<float>, dim3(g), dim3(256), 0, stream, p);
-    } else {
-        const unsigned g = (unsigned)((rows * p.N + 255) / 256);
-        if (p.bf16) hipLaunchKernelGGL(unpack8_kernel<__bf16>, dim3(g), dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL(unpack8_kernel<float>, dim3(g), dim3(256), 0, stream, p);
+    for (long long r0 = (long long)blockIdx.y * RPW * kRows; r0 < rows; r0 += (long long)gridDim.y * RPW * kRows) {
+        // rows past the end repeat the last one and store nothing
+        long long row[kRows];
+        bool live[kRows];
+#pragma unroll
+        for (int q = 0; q < kRows; ++q) {
+            const long long mine = r0 + q * RPW + threadIdx.x / LPR;
+            live[q] = mine < rows && on;
+            row[q] = mine < rows ? mine : rows - 1;
+        }
+        if constexpr (PACK) {
+            Vec<S, 4> v[kRows];
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) v[q] = vload<S, 4>((const S*)p.x.data + row_offset(p, row[q]) + n0);
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = v[q].get(j);
+                store8<4>(x, live[q] ? i - n0 : 4, live[q] && first, p.p.q + row[q] * N + n0, p.p.scale + row[q] * ng + group);
+            }
+        } else {
+            Vec8<4> v[kRows];
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) v[q] = load8<4>(p.p, (size_t)row[q], n0, N, ng);
+#pragma unroll
+            for (int q = 0; q < kRows; ++q) {
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = v[q].get(j);
+                if (live[q]) vstore<S, 4>((S*)p.x.data + row_offset(p, row[q]) + n0, x);
+            }
+        }
     }
+}
+
+template <class S, bool PACK>
+static void run_pack8(const Pack8& p, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    const int lanes = (p.N + kGroup8 - 1) / kGroup8 * (kGroup8 / 4);
+    auto grid = [&](int lpr) {
+        const int per = 256 / lpr * kRows;
+        return dim3((lanes + lpr - 1) / lpr, (unsigned)std::min<long long>((rows + per - 1) / per, 16384));
+    };
+    if (lanes <= 16) hipLaunchKernelGGL((pack8_kernel<S, 16, PACK>), grid(16), dim3(256), 0, stream, p);
+    else if (lanes <= 64) hipLaunchKernelGGL((pack8_kernel<S, 64, PACK>), grid(64), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((pack8_kernel<S, 256, PACK>), grid(256), dim3(256), 0, stream, p);
+}
+
+template <class S>
+static void run_pack8_any(const Pack8& p, bool pack, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    if (p.N >= 4) return pack ? run_pack8<S, true>(p, stream) : run_pack8<S, false>(p, stream);
+    if (pack) hipLaunchKernelGGL(pack8_any_kernel<S>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(unpack8_any_kernel<S>, dim3((unsigned)((rows * p.N + 255) / 256)), dim3(256), 0, stream, p);
+}
+
+void launch_pack8(const Pack8& p, bool pack, hipStream_t stream) {
+    if (p.bf16) run_pack8_any<__bf16>(p, pack, stream);
+    else run_pack8_any<float>(p, pack, stream);
 }
 
 }  // namespace delrec
