@@ -47,17 +47,17 @@ def _run(cmd, verbose):
         raise RuntimeError(f'hipcc failed ({res.returncode}): {cmd[-1]}')
 
 
-EXT_SOURCE = CSRC / 'torch_ext.cpp'
+EXT_SOURCES = (CSRC / 'torch_ext.cpp', CSRC / 'torch_gated.cpp')
 EXT_OUT = PKG / 'delrec_torch.so'
 
 
 def extension_command(out=EXT_OUT):
-    """Host-only compile of the C++ autograd Function (torch_ext.cpp) against torch and the
-    HIP library, which it finds next to itself at run time (rpath $ORIGIN)."""
+    """Host-only compile of the C++ autograd Functions (torch_ext.cpp, torch_gated.cpp) against
+    torch and the HIP library, which it finds next to itself at run time (rpath $ORIGIN)."""
     import sysconfig
     import torch
     tdir = Path(torch.__file__).resolve().parent
-    return [_hipcc(), '--cuda-host-only', '-O2', '-std=c++17', '-fPIC', '-shared', str(EXT_SOURCE), '-o', str(out),
+    return [_hipcc(), '--cuda-host-only', '-O2', '-std=c++17', '-fPIC', '-shared', *map(str, EXT_SOURCES), '-o', str(out),
             f'-I{tdir / "include"}', f'-I{tdir / "include" / "torch" / "csrc" / "api" / "include"}',
             f'-I{sysconfig.get_paths()["include"]}', f'-I{INCLUDE}',
             '-DTORCH_EXTENSION_NAME=delrec_torch', '-DTORCH_API_INCLUDE_EXTENSION_H',

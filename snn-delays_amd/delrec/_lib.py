@@ -239,6 +239,16 @@ def torch_ext():
     return _EXT[0]
 
 
+def require_ext():
+    """The C++ extension, for the operators that have no other host path: ImportError with the
+    build hint where it has not been built."""
+    ext = torch_ext()
+    if ext is None:
+        raise ImportError(f'{EXT_PATH} is not built: run `python -c "import __graft_entry__ as g; '
+                          f'g.build()"` from the repository root')
+    return ext
+
+
 def _check(fn, status):
     if status != 0:
         raise DelrecError(fn, status, load().delrec_strerror(status).decode())
