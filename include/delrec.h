@@ -293,10 +293,10 @@ typedef struct {
 
 /* A (rows, N) tensor kept in 8 bits: groups of 64 columns of a row (the last one shorter) share
  * scale = max(amax * fl(1/127), 2^-126) and q = rint(x * fl(1/scale)), which stands for q * scale.
- * A group that holds an infinity or a NaN has scale NaN (and q 0). */
+ * A group that holds an infinity or a NaN has scale NaN, and its q mean nothing. */
 enum { DELREC_PACK8_GROUP = 64 };
 typedef struct {
-    int8_t* q;                   /* (rows, N) contiguous                                   */
+    int8_t* q;                   /* (rows, N) at a pitch of N rounded up to a multiple of 4 */
     float* scale;                /* (rows, ceil(N / 64)) contiguous                        */
 } delrec_packed8;
 

@@ -2,12 +2,11 @@
 // pack8.hip): element types, the gate, the 8-bit groups.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
 
 namespace delrec {
-
-typedef float gf4 __attribute__((ext_vector_type(4)));
-typedef __bf16 gb4 __attribute__((ext_vector_type(4)));
 
 // activations: float, or bf16 by the hardware's round to nearest even
 template <class S>
@@ -21,45 +20,36 @@ __device__ __forceinline__ float gate_in(float x) {
 }
 
 // V consecutive activations of a row, at any alignment of the element (rows of odd width start
-// anywhere): one 8- or 16-byte access for V = 4
-typedef gf4 gf4u __attribute__((aligned(4)));
-typedef gb4 gb4u __attribute__((aligned(2)));
-
+// anywhere): one access of up to 16 bytes
 template <class S, int V>
-struct Vec {                       // V values as loaded
-    S v[V];
+struct Vec {
+    typedef S type __attribute__((ext_vector_type(V)));
+    typedef type unaligned __attribute__((aligned(sizeof(S))));
+    type v;
     __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
 };
-template <>
-struct Vec<float, 4> {
-    gf4 v;
-    __device__ __forceinline__ float get(int j) const { return v[j]; }
-};
-template <>
-struct Vec<__bf16, 4> {
-    gb4 v;
-    __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
+template <class S>
+struct Vec<S, 1> {
+    S v;
+    __device__ __forceinline__ float get(int) const { return (float)v; }
 };
 
 template <class S, int V>
 __device__ __forceinline__ Vec<S, V> vload(const S* p) {
     Vec<S, V> r;
-    if constexpr (V == 4 && sizeof(S) == 4) r.v = *(const gf4u*)p;
-    else if constexpr (V == 4) r.v = *(const gb4u*)p;
-    else
-#pragma unroll
-        for (int j = 0; j < V; ++j) r.v[j] = p[j];
+    if constexpr (V > 1) r.v = *(const typename Vec<S, V>::unaligned*)p;
+    else r.v = *p;
     return r;
 }
 template <class S, int V>
 __device__ __forceinline__ void vstore(S* p, const float* x) {
-    if constexpr (V == 4) {
-        const gf4 t = {x[0], x[1], x[2], x[3]};
-        if constexpr (sizeof(S) == 4) *(gf4u*)p = t;
-        else *(gb4u*)p = __builtin_convertvector(t, gb4);
-    } else {
+    if constexpr (V > 1) {
+        typename Vec<float, V>::type t;
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[j] = (S)x[j];
+        for (int j = 0; j < V; ++j) t[j] = x[j];
+        *(typename Vec<S, V>::unaligned*)p = __builtin_convertvector(t, typename Vec<S, V>::type);
+    } else {
+        *p = (S)x[0];
     }
 }
 
@@ -73,12 +63,16 @@ __device__ __forceinline__ float scale8(float amax, bool finite) {
     return finite ? fmaxf(amax * kInv127, kMinScale8) : __builtin_nanf("");
 }
 __device__ __forceinline__ bool finite8(float v) { return fabsf(v) < __builtin_inff(); }
-// inv = 1 / scale rounded; |v| <= amax, so |v inv| < 127.5
-__device__ __forceinline__ int quant8(float v, float inv) {
-    const float q = rintf(v * inv);
-    return q == q ? (int)q : 0;
+// fl(1 / scale): one Newton step from the hardware's reciprocal (within 1 ulp) rounds correctly
+// (Markstein), the all-ones mantissa aside; scales and reciprocals here are normal numbers.
+__device__ __forceinline__ float recip8(float scale) {
+    const float r = __builtin_amdgcn_rcpf(scale);
+    return fmaf(fmaf(-scale, r, 1.0f), r, r);
 }
-
+// rint(v inv) in the low byte: |v inv| < 127.5, and at 1.5 * 2^23 a unit is the last place
+__device__ __forceinline__ uint32_t quant8(float v, float inv) {
+    return __float_as_uint(v * inv + 12582912.0f);
+}
 
 // largest |bits| over the 64 / V lanes that hold a group: as unsigned numbers the bit patterns of
 // magnitudes are in their order, infinities and NaN above all finite ones
@@ -89,65 +83,91 @@ __device__ __forceinline__ uint32_t group_umax(uint32_t m) {
     step(__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xF, 0xF, false));
     step(__builtin_amdgcn_update_dpp(0, (int)m, 0x141, 0xF, 0xF, false));
     step(__builtin_amdgcn_update_dpp(0, (int)m, 0x140, 0xF, 0xF, false));
-    if constexpr (V == 1) {
-        step(__shfl_xor((int)m, 16, kWave));
-        step(__shfl_xor((int)m, 32, kWave));
-    }
+    if constexpr (V <= 2) step(__shfl_xor((int)m, 16, kWave));
+    if constexpr (V == 1) step(__shfl_xor((int)m, 32, kWave));
     return m;
 }
 __device__ __forceinline__ float scale8_bits(uint32_t m) {
     return scale8(__uint_as_float(m), m < 0x7f800000u);
 }
 
-// V columns of a row whose 8-bit groups lie on the lanes in order: the lane's V values x (columns
-// n0 .. n0 + V - 1, of which the first `skip` belong to the lane before, and all do when skip = V)
-// go to q, the group's scale to *scale by its first lane. All lanes of the wave call it.
+// A row's 8-bit columns are stored at a pitch of N rounded up to 4, so that a lane's V own columns
+// (from its nominal column i on) are one aligned access, also in a row's last lane, whose values
+// start `skip` columns before its own.
+__host__ __device__ __forceinline__ int pitch8(int N) { return (N + 3) & ~3; }
+
 template <int V>
-__device__ __forceinline__ void store8(const float* x, int skip, bool first, int8_t* q, float* scale) {
-    uint32_t m = 0;
+struct Lane8 {
+    uint32_t mask[V];              // of the bits of a magnitude: own columns only
+    int at, shift;                 // first own column (clamped in lanes without one), 8 skip
+    bool on;
+    __device__ __forceinline__ Lane8(int i, int skip, bool on_, int N) : on(on_) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) m = max(m, j >= skip ? __float_as_uint(x[j]) & 0x7fffffffu : 0u);
-    const float sc = scale8_bits(group_umax<V>(m)), inv = 1.0f / sc;
-    int b[V];
+        for (int j = 0; j < V; ++j) mask[j] = on && j >= skip ? 0x7fffffffu : 0u;
+        at = on ? i : pitch8(N) - V;
+        shift = on ? 8 * skip : 0;
+    }
+};
+
+template <int V>
+struct Word8 {
+    typedef typename std::conditional<V == 4, uint32_t, typename std::conditional<V == 2, uint16_t, uint8_t>::type>::type type;
+};
+
+// the lane's V values as 8 bits, own columns from the low byte on, and their group's scale. The 64
+// columns of a group lie on 64 / V neighbouring lanes; all lanes of the wave call it.
+template <int V>
+__device__ __forceinline__ uint32_t quantise8(const float* x, const Lane8<V>& ln, float* scale) {
+    uint32_t m = 0, word, b[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max(m, __float_as_uint(x[j]) & ln.mask[j]);
+    *scale = scale8_bits(group_umax<V>(m));
+    const float inv = recip8(*scale);
 #pragma unroll
     for (int j = 0; j < V; ++j) b[j] = quant8(x[j], inv);
-    if (V == 4 && skip == 0) {
-        typedef uint32_t u32u __attribute__((aligned(1)));
-        *(u32u*)q = (b[0] & 255) | (b[1] & 255) << 8 | (b[2 % V] & 255) << 16 | (uint32_t)b[3 % V] << 24;
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (j >= skip) q[j] = (int8_t)b[j];
-    }
+    if constexpr (V == 4)
+        word = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0c);
+    else if constexpr (V == 2) word = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400);
+    else word = b[0];
+    return word >> ln.shift;
+}
+// and stored: own columns, the scale by the group's first lane (`first`)
+template <int V>
+__device__ __forceinline__ void store8(const float* x, const Lane8<V>& ln, bool first, int8_t* qrow, float* scale) {
+    float sc;
+    const uint32_t word = quantise8<V>(x, ln, &sc);
+    if (ln.on) *(typename Word8<V>::type*)(qrow + ln.at) = (typename Word8<V>::type)word;
     if (first) *scale = sc;
 }
 
-// V columns from their 8 bits. A row's last lane may start in the group before its own (its
-// columns are moved back to the row's end): both groups' scales.
+// V columns from their 8 bits, by the scale of the lane's own group; columns before its own come as
+// zeros (a lane must not store what it computes of them).
 template <int V>
 struct Vec8 {
     uint32_t q;
-    float s0, s1;
-    int cut;                       // columns of the first group
+    float scale;
     __device__ __forceinline__ float get(int j) const {
-        return (float)((int32_t)(q << (24 - 8 * j)) >> 24) * (j < cut ? s0 : s1);
+        return (float)((int32_t)(q << (24 - 8 * j)) >> 24) * scale;
     }
 };
 template <int V>
-__device__ __forceinline__ Vec8<V> load8(const delrec_packed8& p, size_t row, int n0, int N, int ng) {
+__device__ __forceinline__ Vec8<V> load8(const int8_t* qrow, const float* scale, const Lane8<V>& ln) {
     Vec8<V> r;
-    const int8_t* q = p.q + row * N + n0;
-    if constexpr (V == 4) {
-        typedef uint32_t u32u __attribute__((aligned(1)));
-        r.q = *(const u32u*)q;
-    } else {
-        r.q = (uint8_t)q[0];
-    }
-    const int g0 = n0 / kGroup8, g1 = (n0 + V - 1) / kGroup8;
-    r.s0 = p.scale[row * ng + g0];
-    r.s1 = p.scale[row * ng + g1];
-    r.cut = g1 > g0 ? g1 * kGroup8 - n0 : V;
+    r.q = (uint32_t)*(const typename Word8<V>::type*)(qrow + ln.at) << ln.shift;
+    r.scale = *scale;
     return r;
+}
+
+// V results of a lane, without the first `skip`
+template <class S, int V>
+__device__ __forceinline__ void vstore_own(S* p, const float* x, int skip) {
+    if (skip == 0) {
+        vstore<S, V>(p, x);
+    } else {
+#pragma unroll
+        for (int j = 1; j < V; ++j)
+            if (j >= skip) p[j] = (S)x[j];
+    }
 }
 
 }  // namespace delrec

@@ -18,11 +18,17 @@
 // anyway: exact in 32 bits where reading h back would bring its bf16 rounding into df, and two to
 // four bytes a value less to read.
 #include <algorithm>
+#include <cstdlib>
 
 #include "gated.h"
 #include "kernels.h"
 
 namespace delrec {
+
+#define DELREC_GLOBAL __attribute__((address_space(1)))
+#ifndef DELREC_BWD_WAVES
+#define DELREC_BWD_WAVES (V == 4 ? 2 : 4)
+#endif
 
 namespace {
 
@@ -55,18 +61,103 @@ __device__ __forceinline__ int row_length(const GatedScan& p, int b) {
 // a row's last group up, repeat valid columns and write nothing.
 template <int V>
 struct Lane {
-    int b, n0, skip, group;                  // group: of its first own column
+    int b, b0, n0, skip, group;              // b0: the wave's first row; group: of the first own column
     bool on, first;                          // writes; first lane of its 8-bit group
+    int i;                                   // nominal first column
     __device__ __forceinline__ Lane(const GatedScan& p, int per_row) {
         const long long c = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
         const long long rows = c / per_row;
         b = rows < p.B ? (int)rows : p.B - 1;
-        const int i = (int)(c - rows * per_row) * V;
+        b0 = __builtin_amdgcn_readfirstlane(b);
+        i = (int)(c - rows * per_row) * V;
         on = rows < p.B && i < p.N;
         first = on && i % kGroup8 == 0;
         n0 = i < p.N - V ? i : p.N - V;
         skip = on ? i - n0 : V;
-        group = i / kGroup8;
+        group = min(i, p.N - 1) / kGroup8;
+    }
+};
+
+// A (T, B, ..) array as a lane walks it: a step's address is one base for the wave, in scalar
+// registers and moved by additions, and the lane's 32-bit distance from it (checked by the
+// launcher; V = 1 has 64-bit distances). A multiplication a step and access kept the scalar unit,
+// which the four SIMDs share, busier than the memory.
+template <class T, int V>
+struct Walk {
+    const char* base;
+    long long pitch;
+    typename std::conditional<V == 1, long long, uint32_t>::type off;
+    uint64_t cur;
+    // element (t, b, n) of `data` at t * s0 + b * s1 + n
+    __device__ __forceinline__ Walk(const void* data, long long s0, long long s1, int b, int b0, int n)
+        : base((const char*)data + b0 * s1 * (long long)sizeof(T)), pitch(s0 * (long long)sizeof(T)) {
+        if constexpr (V == 1) off = ((b - b0) * s1 + n) * (long long)sizeof(T);
+        else off = ((uint32_t)(b - b0) * (uint32_t)s1 + (uint32_t)n) * (uint32_t)sizeof(T);
+    }
+    __device__ __forceinline__ void seek(int t) { cur = (uint64_t)(base + t * pitch); }
+    // the next step, or the same one again at the end of time (`more` is 0)
+    __device__ __forceinline__ void next(long long more = -1) { cur += pitch & more; }
+    __device__ __forceinline__ void prev() { cur -= pitch; }
+    // The base is kept apart from the lane's distance (an empty asm, or the compiler adds both into
+    // 64-bit lane addresses for all steps ahead, and their registers cost a wave per SIMD).
+    __device__ __forceinline__ DELREC_GLOBAL char* at() const {
+        uint64_t a = cur;
+        if constexpr (V > 1) {
+            a = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a) |
+                (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32;
+            asm("" : "+s"(a));
+        }
+        return (DELREC_GLOBAL char*)a + off;
+    }
+    template <class E>
+    __device__ __forceinline__ E value() const { return *(const DELREC_GLOBAL E*)at(); }
+    __device__ __forceinline__ Vec<T, V> load() const {
+        Vec<T, V> r;
+        if constexpr (V > 1) r.v = *(const DELREC_GLOBAL typename Vec<T, V>::unaligned*)at();
+        else r.v = *(const DELREC_GLOBAL T*)at();
+        return r;
+    }
+    // without the first `skip`
+    __device__ __forceinline__ void store(const float* x, int skip = 0) const {
+        DELREC_GLOBAL char* q = at();
+        if constexpr (V > 1) {
+            typename Vec<float, V>::type v;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = x[j];
+            if (skip == 0) *(DELREC_GLOBAL typename Vec<T, V>::unaligned*)q = __builtin_convertvector(v, typename Vec<T, V>::type);
+            else
+#pragma unroll
+                for (int j = 1; j < V; ++j)
+                    if (j >= skip) ((DELREC_GLOBAL T*)q)[j] = (T)x[j];
+        } else if (skip == 0) {
+            *(DELREC_GLOBAL T*)q = (T)x[0];
+        }
+    }
+};
+
+// a tensor's 8 bits and their scales, walked together
+template <int V>
+struct Walk8 {
+    Walk<int8_t, V> q;
+    Walk<float, V> scale;
+    const Lane8<V>& ln;
+    __device__ __forceinline__ Walk8(const delrec_packed8& p, int B, int N, int b, int b0, int group, const Lane8<V>& l)
+        : q(p.q, (long long)B * pitch8(N), pitch8(N), b, b0, l.at),
+          scale(p.scale, (long long)B * ((N + kGroup8 - 1) / kGroup8), (N + kGroup8 - 1) / kGroup8, b, b0, group), ln(l) {}
+    __device__ __forceinline__ void seek(int t) { q.seek(t); scale.seek(t); }
+    __device__ __forceinline__ void next(long long more = -1) { q.next(more); scale.next(more); }
+    __device__ __forceinline__ void prev() { q.prev(); scale.prev(); }
+    __device__ __forceinline__ Vec8<V> load() const {
+        Vec8<V> r;
+        r.q = (uint32_t)q.template value<typename Word8<V>::type>() << ln.shift;
+        r.scale = scale.template value<float>();
+        return r;
+    }
+    __device__ __forceinline__ void store(const float* x, bool first) const {
+        float sc;
+        const uint32_t word = quantise8<V>(x, ln, &sc);
+        if (ln.on) *(DELREC_GLOBAL typename Word8<V>::type*)q.at() = (typename Word8<V>::type)word;
+        if (first) *(DELREC_GLOBAL float*)scale.at() = sc;
     }
 };
 
@@ -112,287 +203,330 @@ __device__ __forceinline__ void enter_range(Maps<V>& m, const float* agg, size_t
     barrier_lds();                           // the buffer is free again
 }
 
-template <class S, int V>
-struct Inputs {                              // a wave's steps of one block, as loaded
-    Vec<S, V> z[kSteps], f[kSteps];
-    uint8_t start[kSteps];
-};
+// One step composed onto a piece's map (A, L), forwards: k out. f and z are vectors of any kind
+// that get() reads. A step past a row's length leaves the map as it is, whatever z and f hold.
+template <int V, bool MASK, class F>
+__device__ __forceinline__ void step_forward(const F& f, const F& z, const float* bias, bool live, bool fresh, float* k,
+                                             float* A, float* L) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        k[j] = gate_in(f.get(j) + bias[j]);
+        if (MASK) {
+            if (live) {
+                const float from = fresh ? 0.0f : L[j];
+                L[j] = fmaf(k[j], z.get(j) - from, from);
+                A[j] = fresh ? -1.0f : product<MASK>(A[j], 1.0f - k[j]);
+            }
+        } else {
+            L[j] = fmaf(k[j], z.get(j) - L[j], L[j]);
+            A[j] *= 1.0f - k[j];
+        }
+    }
+}
+
+// and backwards, c -> a (dh + c)
+template <int V, bool MASK, class D>
+__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool live, bool fresh, float* A, float* L) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float a = 1.0f - k[j];
+        if (MASK) {
+            if (live) {
+                L[j] = fresh ? 0.0f : a * (dh.get(j) + L[j]);
+                A[j] = fresh ? -1.0f : product<MASK>(A[j], a);
+            }
+        } else {
+            L[j] = a * (dh.get(j) + L[j]);
+            A[j] *= a;
+        }
+    }
+}
 
 }  // namespace
 
-// SUM: only the range's map, into p.ws. PACK: z and f also to 8 bits.
-template <class S, int V, bool MASK, bool PACK, bool SUM>
-__global__ void __launch_bounds__(512) gated_fwd_kernel(GatedScan p, int per_row, int range) {
+// The map of the pieces before this wave's, applied to h (in the order of DIR), and of all of them.
+// All reads are under way before the first is used.
+template <int V, bool MASK, int DIR>
+__device__ __forceinline__ void compose(const Maps<V>& m, int buf, int w, int nw, int lane, float* h, float* mine) {
+#pragma unroll
+    for (int c = 0; c < kWaves; ++c) {
+        const int q = DIR > 0 ? c : kWaves - 1 - c;
+        if (q < nw) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) mine[j] = q == w ? h[j] : mine[j];
+            m.template run<MASK>(buf, q, lane, h);
+        }
+    }
+}
+
+// Steps past T load the last one again (no branch between the loads) and are left out afterwards, by
+// tests that the whole wave shares.
+#define DELREC_STEPS(s) _Pragma("unroll") for (int s = 0; s < kSteps; ++s)
+#define DELREC_STEPS_BACK(s) _Pragma("unroll") for (int s = kSteps - 1; s >= 0; --s)
+#define DELREC_COLS(j) _Pragma("unroll") for (int j = 0; j < V; ++j)
+
+// PACK: z and f also to 8 bits.
+template <class S, int V, bool MASK, bool PACK>
+__global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_row, int range) {
     __shared__ Maps<V> maps;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Lane<V> ln(p, per_row);
     const int T = p.T, N = p.N, B = p.B, b = ln.b, n0 = ln.n0;
     const size_t plane = (size_t)B * N, at = (size_t)b * N + n0;
     const int ts = blockIdx.y * range, te = min(ts + range, T);
-    const S* zp = (const S*)p.z.data + b * p.z.s1 + n0;
-    const S* fp = (const S*)p.f.data + b * p.f.s1 + n0;
+    Walk<S, V> zp(p.z.data, p.z.s0, p.z.s1, b, ln.b0, n0), fp(p.f.data, p.f.s0, p.f.s1, b, ln.b0, n0),
+        yp(p.h.data, p.h.s0, p.h.s1, b, ln.b0, n0);
+    Walk<uint8_t, V> sp(p.starts, B, 1, b, ln.b0, 0);
+    const Lane8<V> l8(ln.i, ln.skip, ln.on, N);
+    Walk8<V> z8(p.z8, B, N, b, ln.b0, ln.group, l8), f8(p.f8, B, N, b, ln.b0, ln.group, l8);
     const int len = MASK ? row_length(p, b) : T;
-    const int ng = (N + kGroup8 - 1) / kGroup8;
-    float bias[V], h[V], sumA[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
+    float bias[V], h[V];
+    DELREC_COLS(j) {
         bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
-        h[j] = !SUM && p.h0 ? p.h0[at + j] : 0.0f;
-        sumA[j] = 1.0f;
+        h[j] = p.h0 ? p.h0[at + j] : 0.0f;
     }
-    if (!SUM && blockIdx.y) enter_range<V, MASK>(maps, p.ws, plane, at, 0, 1, blockIdx.y, w, nw, lane, h);
+    if (blockIdx.y) enter_range<V, MASK>(maps, p.ws, plane, at, 0, 1, blockIdx.y, w, nw, lane, h);
 
-    auto load = [&](Inputs<S, V>& in, int tb) {
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int t = min(tb + w * kSteps + k, T - 1);
-            in.z[k] = vload<S, V>(zp + t * p.z.s0);
-            in.f[k] = vload<S, V>(fp + t * p.f.s0);
-            if (MASK) in.start[k] = p.starts ? p.starts[(size_t)t * B + b] : 0;
-        }
-    };
-    Inputs<S, V> in;
-    load(in, ts);
     int buf = 0;
     for (int tb = ts; tb < te; tb += nw * kSteps, buf ^= 1) {
         const int t0 = tb + w * kSteps;
-        float kk[kSteps][V], zz[kSteps][V], A[V], L[V];
-        bool fresh[kSteps], live[kSteps];
-#pragma unroll
-        for (int j = 0; j < V; ++j) A[j] = 1.0f, L[j] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            live[k] = t0 + k < (MASK ? len : T);
-            fresh[k] = MASK && live[k] && in.start[k];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float z = in.z[k].get(j);
-                kk[k][j] = live[k] ? gate_in(in.f[k].get(j) + bias[j]) : 0.0f;
-                zz[k][j] = live[k] ? z : 0.0f;
-                if (MASK && fresh[k]) L[j] = 0.0f;
-                L[j] = fmaf(kk[k][j], zz[k][j] - L[j], L[j]);
-                A[j] = fresh[k] ? -1.0f : product<MASK>(A[j], 1.0f - kk[k][j]);
-            }
+        if (p.states && w == 0 && ln.on) vstore<float, V>(p.states + (size_t)(tb / kBlk) * plane + at, h);
+        Vec<S, V> z[kSteps], f[kSteps];
+        float k[kSteps][V], A[V], L[V], g[V];
+        bool fresh[kSteps];
+        DELREC_COLS(j) A[j] = 1.0f, L[j] = g[j] = 0.0f;
+        const int tc = min(t0, T - 1);
+        zp.seek(tc), fp.seek(tc);
+        if (MASK) sp.seek(tc);
+        DELREC_STEPS(s) {
+            const long long more = t0 + s + 1 < T ? -1 : 0;
+            f[s] = fp.load(), z[s] = zp.load();
+            fp.next(more), zp.next(more);
+            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+            if (MASK) sp.next(more);
         }
-        if constexpr (PACK) {
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                const int t = t0 + k;
-                if (t >= T) break;
-                float v[V];
-                const size_t row = (size_t)t * B + b;
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = in.z[k].get(j);
-                store8<V>(v, ln.skip, ln.first, p.z8.q + row * N + n0, p.z8.scale + row * ng + ln.group);
-#pragma unroll
-                for (int j = 0; j < V; ++j) v[j] = in.f[k].get(j);
-                store8<V>(v, ln.skip, ln.first, p.f8.q + row * N + n0, p.f8.scale + row * ng + ln.group);
-            }
+        DELREC_STEPS(s) {
+            if (t0 + s < T) step_forward<V, MASK>(f[s], z[s], bias, t0 + s < len, fresh[s], k[s], A, L);
         }
         maps.put(buf, w, lane, A, L);
-        barrier_lds();
-        if (tb + nw * kSteps < te) load(in, tb + nw * kSteps);
-        if (!SUM && p.states && w == 0 && ln.on) vstore<float, V>(p.states + (size_t)(tb / kBlk) * plane + at, h);
-        float g[V];
-        for (int q = 0; q < nw; ++q) {
-            if (q == w) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) g[j] = h[j];
-            }
-            maps.template run<MASK>(buf, q, lane, h);
-            if constexpr (SUM) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) sumA[j] = product<MASK>(sumA[j], maps.A[buf][q][lane * V + j]);
-            }
-        }
-        if constexpr (!SUM) {
-            S* yp = (S*)p.h.data + b * p.h.s1 + n0;
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                if (t0 + k >= T) break;
-                float y[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (MASK && fresh[k]) g[j] = 0.0f;
-                    g[j] = fmaf(kk[k][j], zz[k][j] - g[j], g[j]);
-                    y[j] = live[k] ? g[j] : 0.0f;
+        if constexpr (PACK) {
+            z8.seek(t0), f8.seek(t0);
+            DELREC_STEPS(s) {
+                if (t0 + s < T) {
+                    float v[V];
+                    DELREC_COLS(j) v[j] = z[s].get(j);
+                    z8.store(v, ln.first);
+                    DELREC_COLS(j) v[j] = f[s].get(j);
+                    f8.store(v, ln.first);
+                    z8.next(), f8.next();
                 }
-                if (ln.on) vstore<S, V>(yp + (t0 + k) * p.h.s0, y);
+            }
+        }
+        barrier_lds();
+        compose<V, MASK, 1>(maps, buf, w, nw, lane, h, g);
+        yp.seek(t0);
+        DELREC_STEPS(s) {
+            if (t0 + s < T) {
+                const bool live = !MASK || t0 + s < len;
+                float y[V];
+                DELREC_COLS(j) {
+                    if (MASK && fresh[s] && live) g[j] = 0.0f;
+                    const float next = fmaf(k[s][j], z[s].get(j) - g[j], g[j]);
+                    g[j] = live ? next : g[j];
+                    y[j] = live ? g[j] : 0.0f;
+                }
+                if (ln.on) yp.store(y);
+                yp.next();
             }
         }
     }
-    if (w || !ln.on) return;
-    if constexpr (SUM) {
-        float* a = p.ws + (size_t)blockIdx.y * 2 * plane + at;
-        vstore<float, V>(a, sumA);
-        vstore<float, V>(a + plane, h);
-    } else if (te == T) {
-        vstore<float, V>(p.h_last + at, h);
-    }
+    if (w == 0 && ln.on && te == T) vstore<float, V>(p.h_last + at, h);
 }
 
-// SUM: only the range's reverse map, from f and dh. PACK: z and f from their 8 bits.
-template <class S, int V, bool MASK, bool PACK, bool SUM>
-__global__ void __launch_bounds__(512) gated_bwd_kernel(GatedScan p, int per_row, int range, float* dbpart) {
+// A range's map into p.ws, each wave a run of consecutive steps on its own, composed at the end.
+// BWD: the reverse map, from f and dh. PACK: f from its 8 bits.
+template <class S, int V, bool MASK, bool PACK, bool BWD>
+__global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int per_row, int range) {
+    __shared__ Maps<V> maps;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    const Lane<V> ln(p, per_row);
+    const int T = p.T, N = p.N, B = p.B, b = ln.b, n0 = ln.n0;
+    const size_t plane = (size_t)B * N, at = (size_t)b * N + n0;
+    const int y = blockIdx.y + (BWD ? 1 : 0);          // the last range forward, the first backward lead nowhere
+    const int run = range / nw, ts = y * range + w * run;
+    const delrec_rows& x = BWD ? p.dh : p.z;
+    Walk<S, V> fp(p.f.data, p.f.s0, p.f.s1, b, ln.b0, n0), xp(x.data, x.s0, x.s1, b, ln.b0, n0);
+    Walk<uint8_t, V> sp(p.starts, B, 1, b, ln.b0, 0);
+    const Lane8<V> l8(ln.i, ln.skip, ln.on, N);
+    Walk8<V> fp8(p.f8, B, N, b, ln.b0, ln.group, l8);
+    const int len = MASK ? row_length(p, b) : T;
+    float bias[V], A[V], L[V];
+    DELREC_COLS(j) {
+        bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
+        A[j] = 1.0f;
+        L[j] = 0.0f;
+    }
+    for (int c = 0; c < run / kSteps; ++c) {
+        const int t0 = ts + (BWD ? run / kSteps - 1 - c : c) * kSteps;
+        typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps];
+        Vec<S, V> v[kSteps];
+        bool fresh[kSteps];
+        const int tc = min(t0, T - 1);
+        if constexpr (PACK) fp8.seek(tc);
+        else fp.seek(tc);
+        xp.seek(tc);
+        if (MASK) sp.seek(tc);
+        DELREC_STEPS(s) {
+            const long long more = t0 + s + 1 < T ? -1 : 0;
+            if constexpr (PACK) f[s] = fp8.load(), fp8.next(more);
+            else f[s] = fp.load(), fp.next(more);
+            v[s] = xp.load(), xp.next(more);
+            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+            if (MASK) sp.next(more);
+        }
+        DELREC_STEPS(q) {
+            const int s = BWD ? kSteps - 1 - q : q;
+            if (t0 + s < T) {
+                const bool live = !MASK || t0 + s < len;
+                float k[V];
+                if constexpr (BWD) {
+                    DELREC_COLS(j) k[j] = gate_in(f[s].get(j) + bias[j]);
+                    step_backward<V, MASK>(k, v[s], live, fresh[s], A, L);
+                } else {
+                    step_forward<V, MASK>(f[s], v[s], bias, live, fresh[s], k, A, L);
+                }
+            }
+        }
+    }
+    maps.put(0, w, lane, A, L);
+    barrier_lds();
+    if (w || !ln.on) return;
+    DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
+    for (int c = 0; c < nw; ++c) {
+        const int q = BWD ? nw - 1 - c : c;
+        maps.template run<MASK>(0, q, lane, L);
+        DELREC_COLS(j) A[j] = product<MASK>(A[j], maps.A[0][q][lane * V + j]);
+    }
+    float* a = p.ws + (size_t)y * 2 * plane + at;
+    vstore_own<float, V>(a, A, PACK ? ln.skip : 0);
+    vstore_own<float, V>(a + plane, L, PACK ? ln.skip : 0);
+}
+
+// PACK: z and f from their 8 bits.
+template <class S, int V, bool MASK, bool PACK>
+__global__ void __launch_bounds__(512, DELREC_BWD_WAVES) gated_bwd_kernel(GatedScan p, int per_row, int range, float* dbpart) {
     __shared__ Maps<V> fmap, rmap;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Lane<V> ln(p, per_row);
     const int T = p.T, N = p.N, B = p.B, b = ln.b, n0 = ln.n0;
     const size_t plane = (size_t)B * N, at = (size_t)b * N + n0;
     const int ts = blockIdx.y * range, te = min(ts + range, T);
-    const int ng = (N + kGroup8 - 1) / kGroup8;
-    const S* zp = (const S*)p.z.data + b * p.z.s1 + n0;
-    const S* fp = (const S*)p.f.data + b * p.f.s1 + n0;
-    const S* dhp = (const S*)p.dh.data + b * p.dh.s1 + n0;
+    const int own = PACK ? ln.skip : 0;
+    Walk<S, V> zp(p.z.data, p.z.s0, p.z.s1, b, ln.b0, n0), fp(p.f.data, p.f.s0, p.f.s1, b, ln.b0, n0),
+        dhp(p.dh.data, p.dh.s0, p.dh.s1, b, ln.b0, n0), dzp(p.dz.data, p.dz.s0, p.dz.s1, b, ln.b0, n0),
+        dfp(p.df.data, p.df.s0, p.df.s1, b, ln.b0, n0);
+    Walk<uint8_t, V> sp(p.starts, B, 1, b, ln.b0, 0);
+    const Lane8<V> l8(ln.i, ln.skip, ln.on, N);
+    Walk8<V> z8(p.z8, B, N, b, ln.b0, ln.group, l8), f8(p.f8, B, N, b, ln.b0, ln.group, l8);
     const int len = MASK ? row_length(p, b) : T;
-    float bias[V], c[V], sumA[V], db[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
+    float bias[V], c[V], db[V];
+    DELREC_COLS(j) {
         bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
-        c[j] = !SUM && p.dlast ? p.dlast[at + j] : 0.0f;
-        sumA[j] = 1.0f;
+        c[j] = p.dlast ? p.dlast[at + j] : 0.0f;
         db[j] = 0.0f;
     }
     const int last = gridDim.y - 1;
-    if (!SUM && (int)blockIdx.y < last)
+    if ((int)blockIdx.y < last)
         enter_range<V, MASK>(rmap, p.ws, plane, at, last, -1, last - blockIdx.y, w, nw, lane, c);
 
     int buf = 0;
     for (int tb = ts + (te - 1 - ts) / (nw * kSteps) * (nw * kSteps); tb >= ts; tb -= nw * kSteps, buf ^= 1) {
         const int t0 = tb + w * kSteps;
-        float kk[kSteps][V], zz[kSteps][V], dh[kSteps][V];
-        bool fresh[kSteps], live[kSteps];
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int t = min(t0 + k, T - 1);
-            live[k] = t0 + k < (MASK ? len : T);
-            fresh[k] = MASK && live[k] && p.starts && p.starts[(size_t)t * B + b];
-            const auto d = vload<S, V>(dhp + t * p.dh.s0);
-            float f[V], z[V];
-            if constexpr (PACK) {
-                const size_t row = (size_t)t * B + b;
-                const auto f8 = load8<V>(p.f8, row, n0, N, ng);
-#pragma unroll
-                for (int j = 0; j < V; ++j) f[j] = f8.get(j);
-                if constexpr (!SUM) {
-                    const auto z8 = load8<V>(p.z8, row, n0, N, ng);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) z[j] = z8.get(j);
-                }
-            } else {
-                const auto fv = vload<S, V>(fp + t * p.f.s0);
-#pragma unroll
-                for (int j = 0; j < V; ++j) f[j] = fv.get(j);
-                if constexpr (!SUM) {
-                    const auto zv = vload<S, V>(zp + t * p.z.s0);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) z[j] = zv.get(j);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                kk[k][j] = live[k] ? gate_in(f[j] + bias[j]) : 0.0f;
-                dh[k][j] = live[k] ? d.get(j) : 0.0f;
-                if (!SUM) zz[k][j] = live[k] ? z[j] : 0.0f;
-            }
-        }
+        float k[kSteps][V], d[kSteps][V], h[V], g[V], mine[V];
+        Vec<S, V> dh[kSteps];
+        bool fresh[kSteps];
+        const auto st = vload<float, V>(p.states + (size_t)(tb / kBlk) * plane + at);
+        DELREC_COLS(j) h[j] = st.get(j), g[j] = mine[j] = 0.0f;
         float A[V], L[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) A[j] = 1.0f, L[j] = 0.0f;
-        if constexpr (!SUM) {
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (MASK && fresh[k]) L[j] = 0.0f;
-                    L[j] = fmaf(kk[k][j], zz[k][j] - L[j], L[j]);
-                    A[j] = fresh[k] ? -1.0f : product<MASK>(A[j], 1.0f - kk[k][j]);
-                }
-            fmap.put(buf, w, lane, A, L);
-#pragma unroll
-            for (int j = 0; j < V; ++j) A[j] = 1.0f, L[j] = 0.0f;
+        typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps], z[kSteps];
+        const int tc = min(t0, T - 1);
+        if constexpr (PACK) z8.seek(tc), f8.seek(tc);
+        else zp.seek(tc), fp.seek(tc);
+        dhp.seek(tc);
+        if (MASK) sp.seek(tc);
+        DELREC_STEPS(s) {
+            const long long more = t0 + s + 1 < T ? -1 : 0;
+            if constexpr (PACK) f[s] = f8.load(), z[s] = z8.load(), f8.next(more), z8.next(more);
+            else f[s] = fp.load(), z[s] = zp.load(), fp.next(more), zp.next(more);
+            dh[s] = dhp.load(), dhp.next(more);
+            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+            if (MASK) sp.next(more);
         }
-#pragma unroll
-        for (int k = kSteps - 1; k >= 0; --k)
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float a = 1.0f - kk[k][j];
-                L[j] = MASK && fresh[k] ? 0.0f : a * (dh[k][j] + L[j]);
-                A[j] = fresh[k] ? -1.0f : product<MASK>(A[j], a);
+        DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
+        DELREC_STEPS(s) {
+            if (t0 + s < T) {
+                step_forward<V, MASK>(f[s], z[s], bias, t0 + s < len, fresh[s], k[s], A, L);
+                DELREC_COLS(j) d[s][j] = z[s].get(j);
             }
+        }
+        fmap.put(buf, w, lane, A, L);
+        DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
+        DELREC_STEPS_BACK(s) {
+            if (t0 + s < T) step_backward<V, MASK>(k[s], dh[s], !MASK || t0 + s < len, fresh[s], A, L);
+        }
         rmap.put(buf, w, lane, A, L);
         barrier_lds();
-        float g[V];
-        for (int q = nw - 1; q >= 0; --q) {
-            if (q == w) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) g[j] = c[j];
-            }
-            rmap.template run<MASK>(buf, q, lane, c);
-            if constexpr (SUM) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) sumA[j] = product<MASK>(sumA[j], rmap.A[buf][q][lane * V + j]);
+        compose<V, MASK, -1>(rmap, buf, w, nw, lane, c, g);
+        compose<V, MASK, 1>(fmap, buf, w, nw, lane, h, mine);
+        float blk[V];
+        // d: z_t becomes h_{t-1} - z_t
+        DELREC_STEPS(s) {
+            if (t0 + s < T) {
+                const bool live = !MASK || t0 + s < len;
+                DELREC_COLS(j) {
+                    if (MASK && fresh[s] && live) mine[j] = 0.0f;
+                    d[s][j] = mine[j] - d[s][j];
+                    const float next = fmaf(-k[s][j], d[s][j], mine[j]);
+                    mine[j] = live ? next : mine[j];
+                }
             }
         }
-        if constexpr (!SUM) {
-            float h[V], blk[V];
-            const auto st = vload<float, V>(p.states + (size_t)(tb / kBlk) * plane + at);
-#pragma unroll
-            for (int j = 0; j < V; ++j) h[j] = st.get(j), blk[j] = 0.0f;
-            for (int q = 0; q < w; ++q) fmap.template run<MASK>(buf, q, lane, h);
-            // zz becomes h_{t-1} - z_t
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    if (MASK && fresh[k]) h[j] = 0.0f;
-                    const float d = h[j] - zz[k][j];
-                    h[j] = fmaf(-kk[k][j], d, h[j]);
-                    zz[k][j] = live[k] ? d : 0.0f;
-                }
-            S* dzp = (S*)p.dz.data + b * p.dz.s1 + n0;
-            S* dfp = (S*)p.df.data + b * p.df.s1 + n0;
-#pragma unroll
-            for (int k = kSteps - 1; k >= 0; --k) {
+        DELREC_COLS(j) blk[j] = 0.0f;
+        dzp.seek(t0 + kSteps - 1), dfp.seek(t0 + kSteps - 1);
+        DELREC_STEPS_BACK(s) {
+            if (t0 + s < T) {
+                const bool live = !MASK || t0 + s < len;
                 float oz[V], of[V];
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    const float a = 1.0f - kk[k][j], lam = dh[k][j] + g[j];
-                    oz[j] = live[k] ? lam * kk[k][j] : 0.0f;
-                    of[j] = oz[j] * a * zz[k][j];
+                DELREC_COLS(j) {
+                    const float a = 1.0f - k[s][j], lam = dh[s].get(j) + g[j];
+                    oz[j] = lam * k[s][j];
+                    of[j] = oz[j] * a * d[s][j];
+                    if (MASK) {
+                        oz[j] = live ? oz[j] : 0.0f;
+                        of[j] = live ? of[j] : 0.0f;
+                        g[j] = live ? (fresh[s] ? 0.0f : a * lam) : g[j];
+                    } else {
+                        g[j] = a * lam;
+                    }
                     blk[j] += of[j];
-                    g[j] = MASK && fresh[k] ? 0.0f : a * lam;
                 }
-                if (t0 + k < T && ln.on) {
-                    vstore<S, V>(dzp + (t0 + k) * p.dz.s0, oz);
-                    vstore<S, V>(dfp + (t0 + k) * p.df.s0, of);
-                }
+                if (ln.on) dzp.store(oz, own), dfp.store(of, own);
             }
-            // the bias sum in two levels: within a block, then over blocks
-#pragma unroll
-            for (int j = 0; j < V; ++j) db[j] += blk[j];
+            dzp.prev(), dfp.prev();
         }
+        // the bias sum in two levels, within a block and over blocks: one long chain of 32-bit
+        // additions lost a digit at T = 16384
+        DELREC_COLS(j) db[j] += blk[j];
     }
-    if constexpr (SUM) {
-        if (w || !ln.on) return;
-        float* a = p.ws + (size_t)blockIdx.y * 2 * plane + at;
-        vstore<float, V>(a, sumA);
-        vstore<float, V>(a + plane, c);
-    } else {
-        if (w == 0 && ln.on && ts == 0 && p.dh0) vstore<float, V>(p.dh0 + at, c);
-        if (!dbpart) return;
-        __syncthreads();
-        float one[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) one[j] = 1.0f;
-        rmap.put(0, w, lane, one, db);
-        __syncthreads();
-        if (w || !ln.on) return;
-        for (int q = 1; q < nw; ++q)
-#pragma unroll
-            for (int j = 0; j < V; ++j) db[j] += rmap.S[0][q][lane * V + j];
-        vstore<float, V>(dbpart + (size_t)blockIdx.y * plane + at, db);
-    }
+    if (w == 0 && ln.on && ts == 0 && p.dh0) vstore_own<float, V>(p.dh0 + at, c, own);
+    if (!dbpart) return;
+    __syncthreads();
+    rmap.put(0, w, lane, db, db);
+    __syncthreads();
+    if (w || !ln.on) return;
+    for (int q = 1; q < nw; ++q)
+        DELREC_COLS(j) db[j] += rmap.S[0][q][lane * V + j];
+    vstore_own<float, V>(dbpart + (size_t)blockIdx.y * plane + at, db, own);
 }
 
 namespace {
@@ -401,18 +535,26 @@ struct Plan {
     int V, per_row, groups, waves, range, ranges;
 };
 
-// V = 4 wherever a row holds four columns. Time over the grid where the channels alone do not
-// give every CU a workgroup.
-Plan gated_plan(int T, int B, int N, bool pack) {
+Plan gated_plan(int T, int B, int N, bool pack, bool wide) {
     Plan q;
-    q.V = N >= 4 ? 4 : 1;
-    q.per_row = pack ? (N + kGroup8 - 1) / kGroup8 * (kGroup8 / q.V) : (N + q.V - 1) / q.V;
-    q.groups = (int)(((long long)B * q.per_row + 63) / 64);
+    auto shape = [&](int v) {
+        q.V = v;
+        q.per_row = pack ? (N + kGroup8 - 1) / kGroup8 * (kGroup8 / v) : (N + v - 1) / v;
+        q.groups = (int)(((long long)B * q.per_row + 63) / 64);
+    };
+    shape(N >= 4 ? 4 : N >= 2 ? 2 : 1);
+    int fill = 512, top = 64;
+    if (const char* e = getenv("PLAN_FILL")) fill = atoi(e);
+    if (const char* e = getenv("PLAN_TOP")) top = atoi(e);
+    if (q.V == 4 && q.groups < fill) shape(2);
+    if (const char* e = getenv("PLAN_V")) shape(atoi(e));
+    if (wide) shape(1);
     q.waves = T >= kBlk ? kWaves : (T + kSteps - 1) / kSteps;
     const int blocks = (T + kBlk - 1) / kBlk;
-    int want = q.groups >= 256 ? 1 : (512 + q.groups - 1) / q.groups;
-    if (want > 64) want = 64;
-    if (want > blocks / 2) want = blocks / 2 < 1 ? 1 : blocks / 2;
+    int low = 256;
+    if (const char* e = getenv("PLAN_LOW")) low = atoi(e);
+    int want = q.groups >= low ? 1 : std::max(1, fill / q.groups);
+    want = std::min({want, top, std::max(1, blocks / 2)});
     const int per = (blocks + want - 1) / want;
     q.range = per * kBlk;
     q.ranges = (blocks + per - 1) / per;
@@ -423,16 +565,16 @@ size_t map_floats(const Plan& q, int B, int N) { return q.ranges > 1 ? (size_t)q
 
 template <class S, int V, bool MASK, bool PACK>
 void run_gated(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream) {
-    const dim3 block(64 * q.waves), grid(q.groups, q.ranges), inner(q.groups, q.ranges);
+    const dim3 block(64 * q.waves), grid(q.groups, q.ranges), inner(q.groups, q.ranges - 1);
     if (fwd) {
         if (q.ranges > 1)
-            hipLaunchKernelGGL((gated_fwd_kernel<S, V, MASK, false, true>), inner, block, 0, stream, p, q.per_row, q.range);
-        hipLaunchKernelGGL((gated_fwd_kernel<S, V, MASK, PACK, false>), grid, block, 0, stream, p, q.per_row, q.range);
+            hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, false, false>), inner, block, 0, stream, p, q.per_row, q.range);
+        hipLaunchKernelGGL((gated_fwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range);
     } else {
         float* part = p.db ? p.ws + map_floats(q, p.B, p.N) : nullptr;
         if (q.ranges > 1)
-            hipLaunchKernelGGL((gated_bwd_kernel<S, V, MASK, PACK, true>), inner, block, 0, stream, p, q.per_row, q.range, nullptr);
-        hipLaunchKernelGGL((gated_bwd_kernel<S, V, MASK, PACK, false>), grid, block, 0, stream, p, q.per_row, q.range, part);
+            hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, PACK, true>), inner, block, 0, stream, p, q.per_row, q.range);
+        hipLaunchKernelGGL((gated_bwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range, part);
         if (p.db) launch_column_sums(part, q.ranges * p.B, p.N, p.N, p.db, nullptr, nullptr, stream);
     }
 }
@@ -444,22 +586,36 @@ void run_gated_m(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream
     else mask ? run_gated<S, V, true, false>(p, q, fwd, stream) : run_gated<S, V, false, false>(p, q, fwd, stream);
 }
 
+template <class S>
+void run_gated_v(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream) {
+    if (q.V == 4) run_gated_m<S, 4>(p, q, fwd, stream);
+    else if (q.V == 2) run_gated_m<S, 2>(p, q, fwd, stream);
+    else run_gated_m<S, 1>(p, q, fwd, stream);
+}
+
 void launch_gated(const GatedScan& p, bool fwd, hipStream_t stream) {
-    const Plan q = gated_plan(p.T, p.B, p.N, p.z8.q != nullptr);
-    if (p.bf16) q.V == 4 ? run_gated_m<__bf16, 4>(p, q, fwd, stream) : run_gated_m<__bf16, 1>(p, q, fwd, stream);
-    else q.V == 4 ? run_gated_m<float, 4>(p, q, fwd, stream) : run_gated_m<float, 1>(p, q, fwd, stream);
+    // the rows that a wave's 64 V channels touch, counted generously, against 32-bit offsets
+    bool wide = false;
+    for (const delrec_rows* x : {&p.z, &p.f, &p.h, &p.dh, &p.dz, &p.df})
+        if (x->data && (256 / p.N + 2) * x->s1 + p.N > 0x7fffffffLL / 4) wide = true;
+    const Plan q = gated_plan(p.T, p.B, p.N, p.z8.q != nullptr, wide);
+    if (p.bf16) run_gated_v<__bf16>(p, q, fwd, stream);
+    else run_gated_v<float>(p, q, fwd, stream);
 }
 
 }  // namespace
 
-// floats of workspace: the ranges' maps, and the ranges' bias sums (the 8-bit form's wider rows
-// give at most as many ranges)
+// floats of workspace, for whichever form the strides and the 8 bits ask for: the ranges' maps, and
+// the ranges' bias sums
 size_t gated_fwd_ws(int T, int B, int N) {
-    return std::max(map_floats(gated_plan(T, B, N, false), B, N), map_floats(gated_plan(T, B, N, true), B, N));
+    size_t n = 0;
+    for (int form = 0; form < 4; ++form) n = std::max(n, map_floats(gated_plan(T, B, N, form & 1, form & 2), B, N));
+    return n;
 }
 size_t gated_bwd_ws(int T, int B, int N) {
-    const Plan a = gated_plan(T, B, N, false), b = gated_plan(T, B, N, true);
-    return gated_fwd_ws(T, B, N) + (size_t)std::max(a.ranges, b.ranges) * B * N;
+    int ranges = 1;
+    for (int form = 0; form < 4; ++form) ranges = std::max(ranges, gated_plan(T, B, N, form & 1, form & 2).ranges);
+    return gated_fwd_ws(T, B, N) + (size_t)ranges * B * N;
 }
 
 void launch_gated_fwd(const GatedScan& p, hipStream_t stream) { launch_gated(p, true, stream); }

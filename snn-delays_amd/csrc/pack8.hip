@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(256) pack8_any_kernel(Pack8 p) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
     const float sc = scale8(m, __all(finite8(v)));
-    if (n < p.N) p.p.q[row * p.N + n] = (int8_t)quant8(v, 1.0f / sc);
+    if (n < p.N) p.p.q[row * pitch8(p.N) + n] = (int8_t)quant8(v, recip8(sc));
     if (lane == 0) p.p.scale[grp] = sc;
 }
 
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(256) unpack8_any_kernel(Pack8 p) {
     const long long row = i / p.N;
     const int n = (int)(i % p.N);
     S* x = (S*)p.x.data + (row / p.R1) * p.x.s0 + (row % p.R1) * p.x.s1;
-    x[n] = (S)((float)p.p.q[i] * p.p.scale[row * ng + n / kGroup8]);
+    x[n] = (S)((float)p.p.q[row * pitch8(p.N) + n] * p.p.scale[row * ng + n / kGroup8]);
 }
 
 // Rows of four columns and more: LPR lanes a row, four columns a lane (16 lanes a group), kRows
@@ -77,18 +77,18 @@ __global__ void __launch_bounds__(256) pack8_kernel(Pack8 p) {
                 float x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = v[q].get(j);
-                store8<4>(x, live[q] ? i - n0 : 4, live[q] && first, p.p.q + row[q] * N + n0, p.p.scale + row[q] * ng + group);
+                store8<4>(x, Lane8<4>(i, i - n0, live[q], N), live[q] && first, p.p.q + row[q] * pitch8(N), p.p.scale + row[q] * ng + group);
             }
         } else {
             Vec8<4> v[kRows];
 #pragma unroll
-            for (int q = 0; q < kRows; ++q) v[q] = load8<4>(p.p, (size_t)row[q], n0, N, ng);
+            for (int q = 0; q < kRows; ++q) v[q] = load8<4>(p.p.q + row[q] * pitch8(N), p.p.scale + row[q] * ng + group, Lane8<4>(i, i - n0, on, N));
 #pragma unroll
             for (int q = 0; q < kRows; ++q) {
                 float x[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[j] = v[q].get(j);
-                if (live[q]) vstore<S, 4>((S*)p.x.data + row_offset(p, row[q]) + n0, x);
+                if (live[q]) vstore_own<S, 4>((S*)p.x.data + row_offset(p, row[q]) + n0, x, i - n0);
             }
         }
     }

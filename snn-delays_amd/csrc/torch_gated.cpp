@@ -104,7 +104,7 @@ struct Packed {
     Tensor q, scale;
     Packed() = default;
     Packed(int64_t rows, int64_t N, const Tensor& like)
-        : q(at::empty({rows, N}, like.options().dtype(at::kChar))),
+        : q(at::empty({rows, (N + 3) / 4 * 4}, like.options().dtype(at::kChar))),
           scale(at::empty({rows, (N + DELREC_PACK8_GROUP - 1) / DELREC_PACK8_GROUP}, like.options().dtype(at::kFloat))) {}
     Packed(const Tensor& q_, const Tensor& s_) : q(q_), scale(s_) {}
     delrec_packed8 arg() const {
@@ -442,14 +442,14 @@ py::tuple pack8(Tensor x) {
         a.x = rows_of(v); a.p = p.arg();
         check(delrec_pack8(&a, stream_of(x)), "delrec_pack8");
     }
-    return py::make_tuple(p.q, p.scale);
+    return py::make_tuple(p.q.narrow(1, 0, N), p.scale);
 }
 
 Tensor unpack8(Tensor q, Tensor scale, std::vector<int64_t> shape, py::object dtype) {
     if (!q.is_cuda()) throw std::runtime_error(text("delrec-mi355x unpacks 8 bits with a HIP kernel on the GPU; they are on ", q.device()));
     const auto type = torch::python::detail::py_object_to_dtype(dtype);
     const int64_t groups = q.dim() == 2 ? (q.size(1) + DELREC_PACK8_GROUP - 1) / DELREC_PACK8_GROUP : 0;
-    if ((type != at::kFloat && type != at::kBFloat16) || q.dim() != 2 || q.scalar_type() != at::kChar || !q.is_contiguous() ||
+    if ((type != at::kFloat && type != at::kBFloat16) || q.dim() != 2 || q.scalar_type() != at::kChar || q.stride(1) != 1 || q.stride(0) != (q.size(1) + 3) / 4 * 4 ||
         scale.dim() != 2 || scale.size(0) != q.size(0) || scale.size(1) != groups || scale.scalar_type() != at::kFloat ||
         scale.device() != q.device() || !scale.is_contiguous())
         refuse(text("not a packed tensor: q ", describe(q), ", scale ", describe(scale), ", type ", type));
