@@ -13,12 +13,16 @@
 // time is cut a second time, over the grid: a first launch composes each range (reading its
 // inputs once more), the second starts from the composition of the ranges before it.
 //
+// Bound by memory where the channels fill the GPU: at T250 B128 N512 bf16 23 us forward (98 MB,
+// 4.2 TB/s) and 35 backward (164 MB, 4.7 TB/s, what a large copy reaches). A block's loads are not
+// taken ahead of the one before: two to four workgroups a CU hide them, and their registers cost
+// one of these.
+//
 // The forward keeps the state before every 64th step in 32 bits (1/16 byte a value and step); the
 // backward starts its blocks there and recomputes the states between from z and f, which it needs
 // anyway: exact in 32 bits where reading h back would bring its bf16 rounding into df, and two to
 // four bytes a value less to read.
 #include <algorithm>
-#include <cstdlib>
 
 #include "gated.h"
 #include "kernels.h"
@@ -26,9 +30,6 @@
 namespace delrec {
 
 #define DELREC_GLOBAL __attribute__((address_space(1)))
-#ifndef DELREC_BWD_WAVES
-#define DELREC_BWD_WAVES (V == 4 ? 2 : 4)
-#endif
 
 namespace {
 
@@ -36,17 +37,18 @@ constexpr int kBlk = DELREC_GATED_BLOCK;
 constexpr int kSteps = 8;                    // steps of a wave in a block
 constexpr int kWaves = kBlk / kSteps;
 
-// A start inside a piece cuts what comes before it off, also where that is infinite: A = -1 says
-// so (products of leaks are never negative). Only the masked forms have it.
+// A start inside a piece cuts what comes before it off, also where that is infinite: the sign of A
+// says so (products of leaks are never negative, and a further leak, zero too, keeps the sign).
+// Only the masked forms have it.
+__device__ __forceinline__ bool cut(float A) { return __float_as_int(A) < 0; }
 template <bool MASK>
 __device__ __forceinline__ float apply(float A, float S, float h) {
-    if (MASK && A < 0.0f) return S;
-    return fmaf(A, h, S);
+    const float r = fmaf(A, h, S);
+    return MASK && cut(A) ? S : r;
 }
 template <bool MASK>
 __device__ __forceinline__ float product(float A, float B) {
-    if (MASK && (A < 0.0f || B < 0.0f)) return -1.0f;
-    return A * B;
+    return MASK && cut(A) && cut(B) ? -1.0f : A * B;
 }
 
 __device__ __forceinline__ int row_length(const GatedScan& p, int b) {
@@ -204,45 +206,47 @@ __device__ __forceinline__ void enter_range(Maps<V>& m, const float* agg, size_t
 }
 
 // One step composed onto a piece's map (A, L), forwards: k out. f and z are vectors of any kind
-// that get() reads. A step past a row's length leaves the map as it is, whatever z and f hold.
+// that get() reads.
 template <int V, bool MASK, class F>
-__device__ __forceinline__ void step_forward(const F& f, const F& z, const float* bias, bool live, bool fresh, float* k,
-                                             float* A, float* L) {
+__device__ __forceinline__ void step_forward(const F& f, const F& z, const float* bias, bool fresh, float* k, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         k[j] = gate_in(f.get(j) + bias[j]);
-        if (MASK) {
-            if (live) {
-                const float from = fresh ? 0.0f : L[j];
-                L[j] = fmaf(k[j], z.get(j) - from, from);
-                A[j] = fresh ? -1.0f : product<MASK>(A[j], 1.0f - k[j]);
-            }
-        } else {
-            L[j] = fmaf(k[j], z.get(j) - L[j], L[j]);
-            A[j] *= 1.0f - k[j];
-        }
+        const float from = MASK && fresh ? 0.0f : L[j], a = A[j] * (1.0f - k[j]);
+        L[j] = fmaf(k[j], z.get(j) - from, from);
+        A[j] = MASK && fresh ? -1.0f : a;
     }
 }
 
 // and backwards, c -> a (dh + c)
 template <int V, bool MASK, class D>
-__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool live, bool fresh, float* A, float* L) {
+__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool fresh, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float a = 1.0f - k[j];
-        if (MASK) {
-            if (live) {
-                L[j] = fresh ? 0.0f : a * (dh.get(j) + L[j]);
-                A[j] = fresh ? -1.0f : product<MASK>(A[j], a);
-            }
-        } else {
-            L[j] = a * (dh.get(j) + L[j]);
-            A[j] *= a;
-        }
+        const float a = 1.0f - k[j], l = a * (dh.get(j) + L[j]), m = A[j] * a;
+        L[j] = MASK && fresh ? 0.0f : l;
+        A[j] = MASK && fresh ? -1.0f : m;
     }
 }
 
-}  // namespace
+// Padding. A wave whose lanes are all past their rows' lengths loads nothing and leaves the state
+// alone; where only some are, these lanes' inputs are replaced, whatever they hold: z and dh by 0
+// and f by a gate that lets nothing in (k = 0).
+template <class S, int V>
+__device__ __forceinline__ void blank(Vec<S, V>& x, float v) {
+    if constexpr (V > 1) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) x.v[j] = (S)v;
+    } else {
+        x.v = (S)v;
+    }
+}
+template <int V>
+__device__ __forceinline__ void blank(Vec8<V>& x, float v) {
+    x.q = 0x01010101u;
+    x.scale = v;
+}
+constexpr float kShut = 1e38f;
 
 // The map of the pieces before this wave's, applied to h (in the order of DIR), and of all of them.
 // All reads are under way before the first is used.
@@ -258,6 +262,8 @@ __device__ __forceinline__ void compose(const Maps<V>& m, int buf, int w, int nw
         }
     }
 }
+
+}  // namespace
 
 // Steps past T load the last one again (no branch between the loads) and are left out afterwards, by
 // tests that the whole wave shares.
@@ -295,21 +301,25 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
         float k[kSteps][V], A[V], L[V], g[V];
         bool fresh[kSteps];
         DELREC_COLS(j) A[j] = 1.0f, L[j] = g[j] = 0.0f;
-        const int tc = min(t0, T - 1);
-        zp.seek(tc), fp.seek(tc);
-        if (MASK) sp.seek(tc);
-        DELREC_STEPS(s) {
-            const long long more = t0 + s + 1 < T ? -1 : 0;
-            f[s] = fp.load(), z[s] = zp.load();
-            fp.next(more), zp.next(more);
-            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
-            if (MASK) sp.next(more);
-        }
-        DELREC_STEPS(s) {
-            if (t0 + s < T) step_forward<V, MASK>(f[s], z[s], bias, t0 + s < len, fresh[s], k[s], A, L);
+        const bool any = MASK ? __any(t0 < len) : t0 < T, part = MASK && !__all(t0 + kSteps <= len);
+        if (any) {
+            zp.seek(t0), fp.seek(t0);
+            if (MASK) sp.seek(t0);
+            DELREC_STEPS(s) {
+                const long long more = t0 + s + 1 < T ? -1 : 0;
+                f[s] = fp.load(), z[s] = zp.load();
+                fp.next(more), zp.next(more);
+                fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+                if (MASK) sp.next(more);
+            }
+            if (part) DELREC_STEPS(s)
+                if (t0 + s >= len) blank(z[s], 0.0f), blank(f[s], kShut), fresh[s] = false;
+            DELREC_STEPS(s) {
+                if (t0 + s < T) step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
+            }
         }
         maps.put(buf, w, lane, A, L);
-        if constexpr (PACK) {
+        if (PACK && any) {
             z8.seek(t0), f8.seek(t0);
             DELREC_STEPS(s) {
                 if (t0 + s < T) {
@@ -327,13 +337,14 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
         yp.seek(t0);
         DELREC_STEPS(s) {
             if (t0 + s < T) {
-                const bool live = !MASK || t0 + s < len;
                 float y[V];
-                DELREC_COLS(j) {
-                    if (MASK && fresh[s] && live) g[j] = 0.0f;
-                    const float next = fmaf(k[s][j], z[s].get(j) - g[j], g[j]);
-                    g[j] = live ? next : g[j];
-                    y[j] = live ? g[j] : 0.0f;
+                DELREC_COLS(j) y[j] = 0.0f;
+                if (any) {
+                    DELREC_COLS(j) {
+                        const float from = MASK && fresh[s] ? 0.0f : g[j];
+                        y[j] = g[j] = fmaf(k[s][j], z[s].get(j) - from, from);
+                    }
+                    if (part && t0 + s >= len) DELREC_COLS(j) y[j] = 0.0f;
                 }
                 if (ln.on) yp.store(y);
                 yp.next();
@@ -371,11 +382,12 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
         typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps];
         Vec<S, V> v[kSteps];
         bool fresh[kSteps];
-        const int tc = min(t0, T - 1);
-        if constexpr (PACK) fp8.seek(tc);
-        else fp.seek(tc);
-        xp.seek(tc);
-        if (MASK) sp.seek(tc);
+        if (MASK ? !__any(t0 < len) : t0 >= T) continue;
+        const bool part = MASK && !__all(t0 + kSteps <= len);
+        if constexpr (PACK) fp8.seek(t0);
+        else fp.seek(t0);
+        xp.seek(t0);
+        if (MASK) sp.seek(t0);
         DELREC_STEPS(s) {
             const long long more = t0 + s + 1 < T ? -1 : 0;
             if constexpr (PACK) f[s] = fp8.load(), fp8.next(more);
@@ -384,16 +396,17 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
             fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
             if (MASK) sp.next(more);
         }
+        if (part) DELREC_STEPS(s)
+            if (t0 + s >= len) blank(v[s], 0.0f), blank(f[s], kShut), fresh[s] = false;
         DELREC_STEPS(q) {
             const int s = BWD ? kSteps - 1 - q : q;
             if (t0 + s < T) {
-                const bool live = !MASK || t0 + s < len;
                 float k[V];
                 if constexpr (BWD) {
                     DELREC_COLS(j) k[j] = gate_in(f[s].get(j) + bias[j]);
-                    step_backward<V, MASK>(k, v[s], live, fresh[s], A, L);
+                    step_backward<V, MASK>(k, v[s], fresh[s], A, L);
                 } else {
-                    step_forward<V, MASK>(f[s], v[s], bias, live, fresh[s], k, A, L);
+                    step_forward<V, MASK>(f[s], v[s], bias, fresh[s], k, A, L);
                 }
             }
         }
@@ -414,7 +427,7 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
 
 // PACK: z and f from their 8 bits.
 template <class S, int V, bool MASK, bool PACK>
-__global__ void __launch_bounds__(512, DELREC_BWD_WAVES) gated_bwd_kernel(GatedScan p, int per_row, int range, float* dbpart) {
+__global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_row, int range, float* dbpart) {
     __shared__ Maps<V> fmap, rmap;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Lane<V> ln(p, per_row);
@@ -447,47 +460,51 @@ __global__ void __launch_bounds__(512, DELREC_BWD_WAVES) gated_bwd_kernel(GatedS
         bool fresh[kSteps];
         const auto st = vload<float, V>(p.states + (size_t)(tb / kBlk) * plane + at);
         DELREC_COLS(j) h[j] = st.get(j), g[j] = mine[j] = 0.0f;
-        float A[V], L[V];
-        typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps], z[kSteps];
-        const int tc = min(t0, T - 1);
-        if constexpr (PACK) z8.seek(tc), f8.seek(tc);
-        else zp.seek(tc), fp.seek(tc);
-        dhp.seek(tc);
-        if (MASK) sp.seek(tc);
-        DELREC_STEPS(s) {
-            const long long more = t0 + s + 1 < T ? -1 : 0;
-            if constexpr (PACK) f[s] = f8.load(), z[s] = z8.load(), f8.next(more), z8.next(more);
-            else f[s] = fp.load(), z[s] = zp.load(), fp.next(more), zp.next(more);
-            dh[s] = dhp.load(), dhp.next(more);
-            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
-            if (MASK) sp.next(more);
-        }
-        DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-        DELREC_STEPS(s) {
-            if (t0 + s < T) {
-                step_forward<V, MASK>(f[s], z[s], bias, t0 + s < len, fresh[s], k[s], A, L);
-                DELREC_COLS(j) d[s][j] = z[s].get(j);
+        const bool any = MASK ? __any(t0 < len) : t0 < T, part = MASK && !__all(t0 + kSteps <= len);
+        {
+            float A[V], L[V];
+            typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps], z[kSteps];
+            if (any) {
+                if constexpr (PACK) z8.seek(t0), f8.seek(t0);
+                else zp.seek(t0), fp.seek(t0);
+                dhp.seek(t0);
+                if (MASK) sp.seek(t0);
+                DELREC_STEPS(s) {
+                    const long long more = t0 + s + 1 < T ? -1 : 0;
+                    if constexpr (PACK) f[s] = f8.load(), z[s] = z8.load(), f8.next(more), z8.next(more);
+                    else f[s] = fp.load(), z[s] = zp.load(), fp.next(more), zp.next(more);
+                    dh[s] = dhp.load(), dhp.next(more);
+                    fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+                    if (MASK) sp.next(more);
+                }
+                if (part) DELREC_STEPS(s)
+                    if (t0 + s >= len) blank(z[s], 0.0f), blank(f[s], kShut), blank(dh[s], 0.0f), fresh[s] = false;
             }
+            DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
+            if (any) DELREC_STEPS(s) {
+                if (t0 + s < T) {
+                    step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
+                    DELREC_COLS(j) d[s][j] = z[s].get(j);
+                }
+            }
+            fmap.put(buf, w, lane, A, L);
+            DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
+            if (any) DELREC_STEPS_BACK(s) {
+                if (t0 + s < T) step_backward<V, MASK>(k[s], dh[s], fresh[s], A, L);
+            }
+            rmap.put(buf, w, lane, A, L);
         }
-        fmap.put(buf, w, lane, A, L);
-        DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-        DELREC_STEPS_BACK(s) {
-            if (t0 + s < T) step_backward<V, MASK>(k[s], dh[s], !MASK || t0 + s < len, fresh[s], A, L);
-        }
-        rmap.put(buf, w, lane, A, L);
         barrier_lds();
         compose<V, MASK, -1>(rmap, buf, w, nw, lane, c, g);
         compose<V, MASK, 1>(fmap, buf, w, nw, lane, h, mine);
         float blk[V];
         // d: z_t becomes h_{t-1} - z_t
-        DELREC_STEPS(s) {
+        if (any) DELREC_STEPS(s) {
             if (t0 + s < T) {
-                const bool live = !MASK || t0 + s < len;
                 DELREC_COLS(j) {
-                    if (MASK && fresh[s] && live) mine[j] = 0.0f;
-                    d[s][j] = mine[j] - d[s][j];
-                    const float next = fmaf(-k[s][j], d[s][j], mine[j]);
-                    mine[j] = live ? next : mine[j];
+                    const float from = MASK && fresh[s] ? 0.0f : mine[j];
+                    d[s][j] = from - d[s][j];
+                    mine[j] = fmaf(-k[s][j], d[s][j], from);
                 }
             }
         }
@@ -495,20 +512,17 @@ __global__ void __launch_bounds__(512, DELREC_BWD_WAVES) gated_bwd_kernel(GatedS
         dzp.seek(t0 + kSteps - 1), dfp.seek(t0 + kSteps - 1);
         DELREC_STEPS_BACK(s) {
             if (t0 + s < T) {
-                const bool live = !MASK || t0 + s < len;
                 float oz[V], of[V];
-                DELREC_COLS(j) {
-                    const float a = 1.0f - k[s][j], lam = dh[s].get(j) + g[j];
-                    oz[j] = lam * k[s][j];
-                    of[j] = oz[j] * a * d[s][j];
-                    if (MASK) {
-                        oz[j] = live ? oz[j] : 0.0f;
-                        of[j] = live ? of[j] : 0.0f;
-                        g[j] = live ? (fresh[s] ? 0.0f : a * lam) : g[j];
-                    } else {
-                        g[j] = a * lam;
+                DELREC_COLS(j) oz[j] = of[j] = 0.0f;
+                if (any) {
+                    DELREC_COLS(j) {
+                        const float a = 1.0f - k[s][j], lam = dh[s].get(j) + g[j], back = a * lam;
+                        oz[j] = lam * k[s][j];
+                        of[j] = oz[j] * a * d[s][j];
+                        g[j] = MASK && fresh[s] ? 0.0f : back;
                     }
-                    blk[j] += of[j];
+                    if (part && t0 + s >= len) DELREC_COLS(j) oz[j] = of[j] = 0.0f;
+                    DELREC_COLS(j) blk[j] += of[j];
                 }
                 if (ln.on) dzp.store(oz, own), dfp.store(of, own);
             }
@@ -535,26 +549,26 @@ struct Plan {
     int V, per_row, groups, waves, range, ranges;
 };
 
-Plan gated_plan(int T, int B, int N, bool pack, bool wide) {
+// Two columns a lane. Four (one access of 8 bytes for bf16, not 4) have the same bytes under way
+// but half the workgroups and, in the backward, 160 registers and 3 waves a SIMD: 480 us for
+// T1024 B64 N2048 with 8 bits, 290 with two; 55 and 35 us for T250 B128 N512. One (rows of one
+// column, and offsets past 32 bits): 548 and 66 us.
+//
+// Time over the grid where the channels give less than a workgroup a CU: each range's inputs are
+// then read twice, and at T1000 N512 bf16 the forward and backward take 124 us whole and 85 in
+// four ranges for B 32 (128 workgroups), 150 and 158 for B 64 (256). As many ranges as make one
+// round of two workgroups a CU (T16384 B2 N700 fp32: 234 us with 43 ranges = 473 workgroups, 253
+// with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 186 us with 3
+// ranges, 135 with 6).
+Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
     Plan q;
-    auto shape = [&](int v) {
-        q.V = v;
-        q.per_row = pack ? (N + kGroup8 - 1) / kGroup8 * (kGroup8 / v) : (N + v - 1) / v;
-        q.groups = (int)(((long long)B * q.per_row + 63) / 64);
-    };
-    shape(N >= 4 ? 4 : N >= 2 ? 2 : 1);
-    int fill = 512, top = 64;
-    if (const char* e = getenv("PLAN_FILL")) fill = atoi(e);
-    if (const char* e = getenv("PLAN_TOP")) top = atoi(e);
-    if (q.V == 4 && q.groups < fill) shape(2);
-    if (const char* e = getenv("PLAN_V")) shape(atoi(e));
-    if (wide) shape(1);
+    q.V = N >= 2 && !wide ? 2 : 1;
+    q.per_row = pack ? (N + kGroup8 - 1) / kGroup8 * (kGroup8 / q.V) : (N + q.V - 1) / q.V;
+    q.groups = (int)(((long long)B * q.per_row + 63) / 64);
     q.waves = T >= kBlk ? kWaves : (T + kSteps - 1) / kSteps;
     const int blocks = (T + kBlk - 1) / kBlk;
-    int low = 256;
-    if (const char* e = getenv("PLAN_LOW")) low = atoi(e);
-    int want = q.groups >= low ? 1 : std::max(1, fill / q.groups);
-    want = std::min({want, top, std::max(1, blocks / 2)});
+    int want = q.groups >= 256 ? 1 : (mask ? 1024 : 512) / q.groups;
+    want = std::max(1, std::min({want, 128, blocks / 2}));
     const int per = (blocks + want - 1) / want;
     q.range = per * kBlk;
     q.ranges = (blocks + per - 1) / per;
@@ -588,8 +602,7 @@ void run_gated_m(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream
 
 template <class S>
 void run_gated_v(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream) {
-    if (q.V == 4) run_gated_m<S, 4>(p, q, fwd, stream);
-    else if (q.V == 2) run_gated_m<S, 2>(p, q, fwd, stream);
+    if (q.V == 2) run_gated_m<S, 2>(p, q, fwd, stream);
     else run_gated_m<S, 1>(p, q, fwd, stream);
 }
 
@@ -598,23 +611,23 @@ void launch_gated(const GatedScan& p, bool fwd, hipStream_t stream) {
     bool wide = false;
     for (const delrec_rows* x : {&p.z, &p.f, &p.h, &p.dh, &p.dz, &p.df})
         if (x->data && (256 / p.N + 2) * x->s1 + p.N > 0x7fffffffLL / 4) wide = true;
-    const Plan q = gated_plan(p.T, p.B, p.N, p.z8.q != nullptr, wide);
+    const Plan q = gated_plan(p.T, p.B, p.N, p.z8.q != nullptr, wide, p.starts || p.lengths);
     if (p.bf16) run_gated_v<__bf16>(p, q, fwd, stream);
     else run_gated_v<float>(p, q, fwd, stream);
 }
 
 }  // namespace
 
-// floats of workspace, for whichever form the strides and the 8 bits ask for: the ranges' maps, and
-// the ranges' bias sums
+// floats of workspace, for whichever form the strides, the 8 bits and the masks ask for: the
+// ranges' maps, and the ranges' bias sums
 size_t gated_fwd_ws(int T, int B, int N) {
     size_t n = 0;
-    for (int form = 0; form < 4; ++form) n = std::max(n, map_floats(gated_plan(T, B, N, form & 1, form & 2), B, N));
+    for (int form = 0; form < 8; ++form) n = std::max(n, map_floats(gated_plan(T, B, N, form & 1, form & 2, form & 4), B, N));
     return n;
 }
 size_t gated_bwd_ws(int T, int B, int N) {
     int ranges = 1;
-    for (int form = 0; form < 4; ++form) ranges = std::max(ranges, gated_plan(T, B, N, form & 1, form & 2).ranges);
+    for (int form = 0; form < 8; ++form) ranges = std::max(ranges, gated_plan(T, B, N, form & 1, form & 2, form & 4).ranges);
     return gated_fwd_ws(T, B, N) + (size_t)ranges * B * N;
 }
 

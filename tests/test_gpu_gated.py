@@ -529,3 +529,25 @@ def test_forward_calls_in_a_graph(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('masks', [False, True])
+def test_scan_offsets_past_32_bits(dev, masks):
+    """Rows of the batch so far apart that their distance in bytes does not fit 32 bits."""
+    from delrec.gated import gated_scan
+    T, B, N, far = 70, 2, 300, (1 << 30) + 512
+    c = scan_case(T, B, N, BF16, masks, seed=11)
+    want = run_scan(c, dev)
+    big = torch.empty(far + T * N, dtype=BF16, device=dev)
+    z = big.as_strided((T, B, N), (N, far, 1))
+    with torch.no_grad():
+        z.copy_(c['z'].to(dev))
+    c2 = {k: (None if v is None else v.to(dev)) for k, v in c.items()}
+    leaves = [z.detach().requires_grad_(True)] + [c2[k].requires_grad_(True) for k in ('f', 'bias', 'h0')]
+    for checkpoint in (False, True):
+        h, last = gated_scan(*leaves, starts=c2['starts'], lengths=c2['lengths'], checkpoint=checkpoint)
+        got = (h, last, *torch.autograd.grad((h, last), leaves, (c2['dh'], c2['dlast'])))
+        ref = want if not checkpoint else run_scan(c, dev, True)
+        for name, a, b in zip(('h', 'last', 'dz', 'df', 'db', 'dh0'), got, ref):
+            close(a, b.detach().double().cpu(), 3e-5, name, mass=float(ref[3].double().abs().sum((0, 1)).max()) if name == 'db' else None)
