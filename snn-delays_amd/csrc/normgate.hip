@@ -9,7 +9,7 @@
 // Bound by memory: a row stays in registers between its loads and its stores, the two row sums
 // are exchanges between its lanes. A row is 16, 64, 256 or 512 lanes, each with NE vectors of
 // four columns, as few lanes as hold it in at most four vectors (16 lanes: four rows a wave, no
-// LDS). The backward recomputes x', e and the gate from o, g and x (or their 8 bits) and the two
+// LDS): forward 31 us for 32000 x 512 bf16 (5.3 TB/s). The backward recomputes x', e and the gate from o, g and x (or their 8 bits) and the two
 // kept norms: one residual tensor is read, not two. Its column sums stay in registers over all the
 // rows a workgroup takes; the workgroups' sums are added in a second launch, in a fixed order.
 #include <algorithm>
@@ -158,14 +158,15 @@ __global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, in
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int n = blockIdx.x * 64 + lane, k = blockIdx.y;
     float* out = k == 0 ? o0 : (k == 1 ? o1 : o2);
-    // eight rows' loads in flight at a time (one at a time: 20 us for 1024 rows of 3 x 512, so 5)
+    // eight rows' loads in flight at a time (past the end the last row again, left out)
     float s8[8] = {};
-    if (n < N) {
-        const float* at = part + (size_t)k * N + n;
-        for (int r = w; r < rows; r += 128)
+    const float* at = part + (size_t)k * N + min(n, N - 1);
+    for (int r = w; r < rows; r += 128) {
+        float v[8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (r + 16 * q < rows) s8[q] += at[(size_t)(r + 16 * q) * pitch];
+        for (int q = 0; q < 8; ++q) v[q] = at[(size_t)min(r + 16 * q, rows - 1) * pitch];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s8[q] += r + 16 * q < rows ? v[q] : 0.0f;
     }
     float s = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
     red[w][lane] = s;
@@ -366,77 +367,104 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_fwd_kernel(NormGate 
     }
 }
 
-// PACK: o, g and x from their 8 bits
+// PACK: o, g and x from their 8 bits. Up to two vectors a lane (N 2048), a row's values are loaded
+// while the one before is computed, and the three column vectors are in LDS, read again in each
+// half of a row. Each row's loads waited for in place, the columns in registers: 77 us for 32000 x
+// 512 bf16 and 660 for 65536 x 2048 with 8 bits; so 50 (5.3 TB/s) and 485 (4.7 TB/s). With four
+// vectors there are no registers for either.
 template <class S, class X, int LPR, int NE, bool BLOCK, bool PACK>
 __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate p) {
-    constexpr int RPW = kRowBlock<LPR> / LPR, W = LPR > 64 ? LPR / 64 : 1;
+    constexpr int RPW = kRowBlock<LPR> / LPR, W = LPR > 64 ? LPR / 64 : 1, ROW = LPR * NE * 4;
+    constexpr bool SHARED = NE <= 2, AHEAD = NE <= 2;
     __shared__ float red[2 * W];
-    __shared__ float slots[RPW > 1 ? RPW : 1][RPW > 1 ? LPR * NE * 4 : 1];
+    __shared__ float slots[RPW > 1 ? RPW : 1][RPW > 1 ? ROW : 1];
+    __shared__ float cols[SHARED ? 3 : 1][SHARED ? ROW : 1];
     const int lane = threadIdx.x % LPR, N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
     const Cols<LPR, NE> c(lane, N);
-    const long long rows = (long long)p.R0 * p.R1;
-    float w[NE][4], sc[NE][4], w2[NE][4], acc[3][NE][4];
-    if constexpr (BLOCK) {
-        load_cols<NE>(w, p.w, c.n0);
-        load_cols<NE>(sc, p.scale, c.n0);
-    }
-    if (p.w2) load_cols<NE>(w2, p.w2, c.n0);
+    const long long rows = (long long)p.R0 * p.R1, step = (long long)gridDim.x * RPW;
+    float held[SHARED ? 1 : 3][NE][4], acc[3][NE][4];
+    auto fill = [&](int k, const float* src) {
 #pragma unroll
-    for (int e = 0; e < NE; ++e)
+        for (int e = 0; e < NE; ++e) {
+            float v[4] = {};
+            if (src) {
+                const auto t = vload<float, 4>(src + c.n0[e]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            acc[0][e][j] = acc[1][e][j] = acc[2][e][j] = 0.0f;
-            if (!p.w2) w2[e][j] = 0.0f;
+                for (int j = 0; j < 4; ++j) v[j] = t.get(j);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (SHARED) cols[k][(e * LPR + lane) * 4 + j] = v[j];
+                else held[k][e][j] = v[j];
+                acc[k][e][j] = 0.0f;
+            }
         }
-    const float inv_n = 1.0f / (float)N;
-    for (long long r0 = (long long)blockIdx.x * RPW; r0 < rows; r0 += (long long)gridDim.x * RPW) {
+    };
+    fill(0, BLOCK ? p.w : nullptr);
+    fill(1, BLOCK ? p.scale : nullptr);
+    fill(2, p.w2);
+    __syncthreads();
+    auto col = [&](int k, int e, int j) {
+        if constexpr (SHARED) return cols[k][(e * LPR + lane) * 4 + j];
+        else return held[k][e][j];
+    };
+
+    typedef typename std::conditional<PACK, Vec8<4>, Vec<S, 4>>::type SV;
+    typedef typename std::conditional<PACK, Vec8<4>, Vec<X, 4>>::type XV;
+    struct Raw {
+        SV o[NE], g[NE];
+        XV x[NE];
+        Vec<X, 4> up[NE];
+        Vec<S, 4> du[NE];
+        float r, r2;
+    } in;
+    // rows past the end repeat the last one, with no gradient, and store nothing
+    auto load = [&](long long r0) {
         const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
-        const bool live = mine < rows;
-        float o[NE][4], g[NE][4], x[NE][4], up[NE][4], du[NE][4];
-        auto take = [&](auto tag, const delrec_rows& src, const delrec_packed8& q, float (&v)[NE][4]) {
-            using T = decltype(tag);
+        const size_t q = (size_t)row * pitch8(N), s = (size_t)row * ng;
+        in.r = p.stats[2 * row];
+        in.r2 = p.stats[2 * row + 1];
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
             if constexpr (PACK) {
-#pragma unroll
-                for (int e = 0; e < NE; ++e) {
-                    const auto t = load8<4>(q.q + row * pitch8(N), q.scale + row * ng + c.group[e], Lane8<4>(c.i[e], c.skip[e], c.on[e], N));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[e][j] = t.get(j);
+                const Lane8<4> l8(c.i[e], c.skip[e], c.on[e], N);
+                if constexpr (BLOCK) {
+                    in.o[e] = load8<4>(p.o8.q + q, p.o8.scale + s + c.group[e], l8);
+                    in.g[e] = load8<4>(p.g8.q + q, p.g8.scale + s + c.group[e], l8);
                 }
+                in.x[e] = load8<4>(p.x8.q + q, p.x8.scale + s + c.group[e], l8);
             } else {
-                const T* b = row_at<const T>(src, row, p);
-#pragma unroll
-                for (int e = 0; e < NE; ++e) {
-                    const auto t = vload<T, 4>(b + c.n0[e]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[e][j] = t.get(j);
+                if constexpr (BLOCK) {
+                    in.o[e] = vload<S, 4>(row_at<const S>(p.o, row, p) + c.n0[e]);
+                    in.g[e] = vload<S, 4>(row_at<const S>(p.g, row, p) + c.n0[e]);
                 }
+                in.x[e] = vload<X, 4>(row_at<const X>(p.x, row, p) + c.n0[e]);
             }
-        };
-        auto grad = [&](auto tag, const delrec_rows& src, float (&v)[NE][4]) {
-            using T = decltype(tag);
-            const T* b = src.data ? row_at<const T>(src, row, p) : nullptr;
-#pragma unroll
-            for (int e = 0; e < NE; ++e) {
-                if (b) {
-                    const auto t = vload<T, 4>(b + c.n0[e]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[e][j] = live ? t.get(j) : 0.0f;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[e][j] = 0.0f;
-                }
-            }
-        };
-        if constexpr (BLOCK) {
-            take(S{}, p.o, p.o8, o);
-            take(S{}, p.g, p.g8, g);
+            if (p.dx_out.data) in.up[e] = vload<X, 4>(row_at<const X>(p.dx_out, row, p) + c.n0[e]);
+            if (p.du.data) in.du[e] = vload<S, 4>(row_at<const S>(p.du, row, p) + c.n0[e]);
         }
-        take(X{}, p.x, p.x8, x);
-        grad(X{}, p.dx_out, up);
-        grad(S{}, p.du, du);
-        const float r = p.stats[2 * row], r2 = p.stats[2 * row + 1];
+    };
+    const float inv_n = 1.0f / (float)N;
+    long long r0 = (long long)blockIdx.x * RPW;
+    if (AHEAD && r0 < rows) load(r0);
+    for (; r0 < rows; r0 += step) {
+        if (!AHEAD) load(r0);
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        const bool live = mine < rows, has_up = live && p.dx_out.data, has_du = live && p.du.data;
+        const float r = in.r, r2 = in.r2;
+        float o[NE][4], g[NE][4], x[NE][4], up[NE][4], du[NE][4], sg[NE][4];
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (BLOCK) o[e][j] = in.o[e].get(j), g[e][j] = in.g[e].get(j);
+                x[e][j] = in.x[e].get(j);
+                up[e][j] = has_up ? in.up[e].get(j) : 0.0f;
+                du[e][j] = has_du ? in.du[e].get(j) : 0.0f;
+            }
+        if (AHEAD && r0 + step < rows) load(r0 + step);
         // o becomes e = o r, x becomes e2 = x' r2
-        float s = 0.0f, si[NE][4], sg[NE][4];
+        float s = 0.0f;
 #pragma unroll
         for (int e = 0; e < NE; ++e)
 #pragma unroll
@@ -444,13 +472,13 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
                 if constexpr (BLOCK) {
                     o[e][j] *= r;
                     sg[e][j] = sigm(g[e][j]);
-                    si[e][j] = g[e][j] * sg[e][j];
-                    x[e][j] = fmaf(sc[e][j], o[e][j] * w[e][j] * si[e][j], x[e][j]);
+                    x[e][j] = fmaf(col(1, e, j), o[e][j] * col(0, e, j) * (g[e][j] * sg[e][j]), x[e][j]);
                 }
                 x[e][j] *= r2;
-                s += j >= c.skip[e] ? w2[e][j] * du[e][j] * x[e][j] : 0.0f;
+                s += j >= c.skip[e] ? col(2, e, j) * du[e][j] * x[e][j] : 0.0f;
             }
         const float m2 = lanes_sum<LPR>(s, red, 0) * inv_n;
+        if constexpr (SHARED) asm volatile("" ::: "memory");   // the columns are read again, not kept
         s = 0.0f;
         X* dxp = row_at<X>(p.dx, row, p);
 #pragma unroll
@@ -458,15 +486,15 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
             float dg[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float dx = fmaf(r2, w2[e][j] * du[e][j] - x[e][j] * m2, up[e][j]);
+                const float dx = fmaf(r2, col(2, e, j) * du[e][j] - x[e][j] * m2, up[e][j]);
                 acc[2][e][j] = fmaf(du[e][j], x[e][j], acc[2][e][j]);
                 up[e][j] = dx;
                 if constexpr (BLOCK) {
-                    const float dxs = dx * si[e][j], dn = sc[e][j] * dxs, ew = o[e][j] * w[e][j];
+                    const float si = g[e][j] * sg[e][j], dxs = dx * si, dn = col(1, e, j) * dxs, ew = o[e][j] * col(0, e, j);
                     acc[0][e][j] = fmaf(dn, o[e][j], acc[0][e][j]);
                     acc[1][e][j] = fmaf(dxs, ew, acc[1][e][j]);
-                    dg[j] = sc[e][j] * dx * ew * fmaf(si[e][j], 1.0f - sg[e][j], sg[e][j]);
-                    g[e][j] = w[e][j] * dn;  // v
+                    dg[j] = col(1, e, j) * dx * ew * fmaf(si, 1.0f - sg[e][j], sg[e][j]);
+                    g[e][j] = col(0, e, j) * dn;   // v
                     s += j >= c.skip[e] ? g[e][j] * o[e][j] : 0.0f;
                 }
             }
@@ -536,11 +564,24 @@ RowPlan row_plan(int N, bool fwd) {
     return q;
 }
 
-// workgroups of the backward, one set of column sums each: enough to fill the GPU, few enough that
-// the sums are small beside the rows
-int norm_gate_parts(long long rows, int N) {
-    const long long wg = in_registers(N) ? (rows + row_plan(N, false).rpw - 1) / row_plan(N, false).rpw : rows;
-    return (int)std::min<long long>(wg, in_registers(N) ? 1024 : 512);
+// Workgroups of the backward, one set of column sums each: those that fit the GPU at once, each
+// with its share of the rows (a second round of some of them leaves CUs idle: 32000 x 512 bf16, of
+// which 768 fit: 50 us with 768, 59 with 1024).
+constexpr int kMostParts = 1280;
+
+long long row_groups(long long rows, int N) {
+    if (!in_registers(N)) return rows;
+    const int rpw = row_plan(N, false).rpw;
+    return (rows + rpw - 1) / rpw;
+}
+int any_parts(long long rows) { return (int)std::min<long long>(rows, 512); }
+
+int resident(const void* kernel, int block) {
+    int per_cu = 0, dev = 0, cus = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, block, 0) != hipSuccess || per_cu < 1) per_cu = 1;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
+        cus = 256;
+    return std::min(per_cu * cus, kMostParts);
 }
 
 template <class S, class X, int LPR, int NE>
@@ -553,22 +594,23 @@ void run_fwd(const NormGate& p, hipStream_t stream) {
     else hipLaunchKernelGGL((norm_gate_fwd_kernel<S, X, LPR, NE, kNormOnly>), grid, block, 0, stream, p);
 }
 
+template <class S, class X, int LPR, int NE, bool BLOCK, bool PACK>
+int run_bwd_k(const NormGate& p, hipStream_t stream) {
+    static const int fit = resident((const void*)norm_gate_bwd_kernel<S, X, LPR, NE, BLOCK, PACK>, kRowBlock<LPR>);
+    const int parts = (int)std::min<long long>(row_groups((long long)p.R0 * p.R1, p.N), fit);
+    hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, BLOCK, PACK>), dim3(parts), dim3(kRowBlock<LPR>), 0, stream, p);
+    return parts;
+}
 template <class S, class X, int LPR, int NE>
-void run_bwd(const NormGate& p, int parts, hipStream_t stream) {
-    const dim3 grid(parts), block(kRowBlock<LPR>);
-    if (p.w) {
-        if (p.x8.q) hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, true, true>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, true, false>), grid, block, 0, stream, p);
-    } else {
-        if (p.x8.q) hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, false, true>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((norm_gate_bwd_kernel<S, X, LPR, NE, false, false>), grid, block, 0, stream, p);
-    }
+int run_bwd(const NormGate& p, hipStream_t stream) {
+    if (p.w) return p.x8.q ? run_bwd_k<S, X, LPR, NE, true, true>(p, stream) : run_bwd_k<S, X, LPR, NE, true, false>(p, stream);
+    return p.x8.q ? run_bwd_k<S, X, LPR, NE, false, true>(p, stream) : run_bwd_k<S, X, LPR, NE, false, false>(p, stream);
 }
 
+// the workgroups of a backward (sets of column sums)
 template <class S, class X>
-void run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
+int run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
     const long long rows = (long long)p.R0 * p.R1;
-    const int parts = norm_gate_parts(rows, p.N);
     if (!in_registers(p.N)) {
         if (fwd) {
             hipLaunchKernelGGL((norm_any_fwd_kernel<S, X>), dim3((unsigned)rows), dim3(kNb), 0, stream, p);
@@ -576,9 +618,9 @@ void run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
             if (p.g8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.g, p.g8}, true, stream);
             if (p.x8.q) launch_pack8({p.R0, p.R1, p.N, p.x_bf16, p.x, p.x8}, true, stream);
         } else {
-            hipLaunchKernelGGL((norm_any_bwd_kernel<S, X>), dim3(parts), dim3(kNb), 0, stream, p);
+            hipLaunchKernelGGL((norm_any_bwd_kernel<S, X>), dim3(any_parts(rows)), dim3(kNb), 0, stream, p);
         }
-        return;
+        return any_parts(rows);
     }
     const RowPlan q = row_plan(p.N, fwd);
     if (fwd) {
@@ -586,17 +628,19 @@ void run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
         else if (q.lanes == 64) q.vecs == 1 ? run_fwd<S, X, 64, 1>(p, stream) : q.vecs == 2 ? run_fwd<S, X, 64, 2>(p, stream) : run_fwd<S, X, 64, 4>(p, stream);
         else if (q.lanes == 256) q.vecs == 2 ? run_fwd<S, X, 256, 2>(p, stream) : run_fwd<S, X, 256, 4>(p, stream);
         else run_fwd<S, X, 512, 4>(p, stream);
-    } else {
-        if (q.lanes == 16) q.vecs == 1 ? run_bwd<S, X, 16, 1>(p, parts, stream) : run_bwd<S, X, 16, 2>(p, parts, stream);
-        else if (q.lanes == 64) q.vecs == 1 ? run_bwd<S, X, 64, 1>(p, parts, stream) : run_bwd<S, X, 64, 2>(p, parts, stream);
-        else if (q.lanes == 256) q.vecs == 1 ? run_bwd<S, X, 256, 1>(p, parts, stream) : q.vecs == 2 ? run_bwd<S, X, 256, 2>(p, parts, stream) : run_bwd<S, X, 256, 4>(p, parts, stream);
-        else run_bwd<S, X, 512, 4>(p, parts, stream);
+        return 0;
     }
+    if (q.lanes == 16) return q.vecs == 1 ? run_bwd<S, X, 16, 1>(p, stream) : run_bwd<S, X, 16, 2>(p, stream);
+    if (q.lanes == 64) return q.vecs == 1 ? run_bwd<S, X, 64, 1>(p, stream) : run_bwd<S, X, 64, 2>(p, stream);
+    if (q.lanes == 512) return run_bwd<S, X, 512, 4>(p, stream);
+    return q.vecs == 1 ? run_bwd<S, X, 256, 1>(p, stream) : q.vecs == 2 ? run_bwd<S, X, 256, 2>(p, stream) : run_bwd<S, X, 256, 4>(p, stream);
 }
 
 }  // namespace
 
-size_t norm_gate_bwd_ws(long long rows, int N) { return (size_t)norm_gate_parts(rows, N) * 3 * N; }
+size_t norm_gate_bwd_ws(long long rows, int N) {
+    return (size_t)(in_registers(N) ? std::min<long long>(row_groups(rows, N), kMostParts) : any_parts(rows)) * 3 * N;
+}
 
 void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
     NormGate p = a;
@@ -613,11 +657,10 @@ void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
             p.R0 = 1;
         }
     }
-    if (!p.bf16) run_norm_gate<float, float>(p, fwd, stream);
-    else if (p.x_bf16) run_norm_gate<__bf16, __bf16>(p, fwd, stream);
-    else run_norm_gate<__bf16, float>(p, fwd, stream);
-    if (!fwd)
-        launch_column_sums(p.part, norm_gate_parts((long long)p.R0 * p.R1, p.N), p.N, 3 * p.N, p.dw, p.dscale, p.dw2, stream);
+    const int parts = !p.bf16 ? run_norm_gate<float, float>(p, fwd, stream)
+                      : p.x_bf16 ? run_norm_gate<__bf16, __bf16>(p, fwd, stream)
+                                 : run_norm_gate<__bf16, float>(p, fwd, stream);
+    if (!fwd) launch_column_sums(p.part, parts, p.N, 3 * p.N, p.dw, p.dscale, p.dw2, stream);
 }
 
 }  // namespace delrec
