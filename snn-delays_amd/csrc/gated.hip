@@ -610,7 +610,7 @@ void launch_gated(const GatedScan& p, bool fwd, hipStream_t stream) {
     // the rows that a wave's 64 V channels touch, counted generously, against 32-bit offsets
     bool wide = false;
     for (const delrec_rows* x : {&p.z, &p.f, &p.h, &p.dh, &p.dz, &p.df})
-        if (x->data && (256 / p.N + 2) * x->s1 + p.N > 0x7fffffffLL / 4) wide = true;
+        if (x->data && (x->s1 < 0 || (256 / p.N + 2) * x->s1 + p.N > 0x7fffffffLL / 4)) wide = true;
     const Plan q = gated_plan(p.T, p.B, p.N, p.z8.q != nullptr, wide, p.starts || p.lengths);
     if (p.bf16) run_gated_v<__bf16>(p, q, fwd, stream);
     else run_gated_v<float>(p, q, fwd, stream);

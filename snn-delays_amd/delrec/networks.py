@@ -6,6 +6,9 @@ hot path this build implements: axonal, synaptic, common, vanilla, fixed and hyb
 recurrent delays (``networks.py:140-400, 802-984, 1128-1204``). Layers are created in the
 reference's order, so a seeded model draws the same initial parameters.
 
+``RNN_gated`` is the non-spiking counterpart on the same (T, B, N) inputs: a residual stack of
+gated linear recurrences (``delrec.gated``), without one in the reference.
+
 Feedforward-delay classes ride DCLS's convolution, not this path, and are not provided;
 ``dcls_module`` exists only so ``isinstance`` checks in callers keep working.
 """
@@ -14,6 +17,8 @@ import torch
 
 from .spike_linear import SpikeLinear
 
+from .checkpoint8 import Linear8
+from .gated import GatedBlock, rms_norm
 from .delay_layers import axonal_recdel, synaptic_recdel, common_recdel
 from .neuron import Dropout
 
@@ -351,3 +356,48 @@ class SNN_fixed_hybrid_recurrent_delays(SNN_recurrent_hybrid_delays):
                 layer.use_sig_p = False
                 if hasattr(layer, 'p_spread'):
                     del layer.p_spread
+
+
+# ---------------------------------------------------------------- without spikes --------
+
+class RNN_gated(torch.nn.Module):
+    """A residual stack of gated linear recurrences over (T, B, N): ``Linear -> rms_norm ->
+    GatedBlock ... -> Linear``, one block for each entry of ``config.hidden_layers`` (all of one
+    width). Trains with ``delrec.training.mem`` like the ``SNN_*`` classes; ``step`` runs it one
+    time step at a time on streaming input. The residual stream is fp32, also under
+    ``torch.autocast('cuda', torch.bfloat16)``. ``config.checkpoint8`` (default False): the
+    blocks keep their activations in 8 bits for the backward pass."""
+
+    def __init__(self, config):
+        super().__init__()
+        widths = set(config.hidden_layers)
+        if len(widths) != 1:
+            raise ValueError(f'RNN_gated needs hidden layers of one width, got {config.hidden_layers}')
+        N = widths.pop()
+        self.config = config
+        self.checkpoint = bool(getattr(config, 'checkpoint8', False))
+        self.embed = torch.nn.Linear(config.input_size, N, bias=config.bias)
+        self.norm_weight = torch.nn.Parameter(torch.ones(N))
+        self.blocks = torch.nn.ModuleList(GatedBlock(N, bias=config.bias, checkpoint=self.checkpoint)
+                                          for _ in config.hidden_layers)
+        self.readout = (Linear8 if self.checkpoint else torch.nn.Linear)(N, config.output_size, bias=config.bias)
+
+    def forward(self, x, starts=None, lengths=None):
+        assert x.dim() == 3  # (T, B, N)
+        x = self.embed(x).float()
+        u = rms_norm(x, self.norm_weight, checkpoint=self.checkpoint)
+        for block in self.blocks:
+            x, u, _ = block(x, u, starts=starts, lengths=lengths)
+        return self.readout(u)
+
+    @torch.no_grad()
+    def step(self, x, state=None):
+        """One time step of inputs (B, input_size): the readout (B, output_size) and the blocks'
+        states, which are updated in place (``None``: all zero)."""
+        x = self.embed(x).float()
+        if state is None:
+            state = [x.new_zeros(x.shape) for _ in self.blocks]
+        u = rms_norm(x, self.norm_weight)
+        for block, h in zip(self.blocks, state):
+            x, u, _ = block.step(x, u, h, h_out=h)
+        return torch.nn.functional.linear(u, self.readout.weight, self.readout.bias), state

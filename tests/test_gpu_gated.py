@@ -551,3 +551,130 @@ def test_scan_offsets_past_32_bits(dev, masks):
         ref = want if not checkpoint else run_scan(c, dev, True)
         for name, a, b in zip(('h', 'last', 'dz', 'df', 'db', 'dh0'), got, ref):
             close(a, b.detach().double().cpu(), 3e-5, name, mass=float(ref[3].double().abs().sum((0, 1)).max()) if name == 'db' else None)
+
+
+# ---------------------------------------------------------------- block and model -----------
+
+def block_reference(block, x, u, dx, du):
+    """A GatedBlock's outputs and gradients in 64 bits."""
+    N = x.shape[-1]
+    p = {k: v.detach().double().cpu() for k, v in block.named_parameters()}
+    leaves = [t.double().cpu().requires_grad_(True) for t in (x, u)] + [v.requires_grad_(True) for v in p.values()]
+    z, f, g = (leaves[1] @ p['proj.weight'].t()).split(N, -1)
+    h, last, _ = og.scan(z, f, p['gate_bias'])
+    xo, uo = og.norm_gate(h, g, leaves[0], p['weight'], p['scale'], p['next_weight'], block.eps)
+    grads = torch.autograd.grad((xo, uo), leaves, (dx.double().cpu(), du.double().cpu()))
+    return xo.detach(), uo.detach(), last.detach(), dict(zip(['x', 'u', *p], grads))
+
+
+@pytest.mark.gpu
+def test_block_forward_and_gradients(dev):
+    """The block's fp32 projection adds a rounding per product (torch's GEMM): 1e-4 of the largest."""
+    from delrec.gated import GatedBlock
+    torch.manual_seed(2)
+    block = GatedBlock(68).to(dev)
+    x, u, dx, du = (torch.randn(90, 3, 68, device=dev) for _ in range(4))
+    xl, ul = x.clone().requires_grad_(True), u.clone().requires_grad_(True)
+    xo, uo, last = block(xl, ul)
+    params = dict(block.named_parameters())
+    grads = torch.autograd.grad((xo, uo), [xl, ul, *params.values()], (dx, du))
+    X, U, L, G = block_reference(block, x, u, dx, du)
+    for name, a, b in (('x', xo, X), ('u', uo, U), ('last', last, L), *((k, g, G[k]) for k, g in zip(['x', 'u', *params], grads))):
+        close(a, b, 1e-4, name)
+
+
+@pytest.mark.gpu
+def test_block_keeps_less_in_8_bits(dev):
+    """Between forward and backward a checkpointed block holds about 7 bytes a channel and step
+    beside its outputs (u, z, f, o, g, x in 8 bits with their scales, the states), an fp32 one 24
+    and more; its gradients stay within some percent."""
+    from delrec.gated import GatedBlock
+    T, B, N = 512, 8, 256
+    held, grads = [], []
+    for checkpoint in (False, True):
+        torch.manual_seed(2)
+        block = GatedBlock(N, checkpoint=checkpoint).to(dev)
+        gen = torch.Generator(device=dev).manual_seed(1)
+        x, u, dx, du = (torch.randn(T, B, N, device=dev, generator=gen) for _ in range(4))
+        x.requires_grad_(True), u.requires_grad_(True)
+        out = block(x * 1.0, u * 1.0)            # inputs that the block alone keeps alive
+        torch.cuda.synchronize()
+        base = torch.cuda.memory_allocated()
+        params = list(block.parameters())
+        grads.append(torch.autograd.grad(out[:2], [x, u, *params], (dx, du)))
+        size = sum(g.numel() * g.element_size() for g in grads[-1])
+        torch.cuda.synchronize()
+        held.append((base + size - torch.cuda.memory_allocated()) / (T * B * N))
+    assert held[1] < 8.0 and held[0] > 20.0, held
+    for a, b in zip(*grads):
+        assert float((a - b).norm() / a.norm()) < 0.05
+
+
+def gated_config(**kw):
+    from configs.perf_MEM import Config
+    cfg = Config()
+    cfg.hidden_layers = [64, 64]
+    cfg.model = 'RNN_gated'
+    for k, v in kw.items():
+        setattr(cfg, k, v)
+    return cfg
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+def test_model_learns_the_memorisation_task(dev, checkpoint):
+    """The task's 256 random patterns of four classes, as the spiking models train on them."""
+    from delrec.training import mem
+    history, final = mem.run(gated_config(epochs=60, checkpoint8=checkpoint), dev)
+    assert history[0]['loss'] > final['loss'] and final['accuracy_percent'] > 90.0, (history[0], final)
+
+
+@pytest.mark.gpu
+def test_model_steps_are_its_scan(dev):
+    """Streaming gives the sequence's outputs (fp32, the errors of 40 steps and two blocks), also
+    through a captured step."""
+    from delrec.networks import RNN_gated
+    torch.manual_seed(4)
+    model = RNN_gated(gated_config(hidden_layers=[72, 72, 72])).to(dev)
+    x = torch.randn(40, 5, 8, device=dev)
+    with torch.no_grad():
+        want = model(x)
+        state, outs = None, []
+        for t in range(40):
+            y, state = model.step(x[t], state)
+            outs.append(y)
+        torch.testing.assert_close(torch.stack(outs), want, rtol=0, atol=1e-4 * float(want.abs().max()))
+        state = [torch.zeros_like(s) for s in state]
+        slot = x[0].clone()
+        model.step(slot, [s.clone() for s in state])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y, _ = model.step(slot, state)
+        for s in state:
+            s.zero_()
+        for t in range(40):
+            slot.copy_(x[t])
+            graph.replay()
+            torch.cuda.synchronize()
+            torch.testing.assert_close(y, outs[t], rtol=0, atol=0)
+
+
+@pytest.mark.gpu
+def test_model_under_autocast_and_masks(dev):
+    """bf16 activations, an fp32 residual stream, and rows of several lengths: each row's outputs
+    are those of the row alone."""
+    from delrec.networks import RNN_gated
+    torch.manual_seed(5)
+    model = RNN_gated(gated_config()).to(dev)
+    x = torch.randn(50, 3, 8, device=dev)
+    lengths = torch.tensor([50, 17, 1], device=dev)
+    with torch.autocast('cuda', torch.bfloat16):
+        y = model(x, lengths=lengths)
+        y.float().square().mean().backward()
+    full = model(x, lengths=lengths)
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in model.parameters())
+    assert float((y.float() - full).norm() / full.norm()) < 0.05
+    for b, n in enumerate(lengths.tolist()):
+        alone = model(x[:n, b:b + 1])
+        torch.testing.assert_close(full[:n, b:b + 1], alone, rtol=0, atol=1e-4 * float(full.abs().max()))
