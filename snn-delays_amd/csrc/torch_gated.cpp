@@ -3,8 +3,12 @@
 // (include/delrec.h), autograd Functions.
 //
 // In C++ because the smallest calls are bound by the host: a training pass of the scan at T32 B64
-// N64 takes 235 us through Python Functions and the ctypes binding, its kernels 20.
+// N64, whose kernels take 15 us, took 235 us through Python Functions and the ctypes binding. The
+// graph's nodes are torch::autograd::Node themselves: torch::autograd::Function keeps its values in
+// a dictionary of boxed ones.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
@@ -20,7 +24,8 @@ namespace py = pybind11;
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::Node;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = c10::optional<Tensor>;
 
@@ -74,6 +79,31 @@ bool wanted(std::initializer_list<const Tensor*> ts) {
 void once_differentiable(const char* what) {
     if (at::GradMode::is_enabled()) throw std::runtime_error(text(what, " has no second derivative (create_graph=True)"));
 }
+
+// A node of the graph: what it keeps is freed after its backward, and a second backward through it
+// raises torch's own error.
+struct KeptNode : public Node {
+    std::vector<SavedVariable> kept;
+    bool released = false;
+    void keep(std::initializer_list<Tensor> ts) {
+        kept.reserve(ts.size());
+        for (const Tensor& t : ts) kept.emplace_back(t, false);
+    }
+    variable_list take() {
+        if (released) throw std::runtime_error(torch::autograd::ERR_BACKWARD_TWICE);
+        variable_list v;
+        v.reserve(kept.size());
+        for (const SavedVariable& t : kept) v.push_back(t.unpack());
+        return v;
+    }
+    void release_variables() override {
+        kept.clear();
+        released = true;
+    }
+};
+
+template <class N>
+std::shared_ptr<N> make_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
 
 // (R0, R1, N) or (R, N), the last axis contiguous; a copy only where there is no such view
 Tensor rows_form(Tensor t) {
@@ -163,38 +193,27 @@ variable_list scan_forward(const Tensor& z, const Tensor& f, const Tensor& bias,
     return {h, last};
 }
 
-struct GatedScan : public torch::autograd::Function<GatedScan> {
-    static variable_list forward(AutogradContext* ctx, Tensor z, Tensor f, OptTensor bias_, OptTensor h0_,
-                                 OptTensor starts_, OptTensor lengths_, bool checkpoint) {
-        ScanKept kept;
-        const Tensor bias = given(bias_), h0 = given(h0_), starts = given(starts_), lengths = given(lengths_);
-        const Tensor b = vector_arg(bias, z.size(2), z, "bias"), h0c = h0.defined() ? h0.contiguous() : h0;
-        variable_list out = scan_forward(rows_form(z), rows_form(f), b, h0c, starts, lengths, checkpoint, &kept);
-        ctx->save_for_backward({kept.z, kept.f, kept.z8.q, kept.z8.scale, kept.f8.q, kept.f8.scale, b, kept.states,
-                                starts, lengths});
-        ctx->saved_data["T"] = z.size(0);
-        ctx->saved_data["type"] = (int64_t)z.scalar_type();
-        // (the type of db where it is wanted, and whether dh0 is)
-        if (bias.defined() && bias.requires_grad()) ctx->saved_data["db"] = (int64_t)bias.scalar_type();
-        if (h0.defined() && h0.requires_grad()) ctx->saved_data["dh0"] = true;
-        return out;
-    }
+struct GatedScanBackward : public KeptNode {
+    std::string name() const override { return "GatedScanBackward"; }
+    int64_t T = 0;
+    at::ScalarType type = at::kFloat;
 
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list apply(variable_list&& grads) override {
         once_differentiable("gated_scan");
-        const variable_list s = ctx->get_saved_variables();
-        const Tensor &states = s[7], dh = rows_form(grads[0]), dlast = grads[1].contiguous();
+        const variable_list s = take();
+        const Tensor& states = s[7];
         const c10::DeviceGuard guard(states.device());
-        const int T = (int)ctx->saved_data["T"].toInt(), B = (int)states.size(1), N = (int)states.size(2);
-        const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const int B = (int)states.size(1), N = (int)states.size(2);
         const auto f32 = states.options();
+        // an output that nothing used
+        const Tensor dh = grads[0].defined() ? rows_form(grads[0]) : at::zeros({1, 1, N}, f32.dtype(type)).expand({T, B, N});
+        const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
         Tensor dz = at::empty({T, B, N}, f32.dtype(type)), df = at::empty({T, B, N}, f32.dtype(type)), db, dh0;
-        const auto want_db = ctx->saved_data.find("db");
-        if (want_db != ctx->saved_data.end()) db = at::empty({N}, f32);
-        if (ctx->saved_data.count("dh0")) dh0 = at::empty({B, N}, f32);
-        const Tensor ws = workspace(DELREC_WS_GATED_BWD, T, B, N, states);
+        if (task_should_compute_output(2)) db = at::empty({N}, f32);
+        if (task_should_compute_output(3)) dh0 = at::empty({B, N}, f32);
+        const Tensor ws = workspace(DELREC_WS_GATED_BWD, (int)T, B, N, states);
         delrec_gated_scan_bwd_args a{};
-        a.T = T; a.B = B; a.N = N; a.bf16 = type == at::kBFloat16;
+        a.T = (int)T; a.B = B; a.N = N; a.bf16 = type == at::kBFloat16;
         a.z = rows_of(s[0]); a.f = rows_of(s[1]);
         a.z8 = Packed(s[2], s[3]).arg(); a.f8 = Packed(s[4], s[5]).arg();
         a.bias = fptr(s[6]); a.states = fptr(states);
@@ -204,10 +223,27 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
         a.db = fptr(db); a.dh0 = fptr(dh0);
         a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
         check(delrec_gated_scan_bwd(&a, stream_of(states)), "delrec_gated_scan_bwd");
-        if (db.defined()) db = db.to((at::ScalarType)want_db->second.toInt());
-        return {dz, df, db, dh0, Tensor(), Tensor(), Tensor()};
+        return {dz, df, db, dh0};     // (the engine casts db to the bias' type)
     }
 };
+
+variable_list scan_with_graph(const Tensor& z, const Tensor& f, const Tensor& bias, const Tensor& h0, const Tensor& starts,
+                              const Tensor& lengths, bool checkpoint) {
+    auto node = make_node<GatedScanBackward>();
+    node->set_next_edges(torch::autograd::collect_next_edges(z, f, bias, h0));
+    variable_list out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ScanKept kept;
+        const Tensor b = vector_arg(bias, z.size(2), z, "bias"), h0c = h0.defined() ? h0.contiguous() : h0;
+        out = scan_forward(rows_form(z), rows_form(f), b, h0c, starts, lengths, checkpoint, &kept);
+        node->T = z.size(0);
+        node->type = z.scalar_type();
+        node->keep({kept.z, kept.f, kept.z8.q, kept.z8.scale, kept.f8.q, kept.f8.scale, b, kept.states, starts, lengths});
+    }
+    torch::autograd::set_history(out, node);
+    return out;
+}
 
 py::tuple pair_of(const variable_list& v) { return py::make_tuple(v[0], v[1]); }
 
@@ -234,9 +270,7 @@ py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTens
         const Tensor last = h0.defined() ? h0.clone() : at::zeros({B, N}, z.options().dtype(at::kFloat));
         return py::make_tuple(at::zeros_like(z), last);
     }
-    auto opt = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
-    if (wanted({&z, &f, &bias, &h0}))
-        return pair_of(GatedScan::apply(z, f, opt(bias), opt(h0), opt(starts), opt(lengths), checkpoint));
+    if (wanted({&z, &f, &bias, &h0})) return pair_of(scan_with_graph(z, f, bias, h0, starts, lengths, checkpoint));
     return pair_of(scan_forward(rows_form(z), rows_form(f), vector_arg(bias, N, z, "bias"), h0.defined() ? h0.contiguous() : h0,
                                 starts, lengths, false, nullptr));
 }
@@ -287,42 +321,22 @@ variable_list norm_forward(const Tensor& o, const Tensor& g, const Tensor& x, co
     return {xo, u};
 }
 
-struct NormGate : public torch::autograd::Function<NormGate> {
-    static variable_list forward(AutogradContext* ctx, OptTensor o_, OptTensor g_, Tensor x, OptTensor w_, OptTensor scale_,
-                                 OptTensor w2_, double eps, bool checkpoint) {
-        const Tensor o = given(o_), g = given(g_), w = given(w_), scale = given(scale_), w2 = given(w2_);
-        const int64_t N = x.size(-1);
-        NormKept kept;
-        const Tensor wc = vector_arg(w, N, x, "weight"), sc = vector_arg(scale, N, x, "scale"),
-                     w2c = vector_arg(w2, N, x, o.defined() ? "next_weight" : "weight"), xr = rows_form(x);
-        const variable_list out = norm_forward(rows_form(o), rows_form(g), xr, wc, sc, w2c, eps, x.sizes(), checkpoint, &kept);
-        ctx->save_for_backward({kept.o, kept.g, kept.x, kept.o8.q, kept.o8.scale, kept.g8.q, kept.g8.scale, kept.x8.q,
-                                kept.x8.scale, wc, sc, w2c, kept.stats});
-        ctx->set_materialize_grads(false);
-        ctx->saved_data["shape"] = x.sizes();
-        ctx->saved_data["types"] = std::vector<int64_t>{
-            (int64_t)(o.defined() ? o : x).scalar_type(), (int64_t)x.scalar_type(),
-            (int64_t)(w.defined() ? w.scalar_type() : at::kFloat), (int64_t)(scale.defined() ? scale.scalar_type() : at::kFloat),
-            (int64_t)(w2.defined() ? w2.scalar_type() : at::kFloat), xr.size(0), xr.dim() == 3 ? xr.size(1) : 1};
-        variable_list res;
-        for (const Tensor& t : out)
-            if (t.defined()) res.push_back(t);
-        return res;
-    }
+struct NormGateBackward : public KeptNode {
+    std::string name() const override { return "NormGateBackward"; }
+    std::vector<int64_t> shape;
+    at::ScalarType act = at::kFloat, res = at::kFloat;
+    int R0 = 0, R1 = 0;
+    bool block = false;
 
-    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list apply(variable_list&& grads) override {
         once_differentiable("norm_gate_residual");
-        const variable_list s = ctx->get_saved_variables();
+        const variable_list s = take();
         const Tensor &w = s[9], &scale = s[10], &w2 = s[11], &stats = s[12];
-        const bool block = w.defined();
         const Tensor dxo = block ? rows_form(grads[0]) : Tensor();
         const Tensor du = !block ? rows_form(grads[0]) : w2.defined() ? rows_form(grads[1]) : Tensor();
-        if (!dxo.defined() && !du.defined()) return variable_list(8);
+        if (!dxo.defined() && !du.defined()) return variable_list(6);
         const c10::DeviceGuard guard(stats.device());
-        const auto shape = ctx->saved_data["shape"].toIntVector();
-        const auto types = ctx->saved_data["types"].toIntVector();
-        const auto act = (at::ScalarType)types[0], res = (at::ScalarType)types[1];
-        const int R0 = (int)types[5], R1 = (int)types[6], N = (int)shape.back();
+        const int N = (int)shape.back();
         const auto f32 = stats.options();
         Tensor d_o, dg, dw, ds, dw2, dx = at::empty(shape, f32.dtype(res));
         if (block) {
@@ -343,10 +357,35 @@ struct NormGate : public torch::autograd::Function<NormGate> {
         a.dw = fptr(dw); a.dscale = fptr(ds); a.dw2 = fptr(dw2);
         a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
         check(delrec_norm_gate_bwd(&a, stream_of(stats)), "delrec_norm_gate_bwd");
-        auto back = [&](const Tensor& t, int k) { return t.defined() ? t.to((at::ScalarType)types[k]) : t; };
-        return {d_o, dg, dx, back(dw, 2), back(ds, 3), back(dw2, 4), Tensor(), Tensor()};
+        return {d_o, dg, dx, dw, ds, dw2};
     }
 };
+
+variable_list norm_with_graph(const Tensor& o, const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& scale,
+                              const Tensor& w2, double eps, bool checkpoint) {
+    auto node = make_node<NormGateBackward>();
+    node->set_next_edges(torch::autograd::collect_next_edges(o, g, x, w, scale, w2));
+    variable_list out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const int64_t N = x.size(-1);
+        NormKept kept;
+        const Tensor wc = vector_arg(w, N, x, "weight"), sc = vector_arg(scale, N, x, "scale"),
+                     w2c = vector_arg(w2, N, x, o.defined() ? "next_weight" : "weight"), xr = rows_form(x);
+        for (const Tensor& t : norm_forward(rows_form(o), rows_form(g), xr, wc, sc, w2c, eps, x.sizes(), checkpoint, &kept))
+            if (t.defined()) out.push_back(t);
+        node->keep({kept.o, kept.g, kept.x, kept.o8.q, kept.o8.scale, kept.g8.q, kept.g8.scale, kept.x8.q, kept.x8.scale, wc,
+                    sc, w2c, kept.stats});
+        node->shape = x.sizes().vec();
+        node->act = (o.defined() ? o : x).scalar_type();
+        node->res = x.scalar_type();
+        node->R0 = (int)xr.size(0);
+        node->R1 = xr.dim() == 3 ? (int)xr.size(1) : 1;
+        node->block = o.defined();
+    }
+    torch::autograd::set_history(out, node);
+    return out;
+}
 
 // over one column v - e <v e> cancels to eps / x^2 of v, which 32-bit norms do not resolve
 void check_width(const Tensor& x) {
@@ -372,8 +411,7 @@ py::tuple norm_gate_residual(Tensor o, Tensor g, Tensor x, OptTensor w_, OptTens
         return py::make_tuple(y, w2.defined() ? py::cast((y * w2).to(o.scalar_type())) : py::none());
     }
     if (wanted({&o, &g, &x, &w, &scale, &w2})) {
-        const variable_list r = NormGate::apply(OptTensor(o), OptTensor(g), x, OptTensor(w), OptTensor(scale), w2.defined() ? OptTensor(w2) : OptTensor(),
-                                                eps, checkpoint);
+        const variable_list r = norm_with_graph(o, g, x, w, scale, w2, eps, checkpoint);
         return py::make_tuple(r[0], r.size() > 1 ? py::cast(r[1]) : py::none());
     }
     const variable_list r = norm_forward(rows_form(o), rows_form(g), rows_form(x), vector_arg(w, N, x, "weight"),
@@ -387,7 +425,7 @@ Tensor rms_norm(Tensor x, OptTensor w_, double eps, bool checkpoint) {
     check_width(x);
     if (!w.defined()) refuse("weight is needed");
     if (x.numel() == 0) return (x * w).to(x.scalar_type());
-    if (wanted({&x, &w})) return NormGate::apply(OptTensor(), OptTensor(), x, OptTensor(), OptTensor(), OptTensor(w), eps, checkpoint)[0];
+    if (wanted({&x, &w})) return norm_with_graph(Tensor(), Tensor(), x, Tensor(), Tensor(), w, eps, checkpoint)[0];
     return norm_forward(Tensor(), Tensor(), rows_form(x), Tensor(), Tensor(), vector_arg(w, x.size(-1), x, "weight"), eps,
                         x.sizes(), false, nullptr)[1];
 }

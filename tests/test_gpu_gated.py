@@ -678,3 +678,26 @@ def test_model_under_autocast_and_masks(dev):
     for b, n in enumerate(lengths.tolist()):
         alone = model(x[:n, b:b + 1])
         torch.testing.assert_close(full[:n, b:b + 1], alone, rtol=0, atol=1e-4 * float(full.abs().max()))
+
+
+@pytest.mark.gpu
+def test_graph_nodes_keep_and_release(dev):
+    """A second backward needs retain_graph, a changed input is noticed, second derivatives are
+    refused, and a parameter's own type comes back as its gradient's."""
+    from delrec.gated import gated_scan, rms_norm
+    z = torch.randn(70, 2, 8, device=dev, requires_grad=True)
+    f = torch.randn(70, 2, 8, device=dev)
+    bias = torch.zeros(8, device=dev, dtype=BF16, requires_grad=True)
+    h, _ = gated_scan(z, f, bias)
+    first = torch.autograd.grad(h.sum(), (z, bias), retain_graph=True)
+    again = torch.autograd.grad(h.sum(), (z, bias))
+    assert all(torch.equal(a, b) for a, b in zip(first, again)) and first[1].dtype == BF16
+    with pytest.raises(RuntimeError, match='second time'):
+        torch.autograd.grad(h.sum(), z)
+    h, _ = gated_scan(z, f)
+    f.add_(1.0)
+    with pytest.raises(RuntimeError, match='inplace'):
+        torch.autograd.grad(h.sum(), z)
+    u = rms_norm(z, torch.ones(8, device=dev))
+    with pytest.raises(RuntimeError, match='second derivative'):
+        torch.autograd.grad(u.sum(), z, create_graph=True)
