@@ -12,12 +12,14 @@ namespace delrec {
 template <class S>
 __device__ __forceinline__ float to_f32(S v) { return (float)v; }
 
-// k = sigmoid(-x) = 1 / (1 + e^x), through the hardware's 2^x and reciprocal (about 1 ulp each;
-// the product x log2(e) adds 6e-8 |x| relative). k is computed by itself and not as 1 - a: at a
-// leak near 1 that difference would lose the small k's digits.
-__device__ __forceinline__ float gate_in(float x) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * 1.4426950408889634f));
+// k = sigmoid(-x) = 1 / (1 + e^x) from y = x log2(e), through the hardware's 2^y and reciprocal
+// (about 1 ulp each; y's rounding adds 6e-8 |x| relative). k is computed by itself and not as 1 - a:
+// at a leak near 1 that difference would lose the small k's digits.
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float gate_in2(float y) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y));
 }
+__device__ __forceinline__ float gate_in(float x) { return gate_in2(x * kLog2e); }
 
 // V consecutive activations of a row, at any alignment of the element (rows of odd width start
 // anywhere): one access of up to 16 bytes

@@ -88,7 +88,7 @@ template <class T, int V>
 struct Walk {
     const char* base;
     long long pitch;
-    typename std::conditional<V == 1, long long, uint32_t>::type off;
+    typename std::conditional<V == 1, long long, uint32_t>::type off, here;
     uint64_t cur;
     // element (t, b, n) of `data` at t * s0 + b * s1 + n
     __device__ __forceinline__ Walk(const void* data, long long s0, long long s1, int b, int b0, int n)
@@ -97,8 +97,13 @@ struct Walk {
         else off = ((uint32_t)(b - b0) * (uint32_t)s1 + (uint32_t)n) * (uint32_t)sizeof(T);
     }
     __device__ __forceinline__ void seek(int t) { cur = (uint64_t)(base + t * pitch); }
-    // the next step, or the same one again at the end of time (`more` is 0)
-    __device__ __forceinline__ void next(long long more = -1) { cur += pitch & more; }
+    // before a run of accesses: the lane's distance anew, in the basic block that uses it (or the
+    // compiler widens it once and for all and adds it to every base in vector registers)
+    __device__ __forceinline__ void start() {
+        here = off;
+        if constexpr (V > 1) asm("" : "+v"(here));
+    }
+    __device__ __forceinline__ void next() { cur += pitch; }
     __device__ __forceinline__ void prev() { cur -= pitch; }
     // The base is kept apart from the lane's distance (an empty asm, or the compiler adds both into
     // 64-bit lane addresses for all steps ahead, and their registers cost a wave per SIMD).
@@ -109,7 +114,7 @@ struct Walk {
                 (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32;
             asm("" : "+s"(a));
         }
-        return (DELREC_GLOBAL char*)a + off;
+        return (DELREC_GLOBAL char*)a + here;
     }
     template <class E>
     __device__ __forceinline__ E value() const { return *(const DELREC_GLOBAL E*)at(); }
@@ -147,7 +152,8 @@ struct Walk8 {
         : q(p.q, (long long)B * pitch8(N), pitch8(N), b, b0, l.at),
           scale(p.scale, (long long)B * ((N + kGroup8 - 1) / kGroup8), (N + kGroup8 - 1) / kGroup8, b, b0, group), ln(l) {}
     __device__ __forceinline__ void seek(int t) { q.seek(t); scale.seek(t); }
-    __device__ __forceinline__ void next(long long more = -1) { q.next(more); scale.next(more); }
+    __device__ __forceinline__ void start() { q.start(); scale.start(); }
+    __device__ __forceinline__ void next() { q.next(); scale.next(); }
     __device__ __forceinline__ void prev() { q.prev(); scale.prev(); }
     __device__ __forceinline__ Vec8<V> load() const {
         Vec8<V> r;
@@ -163,21 +169,30 @@ struct Walk8 {
     }
 };
 
-// the exchange: wave w's maps for the block, in LDS
+// The exchange: the waves' maps of a block in LDS, a lane's V leaks and V sums in one access. Waves
+// that a short T leaves out of the launch count as maps that change nothing.
 template <int V>
 struct Maps {
-    float A[2][kWaves][64 * V], S[2][kWaves][64 * V];
+    typedef float entry __attribute__((ext_vector_type(2 * V)));
+    entry m[2][kWaves][64];
     __device__ __forceinline__ void put(int buf, int w, int lane, const float* a, const float* s) {
+        entry e;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            A[buf][w][lane * V + j] = a[j];
-            S[buf][w][lane * V + j] = s[j];
-        }
+        for (int j = 0; j < V; ++j) e[j] = a[j], e[V + j] = s[j];
+        m[buf][w][lane] = e;
+    }
+    __device__ __forceinline__ void fill_missing(int w, int nw, int lane) {
+        entry e;
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = 1.0f, e[V + j] = 0.0f;
+        for (int q = nw + w; q < kWaves; q += nw) m[0][q][lane] = m[1][q][lane] = e;
     }
     template <bool MASK>
-    __device__ __forceinline__ void run(int buf, int w, int lane, float* h) const {
+    __device__ __forceinline__ entry run(int buf, int w, int lane, float* h) const {
+        const entry e = m[buf][w][lane];
 #pragma unroll
-        for (int j = 0; j < V; ++j) h[j] = apply<MASK>(A[buf][w][lane * V + j], S[buf][w][lane * V + j], h[j]);
+        for (int j = 0; j < V; ++j) h[j] = apply<MASK>(e[j], e[V + j], h[j]);
+        return e;
     }
 };
 
@@ -201,20 +216,23 @@ __device__ __forceinline__ void enter_range(Maps<V>& m, const float* agg, size_t
     }
     m.put(0, w, lane, A, S);
     barrier_lds();
-    for (int q = 0; q < nw; ++q) m.template run<MASK>(0, q, lane, h);
+#pragma unroll
+    for (int q = 0; q < kWaves; ++q) m.template run<MASK>(0, q, lane, h);
     barrier_lds();                           // the buffer is free again
 }
 
 // One step composed onto a piece's map (A, L), forwards: k out. f and z are vectors of any kind
-// that get() reads.
+// that get() reads, bias2 the bias times log2(e).
 template <int V, bool MASK, class F>
-__device__ __forceinline__ void step_forward(const F& f, const F& z, const float* bias, bool fresh, float* k, float* A, float* L) {
+__device__ __forceinline__ void step_forward(const F& f, const F& z, const float* bias2, bool fresh, float* k, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        k[j] = gate_in(f.get(j) + bias[j]);
-        const float from = MASK && fresh ? 0.0f : L[j], a = A[j] * (1.0f - k[j]);
+        k[j] = gate_in2(fmaf(f.get(j), kLog2e, bias2[j]));
+        const float from = MASK && fresh ? 0.0f : L[j];
         L[j] = fmaf(k[j], z.get(j) - from, from);
-        A[j] = MASK && fresh ? -1.0f : a;
+        // (the product keeps a cut's sign also for a leak of 0, where the fma gives +0)
+        if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
+        else A[j] = fmaf(-k[j], A[j], A[j]);
     }
 }
 
@@ -223,15 +241,16 @@ template <int V, bool MASK, class D>
 __device__ __forceinline__ void step_backward(const float* k, const D& dh, bool fresh, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float a = 1.0f - k[j], l = a * (dh.get(j) + L[j]), m = A[j] * a;
+        const float x = dh.get(j) + L[j], l = fmaf(-k[j], x, x);
         L[j] = MASK && fresh ? 0.0f : l;
-        A[j] = MASK && fresh ? -1.0f : m;
+        if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
+        else A[j] = fmaf(-k[j], A[j], A[j]);
     }
 }
 
-// Padding. A wave whose lanes are all past their rows' lengths loads nothing and leaves the state
-// alone; where only some are, these lanes' inputs are replaced, whatever they hold: z and dh by 0
-// and f by a gate that lets nothing in (k = 0).
+// Padding, and the steps past T of the last block. A wave whose lanes are all past their rows' ends
+// loads nothing and leaves the state alone; where only some are, or some of the steps, their inputs
+// are replaced, whatever they hold: z and dh by 0 and f by a gate that lets nothing in (k = 0).
 template <class S, int V>
 __device__ __forceinline__ void blank(Vec<S, V>& x, float v) {
     if constexpr (V > 1) {
@@ -248,25 +267,26 @@ __device__ __forceinline__ void blank(Vec8<V>& x, float v) {
 }
 constexpr float kShut = 1e38f;
 
-// The map of the pieces before this wave's, applied to h (in the order of DIR), and of all of them.
-// All reads are under way before the first is used.
+// The maps of all waves applied to h in the order of DIR, what comes before this wave's own in
+// `mine`. All reads are under way before the first is used.
 template <int V, bool MASK, int DIR>
-__device__ __forceinline__ void compose(const Maps<V>& m, int buf, int w, int nw, int lane, float* h, float* mine) {
+__device__ __forceinline__ void compose(const Maps<V>& m, int buf, int w, int lane, float* h, float* mine) {
 #pragma unroll
     for (int c = 0; c < kWaves; ++c) {
         const int q = DIR > 0 ? c : kWaves - 1 - c;
-        if (q < nw) {
+        if (q == w) {
+            asm volatile("");                // a branch (w is the wave's), not two selects a wave
 #pragma unroll
-            for (int j = 0; j < V; ++j) mine[j] = q == w ? h[j] : mine[j];
-            m.template run<MASK>(buf, q, lane, h);
+            for (int j = 0; j < V; ++j) mine[j] = h[j];
         }
+        m.template run<MASK>(buf, q, lane, h);
     }
 }
 
 }  // namespace
 
-// Steps past T load the last one again (no branch between the loads) and are left out afterwards, by
-// tests that the whole wave shares.
+// (a block's loads come in two forms: without a branch between them, and with a test each where the
+// last steps are past T)
 #define DELREC_STEPS(s) _Pragma("unroll") for (int s = 0; s < kSteps; ++s)
 #define DELREC_STEPS_BACK(s) _Pragma("unroll") for (int s = kSteps - 1; s >= 0; --s)
 #define DELREC_COLS(j) _Pragma("unroll") for (int j = 0; j < V; ++j)
@@ -288,9 +308,10 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
     const int len = MASK ? row_length(p, b) : T;
     float bias[V], h[V];
     DELREC_COLS(j) {
-        bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
+        bias[j] = p.bias ? p.bias[n0 + j] * kLog2e : 0.0f;
         h[j] = p.h0 ? p.h0[at + j] : 0.0f;
     }
+    maps.fill_missing(w, nw, lane);
     if (blockIdx.y) enter_range<V, MASK>(maps, p.ws, plane, at, 0, 1, blockIdx.y, w, nw, lane, h);
 
     int buf = 0;
@@ -301,26 +322,32 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
         float k[kSteps][V], A[V], L[V], g[V];
         bool fresh[kSteps];
         DELREC_COLS(j) A[j] = 1.0f, L[j] = g[j] = 0.0f;
-        const bool any = MASK ? __any(t0 < len) : t0 < T, part = MASK && !__all(t0 + kSteps <= len);
-        if (any) {
+        const bool any = MASK ? __any(t0 < len) : t0 < len, part = MASK ? !__all(t0 + kSteps <= len) : t0 + kSteps > len;
+        if (!MASK || any) {
             zp.seek(t0), fp.seek(t0);
             if (MASK) sp.seek(t0);
-            DELREC_STEPS(s) {
-                const long long more = t0 + s + 1 < T ? -1 : 0;
-                f[s] = fp.load(), z[s] = zp.load();
-                fp.next(more), zp.next(more);
-                fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
-                if (MASK) sp.next(more);
-            }
+            auto load = [&](auto full) {
+                fp.start(), zp.start();
+                if (MASK) sp.start();
+                DELREC_STEPS(s) {
+                    fresh[s] = false;
+                    if (decltype(full)::value || t0 + s < T) {
+                        f[s] = fp.load(), z[s] = zp.load();
+                        fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+                        fp.next(), zp.next();
+                        if (MASK) sp.next();
+                    }
+                }
+            };
+            t0 + kSteps <= T ? load(std::true_type()) : load(std::false_type());
             if (part) DELREC_STEPS(s)
                 if (t0 + s >= len) blank(z[s], 0.0f), blank(f[s], kShut), fresh[s] = false;
-            DELREC_STEPS(s) {
-                if (t0 + s < T) step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
-            }
+            DELREC_STEPS(s) step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
         }
         maps.put(buf, w, lane, A, L);
         if (PACK && any) {
             z8.seek(t0), f8.seek(t0);
+            z8.start(), f8.start();
             DELREC_STEPS(s) {
                 if (t0 + s < T) {
                     float v[V];
@@ -333,22 +360,22 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
             }
         }
         barrier_lds();
-        compose<V, MASK, 1>(maps, buf, w, nw, lane, h, g);
-        yp.seek(t0);
+        compose<V, MASK, 1>(maps, buf, w, lane, h, g);
+        if (MASK && !any) DELREC_STEPS(s) {
+            blank(z[s], 0.0f);
+            DELREC_COLS(j) k[s][j] = 0.0f;
+            fresh[s] = false;
+        }
+        yp.seek(t0), yp.start();
         DELREC_STEPS(s) {
-            if (t0 + s < T) {
-                float y[V];
-                DELREC_COLS(j) y[j] = 0.0f;
-                if (any) {
-                    DELREC_COLS(j) {
-                        const float from = MASK && fresh[s] ? 0.0f : g[j];
-                        y[j] = g[j] = fmaf(k[s][j], z[s].get(j) - from, from);
-                    }
-                    if (part && t0 + s >= len) DELREC_COLS(j) y[j] = 0.0f;
-                }
-                if (ln.on) yp.store(y);
-                yp.next();
+            float y[V];
+            DELREC_COLS(j) {
+                const float from = MASK && fresh[s] ? 0.0f : g[j];
+                y[j] = g[j] = fmaf(k[s][j], z[s].get(j) - from, from);
             }
+            if (MASK && part && t0 + s >= len) DELREC_COLS(j) y[j] = 0.0f;
+            if (t0 + s < T && ln.on) yp.store(y);
+            yp.next();
         }
     }
     if (w == 0 && ln.on && te == T) vstore<float, V>(p.h_last + at, h);
@@ -373,7 +400,7 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
     const int len = MASK ? row_length(p, b) : T;
     float bias[V], A[V], L[V];
     DELREC_COLS(j) {
-        bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
+        bias[j] = p.bias ? p.bias[n0 + j] * kLog2e : 0.0f;
         A[j] = 1.0f;
         L[j] = 0.0f;
     }
@@ -382,32 +409,39 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
         typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps];
         Vec<S, V> v[kSteps];
         bool fresh[kSteps];
-        if (MASK ? !__any(t0 < len) : t0 >= T) continue;
-        const bool part = MASK && !__all(t0 + kSteps <= len);
+        if (MASK ? !__any(t0 < len) : t0 >= len) continue;
+        const bool part = MASK ? !__all(t0 + kSteps <= len) : t0 + kSteps > len;
         if constexpr (PACK) fp8.seek(t0);
         else fp.seek(t0);
         xp.seek(t0);
         if (MASK) sp.seek(t0);
-        DELREC_STEPS(s) {
-            const long long more = t0 + s + 1 < T ? -1 : 0;
-            if constexpr (PACK) f[s] = fp8.load(), fp8.next(more);
-            else f[s] = fp.load(), fp.next(more);
-            v[s] = xp.load(), xp.next(more);
-            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
-            if (MASK) sp.next(more);
-        }
+        auto load = [&](auto full) {
+            if constexpr (PACK) fp8.start();
+            else fp.start();
+            xp.start();
+            if (MASK) sp.start();
+            DELREC_STEPS(s) {
+                fresh[s] = false;
+                if (decltype(full)::value || t0 + s < T) {
+                    if constexpr (PACK) f[s] = fp8.load(), fp8.next();
+                    else f[s] = fp.load(), fp.next();
+                    v[s] = xp.load(), xp.next();
+                    fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+                    if (MASK) sp.next();
+                }
+            }
+        };
+        t0 + kSteps <= T ? load(std::true_type()) : load(std::false_type());
         if (part) DELREC_STEPS(s)
             if (t0 + s >= len) blank(v[s], 0.0f), blank(f[s], kShut), fresh[s] = false;
         DELREC_STEPS(q) {
             const int s = BWD ? kSteps - 1 - q : q;
-            if (t0 + s < T) {
-                float k[V];
-                if constexpr (BWD) {
-                    DELREC_COLS(j) k[j] = gate_in(f[s].get(j) + bias[j]);
-                    step_backward<V, MASK>(k, v[s], fresh[s], A, L);
-                } else {
-                    step_forward<V, MASK>(f[s], v[s], bias, fresh[s], k, A, L);
-                }
+            float k[V];
+            if constexpr (BWD) {
+                DELREC_COLS(j) k[j] = gate_in2(fmaf(f[s].get(j), kLog2e, bias[j]));
+                step_backward<V, MASK>(k, v[s], fresh[s], A, L);
+            } else {
+                step_forward<V, MASK>(f[s], v[s], bias, fresh[s], k, A, L);
             }
         }
     }
@@ -417,8 +451,8 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
     DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
     for (int c = 0; c < nw; ++c) {
         const int q = BWD ? nw - 1 - c : c;
-        maps.template run<MASK>(0, q, lane, L);
-        DELREC_COLS(j) A[j] = product<MASK>(A[j], maps.A[0][q][lane * V + j]);
+        const auto e = maps.template run<MASK>(0, q, lane, L);
+        DELREC_COLS(j) A[j] = product<MASK>(A[j], e[j]);
     }
     float* a = p.ws + (size_t)y * 2 * plane + at;
     vstore_own<float, V>(a, A, PACK ? ln.skip : 0);
@@ -444,10 +478,12 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
     const int len = MASK ? row_length(p, b) : T;
     float bias[V], c[V], db[V];
     DELREC_COLS(j) {
-        bias[j] = p.bias ? p.bias[n0 + j] : 0.0f;
+        bias[j] = p.bias ? p.bias[n0 + j] * kLog2e : 0.0f;
         c[j] = p.dlast ? p.dlast[at + j] : 0.0f;
         db[j] = 0.0f;
     }
+    fmap.fill_missing(w, nw, lane);
+    rmap.fill_missing(w, nw, lane);
     const int last = gridDim.y - 1;
     if ((int)blockIdx.y < last)
         enter_range<V, MASK>(rmap, p.ws, plane, at, last, -1, last - blockIdx.y, w, nw, lane, c);
@@ -457,75 +493,78 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
         const int t0 = tb + w * kSteps;
         float k[kSteps][V], d[kSteps][V], h[V], g[V], mine[V];
         Vec<S, V> dh[kSteps];
+        typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type z[kSteps];
         bool fresh[kSteps];
         const auto st = vload<float, V>(p.states + (size_t)(tb / kBlk) * plane + at);
         DELREC_COLS(j) h[j] = st.get(j), g[j] = mine[j] = 0.0f;
-        const bool any = MASK ? __any(t0 < len) : t0 < T, part = MASK && !__all(t0 + kSteps <= len);
+        const bool any = MASK ? __any(t0 < len) : t0 < len, part = MASK ? !__all(t0 + kSteps <= len) : t0 + kSteps > len;
         {
             float A[V], L[V];
-            typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps], z[kSteps];
-            if (any) {
+            typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type f[kSteps];
+            if (!MASK || any) {
                 if constexpr (PACK) z8.seek(t0), f8.seek(t0);
                 else zp.seek(t0), fp.seek(t0);
                 dhp.seek(t0);
                 if (MASK) sp.seek(t0);
-                DELREC_STEPS(s) {
-                    const long long more = t0 + s + 1 < T ? -1 : 0;
-                    if constexpr (PACK) f[s] = f8.load(), z[s] = z8.load(), f8.next(more), z8.next(more);
-                    else f[s] = fp.load(), z[s] = zp.load(), fp.next(more), zp.next(more);
-                    dh[s] = dhp.load(), dhp.next(more);
-                    fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
-                    if (MASK) sp.next(more);
-                }
+                auto load = [&](auto full) {
+                    if constexpr (PACK) f8.start(), z8.start();
+                    else fp.start(), zp.start();
+                    dhp.start();
+                    if (MASK) sp.start();
+                    DELREC_STEPS(s) {
+                        fresh[s] = false;
+                        if (decltype(full)::value || t0 + s < T) {
+                            if constexpr (PACK) f[s] = f8.load(), z[s] = z8.load(), f8.next(), z8.next();
+                            else f[s] = fp.load(), z[s] = zp.load(), fp.next(), zp.next();
+                            dh[s] = dhp.load(), dhp.next();
+                            fresh[s] = MASK && p.starts && sp.template value<uint8_t>();
+                            if (MASK) sp.next();
+                        }
+                    }
+                };
+                t0 + kSteps <= T ? load(std::true_type()) : load(std::false_type());
                 if (part) DELREC_STEPS(s)
                     if (t0 + s >= len) blank(z[s], 0.0f), blank(f[s], kShut), blank(dh[s], 0.0f), fresh[s] = false;
             }
             DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-            if (any) DELREC_STEPS(s) {
-                if (t0 + s < T) {
-                    step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
-                    DELREC_COLS(j) d[s][j] = z[s].get(j);
-                }
-            }
+            if (!MASK || any) DELREC_STEPS(s) step_forward<V, MASK>(f[s], z[s], bias, fresh[s], k[s], A, L);
             fmap.put(buf, w, lane, A, L);
             DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-            if (any) DELREC_STEPS_BACK(s) {
-                if (t0 + s < T) step_backward<V, MASK>(k[s], dh[s], fresh[s], A, L);
-            }
+            if (!MASK || any) DELREC_STEPS_BACK(s) step_backward<V, MASK>(k[s], dh[s], fresh[s], A, L);
             rmap.put(buf, w, lane, A, L);
         }
         barrier_lds();
-        compose<V, MASK, -1>(rmap, buf, w, nw, lane, c, g);
-        compose<V, MASK, 1>(fmap, buf, w, nw, lane, h, mine);
+        compose<V, MASK, -1>(rmap, buf, w, lane, c, g);
+        // (one exchange's reads at a time: both at once are 64 registers)
+        __builtin_amdgcn_sched_barrier(0);
+        compose<V, MASK, 1>(fmap, buf, w, lane, h, mine);
         float blk[V];
-        // d: z_t becomes h_{t-1} - z_t
-        if (any) DELREC_STEPS(s) {
-            if (t0 + s < T) {
-                DELREC_COLS(j) {
-                    const float from = MASK && fresh[s] ? 0.0f : mine[j];
-                    d[s][j] = from - d[s][j];
-                    mine[j] = fmaf(-k[s][j], d[s][j], from);
-                }
-            }
-        }
         DELREC_COLS(j) blk[j] = 0.0f;
+        if (MASK && !any) DELREC_STEPS(s) {
+            blank(dh[s], 0.0f);
+            blank(z[s], 0.0f);
+            DELREC_COLS(j) k[s][j] = 0.0f;
+            fresh[s] = false;
+        }
+        // d_t = h_{t-1} - z_t
+        DELREC_STEPS(s) DELREC_COLS(j) {
+            const float from = MASK && fresh[s] ? 0.0f : mine[j];
+            d[s][j] = from - z[s].get(j);
+            mine[j] = fmaf(-k[s][j], d[s][j], from);
+        }
+        // (k = 0 outside a row: its gradients come as zeros)
         dzp.seek(t0 + kSteps - 1), dfp.seek(t0 + kSteps - 1);
+        dzp.start(), dfp.start();
         DELREC_STEPS_BACK(s) {
-            if (t0 + s < T) {
-                float oz[V], of[V];
-                DELREC_COLS(j) oz[j] = of[j] = 0.0f;
-                if (any) {
-                    DELREC_COLS(j) {
-                        const float a = 1.0f - k[s][j], lam = dh[s].get(j) + g[j], back = a * lam;
-                        oz[j] = lam * k[s][j];
-                        of[j] = oz[j] * a * d[s][j];
-                        g[j] = MASK && fresh[s] ? 0.0f : back;
-                    }
-                    if (part && t0 + s >= len) DELREC_COLS(j) oz[j] = of[j] = 0.0f;
-                    DELREC_COLS(j) blk[j] += of[j];
-                }
-                if (ln.on) dzp.store(oz, own), dfp.store(of, own);
+            float oz[V], of[V];
+            DELREC_COLS(j) {
+                const float lam = dh[s].get(j) + g[j];
+                oz[j] = lam * k[s][j];
+                of[j] = fmaf(-k[s][j], oz[j], oz[j]) * d[s][j];
+                g[j] = MASK && fresh[s] ? 0.0f : lam - oz[j];
+                blk[j] += of[j];
             }
+            if (t0 + s < T && ln.on) dzp.store(oz, own), dfp.store(of, own);
             dzp.prev(), dfp.prev();
         }
         // the bias sum in two levels, within a block and over blocks: one long chain of 32-bit
@@ -539,7 +578,7 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
     __syncthreads();
     if (w || !ln.on) return;
     for (int q = 1; q < nw; ++q)
-        DELREC_COLS(j) db[j] += rmap.S[0][q][lane * V + j];
+        DELREC_COLS(j) db[j] += rmap.m[0][q][lane][j];
     vstore_own<float, V>(dbpart + (size_t)blockIdx.y * plane + at, db, own);
 }
 
