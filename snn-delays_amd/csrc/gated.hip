@@ -14,9 +14,10 @@
 // inputs once more), the second starts from the composition of the ranges before it.
 //
 // Bound by memory where the channels fill the GPU: at T250 B128 N512 bf16 23 us forward (98 MB,
-// 4.2 TB/s) and 35 backward (164 MB, 4.7 TB/s, what a large copy reaches). A block's loads are not
-// taken ahead of the one before: two to four workgroups a CU hide them, and their registers cost
-// one of these.
+// 4.3 TB/s) and 34 backward (164 MB, 4.8 TB/s, what a large copy reaches); next, by vector issue
+// (some 45 instructions a value backward, two of them at a quarter of the rate). A block's loads are
+// not taken ahead of the one before: two to four workgroups a CU hide them, and their registers
+// cost one of these.
 //
 // The forward keeps the state before every 64th step in 32 bits (1/16 byte a value and step); the
 // backward starts its blocks there and recomputes the states between from z and f, which it needs
@@ -588,17 +589,17 @@ struct Plan {
     int V, per_row, groups, waves, range, ranges;
 };
 
-// Two columns a lane. Four (one access of 8 bytes for bf16, not 4) have the same bytes under way
-// but half the workgroups and, in the backward, 160 registers and 3 waves a SIMD: 480 us for
-// T1024 B64 N2048 with 8 bits, 290 with two; 55 and 35 us for T250 B128 N512. One (rows of one
-// column, and offsets past 32 bits): 548 and 66 us.
+// Two columns a lane. Four have the same bytes under way in half the workgroups, and the backward's
+// registers (k, z, dh of eight steps) do not fit 128: forward and backward of T1024 B64 N2048 with 8
+// bits take 275 + 674 us with four, 313 + 271 with two, 401 + 347 with one; of T250 B128 N512 26 + 64,
+// 23 + 34, 24 + 39. One for rows of one column and for offsets past 32 bits.
 //
 // Time over the grid where the channels give less than a workgroup a CU: each range's inputs are
-// then read twice, and at T1000 N512 bf16 the forward and backward take 124 us whole and 85 in
-// four ranges for B 32 (128 workgroups), 150 and 158 for B 64 (256). As many ranges as make one
-// round of two workgroups a CU (T16384 B2 N700 fp32: 234 us with 43 ranges = 473 workgroups, 253
-// with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 186 us with 3
-// ranges, 135 with 6).
+// then read twice. T1000 N512 bf16, forward and backward, whole and in ranges: B 32 (128
+// workgroups) 103 and 81 us, B 48 (192) 117 and 118, B 64 (256) 127 and 136. As many ranges as make
+// one round of two workgroups a CU (T16384 B2 N700 fp32: 241 us with 22 ranges, 234 with 43, 237
+// with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 174 us with 3
+// ranges, 143 with 4, 128 with 6).
 Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
     Plan q;
     q.V = N >= 2 && !wide ? 2 : 1;
