@@ -701,3 +701,43 @@ def test_graph_nodes_keep_and_release(dev):
     u = rms_norm(z, torch.ones(8, device=dev))
     with pytest.raises(RuntimeError, match='second derivative'):
         torch.autograd.grad(u.sum(), z, create_graph=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+def test_more_than_2_to_32_values(dev, checkpoint):
+    """Tensors past 2^32 values (and bytes, and odd rows): the far end of each against the same
+    channels or rows by themselves, bit for bit."""
+    from delrec.checkpoint8 import pack8, unpack8
+    from delrec.gated import gated_scan, norm_gate_residual
+    T, B, N = 66, 2, 33_000_001
+    cut = (N // 64 - 1) * 64                 # whole 8-bit groups
+    gen = torch.Generator(device=dev).manual_seed(1)
+
+    def fill(*shape):
+        return torch.empty(*shape, dtype=BF16, device=dev).normal_(generator=gen)
+    z, f, dh = (fill(T, B, N) for _ in range(3))
+    bias = torch.rand(N, device=dev, generator=gen) * 6
+
+    def both(z, f, bias, dh):
+        leaves = [t.detach().requires_grad_(True) for t in (z, f)]
+        h, last = gated_scan(*leaves, bias, checkpoint=checkpoint)
+        return h.detach(), last.detach(), *torch.autograd.grad(h, leaves, dh)
+    far = both(*(t[:, 1:, cut:].contiguous() for t in (z, f)), bias[cut:].contiguous(), dh[:, 1:, cut:].contiguous())
+    whole = both(z, f, bias, dh)
+    for a, b in zip(whole, far):
+        assert torch.equal(a[..., 1:, cut:], b)
+    del whole, z, f, dh
+    R, N = 2_150_000, 2001
+    o, g, x, dx = (fill(R, N) for _ in range(4))
+    w = torch.rand(N, device=dev, generator=gen) + 0.5
+    rows = slice(R - 5, R)
+
+    def norms(o, g, x, dx):
+        leaves = [t.detach().requires_grad_(True) for t in (o, g, x)]
+        y, u = norm_gate_residual(*leaves, w, w, w, checkpoint=checkpoint)
+        return y.detach(), u.detach(), *torch.autograd.grad((y, u), leaves, (dx, dx))
+    far = norms(*(t[rows].clone() for t in (o, g, x, dx)))
+    for a, b in zip(norms(o, g, x, dx), far):
+        assert torch.equal(a[rows], b)
+    assert torch.equal(unpack8(pack8(o))[rows], unpack8(pack8(o[rows].clone())))
