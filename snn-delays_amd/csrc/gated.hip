@@ -599,7 +599,9 @@ struct Plan {
 // workgroups) 103 and 81 us, B 48 (192) 117 and 118, B 64 (256) 127 and 136. As many ranges as make
 // one round of two workgroups a CU (T16384 B2 N700 fp32: 241 us with 22 ranges, 234 with 43, 237
 // with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 174 us with 3
-// ranges, 143 with 4, 128 with 6).
+// ranges, 143 with 4, 128 with 6). From five blocks on, a block a range at the least: B20 N333 bf16
+// whole and in ranges 20 and 25 us at T 128, 34 and 31 (and two more launches) at T 256, 41 and 31
+// at T 320.
 Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
     Plan q;
     q.V = N >= 2 && !wide ? 2 : 1;
@@ -607,8 +609,8 @@ Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
     q.groups = (int)(((long long)B * q.per_row + 63) / 64);
     q.waves = T >= kBlk ? kWaves : (T + kSteps - 1) / kSteps;
     const int blocks = (T + kBlk - 1) / kBlk;
-    int want = q.groups >= 256 ? 1 : (mask ? 1024 : 512) / q.groups;
-    want = std::max(1, std::min({want, 128, blocks / 2}));
+    int want = q.groups >= 256 || blocks < 5 ? 1 : (mask ? 1024 : 512) / q.groups;
+    want = std::max(1, std::min({want, 128, blocks}));
     const int per = (blocks + want - 1) / want;
     q.range = per * kBlk;
     q.ranges = (blocks + per - 1) / per;
