@@ -7,11 +7,11 @@
 //     dw2 = sum du e2,  dscale = sum dx y,  dw = sum dn e       (sums over the rows).
 //
 // Bound by memory: a row stays in registers between its loads and its stores, the two row sums
-// are exchanges between its lanes. A row is 16, 64, 256 or 512 lanes, each with NE vectors of
-// four columns, as few lanes as hold it in at most four vectors (16 lanes: four rows a wave, no
-// LDS): forward 31 us for 32000 x 512 bf16 (5.3 TB/s). The backward recomputes x', e and the gate from o, g and x (or their 8 bits) and the two
-// kept norms: one residual tensor is read, not two. Its column sums stay in registers over all the
-// rows a workgroup takes; the workgroups' sums are added in a second launch, in a fixed order.
+// are exchanges between its lanes. A row is 16, 64, 256 or 512 lanes, each with up to four vectors of
+// four columns (16 lanes: four rows a wave, no LDS): forward 31 us for 32000 x 512 bf16 (5.2 TB/s).
+// The backward recomputes x', e and the gate from o, g and x (or their 8 bits) and the two kept
+// norms: one residual tensor is read, not two. Its column sums stay in registers over all the rows
+// a workgroup takes; the workgroups' sums are added in a second launch, in a fixed order.
 #include <algorithm>
 #include <initializer_list>
 
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_fwd_kernel(NormGate 
     }
 }
 
-// PACK: o, g and x from their 8 bits. Up to two vectors a lane (N 2048), a row's values are loaded
+// PACK: o, g and x from their 8 bits. Up to two vectors a lane (N 4096), a row's values are loaded
 // while the one before is computed, and the three column vectors are in LDS, read again in each
 // half of a row. Each row's loads waited for in place, the columns in registers: 77 us for 32000 x
 // 512 bf16 and 660 for 65536 x 2048 with 8 bits; so 50 (5.3 TB/s) and 485 (4.7 TB/s). With four
@@ -545,8 +545,13 @@ namespace {
 
 bool in_registers(int N) { return N >= 4 && N <= 8192; }
 
-// (lanes of a row, vectors of a lane). The backward holds three more rows and the column sums:
-// two vectors a lane up to 2048 columns.
+// (lanes of a row, vectors of a lane): the fewest lanes that hold the row in two vectors; four where
+// a wave or 512 lanes then do without more waves. Forward and backward of 33.5 million bf16 values
+// in us, this plan's form and the next: N 64 66 + 102 with 16 lanes (192 + 293 with 64), N 128 63 +
+// 106 with 16 x 2 (95 + 150 with 64), N 512 63 + 107 with 64 x 2 (115 + 156 with 256), N 1000 forward
+// 61 with 64 x 4 (73 with 256), backward 112 with 256 (139 with 64 x 4, whose column sums leave no
+// registers), N 2048 63 + 105 with 256 x 2 (71 + 101 with 512), N 4096 70 + 117 with 512 x 2 (68 + 146
+// with 256 x 4), N 8192 101 + 137 (219 + 2243 as rows of any width).
 struct RowPlan {
     int lanes, vecs, rpw;
 };
@@ -558,7 +563,7 @@ RowPlan row_plan(int N, bool fwd) {
     else if (N <= 512) q = {64, 2};
     else if (N <= 1024) q = fwd ? RowPlan{64, 4} : RowPlan{256, 1};
     else if (N <= 2048) q = {256, 2};
-    else if (N <= 4096) q = {256, 4};
+    else if (N <= 4096) q = {512, 2};
     else q = {512, 4};
     q.rpw = q.lanes < 256 ? 256 / q.lanes : 1;
     return q;
@@ -626,14 +631,14 @@ int run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
     if (fwd) {
         if (q.lanes == 16) q.vecs == 1 ? run_fwd<S, X, 16, 1>(p, stream) : run_fwd<S, X, 16, 2>(p, stream);
         else if (q.lanes == 64) q.vecs == 1 ? run_fwd<S, X, 64, 1>(p, stream) : q.vecs == 2 ? run_fwd<S, X, 64, 2>(p, stream) : run_fwd<S, X, 64, 4>(p, stream);
-        else if (q.lanes == 256) q.vecs == 2 ? run_fwd<S, X, 256, 2>(p, stream) : run_fwd<S, X, 256, 4>(p, stream);
-        else run_fwd<S, X, 512, 4>(p, stream);
+        else if (q.lanes == 256) run_fwd<S, X, 256, 2>(p, stream);
+        else q.vecs == 2 ? run_fwd<S, X, 512, 2>(p, stream) : run_fwd<S, X, 512, 4>(p, stream);
         return 0;
     }
     if (q.lanes == 16) return q.vecs == 1 ? run_bwd<S, X, 16, 1>(p, stream) : run_bwd<S, X, 16, 2>(p, stream);
     if (q.lanes == 64) return q.vecs == 1 ? run_bwd<S, X, 64, 1>(p, stream) : run_bwd<S, X, 64, 2>(p, stream);
-    if (q.lanes == 512) return run_bwd<S, X, 512, 4>(p, stream);
-    return q.vecs == 1 ? run_bwd<S, X, 256, 1>(p, stream) : q.vecs == 2 ? run_bwd<S, X, 256, 2>(p, stream) : run_bwd<S, X, 256, 4>(p, stream);
+    if (q.lanes == 256) return q.vecs == 1 ? run_bwd<S, X, 256, 1>(p, stream) : run_bwd<S, X, 256, 2>(p, stream);
+    return q.vecs == 2 ? run_bwd<S, X, 512, 2>(p, stream) : run_bwd<S, X, 512, 4>(p, stream);
 }
 
 }  // namespace

@@ -94,6 +94,9 @@ __global__ void __launch_bounds__(256) pack8_kernel(Pack8 p) {
     }
 }
 
+// The fewest lanes, 16, 64 or 256, that hold a row's groups: packing and unpacking of 33.5 million bf16
+// values take 20 + 16 us so; N 64 with 64 lanes 52 + 36, N 256 with 256 40 + 25 and with 16 22 + 21,
+// N 2048 with 64 21 + 18.
 template <class S, bool PACK>
 static void run_pack8(const Pack8& p, hipStream_t stream) {
     const long long rows = (long long)p.R0 * p.R1;

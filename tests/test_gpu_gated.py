@@ -267,7 +267,7 @@ def ref_norm(c, checkpoint=False, eps=1e-6):
 @pytest.mark.parametrize('checkpoint', [False, True])
 @pytest.mark.parametrize('dtype,resid', [(FP32, FP32), (BF16, BF16), (BF16, FP32)])
 @pytest.mark.parametrize('shape', [(3, 2), (5, 3), (7, 64), (33, 65), (4, 5, 127), (9, 3, 256), (600, 260),
-                                   (17, 700), (6, 1500), (5, 2049), (3, 5000), (2, 17000)])
+                                   (17, 700), (6, 1500), (5, 2049), (3, 5000), (4, 4099), (9, 4096), (2, 17000)])
 def test_norm_gate_forward_and_gradients(dev, shape, dtype, resid, checkpoint):
     c = norm_case(shape, dtype, resid)
     got, ref = run_norm(c, dev, checkpoint), ref_norm(c, checkpoint)
