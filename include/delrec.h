@@ -342,7 +342,8 @@ typedef struct {
 /* x' = x + scale * (o r w) * silu(g), r = 1/sqrt(mean o^2 + eps), and u = x' r2 w2, r2 =
  * 1/sqrt(mean x'^2 + eps) (of x' before it is rounded), over R0 * R1 rows of N >= 2. w2 NULL: no u.
  * o.data NULL: no block, u = x r2 w2 alone (x_out not written). stats keeps r and r2 for the
- * backward pass; o8 / g8 / x8 keep the inputs in 8 bits. */
+ * backward pass; o8, g8 and x8 (all three, or none; without a block x8 alone, or none) keep the
+ * inputs in 8 bits. */
 typedef struct {
     int32_t R0, R1, N, bf16, x_bf16;   /* bf16: o, g, u; x_bf16: x, x_out                  */
     delrec_rows o, g, x;
@@ -358,7 +359,7 @@ typedef struct {
 
 typedef struct {
     int32_t R0, R1, N, bf16, x_bf16;
-    delrec_rows o, g, x;         /* as the forward's, not read where the 8-bit form is given */
+    delrec_rows o, g, x;         /* as the forward's, not read with the 8-bit forms        */
     delrec_packed8 o8, g8, x8;
     const float* w;
     const float* scale;

@@ -18,6 +18,13 @@ bool sizes_ok(int R0, int R1, int N) {
 
 bool pair_ok(const delrec_packed8& p) { return (p.q == nullptr) == (p.scale == nullptr); }
 
+// the norms' 8-bit forms: of o, g and x together, of x alone without a block, or none (the kernels
+// go by x8)
+bool eights_ok(const delrec_packed8& o8, const delrec_packed8& g8, const delrec_packed8& x8, bool block) {
+    const bool others = block && x8.q;
+    return pair_ok(o8) && pair_ok(g8) && pair_ok(x8) && (o8.q != nullptr) == others && (g8.q != nullptr) == others;
+}
+
 }  // namespace
 
 extern "C" {
@@ -73,8 +80,8 @@ int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream) {
     const bool block = a->o.data != nullptr;
     if (!a->x.data || !(a->eps >= 0.0f) || (a->w2 && !a->u)) return DELREC_ERR_ARG;
     if (block && (!a->g.data || !a->w || !a->scale || !a->x_out)) return DELREC_ERR_ARG;
-    if (!block && (!a->w2 || a->o8.q || a->g8.q)) return DELREC_ERR_ARG;
-    if (!pair_ok(a->o8) || !pair_ok(a->g8) || !pair_ok(a->x8)) return DELREC_ERR_ARG;
+    if (!block && !a->w2) return DELREC_ERR_ARG;
+    if (!eights_ok(a->o8, a->g8, a->x8, block)) return DELREC_ERR_ARG;
     if (!a->bf16 && a->x_bf16) return DELREC_ERR_UNSUPPORTED;
     NormGate p{};
     p.R0 = a->R0; p.R1 = a->R1; p.N = a->N; p.bf16 = a->bf16 != 0; p.x_bf16 = a->x_bf16 != 0;
@@ -87,7 +94,7 @@ int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream) {
 int delrec_norm_gate_bwd(const delrec_norm_gate_bwd_args* a, void* stream) {
     if (!a || !sizes_ok(a->R0, a->R1, a->N) || a->N < 2) return DELREC_ERR_ARG;
     const bool block = a->o.data || a->o8.q;
-    if (!pair_ok(a->o8) || !pair_ok(a->g8) || !pair_ok(a->x8)) return DELREC_ERR_ARG;
+    if (!eights_ok(a->o8, a->g8, a->x8, block)) return DELREC_ERR_ARG;
     if ((!a->x.data && !a->x8.q) || !a->stats || !a->dx.data) return DELREC_ERR_ARG;
     if (!a->dx_out.data && !a->du.data) return DELREC_ERR_ARG;
     if (block && ((!a->g.data && !a->g8.q) || !a->w || !a->scale || !a->d_o.data || !a->dg.data || !a->dw || !a->dscale))

@@ -137,3 +137,27 @@ def test_oracle_8_bit_gradients_at_exact_values_are_the_gradients():
     want = torch.autograd.grad(og.norm_gate(*leaves, 1e-6), leaves, cot)
     for p, q in zip(og.norm_gate_grads8(o, gg, x, w, s, w2, 1e-6, *cot), want):
         torch.testing.assert_close(p, q, rtol=1e-5, atol=1e-5)
+
+
+def test_abi_refuses_8_bits_of_only_some_inputs():
+    """o, g and x of a block are kept in 8 bits together, x by itself where there is no block: any
+    other mix would have a kernel go through a pointer that was not given."""
+    from delrec import _lib
+    lib = _lib.load()
+    one, rows, packed = ctypes.c_void_p(4096), _lib.Rows(4096, 8, 8), _lib.Packed8(4096, 4096)
+    fwd = dict(R0=3, R1=1, N=8, o=rows, g=rows, x=rows, w=one, scale=one, w2=one, x_out=one, u=one, stats=one, eps=1e-6)
+    bwd = dict(R0=3, R1=1, N=8, w=one, scale=one, w2=one, stats=one, du=rows, d_o=rows, dg=rows, dx=rows, dw=one,
+               dscale=one, dw2=one)                      # no workspace: what passes the checks stops there
+    for given in range(8):
+        eight = {k: packed for i, k in enumerate(('o8', 'g8', 'x8')) if given >> i & 1}
+        plain = {k[0]: rows for k in ('o8', 'g8', 'x8') if k not in eight}
+        if given not in (0, 7):
+            assert lib.delrec_norm_gate_fwd(ctypes.byref(_lib.NormGateFwdArgs(**fwd, **eight)), None) == 1, given
+        want = 3 if given in (0, 7) else 1
+        for args in ({**bwd, **plain, **eight}, {**bwd, 'o': rows, 'g': rows, 'x': rows, **eight}):
+            assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**args)), None) == want, (given, args)
+    alone = dict(R0=3, R1=1, N=8, x=rows, w2=one, stats=one, du=rows, dx=rows, dw2=one)
+    assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**alone, x8=packed)), None) == 3
+    assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**alone, g8=packed)), None) == 1
+    # N = 3: the kernels for rows of any width have the same contract
+    assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**{**bwd, 'N': 3}, o=rows, g=rows, x8=packed)), None) == 1
