@@ -113,6 +113,14 @@ Tensor rows_form(Tensor t) {
     return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
 }
 
+// The same for a tensor that the graph keeps, to be called above the autograd keys: a view taken
+// there shares its tensor's version counter, and one taken below them has its own, so that a change
+// in place between forward and backward would go unnoticed. Detached: no node for the view.
+Tensor kept_rows(const Tensor& t) {
+    if (!t.defined() || ((t.dim() == 2 || t.dim() == 3) && t.stride(-1) == 1)) return t;
+    return rows_form(t.detach());
+}
+
 delrec_rows rows_of(const Tensor& t) {
     if (!t.defined()) return {nullptr, 0, 0};
     if (t.dim() == 3) return {t.data_ptr(), t.stride(0), t.stride(1)};
@@ -366,13 +374,14 @@ variable_list norm_with_graph(const Tensor& o, const Tensor& g, const Tensor& x,
     auto node = make_node<NormGateBackward>();
     node->set_next_edges(torch::autograd::collect_next_edges(o, g, x, w, scale, w2));
     variable_list out;
+    const Tensor orow = kept_rows(o), grow = kept_rows(g), xr = kept_rows(x);
     {
         at::AutoDispatchBelowADInplaceOrView below;
         const int64_t N = x.size(-1);
         NormKept kept;
         const Tensor wc = vector_arg(w, N, x, "weight"), sc = vector_arg(scale, N, x, "scale"),
-                     w2c = vector_arg(w2, N, x, o.defined() ? "next_weight" : "weight"), xr = rows_form(x);
-        for (const Tensor& t : norm_forward(rows_form(o), rows_form(g), xr, wc, sc, w2c, eps, x.sizes(), checkpoint, &kept))
+                     w2c = vector_arg(w2, N, x, o.defined() ? "next_weight" : "weight");
+        for (const Tensor& t : norm_forward(orow, grow, xr, wc, sc, w2c, eps, x.sizes(), checkpoint, &kept))
             if (t.defined()) out.push_back(t);
         node->keep({kept.o, kept.g, kept.x, kept.o8.q, kept.o8.scale, kept.g8.q, kept.g8.scale, kept.x8.q, kept.x8.scale, wc,
                     sc, w2c, kept.stats});

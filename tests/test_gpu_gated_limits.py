@@ -40,3 +40,35 @@ def test_scan_nan_bias_leaves_empty_rows_alone(dev, checkpoint):
     assert torch.equal(last[0], c['h0'][0]) and torch.equal(dh0[0], c['dlast'][0])
     assert not h[:, 0].any() and not dz[:, 0].any() and not df[:, 0].any()
     assert torch.isnan(last[1]).tolist() == torch.isnan(db).tolist() == [False, False, True, False, False, False]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(70,), (5, 70), (2, 3, 70), (2, 2, 3, 70), (2, 1, 2, 2, 70)])
+def test_norm_notices_inputs_changed_in_place(dev, shape):
+    """Whatever the number of axes, a kept input that changes before the backward pass is an error,
+    as torch's own operations have it; without a change the gradients are those of the rows."""
+    from delrec.gated import norm_gate_residual, rms_norm
+    c = {k: v.to(dev) for k, v in norm_case(shape, FP32, FP32, seed=31).items()}
+
+    def forward():
+        leaves = [c[k].clone().requires_grad_(True) for k in NAMES]
+        kept = [t * 1.0 for t in leaves[:3]]
+        return leaves, kept, norm_gate_residual(*kept, *leaves[3:])[0]
+    leaves, _, y = forward()
+    rows = [c[k].clone().reshape(-1, 70).requires_grad_(True) if k in 'ogx' else c[k].clone().requires_grad_(True) for k in NAMES]
+    want = torch.autograd.grad(norm_gate_residual(*rows)[0].sum(), rows, allow_unused=True)
+    for a, b in zip(torch.autograd.grad(y.sum(), leaves, allow_unused=True), want):
+        assert torch.equal(a.reshape(b.shape), b)
+    for k in range(3):
+        leaves, kept, y = forward()
+        with torch.no_grad():
+            kept[k].mul_(2.0)
+        with pytest.raises(RuntimeError, match='inplace'):
+            torch.autograd.grad(y.sum(), leaves, allow_unused=True)
+    x = c['x'].clone().requires_grad_(True)
+    kept = x * 1.0
+    u = rms_norm(kept, c['w'])
+    with torch.no_grad():
+        kept.view(-1)[0] += 1.0
+    with pytest.raises(RuntimeError, match='inplace'):
+        torch.autograd.grad(u.sum(), x)
