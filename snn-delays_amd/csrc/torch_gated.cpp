@@ -448,12 +448,13 @@ py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor
     check_like(f, z, z.scalar_type(), "f");
     if (z.dim() != 2 || z.size(0) == 0) refuse(text("gated_step takes (B, N) tensors with B > 0, got ", z.sizes()));
     check_like(h, z, at::kFloat, "h");
-    if (wanted({&z, &f, &g, &x, &h, &w, &scale, &w2, &bias}))
+    if (wanted({&z, &f, &g, &x, &h, &w, &scale, &w2, &bias, &h_out}))
         throw std::runtime_error("gated_step has no backward pass: call it under torch.no_grad(), or gated_scan and "
                                  "norm_gate_residual");
     const c10::DeviceGuard guard(z.device());
     const int B = as_int(z.size(0)), N = as_int(z.size(1));
-    if (h_out.defined()) {
+    const bool in_place = h_out.defined();
+    if (in_place) {
         check_like(h_out, h, at::kFloat, "h_out");
         if (!h_out.is_contiguous()) refuse("h_out must be contiguous");
     } else {
@@ -473,6 +474,8 @@ py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor
     a.w = fptr(w); a.scale = fptr(scale); a.w2 = fptr(w2); a.eps = (float)eps;
     a.h_out = fptr(h_out); a.x_out = xo.data_ptr(); a.u = u.defined() ? u.data_ptr() : nullptr;
     check(delrec_gated_step(&a, stream_of(z)), "delrec_gated_step");
+    // a graph that kept the old state sees that it is gone, as after any operation in place
+    if (in_place && !h_out.is_inference()) h_out.unsafeGetTensorImpl()->bump_version();
     return py::make_tuple(xo, u.defined() ? py::cast(u) : py::none(), h_out);
 }
 

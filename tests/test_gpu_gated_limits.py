@@ -72,3 +72,35 @@ def test_norm_notices_inputs_changed_in_place(dev, shape):
         kept.view(-1)[0] += 1.0
     with pytest.raises(RuntimeError, match='inplace'):
         torch.autograd.grad(u.sum(), x)
+
+
+@pytest.mark.gpu
+def test_step_in_place_is_seen_by_a_graph(dev):
+    """A state that a graph has kept and a step then overwrites is an error in the backward pass; a
+    state of a graph itself is refused with gradients on; inference tensors go through."""
+    from delrec.gated import gated_scan, gated_step
+    c = {k: v.to(dev) for k, v in norm_case((2, 70), FP32, FP32, seed=32).items()}
+
+    def step(state):
+        return gated_step(c['o'], c['g'], c['g'], c['x'], state, c['w'], c['scale'], c['w2'], h_out=state)
+    z = rnd(torch.Generator().manual_seed(33), 5, 2, 70).to(dev).requires_grad_(True)
+    _, last = gated_scan(z, z)
+    loss = last.square().sum()
+    before = last._version
+    with torch.no_grad():
+        step(last)
+    assert last._version > before
+    with pytest.raises(RuntimeError, match='inplace'):
+        torch.autograd.grad(loss, z)
+    fresh = torch.zeros(2, 70, device=dev)
+    for h, out in ((last, last), (fresh, last)):
+        with pytest.raises(RuntimeError, match='no backward'):
+            gated_step(c['o'], c['g'], c['g'], c['x'], h, c['w'], c['scale'], h_out=out)
+    with torch.no_grad():
+        want = step(fresh)[2].clone()
+    with torch.inference_mode():
+        state = torch.zeros(2, 70, device=dev)
+        assert torch.equal(step(state)[2], want)
+    step(state)                          # an inference tensor, outside of that mode
+    with torch.no_grad():
+        assert torch.equal(step(fresh)[2], state)
