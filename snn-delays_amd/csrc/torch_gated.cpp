@@ -76,6 +76,12 @@ bool wanted(std::initializer_list<const Tensor*> ts) {
     return false;
 }
 
+// torch's own Functions refuse inputs with a forward-mode tangent; bare nodes would drop it
+void check_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(text(what, " has no forward-mode derivative"));
+}
+
 void once_differentiable(const char* what) {
     if (at::GradMode::is_enabled()) throw std::runtime_error(text(what, " has no second derivative (create_graph=True)"));
 }
@@ -259,6 +265,7 @@ py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTens
     const Tensor bias = given(bias_), h0 = given(h0_);
     Tensor starts = given(starts_), lengths = given(lengths_);
     check_activation(z, "z");
+    check_tangents("gated_scan", {&z, &f, &bias, &h0});
     if (z.dim() != 3 || z.size(1) == 0 || z.size(2) == 0) refuse(text("z must be (T, B, N) with B, N > 0, got ", z.sizes()));
     check_like(f, z, z.scalar_type(), "f");
     const int64_t T = z.size(0), B = z.size(1), N = z.size(2);
@@ -414,6 +421,7 @@ void check_rows(const Tensor& o, const Tensor& g, const Tensor& x, const Tensor&
 py::tuple norm_gate_residual(Tensor o, Tensor g, Tensor x, OptTensor w_, OptTensor scale_, OptTensor w2_, double eps, bool checkpoint) {
     const Tensor w = given(w_), scale = given(scale_), w2 = given(w2_);
     check_rows(o, g, x, w, scale);
+    check_tangents("norm_gate_residual", {&o, &g, &x, &w, &scale, &w2});
     const int64_t N = x.size(-1);
     if (o.numel() == 0) {
         const Tensor y = x + (o * w * scale * g).to(x.scalar_type());
@@ -433,6 +441,7 @@ Tensor rms_norm(Tensor x, OptTensor w_, double eps, bool checkpoint) {
     check_activation(x, "x");
     check_width(x);
     if (!w.defined()) refuse("weight is needed");
+    check_tangents("rms_norm", {&x, &w});
     if (x.numel() == 0) return (x * w).to(x.scalar_type());
     if (wanted({&x, &w})) return norm_with_graph(Tensor(), Tensor(), x, Tensor(), Tensor(), w, eps, checkpoint)[0];
     return norm_forward(Tensor(), Tensor(), rows_form(x), Tensor(), Tensor(), vector_arg(w, x.size(-1), x, "weight"), eps,
@@ -448,6 +457,7 @@ py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor
     check_like(f, z, z.scalar_type(), "f");
     if (z.dim() != 2 || z.size(0) == 0) refuse(text("gated_step takes (B, N) tensors with B > 0, got ", z.sizes()));
     check_like(h, z, at::kFloat, "h");
+    check_tangents("gated_step", {&z, &f, &g, &x, &h, &w, &scale, &w2, &bias});
     if (wanted({&z, &f, &g, &x, &h, &w, &scale, &w2, &bias, &h_out}))
         throw std::runtime_error("gated_step has no backward pass: call it under torch.no_grad(), or gated_scan and "
                                  "norm_gate_residual");

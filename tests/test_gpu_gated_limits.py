@@ -104,3 +104,26 @@ def test_step_in_place_is_seen_by_a_graph(dev):
     step(state)                          # an inference tensor, outside of that mode
     with torch.no_grad():
         assert torch.equal(step(fresh)[2], state)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('grad', [False, True])
+def test_forward_mode_tangents_are_refused(dev, grad):
+    """An output without the tangent that its input carries would count as a constant."""
+    import torch.autograd.forward_ad as fw
+    from delrec.gated import gated_scan, gated_step, norm_gate_residual, rms_norm
+    c = {k: v.to(dev) for k, v in norm_case((4, 2, 70), FP32, FP32, seed=34).items()}
+    v, h = c['w'], c['x'][0]
+    calls = {
+        'gated_scan': (gated_scan, [c['o'], c['g'], v, h]),
+        'norm_gate_residual': (norm_gate_residual, [c['o'], c['g'], c['x'], v, v, v]),
+        'rms_norm': (rms_norm, [c['x'], v]),
+        'gated_step': (gated_step, [c['o'][0], c['g'][0], c['g'][1], c['x'][1], h, v, v, v, v]),
+    }
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        for name, (call, args) in calls.items():
+            call(*args)
+            for i, a in enumerate(args):
+                dual = fw.make_dual(a.clone(), torch.ones_like(a))
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    call(*args[:i], dual, *args[i + 1:])
