@@ -233,13 +233,14 @@ __device__ __forceinline__ void gate(const F& f, const float* bias2, bool off, f
     for (int j = 0; j < V; ++j) k[j] = off ? 0.0f : gate_in2(fmaf(f.get(j), kLog2e, bias2[j]));
 }
 
-// One step composed onto a piece's map (A, L), forwards
+// One step composed onto a piece's map (A, L), forwards (past the row's end L stays, and is not
+// multiplied by the shut gate's zero: it may be infinite)
 template <int V, bool MASK, class F>
-__device__ __forceinline__ void step_forward(const float* k, const F& z, bool fresh, float* A, float* L) {
+__device__ __forceinline__ void step_forward(const float* k, const F& z, bool fresh, bool off, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float from = MASK && fresh ? 0.0f : L[j];
-        L[j] = fmaf(k[j], z.get(j) - from, from);
+        const float from = MASK && fresh ? 0.0f : L[j], l = fmaf(k[j], z.get(j) - from, from);
+        L[j] = off ? L[j] : l;
         // (the product keeps a cut's sign also for a leak of 0, where the fma gives +0)
         if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
         else A[j] = fmaf(-k[j], A[j], A[j]);
@@ -248,11 +249,11 @@ __device__ __forceinline__ void step_forward(const float* k, const F& z, bool fr
 
 // and backwards, c -> a (dh + c)
 template <int V, bool MASK, class D>
-__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool fresh, float* A, float* L) {
+__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool fresh, bool off, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float x = dh.get(j) + L[j], l = fmaf(-k[j], x, x);
-        L[j] = MASK && fresh ? 0.0f : l;
+        L[j] = MASK && fresh ? 0.0f : off ? L[j] : l;
         if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
         else A[j] = fmaf(-k[j], A[j], A[j]);
     }
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
                 if (t0 + s >= len) blank(z[s]), fresh[s] = false;
             DELREC_STEPS(s) {
                 gate<V>(f[s], bias, t0 + s >= len, k[s]);
-                step_forward<V, MASK>(k[s], z[s], fresh[s], A, L);
+                step_forward<V, MASK>(k[s], z[s], fresh[s], t0 + s >= len, A, L);
             }
         }
         maps.put(buf, w, lane, A, L);
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
             const int s = BWD ? kSteps - 1 - q : q;
             float k[V];
             gate<V>(f[s], bias, t0 + s >= len, k);
-            if constexpr (BWD) step_backward<V, MASK>(k, v[s], fresh[s], A, L);
-            else step_forward<V, MASK>(k, v[s], fresh[s], A, L);
+            if constexpr (BWD) step_backward<V, MASK>(k, v[s], fresh[s], t0 + s >= len, A, L);
+            else step_forward<V, MASK>(k, v[s], fresh[s], t0 + s >= len, A, L);
         }
     }
     maps.put(0, w, lane, A, L);
@@ -541,11 +542,11 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
             DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
             if (!MASK || any) DELREC_STEPS(s) {
                 gate<V>(f[s], bias, t0 + s >= len, k[s]);
-                step_forward<V, MASK>(k[s], z[s], fresh[s], A, L);
+                step_forward<V, MASK>(k[s], z[s], fresh[s], t0 + s >= len, A, L);
             }
             fmap.put(buf, w, lane, A, L);
             DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-            if (!MASK || any) DELREC_STEPS_BACK(s) step_backward<V, MASK>(k[s], dh[s], fresh[s], A, L);
+            if (!MASK || any) DELREC_STEPS_BACK(s) step_backward<V, MASK>(k[s], dh[s], fresh[s], t0 + s >= len, A, L);
             rmap.put(buf, w, lane, A, L);
         }
         barrier_lds();
@@ -566,15 +567,16 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
             d[s][j] = from - z[s].get(j);
             mine[j] = fmaf(-k[s][j], d[s][j], from);
         }
-        // (k = 0 outside a row: its gradients come as zeros)
+        // (outside a row the gradients are zeros and the carry stays, also an infinite one)
         dzp.seek(t0 + kSteps - 1), dfp.seek(t0 + kSteps - 1);
         dzp.start(), dfp.start();
         DELREC_STEPS_BACK(s) {
             float oz[V], of[V];
             DELREC_COLS(j) {
+                const bool off = t0 + s >= len;
                 const float lam = dh[s].get(j) + g[j];
-                oz[j] = lam * k[s][j];
-                of[j] = fmaf(-k[s][j], oz[j], oz[j]) * d[s][j];
+                oz[j] = off ? 0.0f : lam * k[s][j];
+                of[j] = off ? 0.0f : fmaf(-k[s][j], oz[j], oz[j]) * d[s][j];
                 g[j] = MASK && fresh[s] ? 0.0f : lam - oz[j];
                 blk[j] += of[j];
             }

@@ -127,3 +127,49 @@ def test_forward_mode_tangents_are_refused(dev, grad):
                 dual = fw.make_dual(a.clone(), torch.ones_like(a))
                 with pytest.raises(RuntimeError, match='forward-mode'):
                     call(*args[:i], dual, *args[i + 1:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('T,B,N', [(5, 3, 6), (64, 3, 70), (250, 3, 70), (70, 3, 200), (3001, 3, 6)])
+@pytest.mark.parametrize('dtype', [FP32, BF16])
+def test_scan_infinite_states_outlast_padding(dev, T, B, N, dtype):
+    """A state that the last live step makes infinite stays so over the steps past a row's end,
+    which add nothing to any gradient, and the other channels are as without it."""
+    c = scan_case(T, B, N, dtype, False, seed=41)
+    for lengths in (None, torch.tensor([T, T - 3, max(1, T // 2)])):
+        c['lengths'] = lengths
+        c['z'] = scan_case(T, B, N, dtype, False, seed=41)['z']
+        want = [t.cpu() for t in run_scan(c, dev)]
+        ends = [T] * 3 if lengths is None else lengths.tolist()
+        for b, n in enumerate(ends):
+            c['z'][n - 1, b, 2] = INF if b else -INF
+        got = [t.cpu() for t in run_scan(c, dev)]
+        h, last, dz, df, db, dh0 = got
+        assert last[:, 2].tolist() == [-INF, INF, INF]
+        for b, n in enumerate(ends):
+            assert h[n - 1, b, 2] == last[b, 2] and not h[n:, b].any()
+            assert torch.isinf(df[n - 1, b, 2]) and not df[n:, b].any() and not dz[n:, b].any()
+        others = [i for i in range(N) if i != 2]
+        for name, a, b in zip(('h', 'last', 'dz', 'df', 'db', 'dh0'), got, want):
+            assert torch.equal(a[..., others], b[..., others]), name
+        assert torch.equal(dz, want[2]) and torch.equal(dh0, want[5])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+@pytest.mark.parametrize('bad', [INF, NAN])
+@pytest.mark.parametrize('T,B,N', [(5, 3, 6), (130, 3, 70), (70, 3, 200), (3001, 3, 6)])
+def test_scan_empty_rows_pass_their_state_and_its_gradient_on(dev, T, B, N, bad, checkpoint):
+    """Rows without a step, with a state or a gradient that is not finite: both go through as they
+    are, and reach neither the other gradients nor the bias'."""
+    c = scan_case(T, B, N, FP32, False, seed=42)
+    c['lengths'] = torch.tensor([0, T, max(1, T - 2)])
+    want = [t.cpu() for t in run_scan(c, dev, checkpoint)]
+    for k, i in (('h0', 1), ('dlast', 3)):
+        d = dict(c, **{k: c[k].clone()})
+        d[k][0, i] = bad
+        h, last, dz, df, db, dh0 = (t.cpu() for t in run_scan(d, dev, checkpoint))
+        torch.testing.assert_close(last[0], d['h0'][0], rtol=0, atol=0, equal_nan=True)
+        torch.testing.assert_close(dh0[0], d['dlast'][0], rtol=0, atol=0, equal_nan=True)
+        for a, b in ((h, want[0]), (dz, want[2]), (df, want[3]), (db, want[4])):
+            assert torch.equal(a, b)
