@@ -451,7 +451,8 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
         if (!AHEAD) load(r0);
         const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
         const bool live = mine < rows, has_up = live && p.dx_out.data, has_du = live && p.du.data;
-        const float r = in.r, r2 = in.r2;
+        // (without a second norm r2 and x count as zeros, also where x is not finite)
+        const float r = in.r, r2 = p.w2 ? in.r2 : 0.0f;
         float o[NE][4], g[NE][4], x[NE][4], up[NE][4], du[NE][4], sg[NE][4];
 #pragma unroll
         for (int e = 0; e < NE; ++e)
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
                     sg[e][j] = sigm(g[e][j]);
                     x[e][j] = fmaf(col(1, e, j), o[e][j] * col(0, e, j) * (g[e][j] * sg[e][j]), x[e][j]);
                 }
-                x[e][j] *= r2;
+                x[e][j] = p.w2 ? x[e][j] * r2 : 0.0f;
                 s += j >= c.skip[e] ? col(2, e, j) * du[e][j] * x[e][j] : 0.0f;
             }
         const float m2 = lanes_sum<LPR>(s, red, 0) * inv_n;
@@ -649,6 +650,8 @@ size_t norm_gate_bwd_ws(long long rows, int N) {
 
 void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
     NormGate p = a;
+    // without a gradient of u the second norm has no part in the backward (dw2 = 0)
+    if (!fwd && !p.du.data) p.w2 = nullptr;
     // rows one pitch apart in every tensor need no division by R1
     p.flat = p.R0 == 1;
     if (!p.flat) {

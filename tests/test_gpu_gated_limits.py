@@ -173,3 +173,28 @@ def test_scan_empty_rows_pass_their_state_and_its_gradient_on(dev, T, B, N, bad,
         torch.testing.assert_close(dh0[0], d['dlast'][0], rtol=0, atol=0, equal_nan=True)
         for a, b in ((h, want[0]), (dz, want[2]), (df, want[3]), (db, want[4])):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+@pytest.mark.parametrize('used', ['no next norm', 'u unused'])
+@pytest.mark.parametrize('bad', [INF, NAN])
+@pytest.mark.parametrize('N', [3, 64, 130, 700, 1500, 4099, 9000])
+def test_norm_residual_gradient_without_a_second_norm(dev, N, bad, used, checkpoint):
+    """Without a gradient through u, dx is dx' and do, dg, dw, dscale do not read x: a residual that
+    is not finite reaches none of them."""
+    from delrec.gated import norm_gate_residual
+
+    def grads(x):
+        L = [(x if k == 'x' else c[k]).to(dev).requires_grad_(True) for k in NAMES]
+        y, _ = norm_gate_residual(*L[:5], None if used == 'no next norm' else L[5], checkpoint=checkpoint)
+        return torch.autograd.grad(y, L, c['dxo'].to(dev), allow_unused=True)
+    c = norm_case((9, N), FP32, FP32, seed=43)
+    want = grads(c['x'])
+    x = c['x'].clone()
+    x[4, N // 2] = bad
+    got = grads(x)
+    for k in range(5):
+        assert torch.equal(got[k], want[k]), NAMES[k]
+    assert torch.equal(got[2].cpu(), c['dxo'])
+    assert got[5] is None if used == 'no next norm' else not got[5].any()
