@@ -8,6 +8,10 @@
 
 namespace delrec {
 
+// Workgroups of a launch of up to 1024 threads each: a dimension has room for 2^32 threads. Kernels
+// loop, or are launched again, over what is left.
+constexpr int kMostBlocks = 1 << 20;
+
 // activations: float, or bf16 by the hardware's round to nearest even
 template <class S>
 __device__ __forceinline__ float to_f32(S v) { return (float)v; }

@@ -68,7 +68,7 @@ struct Lane {
     bool on, first;                          // writes; first lane of its 8-bit group
     int i;                                   // nominal first column
     __device__ __forceinline__ Lane(const GatedScan& p, int per_row) {
-        const long long c = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
+        const long long c = ((long long)p.first + blockIdx.x) * 64 + (threadIdx.x & 63);
         const long long rows = c / per_row;
         b = rows < p.B ? (int)rows : p.B - 1;
         b0 = __builtin_amdgcn_readfirstlane(b);
@@ -635,19 +635,25 @@ Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
 size_t map_floats(const Plan& q, int B, int N) { return q.ranges > 1 ? (size_t)q.ranges * 2 * B * N : 0; }
 
 template <class S, int V, bool MASK, bool PACK>
-void run_gated(const GatedScan& p, const Plan& q, bool fwd, hipStream_t stream) {
-    const dim3 block(64 * q.waves), grid(q.groups, q.ranges), inner(q.groups, q.ranges - 1);
-    if (fwd) {
-        if (q.ranges > 1)
-            hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, false, false>), inner, block, 0, stream, p, q.per_row, q.range);
-        hipLaunchKernelGGL((gated_fwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range);
-    } else {
-        float* part = p.db ? p.ws + map_floats(q, p.B, p.N) : nullptr;
-        if (q.ranges > 1)
-            hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, PACK, true>), inner, block, 0, stream, p, q.per_row, q.range);
-        hipLaunchKernelGGL((gated_bwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range, part);
-        if (p.db) launch_column_sums(part, q.ranges * p.B, p.N, p.N, p.db, nullptr, nullptr, stream);
+void run_gated(const GatedScan& a, const Plan& q, bool fwd, hipStream_t stream) {
+    GatedScan p = a;
+    float* part = p.db && !fwd ? p.ws + map_floats(q, p.B, p.N) : nullptr;
+    const dim3 block(64 * q.waves);
+    for (long long first = 0; first < q.groups; first += kMostBlocks) {
+        p.first = (int)first;
+        const int groups = std::min(q.groups - p.first, kMostBlocks);
+        const dim3 grid(groups, q.ranges), inner(groups, q.ranges - 1);
+        if (fwd) {
+            if (q.ranges > 1)
+                hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, false, false>), inner, block, 0, stream, p, q.per_row, q.range);
+            hipLaunchKernelGGL((gated_fwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range);
+        } else {
+            if (q.ranges > 1)
+                hipLaunchKernelGGL((gated_range_kernel<S, V, MASK, PACK, true>), inner, block, 0, stream, p, q.per_row, q.range);
+            hipLaunchKernelGGL((gated_bwd_kernel<S, V, MASK, PACK>), grid, block, 0, stream, p, q.per_row, q.range, part);
+        }
     }
+    if (part) launch_column_sums(part, (unsigned)q.ranges * p.B, p.N, p.N, p.db, nullptr, nullptr, stream);
 }
 
 template <class S, int V>

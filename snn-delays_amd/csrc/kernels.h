@@ -594,6 +594,7 @@ struct GatedScan {               // forward and backward of the gated linear rec
     float* db;
     float* dh0;
     float* ws;                   // workspace, gated_fwd_ws / gated_bwd_ws floats
+    int first;                   // set by the launcher: the launch's first workgroup of channels
 };
 size_t gated_fwd_ws(int T, int B, int N);   // floats
 size_t gated_bwd_ws(int T, int B, int N);
@@ -629,7 +630,7 @@ struct Pack8 {
 };
 void launch_pack8(const Pack8& p, bool pack, hipStream_t stream);
 // o_k[n] = sum over rows r of part[r * pitch + k * N + n], k < pitch / N <= 3 (NULL: skipped)
-void launch_column_sums(const float* part, int rows, int N, int pitch, float* o0, float* o1, float* o2, hipStream_t stream);
+void launch_column_sums(const float* part, unsigned rows, int N, unsigned pitch, float* o0, float* o1, float* o2, hipStream_t stream);
 
 void launch_lif(bool fwd, const delrec_lif_fwd_args* fa, const delrec_lif_bwd_args* ba,
                 const Lif& k, int cus, hipStream_t stream);

@@ -53,46 +53,48 @@ __device__ __forceinline__ float val8(const delrec_rows& x, const delrec_packed8
 template <class S, class X>
 __global__ void __launch_bounds__(kNb) norm_any_fwd_kernel(NormGate p) {
     __shared__ float red[4];
-    const long long row = blockIdx.x;
     const int N = p.N;
     const bool block = p.o.data || p.h;
-    const X* x = row_ptr<const X>(p.x, row, p.R1);
-    float r = 0.0f, r2 = 0.0f, s = 0.0f;
-    if (p.h) {
-        for (int n = threadIdx.x; n < N; n += kNb) {
-            const float k = gate_in(to_f32(row_ptr<const S>(p.f, row, p.R1)[n]) + (p.bias ? p.bias[n] : 0.0f));
-            const float h = p.h[row * N + n];
-            p.h_out[row * N + n] = fmaf(k, to_f32(row_ptr<const S>(p.z, row, p.R1)[n]) - h, h);
+    const long long rows = (long long)p.R0 * p.R1;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const X* x = row_ptr<const X>(p.x, row, p.R1);
+        float r = 0.0f, r2 = 0.0f, s = 0.0f;
+        if (p.h) {
+            for (int n = threadIdx.x; n < N; n += kNb) {
+                const float k = gate_in(to_f32(row_ptr<const S>(p.f, row, p.R1)[n]) + (p.bias ? p.bias[n] : 0.0f));
+                const float h = p.h[row * N + n];
+                p.h_out[row * N + n] = fmaf(k, to_f32(row_ptr<const S>(p.z, row, p.R1)[n]) - h, h);
+            }
+            __syncthreads();
         }
-        __syncthreads();
-    }
-    auto oval = [&](int n) { return p.h ? p.h_out[row * N + n] : to_f32(row_ptr<const S>(p.o, row, p.R1)[n]); };
-    if (block) {
-        for (int n = threadIdx.x; n < N; n += kNb) {
-            const float o = oval(n);
-            s += o * o;
+        auto oval = [&](int n) { return p.h ? p.h_out[row * N + n] : to_f32(row_ptr<const S>(p.o, row, p.R1)[n]); };
+        if (block) {
+            for (int n = threadIdx.x; n < N; n += kNb) {
+                const float o = oval(n);
+                s += o * o;
+            }
+            r = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
         }
-        r = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
-    }
-    auto xval = [&](int n) {
-        const float xv = to_f32(x[n]);
-        if (!block) return xv;
-        const float g = to_f32(row_ptr<const S>(p.g, row, p.R1)[n]);
-        return fmaf(p.scale[n], oval(n) * r * p.w[n] * (g * sigm(g)), xv);
-    };
-    s = 0.0f;
-    for (int n = threadIdx.x; n < N; n += kNb) {
-        const float v = xval(n);
-        if (block) ((X*)p.x_out)[row * N + n] = (X)v;
-        s += v * v;
-    }
-    if (p.w2) {
-        r2 = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
-        for (int n = threadIdx.x; n < N; n += kNb) ((S*)p.u)[row * N + n] = (S)(xval(n) * r2 * p.w2[n]);
-    }
-    if (p.stats && threadIdx.x == 0) {
-        p.stats[2 * row] = r;
-        p.stats[2 * row + 1] = r2;
+        auto xval = [&](int n) {
+            const float xv = to_f32(x[n]);
+            if (!block) return xv;
+            const float g = to_f32(row_ptr<const S>(p.g, row, p.R1)[n]);
+            return fmaf(p.scale[n], oval(n) * r * p.w[n] * (g * sigm(g)), xv);
+        };
+        s = 0.0f;
+        for (int n = threadIdx.x; n < N; n += kNb) {
+            const float v = xval(n);
+            if (block) ((X*)p.x_out)[row * N + n] = (X)v;
+            s += v * v;
+        }
+        if (p.w2) {
+            r2 = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
+            for (int n = threadIdx.x; n < N; n += kNb) ((S*)p.u)[row * N + n] = (S)(xval(n) * r2 * p.w2[n]);
+        }
+        if (p.stats && threadIdx.x == 0) {
+            p.stats[2 * row] = r;
+            p.stats[2 * row + 1] = r2;
+        }
     }
 }
 
@@ -101,8 +103,8 @@ __global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
     __shared__ float red[4];
     const int N = p.N, tid = threadIdx.x;
     const bool block = p.w != nullptr;
-    float* part = p.part + (size_t)blockIdx.x * 3 * N;
-    for (int n = tid; n < 3 * N; n += kNb) part[n] = 0.0f;
+    float *dwp = p.part + (size_t)blockIdx.x * 3 * N, *dsp = dwp + N, *dw2p = dsp + N;
+    for (int n = tid; n < N; n += kNb) dwp[n] = dsp[n] = dw2p[n] = 0.0f;
     __syncthreads();
     const long long rows = (long long)p.R0 * p.R1;
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -131,11 +133,11 @@ __global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
         for (int n = tid; n < N; n += kNb) {
             const float dx = dxval(n);
             row_ptr<X>(p.dx, row, p.R1)[n] = (X)dx;
-            if (p.w2) part[2 * N + n] += duval(n) * e2val(n);
+            if (p.w2) dw2p[n] += duval(n) * e2val(n);
             if (block) {
                 const float g = gval(n), sg = sigm(g), si = g * sg, e = oval(n) * r, dn = p.scale[n] * dx * si;
-                part[n] += dn * e;
-                part[N + n] += dx * e * p.w[n] * si;
+                dwp[n] += dn * e;
+                dsp[n] += dx * e * p.w[n] * si;
                 row_ptr<S>(p.dg, row, p.R1)[n] = (S)(p.scale[n] * dx * e * p.w[n] * (sg + si * (1.0f - sg)));
                 s += p.w[n] * dn * e;
             }
@@ -152,34 +154,37 @@ __global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
 }
 
 // out_k[n] = sum over rows of part[row * pitch + k * N + n], k < 3, in a fixed order
-__global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, int rows, int N, int pitch, float* o0,
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, unsigned rows, int N, unsigned pitch, float* o0,
                                                            float* o1, float* o2) {
     __shared__ float red[16][64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int n = blockIdx.x * 64 + lane, k = blockIdx.y;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, k = blockIdx.y;
     float* out = k == 0 ? o0 : (k == 1 ? o1 : o2);
-    // eight rows' loads in flight at a time (past the end the last row again, left out)
-    float s8[8] = {};
-    const float* at = part + (size_t)k * N + min(n, N - 1);
-    for (int r = w; r < rows; r += 128) {
-        float v[8];
+    for (long long n0 = blockIdx.x * 64LL; n0 < N; n0 += gridDim.x * 64LL) {
+        const int n = (int)n0 + lane;
+        // eight rows' loads in flight at a time (past the end the last row again, left out)
+        float s8[8] = {};
+        const float* at = part + (size_t)k * N + min(n, N - 1);
+        for (unsigned r = w; r < rows; r += 128) {
+            float v[8];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = at[(size_t)min(r + 16 * q, rows - 1) * pitch];
+            for (int q = 0; q < 8; ++q) v[q] = at[(size_t)min(r + 16 * q, rows - 1) * pitch];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s8[q] += r + 16 * q < rows ? v[q] : 0.0f;
-    }
-    float s = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
-    red[w][lane] = s;
-    __syncthreads();
-    if (w == 0 && n < N && out) {
-        s = red[0][lane];
-        for (int q = 1; q < 16; ++q) s += red[q][lane];
-        out[n] = s;
+            for (int q = 0; q < 8; ++q) s8[q] += r + 16 * q < rows ? v[q] : 0.0f;
+        }
+        float s = ((s8[0] + s8[1]) + (s8[2] + s8[3])) + ((s8[4] + s8[5]) + (s8[6] + s8[7]));
+        red[w][lane] = s;
+        __syncthreads();
+        if (w == 0 && n < N && out) {
+            s = red[0][lane];
+            for (int q = 1; q < 16; ++q) s += red[q][lane];
+            out[n] = s;
+        }
+        __syncthreads();
     }
 }
 
-void launch_column_sums(const float* part, int rows, int N, int pitch, float* o0, float* o1, float* o2, hipStream_t stream) {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((N + 63) / 64, pitch / N), dim3(1024), 0, stream, part, rows, N, pitch, o0, o1, o2);
+void launch_column_sums(const float* part, unsigned rows, int N, unsigned pitch, float* o0, float* o1, float* o2, hipStream_t stream) {
+    hipLaunchKernelGGL(column_sums_kernel, dim3(std::min((N - 1) / 64 + 1, kMostBlocks), pitch / N), dim3(1024), 0, stream, part, rows, N, pitch, o0, o1, o2);
 }
 
 // ---- rows of 4 to 8192 columns in registers ----
@@ -619,7 +624,7 @@ int run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
     const long long rows = (long long)p.R0 * p.R1;
     if (!in_registers(p.N)) {
         if (fwd) {
-            hipLaunchKernelGGL((norm_any_fwd_kernel<S, X>), dim3((unsigned)rows), dim3(kNb), 0, stream, p);
+            hipLaunchKernelGGL((norm_any_fwd_kernel<S, X>), dim3((unsigned)std::min<long long>(rows, kMostBlocks)), dim3(kNb), 0, stream, p);
             if (p.o8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.o, p.o8}, true, stream);
             if (p.g8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, p.g, p.g8}, true, stream);
             if (p.x8.q) launch_pack8({p.R0, p.R1, p.N, p.x_bf16, p.x, p.x8}, true, stream);
@@ -668,7 +673,7 @@ void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
     const int parts = !p.bf16 ? run_norm_gate<float, float>(p, fwd, stream)
                       : p.x_bf16 ? run_norm_gate<__bf16, __bf16>(p, fwd, stream)
                                  : run_norm_gate<__bf16, float>(p, fwd, stream);
-    if (!fwd) launch_column_sums(p.part, parts, p.N, 3 * p.N, p.dw, p.dscale, p.dw2, stream);
+    if (!fwd) launch_column_sums(p.part, parts, p.N, 3u * p.N, p.dw, p.dscale, p.dw2, stream);
 }
 
 }  // namespace delrec

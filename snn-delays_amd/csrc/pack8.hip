@@ -7,34 +7,32 @@
 
 namespace delrec {
 
-// one to three columns: a wave a row
+// one to three columns (one group): a wave a row
 template <class S>
 __global__ void __launch_bounds__(256) pack8_any_kernel(Pack8 p) {
     const int lane = threadIdx.x & 63;
-    const long long grp = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int ng = (p.N + kGroup8 - 1) / kGroup8;
-    if (grp >= (long long)p.R0 * p.R1 * ng) return;
-    const long long row = grp / ng;
-    const int n = (int)(grp % ng) * kGroup8 + lane;
-    const S* x = (const S*)p.x.data + (row / p.R1) * p.x.s0 + (row % p.R1) * p.x.s1;
-    const float v = n < p.N ? to_f32(x[n]) : 0.0f;
-    float m = fabsf(v);
+    const long long rows = (long long)p.R0 * p.R1;
+    for (long long row = blockIdx.x * 4LL + (threadIdx.x >> 6); row < rows; row += gridDim.x * 4LL) {
+        const S* x = (const S*)p.x.data + (row / p.R1) * p.x.s0 + (row % p.R1) * p.x.s1;
+        const float v = lane < p.N ? to_f32(x[lane]) : 0.0f;
+        float m = fabsf(v);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
-    const float sc = scale8(m, __all(finite8(v)));
-    if (n < p.N) p.p.q[row * pitch8(p.N) + n] = (int8_t)quant8(v, recip8(sc));
-    if (lane == 0) p.p.scale[grp] = sc;
+        for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, kWave));
+        const float sc = scale8(m, __all(finite8(v)));
+        if (lane < p.N) p.p.q[row * pitch8(p.N) + lane] = (int8_t)quant8(v, recip8(sc));
+        if (lane == 0) p.p.scale[row] = sc;
+    }
 }
 
 template <class S>
 __global__ void __launch_bounds__(256) unpack8_any_kernel(Pack8 p) {
-    const int ng = (p.N + kGroup8 - 1) / kGroup8;
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (long long)p.R0 * p.R1 * p.N) return;
-    const long long row = i / p.N;
-    const int n = (int)(i % p.N);
-    S* x = (S*)p.x.data + (row / p.R1) * p.x.s0 + (row % p.R1) * p.x.s1;
-    x[n] = (S)((float)p.p.q[row * pitch8(p.N) + n] * p.p.scale[row * ng + n / kGroup8]);
+    const long long all = (long long)p.R0 * p.R1 * p.N;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < all; i += gridDim.x * 256LL) {
+        const long long row = i / p.N;
+        const int n = (int)(i % p.N);
+        S* x = (S*)p.x.data + (row / p.R1) * p.x.s0 + (row % p.R1) * p.x.s1;
+        x[n] = (S)((float)p.p.q[row * pitch8(p.N) + n] * p.p.scale[row]);
+    }
 }
 
 // Rows of four columns and more: LPR lanes a row, four columns a lane (16 lanes a group), kRows
@@ -114,8 +112,8 @@ template <class S>
 static void run_pack8_any(const Pack8& p, bool pack, hipStream_t stream) {
     const long long rows = (long long)p.R0 * p.R1;
     if (p.N >= 4) return pack ? run_pack8<S, true>(p, stream) : run_pack8<S, false>(p, stream);
-    if (pack) hipLaunchKernelGGL(pack8_any_kernel<S>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL(unpack8_any_kernel<S>, dim3((unsigned)((rows * p.N + 255) / 256)), dim3(256), 0, stream, p);
+    if (pack) hipLaunchKernelGGL(pack8_any_kernel<S>, dim3((unsigned)std::min<long long>((rows + 3) / 4, kMostBlocks)), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(unpack8_any_kernel<S>, dim3((unsigned)std::min<long long>((rows * p.N + 255) / 256, kMostBlocks)), dim3(256), 0, stream, p);
 }
 
 void launch_pack8(const Pack8& p, bool pack, hipStream_t stream) {

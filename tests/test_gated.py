@@ -161,3 +161,16 @@ def test_abi_refuses_8_bits_of_only_some_inputs():
     assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**alone, g8=packed)), None) == 1
     # N = 3: the kernels for rows of any width have the same contract
     assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(**{**bwd, 'N': 3}, o=rows, g=rows, x8=packed)), None) == 1
+
+
+def test_abi_refuses_columns_past_its_counters():
+    """Column counts whose sums of three, or whose last stride, would pass the kernels' integers."""
+    from delrec import _lib
+    lib = _lib.load()
+    one, rows = ctypes.c_void_p(4096), _lib.Rows(4096, 8, 8)
+    for n in (2 ** 31 - 1, 2 ** 31 - 1023):
+        assert lib.delrec_pack8(ctypes.byref(_lib.Pack8Args(R0=1, R1=1, N=n, x=rows, p=_lib.Packed8(4096, 4096))), None) == 1
+        assert lib.delrec_gated_scan_fwd(ctypes.byref(_lib.GatedScanFwdArgs(T=1, B=1, N=n, z=rows, f=rows, h=rows, h_last=one)), None) == 1
+    bwd = dict(R0=1, R1=1, x=rows, w2=one, stats=one, du=rows, dx=rows, dw2=one)
+    assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(N=2 ** 30 + 1, **bwd)), None) == 1
+    assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(N=2 ** 30, **bwd)), None) == 3      # no workspace

@@ -198,3 +198,60 @@ def test_norm_residual_gradient_without_a_second_norm(dev, N, bad, used, checkpo
         assert torch.equal(got[k], want[k]), NAMES[k]
     assert torch.equal(got[2].cpu(), c['dxo'])
     assert got[5] is None if used == 'no next norm' else not got[5].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+@pytest.mark.parametrize('N', [2, 3])
+def test_norm_past_2_to_24_short_rows(dev, N, checkpoint):
+    """A workgroup a row would be more than 2^32 threads: the last rows against themselves alone."""
+    from delrec.gated import norm_gate_residual
+    R = (1 << 24) + 300
+    gen = torch.Generator(device=dev).manual_seed(1)
+    t = {k: torch.empty(R, N, dtype=BF16, device=dev).normal_(generator=gen) for k in ('o', 'g', 'x', 'dx', 'du')}
+    w = torch.rand(N, device=dev, generator=gen) + 0.5
+
+    def run(o, g, x, dx, du):
+        leaves = [v.detach().requires_grad_(True) for v in (o, g, x)]
+        y, u = norm_gate_residual(*leaves, w, w, w, checkpoint=checkpoint)
+        return y.detach(), u.detach(), *torch.autograd.grad((y, u), leaves, (dx, du))
+    far = slice(R - 300, R)
+    for a, b in zip(run(*t.values()), run(*(v[far].clone() for v in t.values()))):
+        assert torch.equal(a[far], b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('R,N', [((1 << 26) + 5, 1), ((1 << 32) // 3 + 7, 3)])
+def test_pack8_past_2_to_32_threads(dev, R, N):
+    from delrec.checkpoint8 import pack8, unpack8
+    x = torch.empty(R, N, dtype=BF16, device=dev).normal_(generator=torch.Generator(device=dev).manual_seed(2))
+    p = pack8(x)
+    far = slice(R - 9, R)
+    alone = pack8(x[far].clone())
+    assert torch.equal(p.q[far], alone.q) and torch.equal(p.scale[far], alone.scale)
+    assert torch.equal(unpack8(p)[far], unpack8(alone))
+
+
+@pytest.mark.gpu
+def test_scan_past_2_to_32_threads(dev):
+    """Rows of one channel take a wave each in 8 bits: 2^23 rows of 512 threads. And column sums of
+    2^28 columns, whose single row is the sum."""
+    from delrec.gated import gated_scan
+    T, B = 64, (1 << 23) + 3
+    gen = torch.Generator(device=dev).manual_seed(3)
+    z, f, dh = (torch.empty(T, B, 1, dtype=BF16, device=dev).normal_(generator=gen) for _ in range(3))
+
+    def run(z, f, dh):
+        leaves = [v.detach().requires_grad_(True) for v in (z, f)]
+        h, last = gated_scan(*leaves, checkpoint=True)
+        return h.detach(), last.detach()[None], *torch.autograd.grad(h, leaves, dh)
+    far = slice(B - 5, B)
+    for a, b in zip(run(z, f, dh), run(*(v[:, far].clone() for v in (z, f, dh)))):
+        assert torch.equal(a[:, far], b)
+    del z, f, dh
+    N = (1 << 28) + 70
+    z, f, dh = (torch.empty(1, 1, N, device=dev).normal_(generator=gen) for _ in range(3))
+    bias = torch.zeros(N, device=dev, requires_grad=True)
+    f.requires_grad_(True)
+    df, db = torch.autograd.grad(gated_scan(z, f, bias)[0], (f, bias), dh)
+    assert torch.equal(df.view(-1), db)
