@@ -225,38 +225,39 @@ __device__ __forceinline__ void enter_range(Maps<V>& m, const float* agg, size_t
     barrier_lds();                           // the buffer is free again
 }
 
-// A step's gate. f (and z, below) are vectors of any kind that get() reads, bias2 the bias times
-// log2(e); off: the step is past the row's end.
+// A step's gates and leaks (gate_small2). f (and z, below) are vectors of any kind that get() reads,
+// bias2 the bias times log2(e); off: the step is past the row's end.
 template <int V, class F>
-__device__ __forceinline__ void gate(const F& f, const float* bias2, bool off, float* k) {
+__device__ __forceinline__ void gate(const F& f, const float* bias2, bool off, float* m) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) k[j] = off ? 0.0f : gate_in2(fmaf(f.get(j), kLog2e, bias2[j]));
+    for (int j = 0; j < V; ++j) m[j] = off ? 0.0f : gate_small2(f.get_fma(j, kLog2e, bias2[j]));
 }
 
 // One step composed onto a piece's map (A, L), forwards (past the row's end L stays, and is not
 // multiplied by the shut gate's zero: it may be infinite)
 template <int V, bool MASK, class F>
-__device__ __forceinline__ void step_forward(const float* k, const F& z, bool fresh, bool off, float* A, float* L) {
+__device__ __forceinline__ void step_forward(const float* m, const F& z, bool fresh, bool off, float* A, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float from = MASK && fresh ? 0.0f : L[j], l = fmaf(k[j], z.get(j) - from, from);
+        const float from = MASK && fresh ? 0.0f : L[j], l = gate_step(m[j], from - z.get(j), from, z.get(j));
         L[j] = off ? L[j] : l;
-        // (the product keeps a cut's sign also for a leak of 0, where the fma gives +0)
-        if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
-        else A[j] = fmaf(-k[j], A[j], A[j]);
+        A[j] = MASK && fresh ? -1.0f : leak_times(m[j], A[j]);
     }
 }
 
-// and backwards, c -> a (dh + c)
+// and backwards, c -> a (dh + c), whose leak A is the forward map's
 template <int V, bool MASK, class D>
-__device__ __forceinline__ void step_backward(const float* k, const D& dh, bool fresh, bool off, float* A, float* L) {
+__device__ __forceinline__ void step_backward(const float* m, const D& dh, bool fresh, bool off, float* L) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float x = dh.get(j) + L[j], l = fmaf(-k[j], x, x);
+        const float l = leak_times(m[j], dh.get(j) + L[j]);
         L[j] = MASK && fresh ? 0.0f : off ? L[j] : l;
-        if (MASK) A[j] = fresh ? -1.0f : A[j] * (1.0f - k[j]);
-        else A[j] = fmaf(-k[j], A[j], A[j]);
     }
+}
+template <int V, bool MASK>
+__device__ __forceinline__ void step_leak(const float* m, bool fresh, float* A) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) A[j] = MASK && fresh ? -1.0f : leak_times(m[j], A[j]);
 }
 
 // Padding, and the steps past T of the last block. A wave whose lanes are all past their rows' ends
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
         const int t0 = tb + w * kSteps;
         if (p.states && w == 0 && ln.on) vstore<float, V>(p.states + (size_t)(tb / kBlk) * plane + at, h);
         Vec<S, V> z[kSteps], f[kSteps];
-        float k[kSteps][V], A[V], L[V], g[V];
+        float m[kSteps][V], A[V], L[V], g[V];
         bool fresh[kSteps];
         DELREC_COLS(j) A[j] = 1.0f, L[j] = g[j] = 0.0f;
         const bool any = MASK ? __any(t0 < len) : t0 < len, part = MASK ? !__all(t0 + kSteps <= len) : t0 + kSteps > len;
@@ -354,8 +355,8 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
             if (part) DELREC_STEPS(s)
                 if (t0 + s >= len) blank(z[s]), fresh[s] = false;
             DELREC_STEPS(s) {
-                gate<V>(f[s], bias, t0 + s >= len, k[s]);
-                step_forward<V, MASK>(k[s], z[s], fresh[s], t0 + s >= len, A, L);
+                gate<V>(f[s], bias, t0 + s >= len, m[s]);
+                step_forward<V, MASK>(m[s], z[s], fresh[s], t0 + s >= len, A, L);
             }
         }
         maps.put(buf, w, lane, A, L);
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
         compose<V, MASK, 1>(maps, buf, w, lane, h, g);
         if (MASK && !any) DELREC_STEPS(s) {
             blank(z[s]);
-            DELREC_COLS(j) k[s][j] = 0.0f;
+            DELREC_COLS(j) m[s][j] = 0.0f;
             fresh[s] = false;
         }
         yp.seek(t0), yp.start();
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(512, 4) gated_fwd_kernel(GatedScan p, int per_
             float y[V];
             DELREC_COLS(j) {
                 const float from = MASK && fresh[s] ? 0.0f : g[j];
-                y[j] = g[j] = fmaf(k[s][j], z[s].get(j) - from, from);
+                y[j] = g[j] = gate_step(m[s][j], from - z[s].get(j), from, z[s].get(j));
             }
             if (MASK && part && t0 + s >= len) DELREC_COLS(j) y[j] = 0.0f;
             if (t0 + s < T && ln.on) yp.store(y);
@@ -451,10 +452,10 @@ __global__ void __launch_bounds__(512, 4) gated_range_kernel(GatedScan p, int pe
             if (t0 + s >= len) blank(v[s]), fresh[s] = false;
         DELREC_STEPS(q) {
             const int s = BWD ? kSteps - 1 - q : q;
-            float k[V];
-            gate<V>(f[s], bias, t0 + s >= len, k);
-            if constexpr (BWD) step_backward<V, MASK>(k, v[s], fresh[s], t0 + s >= len, A, L);
-            else step_forward<V, MASK>(k, v[s], fresh[s], t0 + s >= len, A, L);
+            float m[V];
+            gate<V>(f[s], bias, t0 + s >= len, m);
+            if constexpr (BWD) step_backward<V, MASK>(m, v[s], fresh[s], t0 + s >= len, L), step_leak<V, MASK>(m, fresh[s], A);
+            else step_forward<V, MASK>(m, v[s], fresh[s], t0 + s >= len, A, L);
         }
     }
     maps.put(0, w, lane, A, L);
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
     int buf = 0;
     for (int tb = ts + (te - 1 - ts) / (nw * kSteps) * (nw * kSteps); tb >= ts; tb -= nw * kSteps, buf ^= 1) {
         const int t0 = tb + w * kSteps;
-        float k[kSteps][V], d[kSteps][V], h[V], g[V], mine[V];
+        float m[kSteps][V], d[kSteps][V], h[V], g[V], mine[V];
         Vec<S, V> dh[kSteps];
         typename std::conditional<PACK, Vec8<V>, Vec<S, V>>::type z[kSteps];
         bool fresh[kSteps];
@@ -541,12 +542,12 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
             }
             DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
             if (!MASK || any) DELREC_STEPS(s) {
-                gate<V>(f[s], bias, t0 + s >= len, k[s]);
-                step_forward<V, MASK>(k[s], z[s], fresh[s], t0 + s >= len, A, L);
+                gate<V>(f[s], bias, t0 + s >= len, m[s]);
+                step_forward<V, MASK>(m[s], z[s], fresh[s], t0 + s >= len, A, L);
             }
             fmap.put(buf, w, lane, A, L);
-            DELREC_COLS(j) A[j] = 1.0f, L[j] = 0.0f;
-            if (!MASK || any) DELREC_STEPS_BACK(s) step_backward<V, MASK>(k[s], dh[s], fresh[s], t0 + s >= len, A, L);
+            DELREC_COLS(j) L[j] = 0.0f;
+            if (!MASK || any) DELREC_STEPS_BACK(s) step_backward<V, MASK>(m[s], dh[s], fresh[s], t0 + s >= len, L);
             rmap.put(buf, w, lane, A, L);
         }
         barrier_lds();
@@ -558,29 +559,32 @@ __global__ void __launch_bounds__(512, 4) gated_bwd_kernel(GatedScan p, int per_
         DELREC_COLS(j) blk[j] = 0.0f;
         if (MASK && !any) DELREC_STEPS(s) {
             blank(dh[s]), blank(z[s]);
-            DELREC_COLS(j) k[s][j] = 0.0f;
+            DELREC_COLS(j) m[s][j] = 0.0f;
             fresh[s] = false;
         }
         // d_t = h_{t-1} - z_t
         DELREC_STEPS(s) DELREC_COLS(j) {
             const float from = MASK && fresh[s] ? 0.0f : mine[j];
             d[s][j] = from - z[s].get(j);
-            mine[j] = fmaf(-k[s][j], d[s][j], from);
+            mine[j] = gate_step(m[s][j], d[s][j], from, z[s].get(j));
         }
         // (outside a row the gradients are zeros and the carry stays, also an infinite one)
         dzp.seek(t0 + kSteps - 1), dfp.seek(t0 + kSteps - 1);
         dzp.start(), dfp.start();
-        DELREC_STEPS_BACK(s) {
+        DELREC_STEPS_BACK(s) if (MASK || t0 + s < T) {
             float oz[V], of[V];
             DELREC_COLS(j) {
-                const bool off = t0 + s >= len;
-                const float lam = dh[s].get(j) + g[j];
-                oz[j] = off ? 0.0f : lam * k[s][j];
-                of[j] = off ? 0.0f : fmaf(-k[s][j], oz[j], oz[j]) * d[s][j];
-                g[j] = MASK && fresh[s] ? 0.0f : lam - oz[j];
+                // the smaller of k lam and a lam, the larger, and k a lam
+                const bool off = MASK && t0 + s >= len, leak = leak_kept(m[s][j]);
+                const float lam = dh[s].get(j) + g[j], few = fabsf(m[s][j]) * lam, most = lam - few;
+                oz[j] = off ? 0.0f : leak ? most : few;
+                of[j] = off ? 0.0f : fmaf(-fabsf(m[s][j]), few, few) * d[s][j];
+                g[j] = MASK && fresh[s] ? 0.0f : off ? lam : leak ? few : most;
                 blk[j] += of[j];
             }
             if (t0 + s < T && ln.on) dzp.store(oz, own), dfp.store(of, own);
+            dzp.prev(), dfp.prev();
+        } else {
             dzp.prev(), dfp.prev();
         }
         // the bias sum in two levels, within a block and over blocks: one long chain of 32-bit

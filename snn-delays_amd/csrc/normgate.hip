@@ -61,9 +61,9 @@ __global__ void __launch_bounds__(kNb) norm_any_fwd_kernel(NormGate p) {
         float r = 0.0f, r2 = 0.0f, s = 0.0f;
         if (p.h) {
             for (int n = threadIdx.x; n < N; n += kNb) {
-                const float k = gate_in(to_f32(row_ptr<const S>(p.f, row, p.R1)[n]) + (p.bias ? p.bias[n] : 0.0f));
-                const float h = p.h[row * N + n];
-                p.h_out[row * N + n] = fmaf(k, to_f32(row_ptr<const S>(p.z, row, p.R1)[n]) - h, h);
+                const float f = to_f32(row_ptr<const S>(p.f, row, p.R1)[n]), z = to_f32(row_ptr<const S>(p.z, row, p.R1)[n]);
+                const float m = gate_small2(fmaf(f, kLog2e, p.bias ? p.bias[n] * kLog2e : 0.0f)), h = p.h[row * N + n];
+                p.h_out[row * N + n] = gate_step(m, h - z, h, z);
             }
             __syncthreads();
         }
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_fwd_kernel(NormGate 
                     const auto h = vload<float, 4>(p.h + row * N + c.n0[e]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float k = gate_in(f.get(j) + (p.bias ? bias[e][j] : 0.0f));
-                        o[e][j] = fmaf(k, z.get(j) - h.get(j), h.get(j));
+                        const float m = gate_small2(f.get_fma(j, kLog2e, p.bias ? bias[e][j] * kLog2e : 0.0f));
+                        o[e][j] = gate_step(m, h.get(j) - z.get(j), h.get(j), z.get(j));
                     }
                 }
             }

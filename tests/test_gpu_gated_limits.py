@@ -255,3 +255,46 @@ def test_scan_past_2_to_32_threads(dev):
     f.requires_grad_(True)
     df, db = torch.autograd.grad(gated_scan(z, f, bias)[0], (f, bias), dh)
     assert torch.equal(df.view(-1), db)
+
+
+def saturated_case(T, B, N, masks, seed):
+    """No input, so that states and gradients are products of gates and leaks: the leaks between e^-4
+    and e^-24 at three steps, the gate e^-60 at the others."""
+    g = torch.Generator().manual_seed(seed)
+    bias = torch.rand(N, generator=g) * 4 - 2
+    x = torch.full((T, B, N), 60.0)
+    for t in {0, T // 2, T - 1}:
+        x[t] = -4 - 20 * torch.rand(B, N, generator=g)
+    c = dict(z=torch.zeros(T, B, N), f=x - bias, bias=bias, h0=1 + torch.rand(B, N, generator=g), dh=torch.zeros(T, B, N),
+             dlast=1 + torch.rand(B, N, generator=g), starts=None, lengths=None)
+    if masks:
+        c['starts'], c['lengths'] = torch.zeros(T, B, dtype=torch.bool), torch.full((B,), T)
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('checkpoint', [False, True])
+@pytest.mark.parametrize('masks', [False, True])
+@pytest.mark.parametrize('T,B,N', [(1, 2, 5), (3, 2, 70), (70, 2, 1), (70, 3, 70), (330, 2, 6)])
+def test_scan_leaks_keep_their_digits(dev, T, B, N, masks, checkpoint):
+    """Each value to its own size. A gate or leak is off by at most 6e-8 (|f + bias| + 2 |bias|) + 4e-7,
+    5e-6 here, and a value is a product of three such leaks, and one more gate and leak in df: 3e-5."""
+    c = saturated_case(T, B, N, masks, seed=51)
+    got = run_scan(c, dev, checkpoint)
+    d = {k: v.double() for k, v in c.items() if k not in ('starts', 'lengths')}
+    ref = og.scan_grads(d['z'], d['f'], d['bias'], d['h0'], c['starts'], c['lengths'], d['dh'], d['dlast'], checkpoint)
+    for name, a, b in zip(('h', 'last', 'dz', 'df', 'db', 'dh0'), got, ref):
+        bad = ~((a.double().cpu() - b).abs() <= 3e-5 * b.abs() + 1e-36)
+        assert not bad.any(), (name, int(bad.sum()), float(((a.double().cpu() - b).abs() / b.abs()).nan_to_num().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('N', [3, 70, 700, 9000])
+def test_step_leaks_keep_their_digits(dev, N):
+    from delrec.gated import gated_step
+    c = saturated_case(1, 4, N, False, seed=52)
+    t = {k: c[k].to(dev) for k in ('z', 'f', 'bias', 'h0')}
+    w = torch.ones(N, device=dev)
+    h = gated_step(t['z'][0], t['f'][0], t['z'][0], t['h0'], t['h0'], w, w, bias=t['bias'])[2]
+    ref = c['h0'].double() * torch.sigmoid(c['f'][0].double() + c['bias'].double())
+    assert ((h.double().cpu() - ref).abs() <= 3e-5 * ref).all()
