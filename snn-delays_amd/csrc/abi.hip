@@ -797,9 +797,15 @@ int delrec_query_workspace(int32_t kind, int32_t T, int32_t B, int32_t N, int32_
         case DELREC_WS_READOUT_CE:
             c.take<float>((size_t)B);
             break;
-        case DELREC_WS_GATED_FWD: c.take<float>(gated_fwd_ws(T, B, N)); break;
-        case DELREC_WS_GATED_BWD: c.take<float>(gated_bwd_ws(T, B, N)); break;
-        case DELREC_WS_NORM_GATE_BWD: c.take<float>(norm_gate_bwd_ws((long long)T * B, N)); break;
+        case DELREC_WS_GATED_FWD:
+        case DELREC_WS_GATED_BWD:
+            if (!gated_scan_sizes_ok(T, B, N)) return DELREC_ERR_ARG;
+            c.take<float>(kind == DELREC_WS_GATED_FWD ? gated_fwd_ws(T, B, N) : gated_bwd_ws(T, B, N));
+            break;
+        case DELREC_WS_NORM_GATE_BWD:
+            if (!norm_gate_sizes_ok(T, B, N)) return DELREC_ERR_ARG;
+            c.take<float>(norm_gate_bwd_ws((long long)T * B, N));
+            break;
         default: return DELREC_ERR_ARG;
     }
     *bytes = c.used;

@@ -4,20 +4,27 @@
 
 #include "kernels.h"
 
+namespace delrec {
+
+// rows fit 31 bits, and so do columns with room for a workgroup's stride past them
+static bool sizes_ok(int R0, int R1, int N) {
+    return R0 > 0 && R1 > 0 && N > 0 && N <= 0x7fffffff - 1024 && (long long)R0 * R1 <= 0x7fffffffLL &&
+           (long long)R0 * R1 <= (0x7fffffffLL * 64) / N;
+}
+
+// (the last of up to 128 ranges of time ends at most as many blocks of 64 steps past T)
+bool gated_scan_sizes_ok(int T, int B, int N) { return sizes_ok(T, B, N) && T <= 0x7fffffff - 128 * DELREC_GATED_BLOCK; }
+
+// (a norm's three column sums side by side count in 32 bits)
+bool norm_gate_sizes_ok(int R0, int R1, int N) { return sizes_ok(R0, R1, N) && N >= 2 && N <= 1 << 30; }
+
+}  // namespace delrec
+
 using namespace delrec;
 
 namespace {
 
 int done() { return hipGetLastError() == hipSuccess ? DELREC_OK : DELREC_ERR_LAUNCH; }
-
-// rows fit 31 bits, and so do columns with room for a workgroup's stride past them
-bool sizes_ok(int R0, int R1, int N) {
-    return R0 > 0 && R1 > 0 && N > 0 && N <= 0x7fffffff - 1024 && (long long)R0 * R1 <= 0x7fffffffLL &&
-           (long long)R0 * R1 <= (0x7fffffffLL * 64) / N;
-}
-
-// (a norm's three column sums side by side count in 32 bits)
-bool norm_sizes_ok(int R0, int R1, int N) { return sizes_ok(R0, R1, N) && N >= 2 && N <= 1 << 30; }
 
 bool pair_ok(const delrec_packed8& p) { return (p.q == nullptr) == (p.scale == nullptr); }
 
@@ -33,7 +40,7 @@ bool eights_ok(const delrec_packed8& o8, const delrec_packed8& g8, const delrec_
 extern "C" {
 
 int delrec_gated_scan_fwd(const delrec_gated_scan_fwd_args* a, void* stream) {
-    if (!a || !sizes_ok(a->T, a->B, a->N)) return DELREC_ERR_ARG;
+    if (!a || !gated_scan_sizes_ok(a->T, a->B, a->N)) return DELREC_ERR_ARG;
     if (!a->z.data || !a->f.data || !a->h.data || !a->h_last) return DELREC_ERR_ARG;
     if (!pair_ok(a->z8) || !pair_ok(a->f8) || (a->z8.q == nullptr) != (a->f8.q == nullptr)) return DELREC_ERR_ARG;
     if (a->z8.q && !a->states) return DELREC_ERR_ARG;
@@ -49,7 +56,7 @@ int delrec_gated_scan_fwd(const delrec_gated_scan_fwd_args* a, void* stream) {
 }
 
 int delrec_gated_scan_bwd(const delrec_gated_scan_bwd_args* a, void* stream) {
-    if (!a || !sizes_ok(a->T, a->B, a->N)) return DELREC_ERR_ARG;
+    if (!a || !gated_scan_sizes_ok(a->T, a->B, a->N)) return DELREC_ERR_ARG;
     if (!pair_ok(a->z8) || !pair_ok(a->f8) || (a->z8.q == nullptr) != (a->f8.q == nullptr)) return DELREC_ERR_ARG;
     if (!a->z8.q && (!a->z.data || !a->f.data)) return DELREC_ERR_ARG;
     if (!a->states || !a->dh.data || !a->dz.data || !a->df.data) return DELREC_ERR_ARG;
@@ -66,7 +73,7 @@ int delrec_gated_scan_bwd(const delrec_gated_scan_bwd_args* a, void* stream) {
 }
 
 int delrec_gated_step(const delrec_gated_step_args* a, void* stream) {
-    if (!a || !norm_sizes_ok(1, a->B, a->N)) return DELREC_ERR_ARG;
+    if (!a || !norm_gate_sizes_ok(1, a->B, a->N)) return DELREC_ERR_ARG;
     if (!a->z.data || !a->f.data || !a->g.data || !a->x.data || !a->h || !a->h_out || !a->x_out) return DELREC_ERR_ARG;
     if (!a->w || !a->scale || (a->w2 && !a->u) || !(a->eps >= 0.0f)) return DELREC_ERR_ARG;
     if (!a->bf16 && a->x_bf16) return DELREC_ERR_UNSUPPORTED;
@@ -79,7 +86,7 @@ int delrec_gated_step(const delrec_gated_step_args* a, void* stream) {
 }
 
 int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream) {
-    if (!a || !norm_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
+    if (!a || !norm_gate_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
     const bool block = a->o.data != nullptr;
     if (!a->x.data || !(a->eps >= 0.0f) || (a->w2 && !a->u)) return DELREC_ERR_ARG;
     if (block && (!a->g.data || !a->w || !a->scale || !a->x_out)) return DELREC_ERR_ARG;
@@ -95,7 +102,7 @@ int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream) {
 }
 
 int delrec_norm_gate_bwd(const delrec_norm_gate_bwd_args* a, void* stream) {
-    if (!a || !norm_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
+    if (!a || !norm_gate_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
     const bool block = a->o.data || a->o8.q;
     if (!eights_ok(a->o8, a->g8, a->x8, block)) return DELREC_ERR_ARG;
     if ((!a->x.data && !a->x8.q) || !a->stats || !a->dx.data) return DELREC_ERR_ARG;

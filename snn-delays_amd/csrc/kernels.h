@@ -596,6 +596,8 @@ struct GatedScan {               // forward and backward of the gated linear rec
     float* ws;                   // workspace, gated_fwd_ws / gated_bwd_ws floats
     int first;                   // set by the launcher: the launch's first workgroup of channels
 };
+bool gated_scan_sizes_ok(int T, int B, int N);   // what the entry points take (gated_abi.hip)
+bool norm_gate_sizes_ok(int R0, int R1, int N);
 size_t gated_fwd_ws(int T, int B, int N);   // floats
 size_t gated_bwd_ws(int T, int B, int N);
 void launch_gated_fwd(const GatedScan& p, hipStream_t stream);

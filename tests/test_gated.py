@@ -174,3 +174,19 @@ def test_abi_refuses_columns_past_its_counters():
     bwd = dict(R0=1, R1=1, x=rows, w2=one, stats=one, du=rows, dx=rows, dw2=one)
     assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(N=2 ** 30 + 1, **bwd)), None) == 1
     assert lib.delrec_norm_gate_bwd(ctypes.byref(_lib.NormGateBwdArgs(N=2 ** 30, **bwd)), None) == 3      # no workspace
+
+
+def test_abi_refuses_steps_past_its_counters():
+    from delrec import _lib
+    lib = _lib.load()
+    one, rows = ctypes.c_void_p(4096), _lib.Rows(4096, 1, 1)
+    for t in (2 ** 31 - 1, 2 ** 31 - 128 * 64):
+        assert lib.delrec_gated_scan_fwd(ctypes.byref(_lib.GatedScanFwdArgs(T=t, B=1, N=1, z=rows, f=rows, h=rows, h_last=one)), None) == 1
+        args = _lib.GatedScanBwdArgs(T=t, B=1, N=1, z=rows, f=rows, states=one, dh=rows, dz=rows, df=rows)
+        assert lib.delrec_gated_scan_bwd(ctypes.byref(args), None) == 1
+    args = _lib.GatedScanFwdArgs(T=2 ** 31 - 128 * 64 - 1, B=1, N=1, z=rows, f=rows, h=rows, h_last=one)
+    assert lib.delrec_gated_scan_fwd(ctypes.byref(args), None) == 3      # no workspace
+    size = ctypes.c_size_t(0)
+    for kind, t, b, n in ((_lib.WS_GATED_FWD, 2 ** 31 - 1, 1, 1), (_lib.WS_GATED_BWD, 1, 1, 2 ** 31 - 1),
+                          (_lib.WS_NORM_GATE_BWD, 1, 1, 2 ** 31 - 1), (_lib.WS_NORM_GATE_BWD, 4, 1, 1)):
+        assert lib.delrec_query_workspace(kind, t, b, n, 1, 0, ctypes.byref(size)) == 1
