@@ -13,6 +13,7 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
+#include <mutex>
 #include <sstream>
 #include <stdexcept>
 #include <string>
@@ -87,7 +88,8 @@ void once_differentiable(const char* what) {
 }
 
 // A node of the graph: what it keeps is freed after its backward, and a second backward through it
-// raises torch's own error.
+// raises torch's own error. Under the node's mutex, since backward passes of several threads may go
+// through one graph.
 struct KeptNode : public Node {
     std::vector<SavedVariable> kept;
     bool released = false;
@@ -96,6 +98,7 @@ struct KeptNode : public Node {
         for (const Tensor& t : ts) kept.emplace_back(t, false);
     }
     variable_list take() {
+        std::lock_guard<std::mutex> lock(mutex_);
         if (released) throw std::runtime_error(torch::autograd::ERR_BACKWARD_TWICE);
         variable_list v;
         v.reserve(kept.size());
@@ -103,6 +106,7 @@ struct KeptNode : public Node {
         return v;
     }
     void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
         kept.clear();
         released = true;
     }

@@ -298,3 +298,31 @@ def test_step_leaks_keep_their_digits(dev, N):
     h = gated_step(t['z'][0], t['f'][0], t['z'][0], t['h0'], t['h0'], w, w, bias=t['bias'])[2]
     ref = c['h0'].double() * torch.sigmoid(c['f'][0].double() + c['bias'].double())
     assert ((h.double().cpu() - ref).abs() <= 3e-5 * ref).all()
+
+
+@pytest.mark.gpu
+def test_backward_passes_of_two_threads_through_one_graph(dev):
+    """Each either gives the graph's gradients or raises that they are gone, as torch's own nodes."""
+    import threading
+    from delrec.gated import gated_scan, rms_norm
+    z = torch.randn(70, 2, 8, device=dev, requires_grad=True)
+    f, w = torch.randn(70, 2, 8, device=dev), torch.ones(8, device=dev)
+    (want,) = torch.autograd.grad(rms_norm(gated_scan(z, f)[0], w).sum(), z)
+    for _ in range(20):
+        loss = rms_norm(gated_scan(z, f)[0], w).sum()
+        done, start = [], threading.Barrier(4)
+
+        def work():
+            start.wait()
+            try:
+                done.append(torch.autograd.grad(loss, z)[0])
+            except RuntimeError as e:
+                assert 'second time' in str(e)
+                done.append(None)
+        threads = [threading.Thread(target=work) for _ in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(done) == 4
+        assert all(g is None or torch.equal(g, want) for g in done)
