@@ -364,9 +364,14 @@ class RNN_gated(torch.nn.Module):
     """A residual stack of gated linear recurrences over (T, B, N): ``Linear -> rms_norm ->
     GatedBlock ... -> Linear``, one block for each entry of ``config.hidden_layers`` (all of one
     width). Trains with ``delrec.training.mem`` like the ``SNN_*`` classes; ``step`` runs it one
-    time step at a time on streaming input. The residual stream is fp32, also under
-    ``torch.autocast('cuda', torch.bfloat16)``. ``config.checkpoint8`` (default False): the
-    blocks keep their activations in 8 bits for the backward pass."""
+    time step at a time on streaming input. Parameters and the residual stream are fp32;
+    activations are bf16 under ``torch.autocast('cuda', torch.bfloat16)`` (a model converted to
+    bf16, and autocast to fp16, raise). ``config.checkpoint8`` (default False): the blocks keep
+    their activations in 8 bits for the backward pass.
+
+    Of the config it takes ``input_size``, ``hidden_layers``, ``output_size`` and ``bias``;
+    ``use_batch_norm`` and a ``feedforward_dropout_rate`` raise, Linears start as
+    ``torch.nn.Linear`` does."""
 
     def __init__(self, config):
         super().__init__()
@@ -374,6 +379,10 @@ class RNN_gated(torch.nn.Module):
         if len(widths) != 1:
             raise ValueError(f'RNN_gated needs hidden layers of one width, got {config.hidden_layers}')
         N = widths.pop()
+        if config.use_batch_norm:
+            _batch_norm(config, N)
+        if config.feedforward_dropout_rate:
+            raise NotImplementedError(f'feedforward_dropout_rate={config.feedforward_dropout_rate}: RNN_gated has no dropout')
         self.config = config
         self.checkpoint = bool(getattr(config, 'checkpoint8', False))
         self.embed = torch.nn.Linear(config.input_size, N, bias=config.bias)

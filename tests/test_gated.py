@@ -190,3 +190,14 @@ def test_abi_refuses_steps_past_its_counters():
     for kind, t, b, n in ((_lib.WS_GATED_FWD, 2 ** 31 - 1, 1, 1), (_lib.WS_GATED_BWD, 1, 1, 2 ** 31 - 1),
                           (_lib.WS_NORM_GATE_BWD, 1, 1, 2 ** 31 - 1), (_lib.WS_NORM_GATE_BWD, 4, 1, 1)):
         assert lib.delrec_query_workspace(kind, t, b, n, 1, 0, ctypes.byref(size)) == 1
+
+
+@pytest.mark.parametrize('field,value', [('use_batch_norm', True), ('feedforward_dropout_rate', 0.1)])
+def test_model_refuses_what_it_does_not_do(field, value):
+    from configs.perf_MEM import Config
+    from delrec.networks import RNN_gated
+    cfg = Config()
+    RNN_gated(cfg)
+    setattr(cfg, field, value)
+    with pytest.raises(NotImplementedError, match=field):
+        RNN_gated(cfg)
