@@ -379,9 +379,9 @@ class RNN_gated(torch.nn.Module):
         if len(widths) != 1:
             raise ValueError(f'RNN_gated needs hidden layers of one width, got {config.hidden_layers}')
         N = widths.pop()
-        if config.use_batch_norm:
+        if getattr(config, 'use_batch_norm', False):
             _batch_norm(config, N)
-        if config.feedforward_dropout_rate:
+        if getattr(config, 'feedforward_dropout_rate', 0.0):
             raise NotImplementedError(f'feedforward_dropout_rate={config.feedforward_dropout_rate}: RNN_gated has no dropout')
         self.config = config
         self.checkpoint = bool(getattr(config, 'checkpoint8', False))

@@ -201,3 +201,9 @@ def test_model_refuses_what_it_does_not_do(field, value):
     setattr(cfg, field, value)
     with pytest.raises(NotImplementedError, match=field):
         RNN_gated(cfg)
+
+
+def test_model_takes_a_config_of_its_own_four_fields():
+    from types import SimpleNamespace
+    from delrec.networks import RNN_gated
+    RNN_gated(SimpleNamespace(input_size=3, hidden_layers=[32, 32], output_size=2, bias=False))
