@@ -87,6 +87,15 @@ void once_differentiable(const char* what) {
     if (at::GradMode::is_enabled()) throw std::runtime_error(text(what, " has no second derivative (create_graph=True)"));
 }
 
+// Forward calls can be captured in a graph. A captured backward pass has ended the process (a
+// segmentation fault in hipStreamEndCapture, cause not known): it is refused before it launches.
+void refuse_capture(const char* what, const Tensor& t) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(t.get_device()).stream(), &status) == hipSuccess &&
+        status != hipStreamCaptureStatusNone)
+        throw std::runtime_error(text("the backward pass of ", what, " cannot be captured in a graph"));
+}
+
 // A node of the graph: what it keeps is freed after its backward, and a second backward through it
 // raises torch's own error. Under the node's mutex, since backward passes of several threads may go
 // through one graph.
@@ -217,9 +226,10 @@ struct GatedScanBackward : public KeptNode {
     at::ScalarType type = at::kFloat;
 
     variable_list apply(variable_list&& grads) override {
-        once_differentiable("gated_scan");
         const variable_list s = take();
         const Tensor& states = s[7];
+        refuse_capture("gated_scan", states);
+        once_differentiable("gated_scan");
         const c10::DeviceGuard guard(states.device());
         const int B = (int)states.size(1), N = (int)states.size(2);
         const auto f32 = states.options();
@@ -348,9 +358,10 @@ struct NormGateBackward : public KeptNode {
     bool block = false;
 
     variable_list apply(variable_list&& grads) override {
-        once_differentiable("norm_gate_residual");
         const variable_list s = take();
         const Tensor &w = s[9], &scale = s[10], &w2 = s[11], &stats = s[12];
+        refuse_capture("norm_gate_residual", stats);
+        once_differentiable("norm_gate_residual");
         const Tensor dxo = block ? rows_form(grads[0]) : Tensor();
         const Tensor du = !block ? rows_form(grads[0]) : w2.defined() ? rows_form(grads[1]) : Tensor();
         if (!dxo.defined() && !du.defined()) return variable_list(6);

@@ -11,7 +11,8 @@ where ``rms(v) = v / sqrt(mean(v^2) + eps)`` over the last axis. The recurrence 
 integrator of ``LIFNode(decay_input=True)`` without its threshold, with a leak that each step's
 input sets. Activations are fp32 or bf16; states, gates, norms and sums are in 32 bits. With
 ``checkpoint=True`` an operator keeps what its backward pass reads in 8 bits
-(``delrec.checkpoint8``). No counterpart in the reference.
+(``delrec.checkpoint8``). Gradients are first-order and reverse-mode; forward calls can be
+captured in a graph, backward passes cannot. No counterpart in the reference.
 """
 
 import torch

@@ -326,3 +326,41 @@ def test_backward_passes_of_two_threads_through_one_graph(dev):
             t.join()
         assert len(done) == 4
         assert all(g is None or torch.equal(g, want) for g in done)
+
+
+@pytest.mark.gpu
+def test_captured_backward_is_refused(dev):
+    """The nodes, called by themselves while the stream is capturing: an error, nothing launched, and
+    the capture, the graph and the nodes stay usable."""
+    from delrec.gated import gated_scan, rms_norm
+    z = torch.randn(70, 2, 8, device=dev, requires_grad=True)
+    h, last = gated_scan(z, z)
+    u = rms_norm(z, torch.ones(8, device=dev))
+    out = torch.ones(3, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        out.mul_(2.0)
+        for node, grads in ((h.grad_fn, (h, last)), (u.grad_fn, (u,))):
+            with pytest.raises(RuntimeError, match='captured'):
+                node(*grads)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert out.tolist() == [8.0] * 3
+    want = torch.autograd.grad(h.sum(), z, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(h.sum(), z)[0], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.skip(reason='a captured backward pass through the autograd engine has ended the process in '
+                         'hipStreamEndCapture; its cause is not known, and the nodes refuse it')
+def test_captured_backward(dev):
+    from delrec.gated import gated_scan
+    z = torch.randn(70, 2, 8, device=dev, requires_grad=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (dz,) = torch.autograd.grad(gated_scan(z, z)[0].sum(), z)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dz, torch.autograd.grad(gated_scan(z, z)[0].sum(), z)[0])
