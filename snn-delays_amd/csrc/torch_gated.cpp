@@ -296,8 +296,12 @@ py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTens
         lengths = lengths.to(at::kLong).contiguous();
     }
     if (T == 0) {
+        // no step: the output is a tensor of the graph all the same, and its gradients are zeros
+        Tensor h = z * f;
+        if (bias.defined()) h = h + vector_arg(bias, N, z, "bias");
+        if (h0.defined()) h = h + h0;
         const Tensor last = h0.defined() ? h0.clone() : at::zeros({B, N}, z.options().dtype(at::kFloat));
-        return py::make_tuple(at::zeros_like(z), last);
+        return py::make_tuple(h.to(z.scalar_type()), last);
     }
     if (wanted({&z, &f, &bias, &h0})) return pair_of(scan_with_graph(z, f, bias, h0, starts, lengths, checkpoint));
     return pair_of(scan_forward(rows_form(z), rows_form(f), vector_arg(bias, N, z, "bias"), h0.defined() ? h0.contiguous() : h0,

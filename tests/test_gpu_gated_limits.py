@@ -364,3 +364,21 @@ def test_captured_backward(dev):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(dz, torch.autograd.grad(gated_scan(z, z)[0].sum(), z)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [FP32, BF16])
+def test_scan_without_steps_has_gradients(dev, dtype):
+    """No step: outputs of the right shapes and types whose gradients are zeros, the state's aside."""
+    from delrec.gated import gated_scan
+    z, f = (torch.empty(0, 3, 4, dtype=dtype, device=dev, requires_grad=True) for _ in range(2))
+    bias, h0 = torch.ones(4, device=dev, requires_grad=True), torch.randn(3, 4, device=dev, requires_grad=True)
+    h, last = gated_scan(z, f, bias, h0)
+    assert h.shape == (0, 3, 4) and h.dtype == dtype and torch.equal(last, h0)
+    grads = torch.autograd.grad(h.float().sum(), (z, f, bias, h0), retain_graph=True)
+    assert [g.shape for g in grads] == [t.shape for t in (z, f, bias, h0)] and not any(g.any() for g in grads)
+    assert torch.equal(torch.autograd.grad(h.float().sum() + last.sum(), h0)[0], torch.ones_like(h0))
+    h, last = gated_scan(z.detach(), f.detach())
+    assert h.dtype == dtype and not h.requires_grad and not last.any()
+    with pytest.raises(ValueError):
+        gated_scan(z, f, torch.ones(5, device=dev))
