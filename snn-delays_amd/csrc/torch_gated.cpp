@@ -528,14 +528,21 @@ Tensor unpack8(Tensor q, Tensor scale, std::vector<int64_t> shape, py::object dt
     if (!q.is_cuda()) throw std::runtime_error(text("delrec-mi355x unpacks 8 bits with a HIP kernel on the GPU; they are on ", q.device()));
     const auto type = torch::python::detail::py_object_to_dtype(dtype);
     const int64_t groups = q.dim() == 2 ? (q.size(1) + DELREC_PACK8_GROUP - 1) / DELREC_PACK8_GROUP : 0;
-    if ((type != at::kFloat && type != at::kBFloat16) || q.dim() != 2 || q.scalar_type() != at::kChar || q.stride(1) != 1 || q.stride(0) != (q.size(1) + 3) / 4 * 4 ||
+    if ((type != at::kFloat && type != at::kBFloat16) || q.dim() != 2 || q.scalar_type() != at::kChar ||
         scale.dim() != 2 || scale.size(0) != q.size(0) || scale.size(1) != groups || scale.scalar_type() != at::kFloat ||
-        scale.device() != q.device() || !scale.is_contiguous())
+        scale.device() != q.device())
         refuse(text("not a packed tensor: q ", describe(q), ", scale ", describe(scale), ", type ", type));
     int64_t n = 1;
     for (int64_t v : shape) n *= v;
     if (n != q.numel() || shape.empty() || shape.back() != q.size(1)) refuse(text("q ", q.sizes(), " does not fill ", at::IntArrayRef(shape)));
     const c10::DeviceGuard guard(q.device());
+    // copies (a tensor saved on the host and brought back) have lost the rows' pitch
+    const int64_t pitch = (q.size(1) + 3) / 4 * 4;
+    if (n && (q.stride(0) != pitch || (q.stride(1) != 1 && q.size(1) > 1) || (uintptr_t)q.data_ptr() % 4)) {
+        const Tensor own = at::empty({q.size(0), pitch}, q.options());
+        q = own.narrow(1, 0, q.size(1)).copy_(q);
+    }
+    scale = scale.contiguous();
     const Tensor out = at::empty(shape, q.options().dtype(type));
     if (n) {
         delrec_pack8_args a{};

@@ -382,3 +382,33 @@ def test_scan_without_steps_has_gradients(dev, dtype):
     assert h.dtype == dtype and not h.requires_grad and not last.any()
     with pytest.raises(ValueError):
         gated_scan(z, f, torch.ones(5, device=dev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('shape', [(5, 70), (1, 70), (7, 3), (6, 1), (2, 3, 64)])
+def test_packed_tensors_may_be_copied(dev, shape):
+    """Copies lose the pitch of the 8-bit rows and keep their values: cloned, sent to the host and
+    back, transposed in memory, sliced."""
+    from delrec.checkpoint8 import Packed8, pack8, unpack8
+    x = rnd(torch.Generator().manual_seed(61), *shape).to(dev)
+    p = pack8(x)
+    want = unpack8(p)
+    for move in (torch.clone, lambda t: t.cpu().to(dev), lambda t: t.contiguous(), lambda t: t.t().contiguous().t(),
+                 lambda t: torch.cat([t[:, :1], t], 1)[:, 1:], lambda t: torch.cat([t, t])[t.shape[0]:]):
+        assert torch.equal(unpack8(Packed8(move(p.q), move(p.scale), p.shape, p.dtype)), want)
+    with pytest.raises(ValueError):
+        unpack8(Packed8(p.q[:-1], p.scale, p.shape, p.dtype))
+    with pytest.raises(ValueError):
+        unpack8(Packed8(p.q.float(), p.scale, p.shape, p.dtype))
+
+
+@pytest.mark.gpu
+def test_linear8_with_its_input_saved_on_the_host(dev):
+    from delrec.checkpoint8 import Linear8
+    lin = Linear8(70, 33).to(dev)
+    x = rnd(torch.Generator().manual_seed(62), 5, 70).to(dev).requires_grad_(True)
+    want = torch.autograd.grad(lin(x).square().sum(), (x, lin.weight, lin.bias))
+    with torch.autograd.graph.save_on_cpu():
+        y = lin(x)
+    for a, b in zip(torch.autograd.grad(y.square().sum(), (x, lin.weight, lin.bias)), want):
+        assert torch.equal(a, b)
