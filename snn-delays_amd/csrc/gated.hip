@@ -14,10 +14,10 @@
 // inputs once more), the second starts from the composition of the ranges before it.
 //
 // Bound by memory where the channels fill the GPU: at T250 B128 N512 bf16 23 us forward (98 MB,
-// 4.3 TB/s) and 34 backward (164 MB, 4.8 TB/s, what a large copy reaches); next, by vector issue
-// (some 45 instructions a value backward, two of them at a quarter of the rate). A block's loads are
-// not taken ahead of the one before: two to four workgroups a CU hide them, and their registers
-// cost one of these.
+// 4.3 TB/s) and 34 backward (164 MB, 4.8 TB/s, what a large copy reaches); next, by vector issue (24
+// instructions a value forward and 42 backward, two of them at a quarter of the rate; 49 and 44 with 8
+// bits). A block's loads are not taken ahead of the one before: two to four workgroups a CU hide
+// them, and their registers cost one of these.
 //
 // The forward keeps the state before every 64th step in 32 bits (1/16 byte a value and step); the
 // backward starts its blocks there and recomputes the states between from z and f, which it needs
@@ -609,17 +609,17 @@ struct Plan {
 };
 
 // Two columns a lane. Four have the same bytes under way in half the workgroups, and the backward's
-// registers (k, z, dh of eight steps) do not fit 128: forward and backward of T1024 B64 N2048 with 8
-// bits take 275 + 674 us with four, 313 + 271 with two, 401 + 347 with one; of T250 B128 N512 26 + 64,
-// 23 + 34, 24 + 39. One for rows of one column and for offsets past 32 bits.
+// registers (gates, z, dh of eight steps) do not fit 128: forward and backward of T1024 B64 N2048 with
+// 8 bits take 299 + 382 us with four, 312 + 291 with two, 410 + 368 with one; of T250 B128 N512 30 +
+// 64, 23 + 34, 28 + 41. One for rows of one column and for offsets past 32 bits.
 //
 // Time over the grid where the channels give less than a workgroup a CU: each range's inputs are
-// then read twice. T1000 N512 bf16, forward and backward, whole and in ranges: B 32 (128
-// workgroups) 103 and 81 us, B 48 (192) 117 and 118, B 64 (256) 127 and 136. As many ranges as make
-// one round of two workgroups a CU (T16384 B2 N700 fp32: 241 us with 22 ranges, 234 with 43, 237
-// with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 174 us with 3
-// ranges, 143 with 4, 128 with 6). From five blocks on, a block a range at the least: B20 N333 bf16
-// whole and in ranges 20 and 25 us at T 128, 34 and 31 (and two more launches) at T 256, 41 and 31
+// then read twice. T1000 N512 bf16, a training pass's kernels whole and in ranges: B 32 (128
+// workgroups) 122 and 89 us, B 48 (192) 132 and 134, B 64 (256) 143 and 147. As many ranges as make
+// one round of two workgroups a CU (T16384 B2 N700 fp32: 255 us with 22 ranges, 244 with 43, 249
+// with 64). With masks twice that, since padded ranges end early (T1000 B50 N333: 188 us with 3
+// ranges, 156 with 4, 141 with 6). From five blocks on, a block a range at the least: B20 N333 bf16
+// whole and in ranges 27 and 29 us at T 128, 41 and 34 (and two more launches) at T 256, 48 and 37
 // at T 320.
 Plan gated_plan(int T, int B, int N, bool pack, bool wide, bool mask) {
     Plan q;

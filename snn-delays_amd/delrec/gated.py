@@ -57,7 +57,7 @@ def gated_step(z, f, g, x, h, weight, scale, next_weight=None, bias=None, eps=1e
     scan rounds its output to z's type): ``(x', u, h')``.
 
     ``z``, ``f``, ``g``, ``x`` (B, N) as there, the state ``h`` (B, N) fp32. ``h_out``: where h'
-    goes, ``h`` itself to update in place. Not differentiable."""
+    goes, ``h`` itself to update in place, or memory that no input shares. Not differentiable."""
     return _lib.require_ext().gated_step(z, f, g, x, h, weight, scale, next_weight, bias, eps, h_out)
 
 
