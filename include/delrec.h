@@ -296,7 +296,8 @@ typedef struct {
  * A group that holds an infinity or a NaN has scale NaN, and its q mean nothing. */
 enum { DELREC_PACK8_GROUP = 64 };
 typedef struct {
-    int8_t* q;                   /* (rows, N) at a pitch of N rounded up to a multiple of 4 */
+    int8_t* q;                   /* (rows, N) at a pitch of N rounded up to a multiple of 4, */
+                                 /* the first row 4-byte aligned                            */
     float* scale;                /* (rows, ceil(N / 64)) contiguous                        */
 } delrec_packed8;
 

@@ -62,12 +62,16 @@ void check_like(const Tensor& t, const Tensor& like, at::ScalarType type, const 
         refuse(text(what, " is ", t.defined() ? describe(t) : "None", ", expected ", like.sizes(), " ", type, " on ", like.device()));
 }
 
+// contiguous, and with its values in memory (the imaginary part of a conjugated tensor has their
+// opposites there); undefined stays so
+Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
+
 // contiguous fp32 (n) on x's device; undefined stays so
 Tensor vector_arg(const Tensor& v, int64_t n, const Tensor& x, const char* what) {
     if (!v.defined()) return v;
     if (v.dim() != 1 || v.size(0) != n || v.device() != x.device())
         refuse(text(what, " is ", describe(v), ", expected [", n, "] on ", x.device()));
-    return v.to(at::kFloat).contiguous();
+    return dense(v.to(at::kFloat));
 }
 
 bool wanted(std::initializer_list<const Tensor*> ts) {
@@ -127,6 +131,7 @@ std::shared_ptr<N> make_node() { return std::shared_ptr<N>(new N(), torch::autog
 // (R0, R1, N) or (R, N), the last axis contiguous; a copy only where there is no such view
 Tensor rows_form(Tensor t) {
     if (!t.defined()) return t;
+    t = t.resolve_neg();
     if (t.dim() == 1) t = t.unsqueeze(0);
     else if (t.dim() > 3) t = t.reshape({-1, t.size(-1)});
     return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
@@ -136,7 +141,7 @@ Tensor rows_form(Tensor t) {
 // there shares its tensor's version counter, and one taken below them has its own, so that a change
 // in place between forward and backward would go unnoticed. Detached: no node for the view.
 Tensor kept_rows(const Tensor& t) {
-    if (!t.defined() || ((t.dim() == 2 || t.dim() == 3) && t.stride(-1) == 1)) return t;
+    if (!t.defined() || ((t.dim() == 2 || t.dim() == 3) && t.stride(-1) == 1 && !t.is_neg())) return t;
     return rows_form(t.detach());
 }
 
@@ -235,7 +240,7 @@ struct GatedScanBackward : public KeptNode {
         const auto f32 = states.options();
         // an output that nothing used
         const Tensor dh = grads[0].defined() ? rows_form(grads[0]) : at::zeros({1, 1, N}, f32.dtype(type)).expand({T, B, N});
-        const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : Tensor();
+        const Tensor dlast = dense(grads[1]);
         Tensor dz = at::empty({T, B, N}, f32.dtype(type)), df = at::empty({T, B, N}, f32.dtype(type)), db, dh0;
         if (task_should_compute_output(2)) db = at::empty({N}, f32);
         if (task_should_compute_output(3)) dh0 = at::empty({B, N}, f32);
@@ -263,7 +268,7 @@ variable_list scan_with_graph(const Tensor& z, const Tensor& f, const Tensor& bi
     {
         at::AutoDispatchBelowADInplaceOrView below;
         ScanKept kept;
-        const Tensor b = vector_arg(bias, z.size(2), z, "bias"), h0c = h0.defined() ? h0.contiguous() : h0;
+        const Tensor b = vector_arg(bias, z.size(2), z, "bias"), h0c = dense(h0);
         out = scan_forward(rows_form(z), rows_form(f), b, h0c, starts, lengths, checkpoint, &kept);
         node->T = z.size(0);
         node->type = z.scalar_type();
@@ -304,7 +309,7 @@ py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTens
         return py::make_tuple(h.to(z.scalar_type()), last);
     }
     if (wanted({&z, &f, &bias, &h0})) return pair_of(scan_with_graph(z, f, bias, h0, starts, lengths, checkpoint));
-    return pair_of(scan_forward(rows_form(z), rows_form(f), vector_arg(bias, N, z, "bias"), h0.defined() ? h0.contiguous() : h0,
+    return pair_of(scan_forward(rows_form(z), rows_form(f), vector_arg(bias, N, z, "bias"), dense(h0),
                                 starts, lengths, false, nullptr));
 }
 
@@ -485,12 +490,12 @@ py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor
     const bool in_place = h_out.defined();
     if (in_place) {
         check_like(h_out, h, at::kFloat, "h_out");
-        if (!h_out.is_contiguous()) refuse("h_out must be contiguous");
+        if (!h_out.is_contiguous() || h_out.is_neg()) refuse("h_out must be contiguous");
     } else {
         h_out = at::empty({B, N}, h.options());
     }
     z = rows_form(z); f = rows_form(f); g = rows_form(g); x = rows_form(x);
-    h = h.contiguous();
+    h = dense(h);
     w = vector_arg(w, N, z, "weight"); scale = vector_arg(scale, N, z, "scale");
     w2 = vector_arg(w2, N, z, "next_weight"); bias = vector_arg(bias, N, z, "bias");
     const Tensor xo = at::empty({B, N}, x.options());

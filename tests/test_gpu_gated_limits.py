@@ -412,3 +412,42 @@ def test_linear8_with_its_input_saved_on_the_host(dev):
         y = lin(x)
     for a, b in zip(torch.autograd.grad(y.square().sum(), (x, lin.weight, lin.bias)), want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_imaginary_parts_of_conjugated_tensors(dev):
+    """Real views whose memory holds the opposite of their values, as every input and gradient; rows of
+    one channel, which any stride makes contiguous, among them."""
+    from delrec.checkpoint8 import pack8, unpack8
+    from delrec.gated import gated_scan, gated_step, norm_gate_residual, rms_norm
+    g = torch.Generator().manual_seed(71)
+
+    def both(*shape):
+        part = torch.randn(*shape, 2, generator=g).to(dev)
+        view = torch.view_as_complex(part).conj().imag
+        assert view.is_neg()
+        return view, -part[..., 1]
+    shape = (70, 2, 8)
+    wide = [both(*shape) for _ in range(7)]
+    thin = [both(70, 2, 1) for _ in range(3)]
+    rows = [both(2, 8) for _ in range(3)]
+    vecs = [both(8) for _ in range(4)]
+
+    def run(i):
+        z, f, gg, x, dh, dx, du = (p[i].detach() for p in wide)
+        h0, dlast, state = (p[i].detach() for p in rows)
+        v = [p[i].detach().requires_grad_(True) for p in vecs]
+        L = [t.detach().requires_grad_(True) for t in (z, f, h0, gg, x)]
+        h, last = gated_scan(L[0], L[1], v[0], L[2])
+        y, u = norm_gate_residual(L[0], L[3], L[4], v[1], v[2], v[3])
+        out = [h, last, y, u, rms_norm(x, v[3].detach()), unpack8(pack8(x)), torch.autograd.grad((h, last), (L[0], L[1], v[0], L[2]), (dh, dlast)),
+               torch.autograd.grad((y, u), (L[0], *L[3:], *v[1:]), (dx, du))]
+        z1, f1 = (p[i].detach().requires_grad_(True) for p in thin[:2])
+        h1, last1 = gated_scan(z1, f1)
+        out += [h1, last1, *torch.autograd.grad(h1, (z1, f1), thin[2][i])]
+        with torch.no_grad():
+            out += gated_step(z[0], f[0], gg[0], x[0], state, *v[1:], v[0])
+            out += norm_gate_residual(*(t.reshape(35, 2, 2, 8) for t in (z, gg, x)), *v[1:3], None)[:1]
+        return [t for o in out for t in (o if isinstance(o, (tuple, list)) else (o,))]
+    for k, (a, b) in enumerate(zip(run(0), run(1))):
+        torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-6, msg=lambda m: f'{k}: {m}')
