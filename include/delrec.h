@@ -392,6 +392,129 @@ typedef struct {
     void* u;                     /* out (B, N) when w2 is given                            */
 } delrec_gated_step_args;
 
+/* x' = x + y and u = x' r w, r = 1/sqrt(mean x'^2 + eps) (of x' before it is rounded), over R0 * R1
+ * rows of N >= 2. stats keeps r for the backward pass; u8: u, as rounded, also in 8 bits. */
+typedef struct {
+    int32_t R0, R1, N, bf16, x_bf16;   /* bf16: y, u; x_bf16: x, x_out                     */
+    delrec_rows x, y;
+    const float* w;              /* (N)                                                    */
+    float eps;
+    void* x_out;                 /* out (R0, R1, N) contiguous                             */
+    void* u;                     /* out (R0, R1, N) contiguous                             */
+    float* stats;                /* out (R0 * R1), or NULL                                 */
+    delrec_packed8 u8;           /* out, or NULL pointers                                  */
+} delrec_add_norm_fwd_args;
+
+/* Its gradients; that of y equals that of x. */
+typedef struct {
+    int32_t R0, R1, N, bf16, x_bf16;
+    delrec_rows x, y;            /* as the forward's; y.data NULL: x is x' itself          */
+    const float* w;
+    const float* stats;
+    delrec_rows dx_out;          /* gradient of x' (data NULL: 0)                          */
+    delrec_rows du;              /* gradient of u (data NULL: 0)                           */
+    void* dx;                    /* out (R0, R1, N) contiguous, x's type                   */
+    void* dy;                    /* out the same in y's type, or NULL                      */
+    float* dw;                   /* out (N)                                                */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_add_norm_bwd_args;
+
+/* ---- Selective state-space block: short causal convolution, recurrence, one step ----
+ * No counterpart in the reference. Activations (T, B, N) and (T, B, S) fp32 or bf16 (bf16 != 0);
+ * states of the recurrence, and all sums, in 32 bits. starts and lengths as above. */
+
+/* p_t = bias + sum_i w[n][i] x_{t-W+1+i}, i < W in [2, 8]; y = p sigmoid(p) with silu, else p. Rows of
+ * steps before the first are those of state (NULL: 0), of steps before a start 0; from lengths[b]
+ * on y is written 0. state_out: the inputs of a row's last W - 1 steps, which a next call takes as
+ * its state (with T = 1 it may be state itself). Other outputs must not overlap inputs. */
+typedef struct {
+    int32_t T, B, N, W, bf16, silu;
+    delrec_rows x;               /* (T, B, N)                                              */
+    const float* w;              /* (N, W)                                                 */
+    const float* bias;           /* (N) or NULL                                            */
+    const void* state;           /* (B, W - 1, N) contiguous, x's type, or NULL            */
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows y;               /* out (T, B, N)                                          */
+    void* state_out;             /* out (B, W - 1, N) contiguous, or NULL                  */
+} delrec_causal_conv_fwd_args;
+
+typedef struct {
+    int32_t T, B, N, W, bf16, silu;
+    delrec_rows x;
+    const float* w;
+    const float* bias;
+    const void* state;
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows dy;              /* (T, B, N)                                              */
+    const void* dstate_out;      /* (B, W - 1, N) or NULL: 0                               */
+    delrec_rows dx;              /* out (T, B, N)                                          */
+    void* dstate;                /* out (B, W - 1, N), or NULL                             */
+    float* dw;                   /* out (N, W)                                             */
+    float* db;                   /* out (N), or NULL                                       */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_causal_conv_bwd_args;
+
+/* d_t = softplus(dt_t + dt_bias); h_t = exp(d_t A) h_{t-1} + d_t x_t B_t; y_t = (<C_t, h_t> + D x_t)
+ * times g_t sigmoid(g_t) where there is a g; S in [1, 64] states a channel. At a start the state before the
+ * step is 0; from lengths[b] on the state stays and y is written 0. states[i] is the state before
+ * step 16 i, which the backward pass starts from. Outputs must not overlap inputs. */
+enum { DELREC_SELECTIVE_BLOCK = 16 };
+typedef struct {
+    int32_t T, B, N, S, bf16;
+    delrec_rows x, dt, g;        /* (T, B, N); g.data NULL: no gate                        */
+    delrec_rows Bm, C;           /* (T, B, S)                                              */
+    const float* A;              /* (N, S)                                                 */
+    const float* D;              /* (N) or NULL: 0                                         */
+    const float* dt_bias;        /* (N) or NULL: 0                                         */
+    const float* h0;             /* (B, N, S) or NULL: 0                                   */
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows y;               /* out (T, B, N)                                          */
+    float* h_last;               /* out (B, N, S)                                          */
+    float* states;               /* out (ceil(T / 16), B, N, S), or NULL                   */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_selective_scan_fwd_args;
+
+typedef struct {
+    int32_t T, B, N, S, bf16;
+    delrec_rows x, dt, g, Bm, C;
+    const float* A;
+    const float* D;
+    const float* dt_bias;
+    const float* states;
+    const uint8_t* starts;
+    const int64_t* lengths;
+    delrec_rows dy;              /* (T, B, N)                                              */
+    const float* dlast;          /* (B, N, S) or NULL: 0                                   */
+    delrec_rows dx, ddt, dg;     /* out (T, B, N); dg with g                               */
+    void* dBm;                   /* out (T, B, S) contiguous                               */
+    void* dC;                    /* out (T, B, S) contiguous                               */
+    float* dA;                   /* out (N, S), or NULL                                    */
+    float* dD;                   /* out (N), or NULL                                       */
+    float* ddt_bias;             /* out (N), or NULL                                       */
+    float* dh0;                  /* out (B, N, S), or NULL                                 */
+    void* workspace;
+    size_t workspace_bytes;
+} delrec_selective_scan_bwd_args;
+
+/* One time step of that recurrence for B rows; h_out may be h. */
+typedef struct {
+    int32_t B, N, S, bf16;
+    delrec_rows x, dt, g;        /* (1, B, N); g.data NULL: no gate                        */
+    delrec_rows Bm, C;           /* (1, B, S)                                              */
+    const float* A;
+    const float* D;
+    const float* dt_bias;
+    const float* h;              /* (B, N, S)                                              */
+    float* h_out;                /* out (B, N, S)                                          */
+    void* y;                     /* out (B, N) contiguous                                  */
+} delrec_selective_step_args;
+
 /* A tensor to 8 bits, and the values that it stands for. */
 typedef struct {
     int32_t R0, R1, N, bf16;
@@ -410,7 +533,9 @@ enum { DELREC_WS_AXONAL_FWD = 1, DELREC_WS_AXONAL_BWD = 2, DELREC_WS_SYN_FWD = 3
        DELREC_WS_SPIKE_LINEAR_DW = 6 /* N = K inputs, L = M outputs */,
        DELREC_WS_READOUT_CE = 7 /* N = C classes, L = 1 */,
        DELREC_WS_GATED_FWD = 8, DELREC_WS_GATED_BWD = 9 /* both: L = 1 */,
-       DELREC_WS_NORM_GATE_BWD = 10 /* T = R0, B = R1, L = 1 */ };
+       DELREC_WS_NORM_GATE_BWD = 10, DELREC_WS_ADD_NORM_BWD = 11 /* both: T = R0, B = R1, L = 1 */,
+       DELREC_WS_CAUSAL_CONV_BWD = 12 /* L = W */,
+       DELREC_WS_SELECTIVE_FWD = 13, DELREC_WS_SELECTIVE_BWD = 14 /* both: L = S */ };
 
 int delrec_axonal_fwd(const delrec_axonal_fwd_args* a, void* stream);
 int delrec_axonal_bwd(const delrec_axonal_bwd_args* a, void* stream);
@@ -447,6 +572,13 @@ int delrec_gated_scan_bwd(const delrec_gated_scan_bwd_args* a, void* stream);
 int delrec_gated_step(const delrec_gated_step_args* a, void* stream);
 int delrec_norm_gate_fwd(const delrec_norm_gate_fwd_args* a, void* stream);
 int delrec_norm_gate_bwd(const delrec_norm_gate_bwd_args* a, void* stream);
+int delrec_add_norm_fwd(const delrec_add_norm_fwd_args* a, void* stream);
+int delrec_add_norm_bwd(const delrec_add_norm_bwd_args* a, void* stream);
+int delrec_causal_conv_fwd(const delrec_causal_conv_fwd_args* a, void* stream);
+int delrec_causal_conv_bwd(const delrec_causal_conv_bwd_args* a, void* stream);
+int delrec_selective_scan_fwd(const delrec_selective_scan_fwd_args* a, void* stream);
+int delrec_selective_scan_bwd(const delrec_selective_scan_bwd_args* a, void* stream);
+int delrec_selective_step(const delrec_selective_step_args* a, void* stream);
 int delrec_pack8(const delrec_pack8_args* a, void* stream);
 int delrec_unpack8(const delrec_pack8_args* a, void* stream);
 int delrec_lif_fwd(const delrec_lif_fwd_args* a, void* stream);
@@ -497,7 +629,7 @@ int delrec_peak_mfma(int32_t kind, int32_t iters, float* sink, size_t sink_bytes
 const char* delrec_strerror(int status);
 /* "delrec-mi355x <DELREC_ABI_VERSION> (gfx950)": a binding checks it before use (the
  * argument structs change between versions). */
-#define DELREC_ABI_VERSION "0.6.0"
+#define DELREC_ABI_VERSION "0.7.0"
 const char* delrec_version(void);
 
 #ifdef __cplusplus

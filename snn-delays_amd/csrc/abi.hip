@@ -806,6 +806,19 @@ int delrec_query_workspace(int32_t kind, int32_t T, int32_t B, int32_t N, int32_
             if (!norm_gate_sizes_ok(T, B, N)) return DELREC_ERR_ARG;
             c.take<float>(norm_gate_bwd_ws((long long)T * B, N));
             break;
+        case DELREC_WS_ADD_NORM_BWD:
+            if (!norm_gate_sizes_ok(T, B, N)) return DELREC_ERR_ARG;
+            c.take<float>(add_norm_bwd_ws((long long)T * B, N));
+            break;
+        case DELREC_WS_CAUSAL_CONV_BWD:
+            if (!conv_sizes_ok(T, B, N, L)) return DELREC_ERR_ARG;
+            c.take<float>(conv_bwd_ws(T, B, N, L));
+            break;
+        case DELREC_WS_SELECTIVE_FWD:
+        case DELREC_WS_SELECTIVE_BWD:
+            if (!selective_sizes_ok(T, B, N, L)) return DELREC_ERR_ARG;
+            c.take<float>(kind == DELREC_WS_SELECTIVE_FWD ? selective_fwd_ws(T, B, N, L) : selective_bwd_ws(T, B, N, L));
+            break;
         default: return DELREC_ERR_ARG;
     }
     *bytes = c.used;

@@ -125,6 +125,32 @@ int delrec_norm_gate_bwd(const delrec_norm_gate_bwd_args* a, void* stream) {
     return done();
 }
 
+int delrec_add_norm_fwd(const delrec_add_norm_fwd_args* a, void* stream) {
+    if (!a || !norm_gate_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
+    if (!a->x.data || !a->y.data || !a->w || !a->x_out || !a->u || !(a->eps >= 0.0f) || !pair_ok(a->u8)) return DELREC_ERR_ARG;
+    if (!a->bf16 && a->x_bf16) return DELREC_ERR_UNSUPPORTED;
+    AddNorm p{};
+    p.R0 = a->R0; p.R1 = a->R1; p.N = a->N; p.bf16 = a->bf16 != 0; p.x_bf16 = a->x_bf16 != 0;
+    p.x = a->x; p.y = a->y; p.w = a->w; p.eps = a->eps; p.x_out = a->x_out; p.u = a->u; p.stats = a->stats; p.u8 = a->u8;
+    launch_add_norm(p, true, static_cast<hipStream_t>(stream));
+    return done();
+}
+
+int delrec_add_norm_bwd(const delrec_add_norm_bwd_args* a, void* stream) {
+    if (!a || !norm_gate_sizes_ok(a->R0, a->R1, a->N)) return DELREC_ERR_ARG;
+    if (!a->x.data || !a->w || !a->stats || !a->dx || !a->dw || (!a->dx_out.data && !a->du.data)) return DELREC_ERR_ARG;
+    if (!a->bf16 && a->x_bf16) return DELREC_ERR_UNSUPPORTED;
+    AddNorm p{};
+    p.R0 = a->R0; p.R1 = a->R1; p.N = a->N; p.bf16 = a->bf16 != 0; p.x_bf16 = a->x_bf16 != 0;
+    p.x = a->x; p.y = a->y; p.w = a->w; p.stats = const_cast<float*>(a->stats); p.dx_out = a->dx_out; p.du = a->du;
+    p.dx = a->dx; p.d_y = a->dy; p.dw = a->dw;
+    const size_t need = add_norm_bwd_ws((long long)a->R0 * a->R1, a->N) * sizeof(float);
+    if (!a->workspace || a->workspace_bytes < need) return DELREC_ERR_WORKSPACE;
+    p.part = static_cast<float*>(a->workspace);
+    launch_add_norm(p, false, static_cast<hipStream_t>(stream));
+    return done();
+}
+
 static int pack_call(const delrec_pack8_args* a, bool pack, void* stream) {
     if (!a || !sizes_ok(a->R0, a->R1, a->N) || !a->x.data || !a->p.q || !a->p.scale) return DELREC_ERR_ARG;
     launch_pack8({a->R0, a->R1, a->N, a->bf16 != 0, a->x, a->p}, pack, static_cast<hipStream_t>(stream));

@@ -634,6 +634,79 @@ void launch_pack8(const Pack8& p, bool pack, hipStream_t stream);
 // o_k[n] = sum over rows r of part[r * pitch + k * N + n], k < pitch / N <= 3 (NULL: skipped)
 void launch_column_sums(const float* part, unsigned rows, int N, unsigned pitch, float* o0, float* o1, float* o2, hipStream_t stream);
 
+struct AddNorm {                 // a residual's addition and its norm, R0 * R1 rows
+    int R0, R1, N, bf16, x_bf16;
+    delrec_rows x, y;
+    const float* w;
+    float eps;
+    void* x_out;
+    void* u;
+    float* stats;                // [rows] r
+    delrec_packed8 u8;
+    delrec_rows dx_out, du;
+    void* dx;
+    void* d_y;                   // NULL: dx is y's gradient too
+    float* dw;
+    float* part;                 // workspace of the backward
+    int flat;                    // set by the launcher, as NormGate's
+};
+size_t add_norm_bwd_ws(long long rows, int N);   // floats
+void launch_add_norm(const AddNorm& p, bool fwd, hipStream_t stream);
+
+// ---- selective state-space block (selective.hip, conv.hip) ----
+struct Selective {               // forward, backward and one step of the selective recurrence
+    int T, B, N, S, bf16;
+    delrec_rows x, dt, g, Bm, C, y;
+    const float* A;
+    const float* D;
+    const float* dt_bias;
+    const float* h0;
+    const uint8_t* starts;
+    const int64_t* lengths;
+    float* h_last;
+    float* states;               // [ceil(T / 16)][B][N][S]
+    delrec_rows dy, dx, ddt, dg;
+    const float* dlast;
+    float* dA;
+    void* dB;
+    void* dC;
+    float* dD;
+    float* dbias;
+    float* dh0;
+    float* ws;                   // workspace, selective_fwd_ws / selective_bwd_ws floats
+    float* bcsums;               // set by the launcher: parts of ws, and
+    float* rowsums;
+    int tiles;                   // workgroups of channels,
+    long long first;             // the launch's first workgroup
+};
+bool selective_sizes_ok(int T, int B, int N, int S);   // what the entry points take (selective_abi.hip)
+bool conv_sizes_ok(int T, int B, int N, int W);
+size_t selective_fwd_ws(int T, int B, int N, int S);   // floats
+size_t selective_bwd_ws(int T, int B, int N, int S);
+void launch_selective_fwd(const Selective& p, hipStream_t stream);
+void launch_selective_bwd(const Selective& p, hipStream_t stream);
+void launch_selective_step(const Selective& p, hipStream_t stream);
+struct CausalConv {
+    int T, B, N, W, bf16, silu;
+    delrec_rows x, y;
+    const float* w;              // (N, W)
+    const float* bias;
+    const void* state;           // (B, W - 1, N)
+    const uint8_t* starts;
+    const int64_t* lengths;
+    void* state_out;
+    delrec_rows dy, dx;
+    const void* dstate_out;
+    void* dstate;
+    float* dw;
+    float* db;
+    float* part;                 // workspace of the backward, conv_bwd_ws floats
+    int groups, steps, runs;     // set by the launcher: lanes a row, steps of a run, runs,
+    long long first;             // the launch's first workgroup
+};
+size_t conv_bwd_ws(int T, int B, int N, int W);   // floats
+void launch_conv(const CausalConv& p, bool fwd, hipStream_t stream);
+
 void launch_lif(bool fwd, const delrec_lif_fwd_args* fa, const delrec_lif_bwd_args* ba,
                 const Lif& k, int cus, hipStream_t stream);
 void launch_delay_grad(const float* C, const float* W, const float* d, float sigma, int N,

@@ -153,6 +153,68 @@ __global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
     }
 }
 
+// ---- a residual's addition and its norm: x' = x + y, r = 1/sqrt(mean x'^2 + eps), u = x' r w ----
+// Backwards, with e = x' r and v = w du: dx = dy = dx' + r (v - e <v e>), dw = sum du e. The same
+// rows in registers; the forward also packs u, as rounded, to 8 bits. Kept for the backward: r, and
+// x' where it is fp32 (exact), else x and y, so that no rounding of x' reaches dw.
+
+template <class S, class X>
+__global__ void __launch_bounds__(kNb) add_norm_any_fwd_kernel(AddNorm p) {
+    __shared__ float red[4];
+    const int N = p.N;
+    const long long rows = (long long)p.R0 * p.R1;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const X* x = row_ptr<const X>(p.x, row, p.R1);
+        const S* y = row_ptr<const S>(p.y, row, p.R1);
+        float s = 0.0f;
+        for (int n = threadIdx.x; n < N; n += kNb) {
+            const float v = to_f32(x[n]) + to_f32(y[n]);
+            s += v * v;
+        }
+        const float r = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
+        for (int n = threadIdx.x; n < N; n += kNb) {
+            const float v = to_f32(x[n]) + to_f32(y[n]);
+            ((X*)p.x_out)[row * N + n] = (X)v;
+            ((S*)p.u)[row * N + n] = (S)(v * r * p.w[n]);
+        }
+        if (p.stats && threadIdx.x == 0) p.stats[row] = r;
+        __syncthreads();
+    }
+}
+
+template <class S, class X>
+__global__ void __launch_bounds__(kNb) add_norm_any_bwd_kernel(AddNorm p) {
+    __shared__ float red[4];
+    const int N = p.N, tid = threadIdx.x;
+    float* dwp = p.part + (size_t)blockIdx.x * N;
+    for (int n = tid; n < N; n += kNb) dwp[n] = 0.0f;
+    __syncthreads();
+    const long long rows = (long long)p.R0 * p.R1;
+    for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float r = p.stats[row];
+        auto eval = [&](int n) {
+            const float v = to_f32(row_ptr<const X>(p.x, row, p.R1)[n]);
+            return (p.y.data ? v + to_f32(row_ptr<const S>(p.y, row, p.R1)[n]) : v) * r;
+        };
+        auto duval = [&](int n) { return p.du.data ? to_f32(row_ptr<const S>(p.du, row, p.R1)[n]) : 0.0f; };
+        float s = 0.0f;
+        if (p.du.data)
+            for (int n = tid; n < N; n += kNb) s += p.w[n] * duval(n) * eval(n);
+        const float m = row_sum(s, red) / (float)N;
+        for (int n = tid; n < N; n += kNb) {
+            float d = p.dx_out.data ? to_f32(row_ptr<const X>(p.dx_out, row, p.R1)[n]) : 0.0f;
+            if (p.du.data) {
+                const float e = eval(n), du = duval(n);
+                d += r * (p.w[n] * du - e * m);
+                dwp[n] += du * e;
+            }
+            ((X*)p.dx)[row * N + n] = (X)d;
+            if (p.d_y) ((S*)p.d_y)[row * N + n] = (S)d;
+        }
+        __syncthreads();
+    }
+}
+
 // out_k[n] = sum over rows of part[row * pitch + k * N + n], k < 3, in a fixed order
 __global__ void __launch_bounds__(1024) column_sums_kernel(const float* part, unsigned rows, int N, unsigned pitch, float* o0,
                                                            float* o1, float* o2) {
@@ -229,8 +291,8 @@ struct Cols {
     }
 };
 
-template <class T>
-__device__ __forceinline__ T* row_at(const delrec_rows& x, long long row, const NormGate& p) {
+template <class T, class P>
+__device__ __forceinline__ T* row_at(const delrec_rows& x, long long row, const P& p) {
     if (p.flat) return (T*)x.data + row * x.s1;
     const unsigned r = (unsigned)row, i = r / (unsigned)p.R1, j = r - i * (unsigned)p.R1;
     return (T*)x.data + i * x.s0 + j * x.s1;
@@ -547,6 +609,140 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
     }
 }
 
+template <class S, class X, int LPR, int NE>
+__global__ void __launch_bounds__(kRowBlock<LPR>) add_norm_fwd_kernel(AddNorm p) {
+    __shared__ float red[2 * (LPR > 64 ? LPR / 64 : 1)];
+    constexpr int RPW = kRowBlock<LPR> / LPR;
+    const int lane = threadIdx.x % LPR, N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
+    const Cols<LPR, NE> c(lane, N);
+    const long long rows = (long long)p.R0 * p.R1;
+    float w[NE][4];
+    load_cols<NE>(w, p.w, c.n0);
+    const float inv_n = 1.0f / (float)N;
+    int slot = 0;
+    // rows past the end repeat the last one and store nothing (its lanes join the exchanges)
+    for (long long r0 = (long long)blockIdx.x * RPW; r0 < rows; r0 += (long long)gridDim.x * RPW, slot ^= 1) {
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        const bool live = mine < rows;
+        Vec<X, 4> xv[NE];
+        Vec<S, 4> yv[NE];
+        const X* xp = row_at<const X>(p.x, row, p);
+        const S* yp = row_at<const S>(p.y, row, p);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) xv[e] = vload<X, 4>(xp + c.n0[e]), yv[e] = vload<S, 4>(yp + c.n0[e]);
+        float x[NE][4], s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[e][j] = xv[e].get(j) + yv[e].get(j);
+                s += j >= c.skip[e] ? x[e][j] * x[e][j] : 0.0f;
+            }
+            if (live && c.on[e]) vstore<X, 4>((X*)p.x_out + row * N + c.n0[e], x[e]);
+        }
+        const float r = 1.0f / sqrtf(lanes_sum<LPR>(s, red, slot) * inv_n + p.eps);
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            float u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = to_f32((S)(x[e][j] * r * w[e][j]));
+            if (live && c.on[e]) vstore<S, 4>((S*)p.u + row * N + c.n0[e], u);
+            if (p.u8.q) {
+                const Lane8<4> l8(c.i[e], c.skip[e], live && c.on[e], N);
+                store8<4>(u, l8, live && c.first[e], p.u8.q + row * pitch8(N), p.u8.scale + row * ng + c.group[e]);
+            }
+        }
+        if (p.stats && live && lane == 0) p.stats[row] = r;
+    }
+}
+
+template <class S, class X, int LPR, int NE>
+__global__ void __launch_bounds__(kRowBlock<LPR>) add_norm_bwd_kernel(AddNorm p) {
+    constexpr int RPW = kRowBlock<LPR> / LPR, W = LPR > 64 ? LPR / 64 : 1, ROW = LPR * NE * 4;
+    __shared__ float red[2 * W];
+    __shared__ float slots[RPW > 1 ? RPW : 1][RPW > 1 ? ROW : 1];
+    const int lane = threadIdx.x % LPR, N = p.N;
+    const Cols<LPR, NE> c(lane, N);
+    const long long rows = (long long)p.R0 * p.R1, step = (long long)gridDim.x * RPW;
+    const bool sum = p.y.data != nullptr;
+    float w[NE][4], acc[NE][4];
+    load_cols<NE>(w, p.w, c.n0);
+#pragma unroll
+    for (int e = 0; e < NE; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[e][j] = 0.0f;
+    struct Raw {
+        Vec<X, 4> x[NE], up[NE];
+        Vec<S, 4> y[NE], du[NE];
+        float r;
+    } in;
+    auto load = [&](long long r0) {
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        in.r = p.stats[row];
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+            if (p.du.data) {
+                in.x[e] = vload<X, 4>(row_at<const X>(p.x, row, p) + c.n0[e]);
+                if (sum) in.y[e] = vload<S, 4>(row_at<const S>(p.y, row, p) + c.n0[e]);
+                in.du[e] = vload<S, 4>(row_at<const S>(p.du, row, p) + c.n0[e]);
+            }
+            if (p.dx_out.data) in.up[e] = vload<X, 4>(row_at<const X>(p.dx_out, row, p) + c.n0[e]);
+        }
+    };
+    const float inv_n = 1.0f / (float)N;
+    long long r0 = (long long)blockIdx.x * RPW;
+    if (r0 < rows) load(r0);
+    for (int slot = 0; r0 < rows; r0 += step, slot ^= 1) {
+        // rows past the end repeat the last one, with no gradient, and store nothing
+        const long long mine = r0 + threadIdx.x / LPR, row = mine < rows ? mine : rows - 1;
+        const bool live = mine < rows, has_du = live && p.du.data, has_up = live && p.dx_out.data;
+        const float r = in.r;
+        float x[NE][4], du[NE][4], up[NE][4], s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[e][j] = has_du ? (sum ? in.x[e].get(j) + in.y[e].get(j) : in.x[e].get(j)) * r : 0.0f;
+                du[e][j] = has_du ? in.du[e].get(j) : 0.0f;
+                up[e][j] = has_up ? in.up[e].get(j) : 0.0f;
+                s += j >= c.skip[e] ? w[e][j] * du[e][j] * x[e][j] : 0.0f;
+            }
+        if (r0 + step < rows) load(r0 + step);
+        const float m = lanes_sum<LPR>(s, red, slot) * inv_n;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                acc[e][j] = fmaf(du[e][j], x[e][j], acc[e][j]);
+                if (has_du) up[e][j] = fmaf(r, w[e][j] * du[e][j] - x[e][j] * m, up[e][j]);
+            }
+            if (live && c.on[e]) {
+                vstore<X, 4>((X*)p.dx + row * N + c.n0[e], up[e]);
+                if (p.d_y) vstore<S, 4>((S*)p.d_y + row * N + c.n0[e], up[e]);
+            }
+        }
+    }
+    float* part = p.part + (size_t)blockIdx.x * N;
+    if constexpr (RPW > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) slots[threadIdx.x / LPR][(e * LPR + lane) * 4 + j] = acc[e][j];
+        __syncthreads();
+        if (threadIdx.x < LPR)
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    for (int q = 1; q < RPW; ++q) acc[e][j] += slots[q][(e * LPR + lane) * 4 + j];
+    }
+    if (threadIdx.x < LPR)
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+            if (c.on[e]) vstore<float, 4>(part + c.n0[e], acc[e]);
+}
+
 namespace {
 
 bool in_registers(int N) { return N >= 4 && N <= 8192; }
@@ -647,6 +843,22 @@ int run_norm_gate(const NormGate& p, bool fwd, hipStream_t stream) {
     return q.vecs == 2 ? run_bwd<S, X, 512, 2>(p, stream) : run_bwd<S, X, 512, 4>(p, stream);
 }
 
+// rows one pitch apart in every tensor need no division by R1
+template <class P>
+void flatten(P& p, std::initializer_list<delrec_rows*> tensors) {
+    p.flat = p.R0 == 1;
+    if (p.flat) return;
+    p.flat = 1;
+    for (const delrec_rows* t : tensors)
+        if (t->data && t->s0 != t->s1 * p.R1) p.flat = 0;
+    if (p.R1 == 1) {
+        p.flat = 1;
+        for (delrec_rows* t : tensors) t->s1 = t->s0;
+        p.R1 = p.R0;
+        p.R0 = 1;
+    }
+}
+
 }  // namespace
 
 size_t norm_gate_bwd_ws(long long rows, int N) {
@@ -657,23 +869,65 @@ void launch_norm_gate(const NormGate& a, bool fwd, hipStream_t stream) {
     NormGate p = a;
     // without a gradient of u the second norm has no part in the backward (dw2 = 0)
     if (!fwd && !p.du.data) p.w2 = nullptr;
-    // rows one pitch apart in every tensor need no division by R1
-    p.flat = p.R0 == 1;
-    if (!p.flat) {
-        p.flat = 1;
-        for (const delrec_rows* t : {&p.o, &p.g, &p.x, &p.dx_out, &p.du, &p.d_o, &p.dg, &p.dx})
-            if (t->data && t->s0 != t->s1 * p.R1) p.flat = 0;
-        if (p.R1 == 1) {
-            p.flat = 1;
-            for (delrec_rows* t : {&p.o, &p.g, &p.x, &p.dx_out, &p.du, &p.d_o, &p.dg, &p.dx}) t->s1 = t->s0;
-            p.R1 = p.R0;
-            p.R0 = 1;
-        }
-    }
+    flatten(p, {&p.o, &p.g, &p.x, &p.dx_out, &p.du, &p.d_o, &p.dg, &p.dx});
     const int parts = !p.bf16 ? run_norm_gate<float, float>(p, fwd, stream)
                       : p.x_bf16 ? run_norm_gate<__bf16, __bf16>(p, fwd, stream)
                                  : run_norm_gate<__bf16, float>(p, fwd, stream);
     if (!fwd) launch_column_sums(p.part, parts, p.N, 3u * p.N, p.dw, p.dscale, p.dw2, stream);
+}
+
+namespace {
+
+template <class S, class X, int LPR, int NE>
+int run_add_norm_k(const AddNorm& p, bool fwd, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    if (fwd) {
+        const int rpw = kRowBlock<LPR> / LPR;
+        hipLaunchKernelGGL((add_norm_fwd_kernel<S, X, LPR, NE>), dim3((unsigned)std::min<long long>((rows + rpw - 1) / rpw, 4096)),
+                           dim3(kRowBlock<LPR>), 0, stream, p);
+        return 0;
+    }
+    static const int fit = resident((const void*)add_norm_bwd_kernel<S, X, LPR, NE>, kRowBlock<LPR>);
+    const int parts = (int)std::min<long long>(row_groups(rows, p.N), fit);
+    hipLaunchKernelGGL((add_norm_bwd_kernel<S, X, LPR, NE>), dim3(parts), dim3(kRowBlock<LPR>), 0, stream, p);
+    return parts;
+}
+
+template <class S, class X>
+int run_add_norm(const AddNorm& p, bool fwd, hipStream_t stream) {
+    const long long rows = (long long)p.R0 * p.R1;
+    if (!in_registers(p.N)) {
+        if (fwd) {
+            hipLaunchKernelGGL((add_norm_any_fwd_kernel<S, X>), dim3((unsigned)std::min<long long>(rows, kMostBlocks)), dim3(kNb), 0, stream, p);
+            if (p.u8.q) launch_pack8({p.R0, p.R1, p.N, p.bf16, {p.u, (int64_t)p.R1 * p.N, p.N}, p.u8}, true, stream);
+        } else {
+            hipLaunchKernelGGL((add_norm_any_bwd_kernel<S, X>), dim3(any_parts(rows)), dim3(kNb), 0, stream, p);
+        }
+        return any_parts(rows);
+    }
+    const RowPlan q = row_plan(p.N, fwd);
+    if (q.lanes == 16) return q.vecs == 1 ? run_add_norm_k<S, X, 16, 1>(p, fwd, stream) : run_add_norm_k<S, X, 16, 2>(p, fwd, stream);
+    if (q.lanes == 64)
+        return q.vecs == 1   ? run_add_norm_k<S, X, 64, 1>(p, fwd, stream)
+               : q.vecs == 2 ? run_add_norm_k<S, X, 64, 2>(p, fwd, stream)
+                             : run_add_norm_k<S, X, 64, 4>(p, fwd, stream);
+    if (q.lanes == 256) return q.vecs == 1 ? run_add_norm_k<S, X, 256, 1>(p, fwd, stream) : run_add_norm_k<S, X, 256, 2>(p, fwd, stream);
+    return q.vecs == 2 ? run_add_norm_k<S, X, 512, 2>(p, fwd, stream) : run_add_norm_k<S, X, 512, 4>(p, fwd, stream);
+}
+
+}  // namespace
+
+size_t add_norm_bwd_ws(long long rows, int N) {
+    return (size_t)(in_registers(N) ? std::min<long long>(row_groups(rows, N), kMostParts) : any_parts(rows)) * N;
+}
+
+void launch_add_norm(const AddNorm& a, bool fwd, hipStream_t stream) {
+    AddNorm p = a;
+    flatten(p, {&p.x, &p.y, &p.dx_out, &p.du});
+    const int parts = !p.bf16 ? run_add_norm<float, float>(p, fwd, stream)
+                      : p.x_bf16 ? run_add_norm<__bf16, __bf16>(p, fwd, stream)
+                                 : run_add_norm<__bf16, float>(p, fwd, stream);
+    if (!fwd) launch_column_sums(p.part, parts, p.N, p.N, p.dw, nullptr, nullptr, stream);
 }
 
 }  // namespace delrec

@@ -200,11 +200,13 @@ Tensor axonal_common(Tensor x, Tensor W, Tensor d, c10::optional<Tensor> bias, c
 
 }  // namespace
 
-void bind_gated(pybind11::module_& m);   // torch_gated.cpp
+void bind_gated(pybind11::module_& m);       // torch_gated.cpp
+void bind_selective(pybind11::module_& m);   // torch_selective.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
-    m.doc() = "C++ autograd Functions: the axonal delayed-LIF layer (common regime), the gated block's operators";
+    m.doc() = "C++ autograd Functions: the axonal delayed-LIF layer (common regime), the gated and selective blocks' operators";
     bind_gated(m);
+    bind_selective(m);
     m.def("axonal_common", &axonal_common, "axonal layer forward (autograd)", py::arg("x"), py::arg("W"),
           py::arg("d"), py::arg("bias"), py::arg("drop"), py::arg("sigma"), py::arg("tau"), py::arg("vth"),
           py::arg("surrogate"), py::arg("gamma"), py::arg("alpha"), py::arg("detach"));

@@ -6,184 +6,9 @@
 // N64, whose kernels take 15 us, took 235 us through Python Functions and the ctypes binding. The
 // graph's nodes are torch::autograd::Node themselves: torch::autograd::Function keeps its values in
 // a dictionary of boxed ones.
-#include <torch/extension.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/saved_variable.h>
-
-#include <c10/hip/HIPStream.h>
-#include <hip/hip_runtime.h>
-
-#include <mutex>
-#include <sstream>
-#include <stdexcept>
-#include <string>
-
-#include "delrec.h"
-
-namespace py = pybind11;
+#include "torch_ops.h"
 
 namespace {
-
-using at::Tensor;
-using torch::autograd::Node;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-using OptTensor = c10::optional<Tensor>;
-
-void check(int status, const char* fn) {
-    if (status != DELREC_OK)
-        throw std::runtime_error(std::string(fn) + " failed: status " + std::to_string(status) + " (" +
-                                 delrec_strerror(status) + ")");
-}
-
-template <class... A>
-std::string text(const A&... a) {
-    std::ostringstream s;
-    (s << ... << a);
-    return s.str();
-}
-
-std::string describe(const Tensor& t) { return text(t.sizes(), " ", t.scalar_type(), " on ", t.device()); }
-
-[[noreturn]] void refuse(const std::string& why) { throw py::value_error(why); }
-
-Tensor given(const OptTensor& t) { return t ? *t : Tensor(); }
-
-bool is_bf16(const Tensor& t) { return t.scalar_type() == at::kBFloat16; }
-
-void check_activation(const Tensor& t, const char* what) {
-    if (!t.is_cuda())
-        throw std::runtime_error(text("delrec-mi355x runs ", what, " with HIP kernels on the GPU; it is on ", t.device()));
-    if (t.scalar_type() != at::kFloat && !is_bf16(t)) refuse(text(what, " must be fp32 or bf16, got ", t.scalar_type()));
-}
-
-void check_like(const Tensor& t, const Tensor& like, at::ScalarType type, const char* what) {
-    if (!t.defined() || t.sizes() != like.sizes() || t.device() != like.device() || t.scalar_type() != type)
-        refuse(text(what, " is ", t.defined() ? describe(t) : "None", ", expected ", like.sizes(), " ", type, " on ", like.device()));
-}
-
-// contiguous, and with its values in memory (the imaginary part of a conjugated tensor has their
-// opposites there); undefined stays so
-Tensor dense(const Tensor& t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
-
-// contiguous fp32 (n) on x's device; undefined stays so
-Tensor vector_arg(const Tensor& v, int64_t n, const Tensor& x, const char* what) {
-    if (!v.defined()) return v;
-    if (v.dim() != 1 || v.size(0) != n || v.device() != x.device())
-        refuse(text(what, " is ", describe(v), ", expected [", n, "] on ", x.device()));
-    return dense(v.to(at::kFloat));
-}
-
-bool wanted(std::initializer_list<const Tensor*> ts) {
-    if (!at::GradMode::is_enabled()) return false;
-    for (const Tensor* t : ts)
-        if (t->defined() && t->requires_grad()) return true;
-    return false;
-}
-
-// torch's own Functions refuse inputs with a forward-mode tangent; bare nodes would drop it
-void check_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
-    for (const Tensor* t : ts)
-        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(text(what, " has no forward-mode derivative"));
-}
-
-void once_differentiable(const char* what) {
-    if (at::GradMode::is_enabled()) throw std::runtime_error(text(what, " has no second derivative (create_graph=True)"));
-}
-
-// Forward calls can be captured in a graph. A captured backward pass has ended the process (a
-// segmentation fault in hipStreamEndCapture, cause not known): it is refused before it launches.
-void refuse_capture(const char* what, const Tensor& t) {
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(c10::hip::getCurrentHIPStream(t.get_device()).stream(), &status) == hipSuccess &&
-        status != hipStreamCaptureStatusNone)
-        throw std::runtime_error(text("the backward pass of ", what, " cannot be captured in a graph"));
-}
-
-// A node of the graph: what it keeps is freed after its backward, and a second backward through it
-// raises torch's own error. Under the node's mutex, since backward passes of several threads may go
-// through one graph.
-struct KeptNode : public Node {
-    std::vector<SavedVariable> kept;
-    bool released = false;
-    void keep(std::initializer_list<Tensor> ts) {
-        kept.reserve(ts.size());
-        for (const Tensor& t : ts) kept.emplace_back(t, false);
-    }
-    variable_list take() {
-        std::lock_guard<std::mutex> lock(mutex_);
-        if (released) throw std::runtime_error(torch::autograd::ERR_BACKWARD_TWICE);
-        variable_list v;
-        v.reserve(kept.size());
-        for (const SavedVariable& t : kept) v.push_back(t.unpack());
-        return v;
-    }
-    void release_variables() override {
-        std::lock_guard<std::mutex> lock(mutex_);
-        kept.clear();
-        released = true;
-    }
-};
-
-template <class N>
-std::shared_ptr<N> make_node() { return std::shared_ptr<N>(new N(), torch::autograd::deleteNode); }
-
-// (R0, R1, N) or (R, N), the last axis contiguous; a copy only where there is no such view
-Tensor rows_form(Tensor t) {
-    if (!t.defined()) return t;
-    t = t.resolve_neg();
-    if (t.dim() == 1) t = t.unsqueeze(0);
-    else if (t.dim() > 3) t = t.reshape({-1, t.size(-1)});
-    return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
-}
-
-// The same for a tensor that the graph keeps, to be called above the autograd keys: a view taken
-// there shares its tensor's version counter, and one taken below them has its own, so that a change
-// in place between forward and backward would go unnoticed. Detached: no node for the view.
-Tensor kept_rows(const Tensor& t) {
-    if (!t.defined() || ((t.dim() == 2 || t.dim() == 3) && t.stride(-1) == 1 && !t.is_neg())) return t;
-    return rows_form(t.detach());
-}
-
-delrec_rows rows_of(const Tensor& t) {
-    if (!t.defined()) return {nullptr, 0, 0};
-    if (t.dim() == 3) return {t.data_ptr(), t.stride(0), t.stride(1)};
-    return {t.data_ptr(), t.dim() == 2 ? t.stride(0) : 0, 0};
-}
-
-// rows of a contiguous (..., N) tensor, counted as (R0, R1)
-delrec_rows dense_rows(const Tensor& t, int64_t R1, int64_t N) {
-    if (!t.defined()) return {nullptr, 0, 0};
-    return {t.data_ptr(), R1 * N, N};
-}
-
-int as_int(int64_t v) {
-    if (v > INT32_MAX) refuse(text("a size of ", v, " is past 31 bits"));
-    return (int)v;
-}
-
-struct Packed {
-    Tensor q, scale;
-    Packed() = default;
-    Packed(int64_t rows, int64_t N, const Tensor& like)
-        : q(at::empty({rows, (N + 3) / 4 * 4}, like.options().dtype(at::kChar))),
-          scale(at::empty({rows, (N + DELREC_PACK8_GROUP - 1) / DELREC_PACK8_GROUP}, like.options().dtype(at::kFloat))) {}
-    Packed(const Tensor& q_, const Tensor& s_) : q(q_), scale(s_) {}
-    delrec_packed8 arg() const {
-        if (!q.defined()) return {nullptr, nullptr};
-        return {(int8_t*)q.data_ptr(), (float*)scale.data_ptr()};
-    }
-};
-
-float* fptr(const Tensor& t) { return t.defined() ? (float*)t.data_ptr() : nullptr; }
-
-Tensor workspace(int kind, int T, int B, int N, const Tensor& like) {
-    size_t n = 0;
-    check(delrec_query_workspace(kind, T, B, N, 1, 0, &n), "delrec_query_workspace");
-    return n ? at::empty({(int64_t)n}, like.options().dtype(at::kByte)) : Tensor();
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
 // ---------------------------------------------------------------- the recurrence ------------
 
@@ -278,8 +103,6 @@ variable_list scan_with_graph(const Tensor& z, const Tensor& f, const Tensor& bi
     return out;
 }
 
-py::tuple pair_of(const variable_list& v) { return py::make_tuple(v[0], v[1]); }
-
 py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTensor starts_, OptTensor lengths_, bool checkpoint) {
     const Tensor bias = given(bias_), h0 = given(h0_);
     Tensor starts = given(starts_), lengths = given(lengths_);
@@ -290,16 +113,7 @@ py::tuple gated_scan(Tensor z, Tensor f, OptTensor bias_, OptTensor h0_, OptTens
     const int64_t T = z.size(0), B = z.size(1), N = z.size(2);
     if (h0.defined() && (h0.dim() != 2 || h0.size(0) != B || h0.size(1) != N || h0.device() != z.device() || h0.scalar_type() != at::kFloat))
         refuse(text("h0 is ", describe(h0), ", expected [", B, ", ", N, "] Float on ", z.device()));
-    if (starts.defined()) {
-        if (starts.dim() != 2 || starts.size(0) != T || starts.size(1) != B || starts.device() != z.device())
-            refuse(text("starts is ", describe(starts), ", expected [", T, ", ", B, "] on ", z.device()));
-        starts = starts.to(at::kBool).contiguous();
-    }
-    if (lengths.defined()) {
-        if (lengths.dim() != 1 || lengths.size(0) != B || lengths.device() != z.device() || !at::isIntegralType(lengths.scalar_type(), false))
-            refuse(text("lengths is ", describe(lengths), ", expected [", B, "] integers on ", z.device()));
-        lengths = lengths.to(at::kLong).contiguous();
-    }
+    check_masks(starts, lengths, T, B, z);
     if (T == 0) {
         // no step: the output is a tensor of the graph all the same, and its gradients are zeros
         Tensor h = z * f;
@@ -472,6 +286,103 @@ Tensor rms_norm(Tensor x, OptTensor w_, double eps, bool checkpoint) {
                         x.sizes(), false, nullptr)[1];
 }
 
+// ---------------------------------------------------------------- residual addition, norm --
+
+// x', u; with `pack` u8, with `stats` the rows' norms
+variable_list add_norm_forward(const Tensor& x, const Tensor& y, const Tensor& w, double eps, at::IntArrayRef shape, Packed* u8, Tensor* stats) {
+    const c10::DeviceGuard guard(x.device());
+    const int R0 = as_int(x.size(0)), R1 = x.dim() == 3 ? as_int(x.size(1)) : 1, N = as_int(x.size(-1));
+    const int64_t rows = (int64_t)R0 * R1;
+    Tensor xo = at::empty(shape, x.options()), u = at::empty(shape, y.options());
+    delrec_add_norm_fwd_args a{};
+    if (stats) {
+        *stats = at::empty({rows}, x.options().dtype(at::kFloat));
+        a.stats = fptr(*stats);
+    }
+    if (u8) {
+        *u8 = Packed(rows, N, x);
+        a.u8 = u8->arg();
+    }
+    a.R0 = R0; a.R1 = R1; a.N = N; a.bf16 = is_bf16(y); a.x_bf16 = is_bf16(x);
+    a.x = rows_of(x); a.y = rows_of(y); a.w = fptr(w); a.eps = (float)eps;
+    a.x_out = xo.data_ptr(); a.u = u.data_ptr();
+    check(delrec_add_norm_fwd(&a, stream_of(x)), "delrec_add_norm_fwd");
+    return {xo, u};
+}
+
+struct AddNormBackward : public KeptNode {
+    std::string name() const override { return "AddNormBackward"; }
+    std::vector<int64_t> shape;
+    at::ScalarType act = at::kFloat, res = at::kFloat;
+    int R0 = 0, R1 = 0;
+
+    variable_list apply(variable_list&& grads) override {
+        const variable_list s = take();
+        const Tensor &w = s[2], &stats = s[3];
+        refuse_capture("add_norm", stats);
+        once_differentiable("add_norm");
+        const Tensor dxo = rows_form(grads[0]), du = rows_form(grads[1]);
+        if (!dxo.defined() && !du.defined()) return variable_list(3);
+        const c10::DeviceGuard guard(stats.device());
+        const int N = (int)shape.back();
+        const auto f32 = stats.options();
+        Tensor dx = at::empty(shape, f32.dtype(res)), dy, dw = at::empty({N}, f32);
+        if (act != res) dy = at::empty(shape, f32.dtype(act));
+        const Tensor ws = workspace(DELREC_WS_ADD_NORM_BWD, R0, R1, N, stats);
+        delrec_add_norm_bwd_args a{};
+        a.R0 = R0; a.R1 = R1; a.N = N; a.bf16 = act == at::kBFloat16; a.x_bf16 = res == at::kBFloat16;
+        a.x = rows_of(s[0]); a.y = rows_of(s[1]); a.w = fptr(w); a.stats = fptr(stats);
+        if (dxo.defined()) a.dx_out = rows_of(dxo);
+        if (du.defined()) a.du = rows_of(du);
+        a.dx = dx.data_ptr(); a.dy = dy.defined() ? dy.data_ptr() : nullptr; a.dw = fptr(dw);
+        a.workspace = ws.data_ptr(); a.workspace_bytes = (size_t)ws.numel();
+        check(delrec_add_norm_bwd(&a, stream_of(stats)), "delrec_add_norm_bwd");
+        return {dx, dy.defined() ? dy : dx, dw};
+    }
+};
+
+py::tuple add_norm(Tensor x, Tensor y, OptTensor w_, double eps, bool pack) {
+    const Tensor w = given(w_);
+    check_activation(y, "y");
+    if (x.scalar_type() != y.scalar_type() && x.scalar_type() != at::kFloat)
+        refuse(text("x must be ", y.scalar_type(), " or Float, got ", x.scalar_type()));
+    check_like(x, y, x.scalar_type(), "x");
+    check_width(x);
+    if (!w.defined()) refuse("weight is needed");
+    check_tangents("add_norm", {&x, &y, &w});
+    const int64_t N = x.size(-1);
+    Packed u8;
+    variable_list out;
+    if (x.numel() == 0) {
+        const Tensor sum = x + y.to(x.scalar_type());
+        out = {sum, (sum * w).to(y.scalar_type())};
+        if (pack) u8 = Packed(x.numel() / N, N, x);
+    } else if (wanted({&x, &y, &w})) {
+        auto node = make_node<AddNormBackward>();
+        node->set_next_edges(torch::autograd::collect_next_edges(x, y, w));
+        const Tensor xr = kept_rows(x), yr = kept_rows(y);
+        Tensor wc, stats;
+        {
+            at::AutoDispatchBelowADInplaceOrView below;
+            wc = vector_arg(w, N, x, "weight");
+            out = add_norm_forward(xr, yr, wc, eps, x.sizes(), pack ? &u8 : nullptr, &stats);
+        }
+        // x' in 32 bits is the sum itself; of bf16 the addends are kept. Detached (above the autograd
+        // keys, so that changes in place are noticed): the node is not to hold what holds the node.
+        const bool sum = x.scalar_type() == at::kFloat;
+        node->keep({sum ? kept_rows(out[0].detach()) : xr, sum ? Tensor() : yr, wc, stats});
+        node->shape = x.sizes().vec();
+        node->act = y.scalar_type();
+        node->res = x.scalar_type();
+        node->R0 = (int)xr.size(0);
+        node->R1 = xr.dim() == 3 ? (int)xr.size(1) : 1;
+        torch::autograd::set_history(out, node);
+    } else {
+        out = add_norm_forward(rows_form(x), rows_form(y), vector_arg(w, N, x, "weight"), eps, x.sizes(), pack ? &u8 : nullptr, nullptr);
+    }
+    return py::make_tuple(out[0], out[1], pack ? py::cast(u8.q.narrow(1, 0, N)) : py::none(), pack ? py::cast(u8.scale) : py::none());
+}
+
 // ---------------------------------------------------------------- one step, 8 bits ----------
 
 py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor w_, OptTensor scale_, OptTensor w2_,
@@ -567,6 +478,8 @@ void bind_gated(py::module_& m) {
     m.def("norm_gate_residual", &norm_gate_residual, "norms, gate and residual (autograd)", py::arg("o"), py::arg("g"),
           py::arg("x"), py::arg("weight"), py::arg("scale"), py::arg("next_weight"), py::arg("eps"), py::arg("checkpoint"));
     m.def("rms_norm", &rms_norm, "norm of rows (autograd)", py::arg("x"), py::arg("weight"), py::arg("eps"), py::arg("checkpoint"));
+    m.def("add_norm", &add_norm, "residual addition and norm (autograd)", py::arg("x"), py::arg("y"), py::arg("weight"), py::arg("eps"),
+          py::arg("pack"));
     m.def("gated_step", &gated_step, "one time step of the block", py::arg("z"), py::arg("f"), py::arg("g"), py::arg("x"),
           py::arg("h"), py::arg("weight"), py::arg("scale"), py::arg("next_weight"), py::arg("bias"), py::arg("eps"), py::arg("h_out"));
     m.def("pack8", &pack8, "rows to 8 bits", py::arg("x"));

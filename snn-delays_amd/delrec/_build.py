@@ -19,8 +19,8 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG.parent / 'csrc'
 INCLUDE = PKG.parent.parent / 'include'
 OUT = PKG / 'libdelrec_hip.so'
-SOURCES = ('abi.hip', 'axonal.hip', 'axwide.hip', 'farsparse.hip', 'gated.hip', 'gated_abi.hip', 'gemm.hip', 'hybblock.hip', 'hybstep.hip', 'lagmm.hip', 'lagstep.hip', 'normgate.hip',
-           'pack8.hip', 'peaks.hip', 'readout.hip', 'spikelinear.hip', 'synaptic.hip', 'synlin.hip')
+SOURCES = ('abi.hip', 'axonal.hip', 'axwide.hip', 'conv.hip', 'farsparse.hip', 'gated.hip', 'gated_abi.hip', 'gemm.hip', 'hybblock.hip', 'hybstep.hip', 'lagmm.hip', 'lagstep.hip', 'normgate.hip',
+           'pack8.hip', 'peaks.hip', 'readout.hip', 'selective.hip', 'selective_abi.hip', 'spikelinear.hip', 'synaptic.hip', 'synlin.hip')
 ARCH = os.environ.get('DELREC_OFFLOAD_ARCH', 'gfx950')
 
 
@@ -47,12 +47,13 @@ def _run(cmd, verbose):
         raise RuntimeError(f'hipcc failed ({res.returncode}): {cmd[-1]}')
 
 
-EXT_SOURCES = (CSRC / 'torch_ext.cpp', CSRC / 'torch_gated.cpp')
+EXT_SOURCES = (CSRC / 'torch_ext.cpp', CSRC / 'torch_gated.cpp', CSRC / 'torch_selective.cpp')
 EXT_OUT = PKG / 'delrec_torch.so'
 
 
 def extension_command(out=EXT_OUT):
-    """Host-only compile of the C++ autograd Functions (torch_ext.cpp, torch_gated.cpp) against
+    """Host-only compile of the C++ autograd Functions (torch_ext.cpp, torch_gated.cpp,
+    torch_selective.cpp) against
     torch and the HIP library, which it finds next to itself at run time (rpath $ORIGIN)."""
     import sysconfig
     import torch

@@ -29,8 +29,9 @@ DELREC_ERR_WINDOW = 5
 DELREC_ERR_SCRATCH = 9
 WS_AXONAL_FWD, WS_AXONAL_BWD, WS_SYN_FWD, WS_SYN_BWD, WS_SPIKE_LINEAR = 1, 2, 3, 4, 5
 WS_SPIKE_LINEAR_DW, WS_READOUT_CE = 6, 7
-WS_GATED_FWD, WS_GATED_BWD, WS_NORM_GATE_BWD = 8, 9, 10
-GATED_BLOCK, PACK8_GROUP = 64, 64
+WS_GATED_FWD, WS_GATED_BWD, WS_NORM_GATE_BWD, WS_ADD_NORM_BWD = 8, 9, 10, 11
+WS_CAUSAL_CONV_BWD, WS_SELECTIVE_FWD, WS_SELECTIVE_BWD = 12, 13, 14
+GATED_BLOCK, PACK8_GROUP, SELECTIVE_BLOCK = 64, 64, 16
 READOUT_SUM, READOUT_MEAN, READOUT_MAX = 0, 1, 2
 
 # Every symbol include/delrec.h declares (checked by the CPU test suite).
@@ -41,6 +42,8 @@ EXPORTS = ('delrec_axonal_fwd', 'delrec_axonal_bwd', 'delrec_axonal_bwd_noalloc'
            'delrec_max_post', 'delrec_max_take', 'delrec_peak_mfma', 'delrec_spike_linear_dw',
            'delrec_spike_linear_dx_split', 'delrec_readout_ce', 'delrec_gated_scan_fwd',
            'delrec_gated_scan_bwd', 'delrec_gated_step', 'delrec_norm_gate_fwd', 'delrec_norm_gate_bwd',
+           'delrec_add_norm_fwd', 'delrec_add_norm_bwd', 'delrec_causal_conv_fwd', 'delrec_causal_conv_bwd',
+           'delrec_selective_scan_fwd', 'delrec_selective_scan_bwd', 'delrec_selective_step',
            'delrec_pack8', 'delrec_unpack8')
 
 
@@ -166,12 +169,57 @@ class GatedStepArgs(ctypes.Structure):
                 ('w2', c_vp), ('eps', c_f32), ('h_out', c_vp), ('x_out', c_vp), ('u', c_vp)]
 
 
+class AddNormFwdArgs(ctypes.Structure):
+    _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x_bf16', c_i32), ('x', Rows), ('y', Rows),
+                ('w', c_vp), ('eps', c_f32), ('x_out', c_vp), ('u', c_vp), ('stats', c_vp), ('u8', Packed8)]
+
+
+class AddNormBwdArgs(ctypes.Structure):
+    _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x_bf16', c_i32), ('x', Rows), ('y', Rows),
+                ('w', c_vp), ('stats', c_vp), ('dx_out', Rows), ('du', Rows), ('dx', c_vp), ('dy', c_vp), ('dw', c_vp),
+                ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class CausalConvFwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('W', c_i32), ('bf16', c_i32), ('silu', c_i32), ('x', Rows),
+                ('w', c_vp), ('bias', c_vp), ('state', c_vp), ('starts', c_vp), ('lengths', c_vp), ('y', Rows),
+                ('state_out', c_vp)]
+
+
+class CausalConvBwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('W', c_i32), ('bf16', c_i32), ('silu', c_i32), ('x', Rows),
+                ('w', c_vp), ('bias', c_vp), ('state', c_vp), ('starts', c_vp), ('lengths', c_vp), ('dy', Rows),
+                ('dstate_out', c_vp), ('dx', Rows), ('dstate', c_vp), ('dw', c_vp), ('db', c_vp), ('workspace', c_vp),
+                ('workspace_bytes', c_size)]
+
+
+class SelectiveScanFwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('S', c_i32), ('bf16', c_i32), ('x', Rows), ('dt', Rows),
+                ('g', Rows), ('Bm', Rows), ('C', Rows), ('A', c_vp), ('D', c_vp), ('dt_bias', c_vp), ('h0', c_vp),
+                ('starts', c_vp), ('lengths', c_vp), ('y', Rows), ('h_last', c_vp), ('states', c_vp),
+                ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class SelectiveScanBwdArgs(ctypes.Structure):
+    _fields_ = [('T', c_i32), ('B', c_i32), ('N', c_i32), ('S', c_i32), ('bf16', c_i32), ('x', Rows), ('dt', Rows),
+                ('g', Rows), ('Bm', Rows), ('C', Rows), ('A', c_vp), ('D', c_vp), ('dt_bias', c_vp), ('states', c_vp),
+                ('starts', c_vp), ('lengths', c_vp), ('dy', Rows), ('dlast', c_vp), ('dx', Rows), ('ddt', Rows),
+                ('dg', Rows), ('dBm', c_vp), ('dC', c_vp), ('dA', c_vp), ('dD', c_vp), ('ddt_bias', c_vp), ('dh0', c_vp),
+                ('workspace', c_vp), ('workspace_bytes', c_size)]
+
+
+class SelectiveStepArgs(ctypes.Structure):
+    _fields_ = [('B', c_i32), ('N', c_i32), ('S', c_i32), ('bf16', c_i32), ('x', Rows), ('dt', Rows), ('g', Rows),
+                ('Bm', Rows), ('C', Rows), ('A', c_vp), ('D', c_vp), ('dt_bias', c_vp), ('h', c_vp), ('h_out', c_vp),
+                ('y', c_vp)]
+
+
 class Pack8Args(ctypes.Structure):
     _fields_ = [('R0', c_i32), ('R1', c_i32), ('N', c_i32), ('bf16', c_i32), ('x', Rows), ('p', Packed8)]
 
 
 # the DELREC_ABI_VERSION of include/delrec.h these ctypes structs mirror
-ABI_VERSION = '0.6.0'
+ABI_VERSION = '0.7.0'
 
 _lib = None
 
@@ -188,8 +236,9 @@ def load():
     for name in ('delrec_axonal_fwd', 'delrec_axonal_bwd', 'delrec_axonal_bwd_noalloc', 'delrec_syn_fwd',
                  'delrec_syn_bwd', 'delrec_spike_linear_fwd', 'delrec_spike_linear_dw', 'delrec_readout_ce',
                  'delrec_lif_fwd', 'delrec_lif_bwd', 'delrec_gated_scan_fwd', 'delrec_gated_scan_bwd',
-                 'delrec_gated_step', 'delrec_norm_gate_fwd', 'delrec_norm_gate_bwd', 'delrec_pack8',
-                 'delrec_unpack8'):
+                 'delrec_gated_step', 'delrec_norm_gate_fwd', 'delrec_norm_gate_bwd', 'delrec_add_norm_fwd',
+                 'delrec_add_norm_bwd', 'delrec_causal_conv_fwd', 'delrec_causal_conv_bwd', 'delrec_selective_scan_fwd',
+                 'delrec_selective_scan_bwd', 'delrec_selective_step', 'delrec_pack8', 'delrec_unpack8'):
         getattr(lib, name).restype = c_i32
         getattr(lib, name).argtypes = [c_vp, c_vp]
     lib.delrec_delay_grad.restype = c_i32

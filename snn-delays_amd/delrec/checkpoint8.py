@@ -42,8 +42,9 @@ def unpack8(p):
 
 class Linear8Fn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        p = pack8(x)
+    def forward(ctx, x, weight, bias, p):
+        if p is None:
+            p = pack8(x)
         ctx.save_for_backward(weight, p.q, p.scale)
         ctx.meta = (p.shape, p.dtype)
         ctx.has_bias = bias is not None
@@ -62,17 +63,21 @@ class Linear8Fn(torch.autograd.Function):
             dw = g2.t() @ x
         if ctx.has_bias and ctx.needs_input_grad[2]:
             db = g2.sum(0)
-        return dx, dw, db
+        return dx, dw, db, None
 
 
-def linear8(x, weight, bias=None):
-    """``torch.nn.functional.linear`` that keeps x in 8 bits for the weight's gradient."""
+def linear8(x, weight, bias=None, packed=None):
+    """``torch.nn.functional.linear`` that keeps x in 8 bits for the weight's gradient.
+    ``packed``: x's ``Packed8``, where what made x has packed it already (``gated.add_norm``)."""
     if not (torch.is_grad_enabled() and weight.requires_grad):
         return torch.nn.functional.linear(x, weight, bias)
     if torch.is_autocast_enabled('cuda'):
         dt = torch.get_autocast_dtype('cuda')
         x, weight, bias = x.to(dt), weight.to(dt), None if bias is None else bias.to(dt)
-    return Linear8Fn.apply(x, weight, bias)
+    if packed is not None and (packed.shape != x.shape or packed.dtype != x.dtype or packed.q.device != x.device):
+        raise ValueError(f'packed is {tuple(packed.shape)} {packed.dtype} on {packed.q.device}, x is {tuple(x.shape)} {x.dtype} '
+                         f'on {x.device}')
+    return Linear8Fn.apply(x, weight, bias, packed)
 
 
 class Linear8(torch.nn.Linear):

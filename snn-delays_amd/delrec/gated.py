@@ -4,6 +4,7 @@ same time-major (T, B, N) sequences as the delayed-LIF layers.
     gated_scan           h_t = h_{t-1} + k_t (z_t - h_{t-1}), k_t = sigmoid(-(f_t + bias))
     norm_gate_residual   x' = x + scale * rms(o) * weight * silu(g), u = rms(x') * next_weight
     rms_norm             u = rms(x) * weight
+    add_norm             x' = x + y, u = rms(x') * weight, u also in 8 bits
     gated_step           one time step of both, for streaming input
     GatedBlock           the residual block they make with its Linear
 
@@ -18,7 +19,7 @@ captured in a graph, backward passes cannot. No counterpart in the reference.
 import torch
 
 from . import _lib
-from .checkpoint8 import Linear8
+from .checkpoint8 import Linear8, Packed8
 
 
 def gated_scan(z, f, bias=None, h0=None, starts=None, lengths=None, checkpoint=False):
@@ -49,6 +50,17 @@ def rms_norm(x, weight, eps=1e-6, checkpoint=False):
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis of an fp32 or bf16 (..., N)
     tensor; ``checkpoint=True`` keeps x in 8 bits for the backward pass."""
     return _lib.require_ext().rms_norm(x, weight, eps, checkpoint)
+
+
+def add_norm(x, y, weight, eps=1e-6, pack=False):
+    """The residual stream and the next block's input: ``x' = x + y``, ``u = rms(x') * weight``:
+    ``(x', u)``, or with ``pack`` ``(x', u, packed)``, u's ``checkpoint8.Packed8`` as ``pack8(u)`` makes
+    it, in the same pass (not differentiable; for ``linear8``).
+
+    ``y`` (..., N) fp32 or bf16, ``x`` of its type or fp32; ``weight`` (N,). x' has x's type, u has
+    y's; u's norm is taken before x' is rounded. Differentiable in all three."""
+    x, u, q, scale = _lib.require_ext().add_norm(x, y, weight, eps, pack)
+    return (x, u, Packed8(q, scale, u.shape, u.dtype)) if pack else (x, u)
 
 
 def gated_step(z, f, g, x, h, weight, scale, next_weight=None, bias=None, eps=1e-6, h_out=None):

@@ -7,7 +7,8 @@ recurrent delays (``networks.py:140-400, 802-984, 1128-1204``). Layers are creat
 reference's order, so a seeded model draws the same initial parameters.
 
 ``RNN_gated`` is the non-spiking counterpart on the same (T, B, N) inputs: a residual stack of
-gated linear recurrences (``delrec.gated``), without one in the reference.
+gated linear recurrences (``delrec.gated``), ``RNN_selective`` one of selective state-space blocks
+(``delrec.selective``), without ones in the reference.
 
 Feedforward-delay classes ride DCLS's convolution, not this path, and are not provided;
 ``dcls_module`` exists only so ``isinstance`` checks in callers keep working.
@@ -17,8 +18,9 @@ import torch
 
 from .spike_linear import SpikeLinear
 
-from .checkpoint8 import Linear8
+from .checkpoint8 import Linear8, linear8
 from .gated import GatedBlock, rms_norm
+from .selective import SelectiveBlock
 from .delay_layers import axonal_recdel, synaptic_recdel, common_recdel
 from .neuron import Dropout
 
@@ -409,4 +411,58 @@ class RNN_gated(torch.nn.Module):
         u = rms_norm(x, self.norm_weight)
         for block, h in zip(self.blocks, state):
             x, u, _ = block.step(x, u, h, h_out=h)
+        return torch.nn.functional.linear(u, self.readout.weight, self.readout.bias), state
+
+
+class RNN_selective(torch.nn.Module):
+    """A residual stack of selective state-space blocks over (T, B, N): ``Linear -> rms_norm ->
+    SelectiveBlock ... -> Linear``, one block for each entry of ``config.hidden_layers`` (all of one
+    width). Trains with ``delrec.training.mem`` like the ``SNN_*`` classes; ``step`` runs it one time
+    step at a time on streaming input, from where ``forward(..., return_state=True)`` left off.
+    Types and config as ``RNN_gated``'s; ``config.state_size`` (default 16) and
+    ``config.conv_width`` (default 4) are the blocks' S and W. ``config.checkpoint8`` (default False):
+    the Linears that read a block's norm keep that input in 8 bits for the backward pass."""
+
+    def __init__(self, config):
+        super().__init__()
+        widths = set(config.hidden_layers)
+        if len(widths) != 1:
+            raise ValueError(f'RNN_selective needs hidden layers of one width, got {config.hidden_layers}')
+        N = widths.pop()
+        if getattr(config, 'use_batch_norm', False):
+            _batch_norm(config, N)
+        if getattr(config, 'feedforward_dropout_rate', 0.0):
+            raise NotImplementedError(f'feedforward_dropout_rate={config.feedforward_dropout_rate}: RNN_selective has no dropout')
+        self.config = config
+        self.checkpoint = bool(getattr(config, 'checkpoint8', False))
+        S, W = int(getattr(config, 'state_size', 16)), int(getattr(config, 'conv_width', 4))
+        self.embed = torch.nn.Linear(config.input_size, N, bias=config.bias)
+        self.norm_weight = torch.nn.Parameter(torch.ones(N))
+        self.blocks = torch.nn.ModuleList(SelectiveBlock(N, S=S, W=W, bias=config.bias, checkpoint=self.checkpoint)
+                                          for _ in config.hidden_layers)
+        self.readout = (Linear8 if self.checkpoint else torch.nn.Linear)(N, config.output_size, bias=config.bias)
+
+    def forward(self, x, starts=None, lengths=None, state=None, return_state=False):
+        """The readout (T, B, output_size); with ``return_state`` also the blocks' states after the
+        last step, which ``step`` and a further call (as ``state``) go on from."""
+        assert x.dim() == 3  # (T, B, N)
+        x = self.embed(x).float()
+        u, packed, after = rms_norm(x, self.norm_weight, checkpoint=self.checkpoint), None, []
+        for block, before in zip(self.blocks, [None] * len(self.blocks) if state is None else state):
+            x, u, packed, new = block(x, u, packed, before, starts, lengths)
+            after.append(new)
+        y = linear8(u, self.readout.weight, self.readout.bias, packed=packed) if self.checkpoint else self.readout(u)
+        return (y, after) if return_state else y
+
+    @torch.no_grad()
+    def step(self, x, state=None):
+        """One time step of inputs (B, input_size): the readout (B, output_size) and the blocks'
+        states, which are updated in place (``None``: all zero)."""
+        x = self.embed(x)
+        if state is None:
+            state = [block.zero_state(x.shape[0], x.dtype) for block in self.blocks]
+        x = x.float()
+        u = rms_norm(x, self.norm_weight)
+        for block, before in zip(self.blocks, state):
+            x, u = block.step(x, u, before)
         return torch.nn.functional.linear(u, self.readout.weight, self.readout.bias), state
