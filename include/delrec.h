@@ -461,8 +461,8 @@ typedef struct {
 /* d_t = softplus(dt_t + dt_bias); h_t = exp(d_t A) h_{t-1} + d_t x_t B_t; y_t = (<C_t, h_t> + D x_t)
  * times g_t sigmoid(g_t) where there is a g; S in [1, 64] states a channel. At a start the state before the
  * step is 0; from lengths[b] on the state stays and y is written 0. states[i] is the state before
- * step 16 i, which the backward pass starts from. Outputs must not overlap inputs. */
-enum { DELREC_SELECTIVE_BLOCK = 16 };
+ * step 8 i, which the backward pass starts from. Outputs must not overlap inputs. */
+enum { DELREC_SELECTIVE_BLOCK = 8 };
 typedef struct {
     int32_t T, B, N, S, bf16;
     delrec_rows x, dt, g;        /* (T, B, N); g.data NULL: no gate                        */
@@ -475,7 +475,7 @@ typedef struct {
     const int64_t* lengths;
     delrec_rows y;               /* out (T, B, N)                                          */
     float* h_last;               /* out (B, N, S)                                          */
-    float* states;               /* out (ceil(T / 16), B, N, S), or NULL                   */
+    float* states;               /* out (ceil(T / 8), B, N, S), or NULL                    */
     void* workspace;
     size_t workspace_bytes;
 } delrec_selective_scan_fwd_args;

@@ -664,7 +664,7 @@ struct Selective {               // forward, backward and one step of the select
     const uint8_t* starts;
     const int64_t* lengths;
     float* h_last;
-    float* states;               // [ceil(T / 16)][B][N][S]
+    float* states;               // [ceil(T / 8)][B][N][S]
     delrec_rows dy, dx, ddt, dg;
     const float* dlast;
     float* dA;
@@ -676,7 +676,9 @@ struct Selective {               // forward, backward and one step of the select
     float* ws;                   // workspace, selective_fwd_ws / selective_bwd_ws floats
     float* bcsums;               // set by the launcher: parts of ws, and
     float* rowsums;
-    int tiles;                   // workgroups of channels,
+    float* maps;                 // [ranges][B][N][S], [ranges][B][N]
+    float* mapsums;
+    int tiles, range;            // workgroups of channels, steps of a range,
     long long first;             // the launch's first workgroup
 };
 bool selective_sizes_ok(int T, int B, int N, int S);   // what the entry points take (selective_abi.hip)

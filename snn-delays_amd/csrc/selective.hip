@@ -28,9 +28,11 @@ namespace delrec {
 
 namespace {
 
-constexpr int kStepsB = DELREC_SELECTIVE_BLOCK;
+constexpr int kStepsB = 16;                       // steps of a block
+constexpr int kKept = DELREC_SELECTIVE_BLOCK;     // steps from one kept state to the next
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWavesWg = 4;
+constexpr int kGroupsFwd = 1024, kGroupsBwd = 512;
 
 template <int... I, class F>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I>()), ...); }
@@ -85,6 +87,32 @@ __device__ __forceinline__ float sums_by_lane(float* v, int j) {
     hand_over<1, 0xB1>(v, j & 1);
     return v[0];
 }
+// A step's partial sums of a group's lanes, taken in until the lanes' own steps are complete: then each
+// lane has its step's total. Four steps at a time are reduced over quads of lanes (16 lanes: the quads'
+// sums over the row's four quads at the end), so that few registers wait.
+template <int Q>
+struct Sums {
+    float v[4], quad[Q == 16 ? 4 : 1];
+    template <int I>
+    __device__ __forceinline__ void add(float x, int j) {
+        v[I % 4] = x;
+        if constexpr (Q == 16 && I % 4 == 0) {      // (steps come last first)
+            hand_over<2, 0x4E>(v, j & 2);
+            hand_over<1, 0xB1>(v, j & 1);
+            quad[I / 4] = v[0];
+        }
+    }
+    __device__ __forceinline__ float total(int j) {
+        if constexpr (Q == 4) return sums_by_lane<4>(v, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            quad[i % (Q / 4)] = add_dpp<0x124>(quad[i % (Q / 4)], quad[i % (Q / 4)]);   // row_ror:4
+            quad[i % (Q / 4)] = add_dpp<0x128>(quad[i % (Q / 4)], quad[i % (Q / 4)]);   // row_ror:8
+        }
+        const float lo = j & 4 ? quad[1 % (Q / 4)] : quad[0], hi = j & 4 ? quad[3 % (Q / 4)] : quad[2 % (Q / 4)];
+        return j & 8 ? hi : lo;
+    }
+};
 template <int Q>
 __device__ __forceinline__ float lanes_total(float v) {
     return group_sum_t<Q>(v);
@@ -122,6 +150,13 @@ __device__ __forceinline__ void store_states(float* row, const float* v, int s0,
         for (int k = 0; k < K; ++k)
             if (on && s0 + k < S) row[s0 + k] = v[k];
     }
+}
+
+// What stands before is finished before what stands after begins, and LDS is read again: the compiler
+// otherwise keeps what it read once, and mixes the steps, until registers run out.
+__device__ __forceinline__ void fence() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 template <int Q>
@@ -185,229 +220,348 @@ struct Stage {
     }
 };
 
-// a lane's own steps of a block of one of the (T, B, N) inputs; zeros past the row's end
+// A lane's own steps of a block in one of the (T, B, N) tensors: the block's first step is a base for the
+// workgroup, moved in scalar registers, the lane's distance from it stays.
+template <class E, int Q>
+struct Column {
+    const E* base;
+    long long pitch, lane;
+    __device__ __forceinline__ Column(const delrec_rows& x, int b, int n, int j)
+        : base((const E*)x.data + b * x.s1), pitch(x.s0), lane(j * x.s0 + n) {}
+    __device__ __forceinline__ E* at(int t0, int i) const { return (E*)(base + (t0 + i * Q) * pitch) + lane; }
+};
+// zeros past the row's end and in lanes without a channel
 template <class E, int Q>
 struct Own {
     E v[Shape<Q>::own];
-    __device__ __forceinline__ void load(const delrec_rows& x, const char* at, int t0, int j, int tend, bool on) {
+    template <bool FULL, int FROM = 0, int COUNT = Shape<Q>::own>
+    __device__ __forceinline__ void load(const Column<E, Q>& x, int t0, int j, int tend, bool on) {
 #pragma unroll
-        for (int i = 0; i < Shape<Q>::own; ++i) {
-            const int t = t0 + i * Q + j;
-            v[i] = (E)0.0f;
-            if (on && t < tend) v[i] = ((const E*)at)[t * x.s0];
+        for (int i = FROM; i < FROM + COUNT; ++i) {
+            if (FULL) {
+                v[i] = *x.at(t0, i);
+            } else {
+                v[i] = (E)0.0f;
+                if (on && t0 + i * Q + j < tend) v[i] = *x.at(t0, i);
+            }
         }
     }
 };
-template <class E>
-__device__ __forceinline__ const char* column(const delrec_rows& x, int b, int n) {
-    return (const char*)((const E*)x.data + b * x.s1 + n);
+
+// The states that ranges of time start from. A range's map is h -> exp(A sum d) h + L (and of the carry,
+// backwards, the same with its own L); a start in it cuts off what comes before: sum d is then -1.
+template <int K>
+__device__ __forceinline__ void enter_range(float* h, const Selective& p, const float* A2, size_t row, size_t chan, int s0, bool on,
+                                            int from, int dir, int count) {
+    const size_t plane = (size_t)p.B * p.N * p.S;
+    for (int q = 0; q < count; ++q) {
+        const size_t r = from + dir * q;
+        float L[K];
+        load_states<K>(L, p.maps + r * plane + row, s0, p.S, on);
+        const float sd = on ? p.mapsums[r * p.B * p.N + chan] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) h[k] = sd < 0.0f ? L[k] : fmaf(__builtin_amdgcn_exp2f(A2[k] * sd), h[k], L[k]);
+    }
 }
+
+// what a step needs of its own lane
+struct Gate {
+    float value, slope;
+    __device__ __forceinline__ Gate(float g, bool has) {
+        const float s = sigmoid(g), v = g * s;
+        value = has ? v : 1.0f;
+        slope = fmaf(v, 1.0f - s, s);
+    }
+};
 
 }  // namespace
 
-template <class E, int Q, int K>
+// A launch without ranges takes all steps; with them blockIdx.y is the range.
+template <class E, int Q, int K, bool STARTS>
 __global__ void __launch_bounds__(256) selective_fwd_kernel(Selective p) {
-    constexpr int SP = Q * K;
+    constexpr int SP = Q * K, OWN = Shape<Q>::own;
     __shared__ __align__(16) float bc[2][kStepsB][2][SP];
     const Place<Q, K> at(p);
-    const int b = at.b, n = at.n, j = at.j, N = p.N, S = p.S;
-    const size_t row = ((size_t)b * N + n) * S, plane = (size_t)p.B * N * S;
-    const int tend = row_steps(p, b);
+    const int b = at.b, n = at.n, j = at.j, S = p.S;
+    const size_t chan = (size_t)b * p.N + n, row = chan * S, plane = (size_t)p.B * p.N * S;
+    const int len = row_steps(p, b), ts = blockIdx.y * p.range, te = min(ts + p.range, p.T), tend = min(te, len);
+    const bool whole = (at.tile + 1) * Shape<Q>::channels <= p.N, gated = p.g.data != nullptr;
     float A2[K], h[K];
     load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
     load_states<K>(h, p.h0 + row, at.s0, S, p.h0 && at.on);
 #pragma unroll
     for (int k = 0; k < K; ++k) A2[k] *= kLog2e;
+    if (blockIdx.y) enter_range<K>(h, p, A2, row, chan, at.s0, at.on, 0, 1, blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
-    const char *xp = column<E>(p.x, b, n), *dp = column<E>(p.dt, b, n), *gp = column<E>(p.g, b, n);
-    E* yp = (E*)column<E>(p.y, b, n);
+    const Column<E, Q> xc(p.x, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : p.x, b, n, j), yc(p.y, b, n, j);
 
     Stage<E, SP> bcv;
     Own<E, Q> xv, dv, gv;
     auto load = [&](int t0) {
         bcv.load(p, b, t0, tend);
-        dv.load(p.dt, dp, t0, j, tend, at.on);
-        xv.load(p.x, xp, t0, j, tend, at.on);
-        if (p.g.data) gv.load(p.g, gp, t0, j, tend, at.on);
+        auto three = [&](auto full) {
+            constexpr bool F = decltype(full)::value;
+            dv.template load<F>(dc, t0, j, tend, at.on);
+            xv.template load<F>(xc, t0, j, tend, at.on);
+            gv.template load<F>(gc, t0, j, tend, at.on);
+        };
+        whole && t0 + kStepsB <= tend ? three(std::true_type()) : three(std::false_type());
     };
-    if (tend > 0) load(0);
+    if (ts < tend) load(ts);
     int buf = 0;
-    for (int t0 = 0; t0 < tend; t0 += kStepsB, buf ^= 1) {
+    for (int t0 = ts; t0 < tend; t0 += kStepsB, buf ^= 1) {
         bcv.put(&bc[buf][0][0][0]);
         const Own<E, Q> x = xv, d = dv, g = gv;
         const uint32_t starts = start_bits(p, b, t0, tend, at.lane);
         barrier_lds();
         if (t0 + kStepsB < tend) load(t0 + kStepsB);
-        if (p.states) store_states<K>(p.states + (size_t)(t0 / kStepsB) * plane + row, h, at.s0, S, at.on);
-        auto walk = [&](auto masked) {
-            each<Shape<Q>::own>([&](auto sub) {
-                constexpr int c = decltype(sub)::value;
-                const int t = t0 + c * Q + j;
-                const bool valid = at.on && t < tend;
-                float slope, ys[Q];
-                const float xs = (float)x.v[c], delta = valid ? softplus((float)d.v[c] + bias, &slope) : 0.0f, u = delta * xs;
-                each<Q>([&](auto step) {
-                    constexpr int i = decltype(step)::value;
-                    if (decltype(masked)::value && starts >> (c * Q + i) & 1)
-#pragma unroll
-                        for (int k = 0; k < K; ++k) h[k] = 0.0f;
-                    const auto Bv = *(const Vec<float, K>*)&bc[buf][c * Q + i][0][at.s0];
-                    const auto Cv = *(const Vec<float, K>*)&bc[buf][c * Q + i][1][at.s0];
-                    const float di = from_lane<Q, i>(delta), ui = from_lane<Q, i>(u);
-                    ys[i] = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        h[k] = fmaf(__builtin_amdgcn_exp2f(di * A2[k]), h[k], ui * Bv.get(k));
-                        ys[i] = fmaf(h[k], Cv.get(k), ys[i]);
-                    }
-                });
-                float y = fmaf(D, xs, sums_by_lane<Q>(ys, j));
-                if (p.g.data) {
-                    const float gs = (float)g.v[c];
-                    y *= gs * sigmoid(gs);
-                }
-                if (valid) yp[t * p.y.s0] = (E)y;
-            });
+        auto keep = [&](int step) {
+            if (p.states && t0 + step < tend)
+                store_states<K>(p.states + (size_t)((t0 + step) / kKept) * plane + row, h, at.s0, S, at.on);
         };
-        starts ? walk(std::true_type()) : walk(std::false_type());
+        const bool full = whole && t0 + kStepsB <= tend;
+        each<OWN>([&](auto sub) {
+            constexpr int c = decltype(sub)::value;
+            const bool valid = at.on && t0 + c * Q + j < tend;
+            float slope, ys[Q];
+            const float xs = (float)x.v[c], soft = softplus((float)d.v[c] + bias, &slope), delta = valid ? soft : 0.0f, u = delta * xs;
+            each<Q>([&](auto step) {
+                constexpr int i = decltype(step)::value, s = c * Q + i;
+                if constexpr (s % kKept == 0) keep(s);
+                if (STARTS && starts >> s & 1)
+#pragma unroll
+                    for (int k = 0; k < K; ++k) h[k] = 0.0f;
+                const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
+                const auto Cv = *(const Vec<float, K>*)&bc[buf][s][1][at.s0];
+                const float di = from_lane<Q, i>(delta), ui = from_lane<Q, i>(u);
+                ys[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    h[k] = fmaf(__builtin_amdgcn_exp2f(di * A2[k]), h[k], ui * Bv.get(k));
+                    ys[i] = fmaf(h[k], Cv.get(k), ys[i]);
+                }
+            });
+            const float y = fmaf(D, xs, sums_by_lane<Q>(ys, j)) * Gate((float)g.v[c], gated).value;
+            if (full || valid) *yc.at(t0, c) = (E)y;
+        });
     }
-    for (int t = tend + j; t < p.T; t += Q)
-        if (at.on) yp[t * p.y.s0] = (E)0.0f;
-    store_states<K>(p.h_last + row, h, at.s0, S, at.on);
+    for (int t = max(ts, tend) / Q * Q; t < te; t += Q)
+        if (at.on && t + j >= tend && t + j < te) *yc.at(t, 0) = (E)0.0f;
+    if (te == p.T) store_states<K>(p.h_last + row, h, at.s0, S, at.on);
 }
 
-template <class E, int Q, int K>
-__global__ void __launch_bounds__(256) selective_bwd_kernel(Selective p) {
+// A range's map into p.maps and p.mapsums, forwards (of the states) or backwards (of the carry).
+template <class E, int Q, int K, bool STARTS, bool BWD>
+__global__ void __launch_bounds__(256) selective_range_kernel(Selective p) {
     constexpr int SP = Q * K, OWN = Shape<Q>::own;
+    __shared__ __align__(16) float bc[2][kStepsB][2][SP];
+    const Place<Q, K> at(p);
+    const int b = at.b, n = at.n, j = at.j, S = p.S;
+    const int y = blockIdx.y + (BWD ? 1 : 0);          // the last range forward, the first backward lead nowhere
+    const size_t chan = (size_t)b * p.N + n, row = chan * S, plane = (size_t)p.B * p.N * S;
+    const int ts = y * p.range, te = min(ts + p.range, p.T), tend = min(te, row_steps(p, b));
+    const bool whole = (at.tile + 1) * Shape<Q>::channels <= p.N, gated = p.g.data != nullptr;
+    float A2[K], h[K], total = 0.0f;
+    load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
+#pragma unroll
+    for (int k = 0; k < K; ++k) A2[k] *= kLog2e, h[k] = 0.0f;
+    const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f;
+    const delrec_rows& xr = BWD ? p.dy : p.x;
+    const Column<E, Q> xc(xr, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : xr, b, n, j);
+    Stage<E, SP> bcv;
+    Own<E, Q> xv, dv, gv;
+    auto load = [&](int t0) {
+        bcv.load(p, b, t0, tend);
+        auto all = [&](auto full) {
+            constexpr bool F = decltype(full)::value;
+            dv.template load<F>(dc, t0, j, tend, at.on);
+            xv.template load<F>(xc, t0, j, tend, at.on);
+            if constexpr (BWD) gv.template load<F>(gc, t0, j, tend, at.on);
+        };
+        whole && t0 + kStepsB <= tend ? all(std::true_type()) : all(std::false_type());
+    };
+    bool cut = false;
+    int buf = 0;
+    const int blocks = tend > ts ? (tend - ts + kStepsB - 1) / kStepsB : 0;
+    auto first = [&](int i) { return ts + (BWD ? blocks - 1 - i : i) * kStepsB; };
+    if (blocks) load(first(0));
+    for (int i = 0; i < blocks; ++i, buf ^= 1) {
+        const int t0 = first(i);
+        bcv.put(&bc[buf][0][0][0]);
+        const Own<E, Q> x = xv, d = dv, g = gv;
+        const uint32_t starts = start_bits(p, b, t0, tend, at.lane);
+        cut |= starts != 0;
+        barrier_lds();
+        if (i + 1 < blocks) load(first(i + 1));
+        each<OWN>([&](auto sub) {
+            constexpr int c = BWD ? OWN - 1 - decltype(sub)::value : decltype(sub)::value;
+            const bool valid = at.on && t0 + c * Q + j < tend;
+            float slope, soft = softplus((float)d.v[c] + bias, &slope);
+            const float delta = valid ? soft : 0.0f;
+            const float u = BWD ? (float)x.v[c] * Gate((float)g.v[c], gated).value : delta * (float)x.v[c];
+            total += delta;
+            each<Q>([&](auto step) {
+                constexpr int k0 = decltype(step)::value, q = BWD ? Q - 1 - k0 : k0, s = c * Q + q;
+                const bool fresh = STARTS && (starts >> s & 1);
+                const auto Mv = *(const Vec<float, K>*)&bc[buf][s][BWD ? 1 : 0][at.s0];
+                const float di = from_lane<Q, q>(delta), ui = from_lane<Q, q>(u);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float a = __builtin_amdgcn_exp2f(di * A2[k]);
+                    if constexpr (BWD) h[k] = fresh ? 0.0f : a * fmaf(ui, Mv.get(k), h[k]);
+                    else h[k] = fmaf(a, fresh ? 0.0f : h[k], ui * Mv.get(k));
+                }
+            });
+        });
+    }
+    store_states<K>(p.maps + y * plane + row, h, at.s0, S, at.on);
+    total = lanes_total<Q>(total);
+    if (at.on && j == 0) p.mapsums[(size_t)y * p.B * p.N + chan] = cut ? -1.0f : total;
+}
+
+template <class E, int Q, int K, bool STARTS>
+__global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
+    constexpr int SP = Q * K, OWN = Shape<Q>::own;
+    constexpr int HALF = OWN > 1 ? OWN / 2 : 1;       // own steps of a kept state's eight
     __shared__ __align__(16) float bc[2][kStepsB][2][SP];
     __shared__ __align__(16) float sums[kWavesWg][kStepsB][2][SP];
     const Place<Q, K> at(p);
     const int b = at.b, n = at.n, j = at.j, N = p.N, S = p.S;
-    const size_t row = ((size_t)b * N + n) * S, plane = (size_t)p.B * N * S;
-    const int tend = row_steps(p, b);
+    const size_t chan = (size_t)b * N + n, row = chan * S, plane = (size_t)p.B * N * S;
+    const int ts = blockIdx.y * p.range, te = min(ts + p.range, p.T), tend = min(te, row_steps(p, b));
+    const bool whole = (at.tile + 1) * Shape<Q>::channels <= N, gated = p.g.data != nullptr;
     float A2[K], kc[K], dA[K], dD = 0.0f, dbias = 0.0f;
     load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
     load_states<K>(kc, p.dlast + row, at.s0, S, p.dlast && at.on);
 #pragma unroll
     for (int k = 0; k < K; ++k) A2[k] *= kLog2e, dA[k] = 0.0f;
+    enter_range<K>(kc, p, A2, row, chan, at.s0, at.on, gridDim.y - 1, -1, gridDim.y - 1 - blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
-    const char *xp = column<E>(p.x, b, n), *dp = column<E>(p.dt, b, n), *gp = column<E>(p.g, b, n), *yp = column<E>(p.dy, b, n);
-    E *dxp = (E*)column<E>(p.dx, b, n), *ddp = (E*)column<E>(p.ddt, b, n), *dgp = (E*)column<E>(p.dg, b, n);
+    const Column<E, Q> xc(p.x, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : p.x, b, n, j), yc(p.dy, b, n, j);
+    const Column<E, Q> dxc(p.dx, b, n, j), ddc(p.ddt, b, n, j), dgc(gated ? p.dg : p.dx, b, n, j);
 
     Stage<E, SP> bcv;
     Own<E, Q> xv, dv, gv, yv;
-    auto load = [&](int t0) {
-        bcv.load(p, b, t0, tend);
-        dv.load(p.dt, dp, t0, j, tend, at.on);
-        xv.load(p.x, xp, t0, j, tend, at.on);
-        if (p.g.data) gv.load(p.g, gp, t0, j, tend, at.on);
-        yv.load(p.dy, yp, t0, j, tend, at.on);
+    // the own steps of a block, from the one after the last half's on (Q 16: one, with the first half)
+    auto load = [&](int t0, auto half) {
+        constexpr int from = OWN > 1 ? decltype(half)::value * HALF : 0;
+        auto four = [&](auto full) {
+            constexpr bool F = decltype(full)::value;
+            dv.template load<F, from, HALF>(dc, t0, j, tend, at.on);
+            xv.template load<F, from, HALF>(xc, t0, j, tend, at.on);
+            gv.template load<F, from, HALF>(gc, t0, j, tend, at.on);
+            yv.template load<F, from, HALF>(yc, t0, j, tend, at.on);
+        };
+        whole && t0 + kStepsB <= tend ? four(std::true_type()) : four(std::false_type());
     };
-    const int last = (tend - 1) / kStepsB * kStepsB;
-    if (tend > 0) load(last);
+    const int last = ts + (tend > ts ? (tend - ts - 1) / kStepsB * kStepsB : 0);
+    if (tend > ts) {
+        bcv.load(p, b, last, tend);
+        load(last, std::integral_constant<int, 1>());
+        if (OWN > 1) load(last, std::integral_constant<int, 0>());
+    }
     int buf = 0;
-    for (int t0 = last; tend > 0 && t0 >= 0; t0 -= kStepsB, buf ^= 1) {
+    for (int t0 = last; tend > ts && t0 >= ts; t0 -= kStepsB, buf ^= 1) {
         bcv.put(&bc[buf][0][0][0]);
-        const Own<E, Q> x = xv, d = dv, g = gv, dy = yv;
-        const uint32_t starts = start_bits(p, b, t0, tend, at.lane);
-        float h0[K];
-        load_states<K>(h0, p.states + (size_t)(t0 / kStepsB) * plane + row, at.s0, S, at.on);
+        const uint32_t starts = STARTS ? start_bits(p, b, t0, tend, at.lane) : 0;
+        const bool full = whole && t0 + kStepsB <= tend;
         barrier_lds();
-        if (t0 >= kStepsB) load(t0 - kStepsB);
-        auto walk = [&](auto masked) {
-            constexpr bool MASK = decltype(masked)::value;
-            float a[kStepsB][K], h[kStepsB][K], delta[OWN], slope[OWN], u[OWN], w[OWN], gate[OWN], gslope[OWN];
-            each<OWN>([&](auto sub) {
-                constexpr int c = decltype(sub)::value;
-                const bool valid = at.on && t0 + c * Q + j < tend;
-                delta[c] = softplus((float)d.v[c] + bias, &slope[c]);
-                delta[c] = valid ? delta[c] : 0.0f;
-                u[c] = delta[c] * (float)x.v[c];
-                gate[c] = 1.0f;
-                if (p.g.data) {
-                    const float gs = (float)g.v[c], sg = sigmoid(gs);
-                    gate[c] = gs * sg;
-                    gslope[c] = fmaf(gate[c], 1.0f - sg, sg);
+        if (t0 > ts) bcv.load(p, b, t0 - kStepsB, tend);
+        // the values of a lane's own steps of half a block (Q 4), or of its one (Q 16)
+        float delta[HALF], slope[HALF], u[HALF], w[HALF], ga[HALF], xs[HALF];
+        Sums<Q> ys, lb, aq;
+        each_back<2>([&](auto half) {
+            constexpr int hf = decltype(half)::value, s0 = hf * kKept;
+            float hk[K], a[kKept][K], h[kKept][K];
+            // (0 where all eight steps are padding: an infinite state times their step size of 0)
+            load_states<K>(hk, p.states + (size_t)((t0 + s0) / kKept) * plane + row, at.s0, S, at.on && t0 + s0 < tend);
+            if constexpr (OWN > 1 || hf == 1) {
+                each<HALF>([&](auto own) {
+                    constexpr int o = decltype(own)::value, c = (OWN > 1 ? hf * HALF : 0) + o;
+                    const bool valid = at.on && t0 + c * Q + j < tend;
+                    const float soft = softplus((float)dv.v[c] + bias, &slope[o]);
+                    delta[o] = valid ? soft : 0.0f;
+                    xs[o] = (float)xv.v[c];
+                    u[o] = delta[o] * xs[o];
+                    const Gate gate((float)gv.v[c], gated);
+                    w[o] = (float)yv.v[c] * gate.value;
+                    ga[o] = (float)yv.v[c] * gate.slope;
+                });
+                if (t0 > ts) load(t0 - kStepsB, half);
+            }
+            each<kKept>([&](auto step) {
+                constexpr int e = decltype(step)::value, s = s0 + e, o = OWN > 1 ? e / Q : 0, i = s % Q;
+                const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
+                const float di = from_lane<Q, i>(delta[o]), ui = from_lane<Q, i>(u[o]);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float before = STARTS && (starts >> s & 1) ? 0.0f : e ? h[e ? e - 1 : 0][k] : hk[k];
+                    a[e][k] = __builtin_amdgcn_exp2f(di * A2[k]);
+                    h[e][k] = fmaf(a[e][k], before, ui * Bv.get(k));
                 }
-                w[c] = (float)dy.v[c] * gate[c];
-                each<Q>([&](auto step) {
-                    constexpr int i = decltype(step)::value, s = c * Q + i;
-                    const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
-                    const float di = from_lane<Q, i>(delta[c]), ui = from_lane<Q, i>(u[c]);
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        const float before = MASK && (starts >> s & 1) ? 0.0f : s ? h[s ? s - 1 : 0][k] : h0[k];
-                        a[s][k] = __builtin_amdgcn_exp2f(di * A2[k]);
-                        h[s][k] = fmaf(a[s][k], before, ui * Bv.get(k));
-                    }
-                });
             });
-            each_back<OWN>([&](auto sub) {
-                constexpr int c = decltype(sub)::value;
-                float ys[Q], lb[Q], aq[Q], left[Q][K / 2];
-                each_back<Q>([&](auto step) {
-                    constexpr int i = decltype(step)::value, s = c * Q + i;
-                    const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
-                    const auto Cv = *(const Vec<float, K>*)&bc[buf][s][1][at.s0];
-                    const float di = from_lane<Q, i>(delta[c]), ui = from_lane<Q, i>(u[c]), wi = from_lane<Q, i>(w[c]);
-                    const bool fresh = MASK && (starts >> s & 1);
-                    float db[K], dc[K];
-                    ys[i] = lb[i] = aq[i] = 0.0f;
+            fence();
+            float left[Q == 4 ? 4 : 1][K / 2];
+            each_back<kKept>([&](auto step) {
+                constexpr int e = decltype(step)::value, s = s0 + e, o = OWN > 1 ? e / Q : 0, i = s % Q;
+                const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
+                const auto Cv = *(const Vec<float, K>*)&bc[buf][s][1][at.s0];
+                const float di = from_lane<Q, i>(delta[o]), ui = from_lane<Q, i>(u[o]), wi = from_lane<Q, i>(w[o]);
+                const bool fresh = STARTS && (starts >> s & 1);
+                float db[K], dc[K], sy = 0.0f, sl = 0.0f, sq = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        const float before = fresh ? 0.0f : s ? h[s ? s - 1 : 0][k] : h0[k];
-                        const float l = fmaf(wi, Cv.get(k), kc[k]);
-                        ys[i] = fmaf(h[s][k], Cv.get(k), ys[i]);
-                        lb[i] = fmaf(l, Bv.get(k), lb[i]);
-                        db[k] = l * ui;
-                        dc[k] = wi * h[s][k];
-                        kc[k] = fresh ? 0.0f : a[s][k] * l;
-                        const float q = kc[k] * before;
-                        aq[i] = fmaf(A2[k], q, aq[i]);
-                        dA[k] = fmaf(di, q, dA[k]);
-                    }
-                    // over the wave's rows of lanes: lanes below 32 go on with dB, the others with
-                    // dC; odd rows with the upper half of the states
+                for (int k = 0; k < K; ++k) {
+                    const float before = fresh ? 0.0f : e ? h[e ? e - 1 : 0][k] : hk[k];
+                    const float l = fmaf(wi, Cv.get(k), kc[k]);
+                    sy = fmaf(h[e][k], Cv.get(k), sy);
+                    sl = fmaf(l, Bv.get(k), sl);
+                    db[k] = l * ui;
+                    dc[k] = wi * h[e][k];
+                    kc[k] = fresh ? 0.0f : a[e][k] * l;
+                    const float q = kc[k] * before;
+                    sq = fmaf(A2[k], q, sq);
+                    dA[k] = fmaf(di, q, dA[k]);
+                }
+                ys.template add<i>(sy, j), lb.template add<i>(sl, j), aq.template add<i>(sq, j);
+                // over the wave's rows of lanes: lanes below 32 go on with dB, the others with dC; odd
+                // rows with the upper half of the states
 #pragma unroll
-                    for (int k = 0; k < K; ++k) swap32(db[k], dc[k]), db[k] += dc[k];
-#pragma unroll
-                    for (int k = 0; k < K / 2; ++k) swap16(db[k], db[k + K / 2]), left[i][k] = db[k] + db[k + K / 2];
-                });
+                for (int k = 0; k < K; ++k) swap32(db[k], dc[k]), db[k] += dc[k];
                 const int kind = at.lane >> 5, part = at.s0 + (at.lane >> 4 & 1) * (K / 2);
-                if constexpr (Q == 4) {
+                constexpr int r = Q == 4 ? i : 0;
+#pragma unroll
+                for (int k = 0; k < K / 2; ++k) swap16(db[k], db[k + K / 2]), left[r][k] = db[k] + db[k + K / 2];
+                if constexpr (Q == 16) {
+                    vstore<float, K / 2>(&sums[at.w][s][kind][part], left[0]);
+                } else if constexpr (i == 0) {
                     // over the row's four groups of lanes, each of which writes a step
                     float mine[K / 2];
 #pragma unroll
                     for (int k = 0; k < K / 2; ++k) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            left[i][k] = add_dpp<0x124>(left[i][k], left[i][k]);   // row_ror:4
-                            left[i][k] = add_dpp<0x128>(left[i][k], left[i][k]);   // row_ror:8
+                        for (int v = 0; v < 4; ++v) {
+                            left[v][k] = add_dpp<0x124>(left[v][k], left[v][k]);   // row_ror:4
+                            left[v][k] = add_dpp<0x128>(left[v][k], left[v][k]);   // row_ror:8
                         }
                         const float lo = at.lane & 4 ? left[1][k] : left[0][k], hi = at.lane & 4 ? left[3][k] : left[2][k];
                         mine[k] = at.lane & 8 ? hi : lo;
                     }
-                    vstore<float, K / 2>(&sums[at.w][c * 4 + (at.lane >> 2 & 3)][kind][part], mine);
-                } else {
-                    each<Q>([&](auto step) {
-                        constexpr int i = decltype(step)::value;
-                        vstore<float, K / 2>(&sums[at.w][i][kind][part], left[i]);
-                    });
+                    vstore<float, K / 2>(&sums[at.w][s + (at.lane >> 2 & 3)][kind][part], mine);
                 }
-                const int t = t0 + c * Q + j;
-                const float xs = (float)x.v[c], core = fmaf(D, xs, sums_by_lane<Q>(ys, j));
-                const float slb = sums_by_lane<Q>(lb, j), saq = sums_by_lane<Q>(aq, j);
-                const float ddt = fmaf(saq, kLn2, xs * slb) * slope[c];
-                if (at.on && t < tend) {
-                    dD = fmaf(w[c], xs, dD);
-                    dbias += ddt;
-                    dxp[t * p.dx.s0] = (E)fmaf(delta[c], slb, D * w[c]);
-                    ddp[t * p.ddt.s0] = (E)ddt;
-                    if (p.g.data) dgp[t * p.dg.s0] = (E)((float)dy.v[c] * core * gslope[c]);
+                fence();
+                if constexpr (i == 0) {
+                    constexpr int c = s / Q;
+                    const float core = fmaf(D, xs[o], ys.total(j)), slb = lb.total(j), ddt = fmaf(aq.total(j), kLn2, xs[o] * slb) * slope[o];
+                    if (full || (at.on && t0 + c * Q + j < tend)) {
+                        dD = fmaf(w[o], xs[o], dD);
+                        dbias += ddt;
+                        if (gated) *dgc.at(t0, c) = (E)(ga[o] * core);
+                        *dxc.at(t0, c) = (E)fmaf(delta[o], slb, D * w[o]);
+                        *ddc.at(t0, c) = (E)ddt;
+                    }
                 }
             });
-        };
-        starts ? walk(std::true_type()) : walk(std::false_type());
+        });
         barrier_lds();
         // the waves' sums added up, to the workgroup's place in memory
         for (int e = threadIdx.x; e < kStepsB * 2 * SP; e += 256) {
@@ -417,14 +571,14 @@ __global__ void __launch_bounds__(256) selective_bwd_kernel(Selective p) {
             if (t < tend) p.bcsums[(((size_t)at.tile * p.T + t) * p.B + b) * (2 * SP) + e % (2 * SP)] = (v[0] + v[pitch]) + (v[2 * pitch] + v[3 * pitch]);
         }
     }
-    for (int t = tend + j; t < p.T; t += Q)
-        if (at.on) {
-            dxp[t * p.dx.s0] = (E)0.0f;
-            ddp[t * p.ddt.s0] = (E)0.0f;
-            if (p.g.data) dgp[t * p.dg.s0] = (E)0.0f;
+    for (int t = max(ts, tend) / Q * Q; t < te; t += Q)
+        if (at.on && t + j >= tend && t + j < te) {
+            if (gated) *dgc.at(t, 0) = (E)0.0f;
+            *dxc.at(t, 0) = (E)0.0f;
+            *ddc.at(t, 0) = (E)0.0f;
         }
-    if (p.dh0) store_states<K>(p.dh0 + row, kc, at.s0, S, at.on);
-    float* rows = p.rowsums + (size_t)b * N * (S + 2);
+    if (p.dh0 && blockIdx.y == 0) store_states<K>(p.dh0 + row, kc, at.s0, S, at.on);
+    float* rows = p.rowsums + ((size_t)blockIdx.y * p.B + b) * N * (S + 2);
     store_states<K>(rows + (size_t)n * S, dA, at.s0, S, at.on);
     dD = lanes_total<Q>(dD);
     dbias = lanes_total<Q>(dbias);
@@ -462,6 +616,9 @@ __global__ void __launch_bounds__(256) selective_sums_kernel(Selective p, int SP
 }
 
 // one time step
+template <class E>
+__device__ __forceinline__ E* row_of(const delrec_rows& x, int b) { return (E*)x.data + b * x.s1; }
+
 template <class E, int Q, int K>
 __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     const Place<Q, K> at(p);
@@ -470,9 +627,9 @@ __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     float A[K], h[K], slope, y = 0.0f;
     load_states<K>(A, p.A + (size_t)n * S, at.s0, S, true);
     load_states<K>(h, p.h0 + row, at.s0, S, at.on);
-    const float x = (float)*(const E*)column<E>(p.x, b, n);
-    const float delta = softplus((float)*(const E*)column<E>(p.dt, b, n) + (p.dt_bias ? p.dt_bias[n] : 0.0f), &slope);
-    const E *Bv = (const E*)p.Bm.data + b * p.Bm.s1, *Cv = (const E*)p.C.data + b * p.C.s1;
+    const float x = (float)row_of<E>(p.x, b)[n];
+    const float delta = softplus((float)row_of<E>(p.dt, b)[n] + (p.dt_bias ? p.dt_bias[n] : 0.0f), &slope);
+    const E *Bv = row_of<E>(p.Bm, b), *Cv = row_of<E>(p.C, b);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const bool in = at.s0 + k < S;
@@ -484,57 +641,81 @@ __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     if (!at.on || at.j) return;
     if (p.D) y = fmaf(p.D[n], x, y);
     if (p.g.data) {
-        const float g = (float)*(const E*)column<E>(p.g, b, n);
+        const float g = (float)row_of<E>(p.g, b)[n];
         y *= g * sigmoid(g);
     }
-    *(E*)column<E>(p.y, b, n) = (E)y;
+    row_of<E>(p.y, b)[n] = (E)y;
 }
 
 namespace {
 
 struct Plan {
-    int Q, K, tiles;
+    int Q, K, tiles, range, ranges;
 };
-Plan selective_plan(int N, int S) {
+Plan selective_plan(int T, int B, int N, int S, bool fwd) {
     Plan q;
     q.Q = S <= 16 ? 4 : 16;
     q.K = S <= 8 || (S > 16 && S <= 32) ? 2 : 4;
     const int channels = 64 / q.Q * kWavesWg;
     q.tiles = (N + channels - 1) / channels;
+    const long long groups = (long long)B * q.tiles;
+    const int blocks = (T + kStepsB - 1) / kStepsB;
+    int want = (int)std::min<long long>(64, (fwd ? kGroupsFwd : kGroupsBwd) / groups);
+    want = std::max(1, std::min(want, blocks / 4));
+    const int per = (blocks + want - 1) / want;
+    q.range = per * kStepsB;
+    q.ranges = (blocks + per - 1) / per;
     return q;
 }
 
 enum { kFwd, kBwd, kStep };
 
-template <class E, int Q, int K>
-void run_selective(Selective p, int what, hipStream_t stream) {
+template <class E, int Q, int K, bool STARTS>
+void run_selective(Selective p, const Plan& q, int what, hipStream_t stream) {
     const long long groups = (long long)p.B * p.tiles;
-    for (long long first = 0; first < groups; first += kMostBlocks) {
-        p.first = first;
-        const dim3 grid((unsigned)std::min<long long>(groups - first, kMostBlocks)), block(64 * kWavesWg);
-        if (what == kFwd) hipLaunchKernelGGL((selective_fwd_kernel<E, Q, K>), grid, block, 0, stream, p);
-        else if (what == kBwd) hipLaunchKernelGGL((selective_bwd_kernel<E, Q, K>), grid, block, 0, stream, p);
-        else hipLaunchKernelGGL((selective_step_kernel<E, Q, K>), grid, block, 0, stream, p);
-    }
+    for (int pass = what != kStep && q.ranges > 1 ? 0 : 1; pass < 2; ++pass)
+        for (long long first = 0; first < groups; first += kMostBlocks) {
+            p.first = first;
+            const unsigned wgs = (unsigned)std::min<long long>(groups - first, kMostBlocks);
+            const dim3 grid(wgs, q.ranges), inner(wgs, q.ranges - 1), block(64 * kWavesWg);
+            if (what == kStep) hipLaunchKernelGGL((selective_step_kernel<E, Q, K>), dim3(wgs), block, 0, stream, p);
+            else if (pass == 0 && what == kFwd) hipLaunchKernelGGL((selective_range_kernel<E, Q, K, STARTS, false>), inner, block, 0, stream, p);
+            else if (pass == 0) hipLaunchKernelGGL((selective_range_kernel<E, Q, K, STARTS, true>), inner, block, 0, stream, p);
+            else if (what == kFwd) hipLaunchKernelGGL((selective_fwd_kernel<E, Q, K, STARTS>), grid, block, 0, stream, p);
+            else hipLaunchKernelGGL((selective_bwd_kernel<E, Q, K, STARTS>), grid, block, 0, stream, p);
+        }
     if (what == kBwd) {
         const long long a = ((long long)p.T * p.B * 2 * p.S + 255) / 256, c = ((long long)p.N * (p.S + 2) + 255) / 256;
         const unsigned wide = (unsigned)std::min<long long>(a, 4096), rest = (unsigned)std::min<long long>(c, 4096);
-        hipLaunchKernelGGL((selective_sums_kernel<E>), dim3(wide + rest), dim3(256), 0, stream, p, Q * K, wide, p.B);
+        hipLaunchKernelGGL((selective_sums_kernel<E>), dim3(wide + rest), dim3(256), 0, stream, p, Q * K, wide, q.ranges * p.B);
     }
 }
 
+template <class E, int Q, int K>
+void run_selective_s(const Selective& p, const Plan& q, int what, hipStream_t stream) {
+    p.starts ? run_selective<E, Q, K, true>(p, q, what, stream) : run_selective<E, Q, K, false>(p, q, what, stream);
+}
 template <class E>
 void run_selective_q(const Selective& p, const Plan& q, int what, hipStream_t stream) {
-    if (q.Q == 4) q.K == 2 ? run_selective<E, 4, 2>(p, what, stream) : run_selective<E, 4, 4>(p, what, stream);
-    else q.K == 2 ? run_selective<E, 16, 2>(p, what, stream) : run_selective<E, 16, 4>(p, what, stream);
+    if (q.Q == 4) q.K == 2 ? run_selective_s<E, 4, 2>(p, q, what, stream) : run_selective_s<E, 4, 4>(p, q, what, stream);
+    else q.K == 2 ? run_selective_s<E, 16, 2>(p, q, what, stream) : run_selective_s<E, 16, 4>(p, q, what, stream);
 }
 
+size_t map_floats(const Plan& q, int B, int N, int S) { return q.ranges > 1 ? (size_t)q.ranges * B * N * (S + 1) : 0; }
+
 void launch_selective(Selective p, int what, hipStream_t stream) {
-    const Plan q = selective_plan(p.N, p.S);
+    const Plan q = selective_plan(p.T, p.B, p.N, p.S, what != kBwd);
     p.tiles = q.tiles;
+    p.range = q.range;
+    float* ws = p.ws;
+    if (what != kStep && q.ranges > 1) {
+        p.maps = ws;
+        p.mapsums = ws + (size_t)q.ranges * p.B * p.N * p.S;
+        ws += map_floats(q, p.B, p.N, p.S);
+    }
     if (what == kBwd) {
-        p.bcsums = p.ws;
-        p.rowsums = p.ws + (size_t)q.tiles * p.T * p.B * 2 * q.Q * q.K;
+        p.bcsums = ws;
+        p.rowsums = ws + (size_t)q.tiles * p.T * p.B * 2 * q.Q * q.K;
     }
     if (p.bf16) run_selective_q<__bf16>(p, q, what, stream);
     else run_selective_q<float>(p, q, what, stream);
@@ -542,10 +723,10 @@ void launch_selective(Selective p, int what, hipStream_t stream) {
 
 }  // namespace
 
-size_t selective_fwd_ws(int, int, int, int) { return 0; }
+size_t selective_fwd_ws(int T, int B, int N, int S) { return map_floats(selective_plan(T, B, N, S, true), B, N, S); }
 size_t selective_bwd_ws(int T, int B, int N, int S) {
-    const Plan q = selective_plan(N, S);
-    return (size_t)q.tiles * T * B * 2 * q.Q * q.K + (size_t)B * N * (S + 2);
+    const Plan q = selective_plan(T, B, N, S, false);
+    return map_floats(q, B, N, S) + (size_t)q.tiles * T * B * 2 * q.Q * q.K + (size_t)q.ranges * B * N * (S + 2);
 }
 void launch_selective_fwd(const Selective& p, hipStream_t stream) { launch_selective(p, kFwd, stream); }
 void launch_selective_bwd(const Selective& p, hipStream_t stream) { launch_selective(p, kBwd, stream); }

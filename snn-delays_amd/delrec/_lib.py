@@ -31,7 +31,7 @@ WS_AXONAL_FWD, WS_AXONAL_BWD, WS_SYN_FWD, WS_SYN_BWD, WS_SPIKE_LINEAR = 1, 2, 3,
 WS_SPIKE_LINEAR_DW, WS_READOUT_CE = 6, 7
 WS_GATED_FWD, WS_GATED_BWD, WS_NORM_GATE_BWD, WS_ADD_NORM_BWD = 8, 9, 10, 11
 WS_CAUSAL_CONV_BWD, WS_SELECTIVE_FWD, WS_SELECTIVE_BWD = 12, 13, 14
-GATED_BLOCK, PACK8_GROUP, SELECTIVE_BLOCK = 64, 64, 16
+GATED_BLOCK, PACK8_GROUP, SELECTIVE_BLOCK = 64, 64, 8
 READOUT_SUM, READOUT_MEAN, READOUT_MAX = 0, 1, 2
 
 # Every symbol include/delrec.h declares (checked by the CPU test suite).
