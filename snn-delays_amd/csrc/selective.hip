@@ -32,7 +32,6 @@ constexpr int kStepsB = 16;                       // steps of a block
 constexpr int kKept = DELREC_SELECTIVE_BLOCK;     // steps from one kept state to the next
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWavesWg = 4;
-constexpr int kGroupsFwd = 1024, kGroupsBwd = 512;
 
 template <int... I, class F>
 __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I>()), ...); }
@@ -190,6 +189,9 @@ __device__ __forceinline__ int row_steps(const Selective& p, int b) {
     return v < 0 ? 0 : (v < p.T ? (int)v : p.T);
 }
 
+template <class E>
+__device__ __forceinline__ E* row_of(const delrec_rows& x, int b) { return (E*)x.data + b * x.s1; }
+
 // bit i: a sequence starts at step t0 + i
 __device__ __forceinline__ uint32_t start_bits(const Selective& p, int b, int t0, int tend, int lane) {
     if (!p.starts) return 0;
@@ -197,52 +199,72 @@ __device__ __forceinline__ uint32_t start_bits(const Selective& p, int b, int t0
     return (uint32_t)__ballot(lane < kStepsB && t < tend && p.starts[(size_t)min(t, p.T - 1) * p.B + b] != 0);
 }
 
-// B and C of a block of steps, from memory to LDS as fp32; zeros past the row's end and past S
+// B and C of a block of steps, from memory to LDS as fp32; zeros past the row's end and past S. A thread
+// takes the same column of B or C in every `every`-th step.
 template <class E, int SP>
 struct Stage {
-    static constexpr int count = kStepsB * 2 * SP, per = (count + 255) / 256;
+    static constexpr int count = kStepsB * 2 * SP, per = (count + 255) / 256, every = 256 / (2 * SP);
     E v[per];
-    __device__ __forceinline__ void load(const Selective& p, int b, int t0, int tend) {
-#pragma unroll
-        for (int r = 0; r < per; ++r) {
-            const int e = threadIdx.x + 256 * r, t = t0 + e / (2 * SP), s = e % SP;
-            const delrec_rows& m = e / SP % 2 ? p.C : p.Bm;
-            v[r] = (E)0.0f;
-            if (e < count && t < tend && s < p.S) v[r] = ((const E*)m.data)[t * m.s0 + b * m.s1 + s];
-        }
+    const E* at;                                            // the thread's first element of block t0
+    long long pitch;
+    int t, lds;
+    bool in;
+    __device__ __forceinline__ Stage(const Selective& p, int b, int t0) {
+        const int tid = threadIdx.x, s = tid % SP;
+        const delrec_rows& m = tid / SP % 2 ? p.C : p.Bm;
+        t = tid / (2 * SP);
+        lds = tid;
+        in = s < p.S && t < kStepsB;
+        pitch = m.s0;
+        at = (const E*)m.data + (t0 + t) * pitch + b * m.s1 + s;
     }
-    __device__ __forceinline__ void put(float* lds) const {
+    // block t0; then on to the next one, `move` steps away
+    __device__ __forceinline__ void load(int t0, int tend, int move) {
 #pragma unroll
         for (int r = 0; r < per; ++r) {
-            const int e = threadIdx.x + 256 * r;
-            if (e < count) lds[e] = (float)v[r];
+            v[r] = (E)0.0f;
+            if (in && t0 + t + r * every < tend) v[r] = at[r * every * pitch];
         }
+        at += move * pitch;
+    }
+    __device__ __forceinline__ void put(float* to) const {
+#pragma unroll
+        for (int r = 0; r < per; ++r)
+            if (256 * per <= count || lds < count) to[lds + 256 * r] = (float)v[r];
     }
 };
 
-// A lane's own steps of a block in one of the (T, B, N) tensors: the block's first step is a base for the
-// workgroup, moved in scalar registers, the lane's distance from it stays.
-template <class E, int Q>
+// A lane's place in one of the (T, B, N) tensors, moved from own step to own step: one addition an access
+// and none in scalar registers.
+template <class E, int Q, int DIR>
 struct Column {
-    const E* base;
-    long long pitch, lane;
-    __device__ __forceinline__ Column(const delrec_rows& x, int b, int n, int j)
-        : base((const E*)x.data + b * x.s1), pitch(x.s0), lane(j * x.s0 + n) {}
-    __device__ __forceinline__ E* at(int t0, int i) const { return (E*)(base + (t0 + i * Q) * pitch) + lane; }
+    E* at;
+    long long move;
+    // of own step t0 + i Q + j
+    __device__ __forceinline__ Column(const delrec_rows& x, int b, int n, int t)
+        : at((E*)x.data + t * x.s0 + b * x.s1 + n), move(DIR * Q * x.s0) {}
+    __device__ __forceinline__ E* next() {
+        E* r = at;
+        at += move;
+        return r;
+    }
 };
-// zeros past the row's end and in lanes without a channel
-template <class E, int Q>
+// COUNT own steps from FROM on, the last one first where DIR < 0; zeros past the row's end and in lanes
+// without a channel
+template <class E, int Q, int DIR>
 struct Own {
     E v[Shape<Q>::own];
     template <bool FULL, int FROM = 0, int COUNT = Shape<Q>::own>
-    __device__ __forceinline__ void load(const Column<E, Q>& x, int t0, int j, int tend, bool on) {
+    __device__ __forceinline__ void load(Column<E, Q, DIR>& x, int t0, int j, int tend, bool on) {
 #pragma unroll
-        for (int i = FROM; i < FROM + COUNT; ++i) {
+        for (int k = 0; k < COUNT; ++k) {
+            const int i = DIR > 0 ? FROM + k : FROM + COUNT - 1 - k;
+            const E* from = x.next();
             if (FULL) {
-                v[i] = *x.at(t0, i);
+                v[i] = *from;
             } else {
                 v[i] = (E)0.0f;
-                if (on && t0 + i * Q + j < tend) v[i] = *x.at(t0, i);
+                if (on && t0 + i * Q + j < tend) v[i] = *from;
             }
         }
     }
@@ -293,12 +315,12 @@ __global__ void __launch_bounds__(256) selective_fwd_kernel(Selective p) {
     for (int k = 0; k < K; ++k) A2[k] *= kLog2e;
     if (blockIdx.y) enter_range<K>(h, p, A2, row, chan, at.s0, at.on, 0, 1, blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
-    const Column<E, Q> xc(p.x, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : p.x, b, n, j), yc(p.y, b, n, j);
+    Column<E, Q, 1> xc(p.x, b, n, ts + j), dc(p.dt, b, n, ts + j), gc(gated ? p.g : p.x, b, n, ts + j), yc(p.y, b, n, ts + j);
 
-    Stage<E, SP> bcv;
-    Own<E, Q> xv, dv, gv;
+    Stage<E, SP> bcv(p, b, ts);
+    Own<E, Q, 1> xv, dv, gv;
     auto load = [&](int t0) {
-        bcv.load(p, b, t0, tend);
+        bcv.load(t0, tend, kStepsB);
         auto three = [&](auto full) {
             constexpr bool F = decltype(full)::value;
             dv.template load<F>(dc, t0, j, tend, at.on);
@@ -311,8 +333,8 @@ __global__ void __launch_bounds__(256) selective_fwd_kernel(Selective p) {
     int buf = 0;
     for (int t0 = ts; t0 < tend; t0 += kStepsB, buf ^= 1) {
         bcv.put(&bc[buf][0][0][0]);
-        const Own<E, Q> x = xv, d = dv, g = gv;
-        const uint32_t starts = start_bits(p, b, t0, tend, at.lane);
+        const Own<E, Q, 1> x = xv, d = dv, g = gv;
+        const uint32_t starts = STARTS ? start_bits(p, b, t0, tend, at.lane) : 0;
         barrier_lds();
         if (t0 + kStepsB < tend) load(t0 + kStepsB);
         auto keep = [&](int step) {
@@ -342,11 +364,12 @@ __global__ void __launch_bounds__(256) selective_fwd_kernel(Selective p) {
                 }
             });
             const float y = fmaf(D, xs, sums_by_lane<Q>(ys, j)) * Gate((float)g.v[c], gated).value;
-            if (full || valid) *yc.at(t0, c) = (E)y;
+            E* to = yc.next();
+            if (full || valid) *to = (E)y;
         });
     }
-    for (int t = max(ts, tend) / Q * Q; t < te; t += Q)
-        if (at.on && t + j >= tend && t + j < te) *yc.at(t, 0) = (E)0.0f;
+    for (int t = max(ts, tend) + j; t < te; t += Q)
+        if (at.on) row_of<E>(p.y, b)[t * p.y.s0 + n] = (E)0.0f;
     if (te == p.T) store_states<K>(p.h_last + row, h, at.s0, S, at.on);
 }
 
@@ -367,11 +390,15 @@ __global__ void __launch_bounds__(256) selective_range_kernel(Selective p) {
     for (int k = 0; k < K; ++k) A2[k] *= kLog2e, h[k] = 0.0f;
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f;
     const delrec_rows& xr = BWD ? p.dy : p.x;
-    const Column<E, Q> xc(xr, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : xr, b, n, j);
-    Stage<E, SP> bcv;
-    Own<E, Q> xv, dv, gv;
+    constexpr int DIR = BWD ? -1 : 1;
+    const int blocks = tend > ts ? (tend - ts + kStepsB - 1) / kStepsB : 0;
+    auto first = [&](int i) { return ts + (BWD ? blocks - 1 - i : i) * kStepsB; };
+    const int t1 = first(0) + j + (BWD ? (OWN - 1) * Q : 0);
+    Column<E, Q, DIR> xc(xr, b, n, t1), dc(p.dt, b, n, t1), gc(gated ? p.g : xr, b, n, t1);
+    Stage<E, SP> bcv(p, b, first(0));
+    Own<E, Q, DIR> xv, dv, gv;
     auto load = [&](int t0) {
-        bcv.load(p, b, t0, tend);
+        bcv.load(t0, tend, DIR * kStepsB);
         auto all = [&](auto full) {
             constexpr bool F = decltype(full)::value;
             dv.template load<F>(dc, t0, j, tend, at.on);
@@ -382,14 +409,12 @@ __global__ void __launch_bounds__(256) selective_range_kernel(Selective p) {
     };
     bool cut = false;
     int buf = 0;
-    const int blocks = tend > ts ? (tend - ts + kStepsB - 1) / kStepsB : 0;
-    auto first = [&](int i) { return ts + (BWD ? blocks - 1 - i : i) * kStepsB; };
     if (blocks) load(first(0));
     for (int i = 0; i < blocks; ++i, buf ^= 1) {
         const int t0 = first(i);
         bcv.put(&bc[buf][0][0][0]);
-        const Own<E, Q> x = xv, d = dv, g = gv;
-        const uint32_t starts = start_bits(p, b, t0, tend, at.lane);
+        const Own<E, Q, DIR> x = xv, d = dv, g = gv;
+        const uint32_t starts = STARTS ? start_bits(p, b, t0, tend, at.lane) : 0;
         cut |= starts != 0;
         barrier_lds();
         if (i + 1 < blocks) load(first(i + 1));
@@ -437,12 +462,12 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
     for (int k = 0; k < K; ++k) A2[k] *= kLog2e, dA[k] = 0.0f;
     enter_range<K>(kc, p, A2, row, chan, at.s0, at.on, gridDim.y - 1, -1, gridDim.y - 1 - blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
-    const Column<E, Q> xc(p.x, b, n, j), dc(p.dt, b, n, j), gc(gated ? p.g : p.x, b, n, j), yc(p.dy, b, n, j);
-    const Column<E, Q> dxc(p.dx, b, n, j), ddc(p.ddt, b, n, j), dgc(gated ? p.dg : p.dx, b, n, j);
-
-    Stage<E, SP> bcv;
-    Own<E, Q> xv, dv, gv, yv;
-    // the own steps of a block, from the one after the last half's on (Q 16: one, with the first half)
+    const int last = ts + (tend > ts ? (tend - ts - 1) / kStepsB * kStepsB : 0), t1 = last + (OWN - 1) * Q + j;
+    Column<E, Q, -1> xc(p.x, b, n, t1), dc(p.dt, b, n, t1), gc(gated ? p.g : p.x, b, n, t1), yc(p.dy, b, n, t1);
+    Column<E, Q, -1> dxc(p.dx, b, n, t1), ddc(p.ddt, b, n, t1), dgc(gated ? p.dg : p.dx, b, n, t1);
+    Stage<E, SP> bcv(p, b, last);
+    Own<E, Q, -1> xv, dv, gv, yv;
+    // a half's own steps of a block (Q 16: the one, with the upper half)
     auto load = [&](int t0, auto half) {
         constexpr int from = OWN > 1 ? decltype(half)::value * HALF : 0;
         auto four = [&](auto full) {
@@ -454,9 +479,8 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
         };
         whole && t0 + kStepsB <= tend ? four(std::true_type()) : four(std::false_type());
     };
-    const int last = ts + (tend > ts ? (tend - ts - 1) / kStepsB * kStepsB : 0);
     if (tend > ts) {
-        bcv.load(p, b, last, tend);
+        bcv.load(last, tend, -kStepsB);
         load(last, std::integral_constant<int, 1>());
         if (OWN > 1) load(last, std::integral_constant<int, 0>());
     }
@@ -466,7 +490,7 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
         const uint32_t starts = STARTS ? start_bits(p, b, t0, tend, at.lane) : 0;
         const bool full = whole && t0 + kStepsB <= tend;
         barrier_lds();
-        if (t0 > ts) bcv.load(p, b, t0 - kStepsB, tend);
+        if (t0 > ts) bcv.load(t0 - kStepsB, tend, -kStepsB);
         // the values of a lane's own steps of half a block (Q 4), or of its one (Q 16)
         float delta[HALF], slope[HALF], u[HALF], w[HALF], ga[HALF], xs[HALF];
         Sums<Q> ys, lb, aq;
@@ -552,12 +576,13 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
                 if constexpr (i == 0) {
                     constexpr int c = s / Q;
                     const float core = fmaf(D, xs[o], ys.total(j)), slb = lb.total(j), ddt = fmaf(aq.total(j), kLn2, xs[o] * slb) * slope[o];
+                    E *dgp = dgc.next(), *dxp = dxc.next(), *ddp = ddc.next();
                     if (full || (at.on && t0 + c * Q + j < tend)) {
                         dD = fmaf(w[o], xs[o], dD);
                         dbias += ddt;
-                        if (gated) *dgc.at(t0, c) = (E)(ga[o] * core);
-                        *dxc.at(t0, c) = (E)fmaf(delta[o], slb, D * w[o]);
-                        *ddc.at(t0, c) = (E)ddt;
+                        if (gated) *dgp = (E)(ga[o] * core);
+                        *dxp = (E)fmaf(delta[o], slb, D * w[o]);
+                        *ddp = (E)ddt;
                     }
                 }
             });
@@ -571,11 +596,11 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
             if (t < tend) p.bcsums[(((size_t)at.tile * p.T + t) * p.B + b) * (2 * SP) + e % (2 * SP)] = (v[0] + v[pitch]) + (v[2 * pitch] + v[3 * pitch]);
         }
     }
-    for (int t = max(ts, tend) / Q * Q; t < te; t += Q)
-        if (at.on && t + j >= tend && t + j < te) {
-            if (gated) *dgc.at(t, 0) = (E)0.0f;
-            *dxc.at(t, 0) = (E)0.0f;
-            *ddc.at(t, 0) = (E)0.0f;
+    for (int t = max(ts, tend) + j; t < te; t += Q)
+        if (at.on) {
+            if (gated) row_of<E>(p.dg, b)[t * p.dg.s0 + n] = (E)0.0f;
+            row_of<E>(p.dx, b)[t * p.dx.s0 + n] = (E)0.0f;
+            row_of<E>(p.ddt, b)[t * p.ddt.s0 + n] = (E)0.0f;
         }
     if (p.dh0 && blockIdx.y == 0) store_states<K>(p.dh0 + row, kc, at.s0, S, at.on);
     float* rows = p.rowsums + ((size_t)blockIdx.y * p.B + b) * N * (S + 2);
@@ -588,37 +613,71 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
     }
 }
 
-// what the workgroups left: dB and dC over the tiles of channels (workgroups [0, wide)), dA, dD and
-// the bias' over the rows
-template <class E>
-__global__ void __launch_bounds__(256) selective_sums_kernel(Selective p, int SP, unsigned wide, int rows) {
+// What the workgroups left, added up in a fixed order: dB and dC over the tiles of channels (workgroups
+// [0, wide), four columns a thread), and dA, dD and the bias' over the rows and ranges (64 columns a
+// workgroup, the rows over its waves).
+template <class E, int SP>
+__global__ void __launch_bounds__(1024) selective_sums_kernel(Selective p, unsigned wide, unsigned rows) {
     if (blockIdx.x < wide) {
-        const size_t steps = (size_t)p.T * p.B, all = steps * 2 * p.S;
-        for (size_t e = blockIdx.x * 256ULL + threadIdx.x; e < all; e += wide * 256ULL) {
-            const size_t r = e / (2 * p.S);
-            const int c = (int)(e - r * (2 * p.S)), kind = c >= p.S, s = c - kind * p.S;
-            const int t = (int)(r / p.B), b = (int)(r - (size_t)t * p.B);
-            float v = 0.0f;
-            if (t < row_steps(p, b))
-                for (int q = 0; q < p.tiles; ++q) v += p.bcsums[(q * steps + r) * (2 * SP) + kind * SP + s];
-            ((E*)(kind ? p.dC : p.dB))[r * p.S + s] = (E)v;
+        constexpr int PER = 2 * SP / 4;
+        const size_t steps = (size_t)p.T * p.B, all = steps * PER;
+        for (size_t e = blockIdx.x * 1024ULL + threadIdx.x; e < all; e += wide * 1024ULL) {
+            const size_t r = e / PER;
+            const int c = (int)(e % PER) * 4, kind = c / SP, s = c % SP;
+            bool on = true;
+            if (p.lengths) {
+                const unsigned t = (unsigned)r / (unsigned)p.B, b = (unsigned)r - t * (unsigned)p.B;
+                on = (int)t < row_steps(p, b);
+            }
+            float v[4] = {};
+            if (on) {
+                const float* at = p.bcsums + r * (2 * SP) + c;
+#pragma unroll 4
+                for (int q = 0; q < p.tiles; ++q, at += steps * (2 * SP)) {
+                    const auto x = vload<float, 4>(at);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] += x.get(i);
+                }
+            }
+            E* out = (E*)(kind ? p.dC : p.dB) + r * p.S + s;
+            if (s + 4 <= p.S) {
+                vstore<E, 4>(out, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (s + i < p.S) out[i] = (E)v[i];
+            }
         }
         return;
     }
-    const size_t all = (size_t)p.N * (p.S + 2);
-    for (size_t e = (blockIdx.x - wide) * 256ULL + threadIdx.x; e < all; e += (gridDim.x - wide) * 256ULL) {
-        float v = 0.0f;
-        for (int q = 0; q < rows; ++q) v += p.rowsums[q * all + e];
-        const size_t A = (size_t)p.N * p.S;
-        float* out = e < A ? p.dA : e < A + p.N ? p.dD : p.dbias;
-        if (out) out[e < A ? e : e < A + p.N ? e - A : e - A - p.N] = v;
+    __shared__ float red[16][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const size_t all = (size_t)p.N * (p.S + 2), A = (size_t)p.N * p.S;
+    for (size_t c0 = (blockIdx.x - wide) * 64ULL; c0 < all; c0 += (gridDim.x - wide) * 64ULL) {
+        const size_t c = c0 + lane;
+        const float* at = p.rowsums + min(c, all - 1);
+        float s4[4] = {};
+        // four rows' loads in flight at a time (past the end the last row again, left out)
+        for (unsigned r = w; r < rows; r += 64) {
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = at[(size_t)min(r + 16 * q, rows - 1) * all];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s4[q] += r + 16 * q < rows ? v[q] : 0.0f;
+        }
+        red[w][lane] = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+        __syncthreads();
+        if (w == 0 && c < all) {
+            float v = red[0][lane];
+            for (int q = 1; q < 16; ++q) v += red[q][lane];
+            float* out = c < A ? p.dA : c < A + p.N ? p.dD : p.dbias;
+            if (out) out[c < A ? c : c < A + p.N ? c - A : c - A - p.N] = v;
+        }
+        __syncthreads();
     }
 }
 
 // one time step
-template <class E>
-__device__ __forceinline__ E* row_of(const delrec_rows& x, int b) { return (E*)x.data + b * x.s1; }
-
 template <class E, int Q, int K>
 __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     const Place<Q, K> at(p);
@@ -652,7 +711,7 @@ namespace {
 struct Plan {
     int Q, K, tiles, range, ranges;
 };
-Plan selective_plan(int T, int B, int N, int S, bool fwd) {
+Plan selective_plan(int T, int B, int N, int S, bool fwd, bool mask) {
     Plan q;
     q.Q = S <= 16 ? 4 : 16;
     q.K = S <= 8 || (S > 16 && S <= 32) ? 2 : 4;
@@ -660,7 +719,7 @@ Plan selective_plan(int T, int B, int N, int S, bool fwd) {
     q.tiles = (N + channels - 1) / channels;
     const long long groups = (long long)B * q.tiles;
     const int blocks = (T + kStepsB - 1) / kStepsB;
-    int want = (int)std::min<long long>(64, (fwd ? kGroupsFwd : kGroupsBwd) / groups);
+    int want = groups >= (fwd && !mask ? 256 : 512) ? 1 : (int)std::min<long long>(64, (fwd && mask ? 4096 : 1024) / groups);
     want = std::max(1, std::min(want, blocks / 4));
     const int per = (blocks + want - 1) / want;
     q.range = per * kStepsB;
@@ -685,9 +744,9 @@ void run_selective(Selective p, const Plan& q, int what, hipStream_t stream) {
             else hipLaunchKernelGGL((selective_bwd_kernel<E, Q, K, STARTS>), grid, block, 0, stream, p);
         }
     if (what == kBwd) {
-        const long long a = ((long long)p.T * p.B * 2 * p.S + 255) / 256, c = ((long long)p.N * (p.S + 2) + 255) / 256;
-        const unsigned wide = (unsigned)std::min<long long>(a, 4096), rest = (unsigned)std::min<long long>(c, 4096);
-        hipLaunchKernelGGL((selective_sums_kernel<E>), dim3(wide + rest), dim3(256), 0, stream, p, Q * K, wide, q.ranges * p.B);
+        const long long a = ((long long)p.T * p.B * (Q * K / 2) + 1023) / 1024, c = ((long long)p.N * (p.S + 2) + 63) / 64;
+        const unsigned wide = (unsigned)std::min<long long>(a, 2048), rest = (unsigned)std::min<long long>(c, 8192);
+        hipLaunchKernelGGL((selective_sums_kernel<E, Q * K>), dim3(wide + rest), dim3(1024), 0, stream, p, wide, (unsigned)q.ranges * p.B);
     }
 }
 
@@ -704,7 +763,7 @@ void run_selective_q(const Selective& p, const Plan& q, int what, hipStream_t st
 size_t map_floats(const Plan& q, int B, int N, int S) { return q.ranges > 1 ? (size_t)q.ranges * B * N * (S + 1) : 0; }
 
 void launch_selective(Selective p, int what, hipStream_t stream) {
-    const Plan q = selective_plan(p.T, p.B, p.N, p.S, what != kBwd);
+    const Plan q = selective_plan(p.T, p.B, p.N, p.S, what != kBwd, p.starts || p.lengths);
     p.tiles = q.tiles;
     p.range = q.range;
     float* ws = p.ws;
@@ -723,10 +782,17 @@ void launch_selective(Selective p, int what, hipStream_t stream) {
 
 }  // namespace
 
-size_t selective_fwd_ws(int T, int B, int N, int S) { return map_floats(selective_plan(T, B, N, S, true), B, N, S); }
+// floats of workspace, with and without masks
+size_t selective_fwd_ws(int T, int B, int N, int S) {
+    return std::max(map_floats(selective_plan(T, B, N, S, true, false), B, N, S), map_floats(selective_plan(T, B, N, S, true, true), B, N, S));
+}
 size_t selective_bwd_ws(int T, int B, int N, int S) {
-    const Plan q = selective_plan(T, B, N, S, false);
-    return map_floats(q, B, N, S) + (size_t)q.tiles * T * B * 2 * q.Q * q.K + (size_t)q.ranges * B * N * (S + 2);
+    size_t n = 0;
+    for (const bool mask : {false, true}) {
+        const Plan q = selective_plan(T, B, N, S, false, mask);
+        n = std::max(n, map_floats(q, B, N, S) + (size_t)q.tiles * T * B * 2 * q.Q * q.K + (size_t)q.ranges * B * N * (S + 2));
+    }
+    return n;
 }
 void launch_selective_fwd(const Selective& p, hipStream_t stream) { launch_selective(p, kFwd, stream); }
 void launch_selective_bwd(const Selective& p, hipStream_t stream) { launch_selective(p, kBwd, stream); }
