@@ -4,9 +4,12 @@
 // a row's steps from its length on are padding. Backwards, with r_t = dy_t times the activation's
 // slope at p_t: dx_s = sum_i w_i r_{s+W-1-i}, dw_i = sum_t r_t x_{t-W+1+i}, dbias = sum r.
 //
-// Bound by memory. A lane takes V neighbouring channels and a run of steps, and keeps the window of
-// the last W inputs in registers: x is read once, but for the W - 1 steps before each run (from the
-// cache). The backward computes p again from x and carries W unfinished dx along.
+// Bound by memory. A lane takes V neighbouring channels and a run of steps, in blocks of U whose loads are
+// under way together, and keeps the last W - 1 inputs in registers: x is read once, but for the W - 1
+// steps before each run (from the cache). The backward computes p again from x and carries the last W - 1
+// values of r along; the W - 1 steps after a run that its last dx need are computed twice. The sums of
+// dw go over a lane's steps, then through LDS over the workgroup's runs of the same channels, then from
+// memory over the workgroups, each in a fixed order.
 #include <algorithm>
 
 #include "gated.h"
@@ -15,6 +18,9 @@
 namespace delrec {
 
 namespace {
+
+constexpr int kVec = 4;          // channels of a lane
+constexpr int kBwdBlock = 4;     // steps of a block, backwards (of the 32 that a run and its rest take)
 
 __device__ __forceinline__ int conv_steps(const CausalConv& p, int b) {
     if (!p.lengths) return p.T;
@@ -45,38 +51,27 @@ __device__ __forceinline__ void store_part(E* at, const float* v, int have) {
     }
 }
 
-// the lane's channels n .. n + have - 1 of row b, and its run's first step
+// the lane's channels n .. n + have - 1 of row b, and its run's steps t0 .. te - 1
 struct Run {
-    int b, n, have, t0, run;
+    int b, n, have, t0, te, slot;
     bool on;
+    long long tasks;                          // first run of the workgroup
     __device__ __forceinline__ Run(const CausalConv& p, int V) {
-        const long long id = (p.first + blockIdx.x) * 256LL + threadIdx.x;
-        const long long r = id / p.groups;
-        n = (int)(id - r * p.groups) * V;
-        run = (int)(r / p.B);
-        b = (int)(r - (long long)run * p.B);
+        const long long id = p.first + blockIdx.x;
+        const long long tb = id / p.lane_blocks;
+        const int lane = threadIdx.x & (p.lanes - 1);
+        slot = threadIdx.x / p.lanes;
+        tasks = tb * (256 / p.lanes);
+        const long long task = tasks + slot;
+        const int run = (int)(task / p.B);
+        n = ((int)(id - tb * p.lane_blocks) * p.lanes + lane) * V;
+        b = (int)(task - (long long)run * p.B);
         t0 = run * p.steps;
+        te = min(t0 + p.steps, p.T);
         have = min(p.N - n, V);
-        on = run < p.runs;
+        on = run < p.runs && have > 0;
     }
 };
-
-// input row of step t (before the first step: of the state)
-template <class E, int W, int V>
-__device__ __forceinline__ void input_row(float* v, const CausalConv& p, const Run& r, int t) {
-    if (t >= 0) {
-        load_part<E, V>(v, (const E*)p.x.data + t * p.x.s0 + r.b * p.x.s1 + r.n, r.have);
-    } else if (p.state) {
-        load_part<E, V>(v, (const E*)p.state + ((size_t)r.b * (W - 1) + t + W - 1) * p.N + r.n, r.have);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = 0.0f;
-    }
-}
-
-__device__ __forceinline__ bool starts_at(const CausalConv& p, int b, int t) {
-    return p.starts && t >= 0 && p.starts[(size_t)t * p.B + b] != 0;
-}
 
 template <int V, int W>
 __device__ __forceinline__ void load_weights(float (&w)[W][V], float* bias, const CausalConv& p, const Run& r) {
@@ -88,163 +83,246 @@ __device__ __forceinline__ void load_weights(float (&w)[W][V], float* bias, cons
     }
 }
 
-}  // namespace
+// the state's row of step t < 0
+template <class E, int W, int V>
+__device__ __forceinline__ void state_row(float* v, const CausalConv& p, const Run& r, int t) {
+    if (p.state) {
+        load_part<E, V>(v, (const E*)p.state + ((size_t)r.b * (W - 1) + t + W - 1) * p.N + r.n, r.have);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = 0.0f;
+    }
+}
 
+// Steps of a (T, B, N) tensor as a lane reads them, rows t .. t + C - 1 below `end` (the others 0)
+template <class E, int V, int C>
+__device__ __forceinline__ void load_rows(float (*v)[V], const E* at, long long pitch, int t, int end, int have) {
+    if (t + C <= end && have == V) {
+        Vec<E, V> x[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) x[c] = vload<E, V>(at + (t + c) * pitch);
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[c][j] = x[c].get(j);
+    } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c) load_part<E, V>(v[c], at + (t + c) * pitch, t + c < end ? have : 0);
+    }
+}
+
+// bit c: a sequence starts at step t + c, of those below `end`
+template <int C>
+__device__ __forceinline__ uint32_t start_bits(const CausalConv& p, int b, int t, int end) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+        if (t + c >= 0 && t + c < end && p.starts[(size_t)(t + c) * p.B + b] != 0) bits |= 1u << c;
+    return bits;
+}
+// whether step i of the bits' window and a step `ahead` of it are of one sequence: no start after i
+__device__ __forceinline__ constexpr uint32_t between(int i, int ahead) { return ((1u << ahead) - 1u) << (i + 1); }
+
+// the W - 1 steps before the run
 template <class E, int V, int W>
-__global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
-    const Run r(p, V);
-    if (!r.on) return;
-    const int len = conv_steps(p, r.b), te = min(r.t0 + p.steps, p.T);
-    float w[W][V], bias[V], x[W][V];
-    load_weights<V, W>(w, bias, p, r);
-    // x[i]: the row of step t - W + 1 + i, zero where a start cuts it off
+__device__ __forceinline__ void load_before(float (*x)[V], const CausalConv& p, const Run& r, const E* xp, int len) {
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
         const int t = r.t0 - (W - 1) + i;
-        if (starts_at(p, r.b, t) && t < len)
-#pragma unroll
-            for (int q = 0; q < i; ++q)
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[q][j] = 0.0f;
-        if (t < len) input_row<E, W, V>(x[i], p, r, t);
+        if (t < 0) state_row<E, W, V>(x[i], p, r, t);
+        else load_part<E, V>(x[i], xp + t * p.x.s0, t < len ? r.have : 0);
     }
+}
+
+}  // namespace
+
+template <class E, int V, int W, bool STARTS>
+__global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
+    constexpr int U = 8;
+    const Run r(p, V);
+    if (!r.on) return;
+    const int len = conv_steps(p, r.b), end = min(len, r.te);
+    const E* xp = (const E*)p.x.data + r.b * p.x.s1 + r.n;
     E* yp = (E*)p.y.data + r.b * p.y.s1 + r.n;
-    for (int t = r.t0; t < te; ++t) {
-        float y[V];
-        if (t < len) {
-            if (starts_at(p, r.b, t))
+    float w[W][V], bias[V], x[W - 1 + U][V];
+    load_weights<V, W>(w, bias, p, r);
+    load_before<E, V, W>(x, p, r, xp, len);
+    uint32_t starts = STARTS ? start_bits<W - 1>(p, r.b, r.t0 - (W - 1), len) : 0;
+    for (int t = r.t0; t < r.te; t += U) {
+        load_rows<E, V, U>(x + W - 1, xp, p.x.s0, t, end, r.have);
+        if (STARTS) starts |= start_bits<U>(p, r.b, t, end) << (W - 1);
 #pragma unroll
-                for (int i = 0; i < W - 1; ++i)
+        for (int u = 0; u < U; ++u) {
+            float y[V];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) x[i][j] = 0.0f;
-            input_row<E, W, V>(x[W - 1], p, r, t);
+            for (int j = 0; j < V; ++j) y[j] = bias[j];
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                y[j] = bias[j];
+            for (int i = 0; i < W; ++i) {
+                const bool cut = STARTS && i < W - 1 && starts & between(u + i, W - 1 - i);
 #pragma unroll
-                for (int i = 0; i < W; ++i) y[j] = fmaf(w[i][j], x[i][j], y[j]);
-                if (p.silu) y[j] *= gate_in(-y[j]);
+                for (int j = 0; j < V; ++j) y[j] = fmaf(w[i][j], cut ? 0.0f : x[u + i][j], y[j]);
             }
 #pragma unroll
-            for (int i = 0; i < W - 1; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[i][j] = x[i + 1][j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j) y[j] = 0.0f;
+            for (int j = 0; j < V; ++j) {
+                if (p.silu) y[j] *= gate_in(-y[j]);
+                if (t + u >= end) y[j] = 0.0f;
+            }
+            if (t + u < r.te) store_part<E, V>(yp + (t + u) * p.y.s0, y, r.have);
         }
-        store_part<E, V>(yp + t * p.y.s0, y, r.have);
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[i][j] = x[U + i][j];
+        starts >>= U;
     }
-    // the rows that the next call starts from: the window after the row's last step, by the lane
-    // whose run holds it (the first run's for a row without steps)
-    if (!p.state_out || (len > r.t0 ? len > te : !(r.t0 == 0))) return;
+    // The rows that the next call starts from, by the first run's lanes. All are read before the first is
+    // written: with one step they may lie where the state does.
+    if (!p.state_out || r.t0) return;
+    const uint32_t ends = STARTS ? start_bits<W - 1>(p, r.b, len - (W - 1), len) : 0;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        const int t = len - (W - 1) + i;
+        if (t < 0) state_row<E, W, V>(x[i], p, r, t);
+        else load_part<E, V>(x[i], xp + t * p.x.s0, r.have);
+        if (STARTS && i < W - 2 && ends & between(i, W - 2 - i))
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[i][j] = 0.0f;
+    }
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) store_part<E, V>((E*)p.state_out + ((size_t)r.b * (W - 1) + i) * p.N + r.n, x[i], r.have);
 }
 
-template <class E, int V, int W>
+template <class E, int V, int W, bool STARTS>
 __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
+    constexpr int U = kBwdBlock;
+    __shared__ float red[256][V * (W + 1) + 1];
     const Run r(p, V);
-    if (!r.on) return;
-    const int len = conv_steps(p, r.b), te = min(r.t0 + p.steps, p.T);
-    float w[W][V], bias[V], x[W][V], dx[W][V], dw[W][V], db[V];
-    load_weights<V, W>(w, bias, p, r);
+    const int len = r.on ? conv_steps(p, r.b) : 0;
+    float dw[W][V], db[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         db[j] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) x[i][j] = dx[i][j] = dw[i][j] = 0.0f;
+        for (int i = 0; i < W; ++i) dw[i][j] = 0.0f;
     }
-    // bit i: the row of step t - W + 1 + i is not cut off
-    uint32_t joined = 0;
+    if (r.on) {
+        const E* xp = (const E*)p.x.data + r.b * p.x.s1 + r.n;
+        const E* dyp = (const E*)p.dy.data + r.b * p.dy.s1 + r.n;
+        E* dxp = (E*)p.dx.data + r.b * p.dx.s1 + r.n;
+        float w[W][V], bias[V], x[W - 1 + U][V], d[W - 1 + U][V];
+        load_weights<V, W>(w, bias, p, r);
+        load_before<E, V, W>(x, p, r, xp, len);
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) {
-        const int t = r.t0 - (W - 1) + i;
-        if (t < len) {
-            if (starts_at(p, r.b, t)) {
-                joined = 0;
+        for (int i = 0; i < W - 1; ++i)
 #pragma unroll
-                for (int q = 0; q < i; ++q)
+            for (int j = 0; j < V; ++j) d[i][j] = 0.0f;
+        uint32_t starts = STARTS ? start_bits<W - 1>(p, r.b, r.t0 - (W - 1), len) : 0;
+        const int end = min(len, r.te + W - 1);
+        // the run's own steps, and W - 1 more that finish their gradients; row i of the windows is step
+        // t - (W - 1) + i
+        for (int t = r.t0; t < r.te + W - 1; t += U) {
+            load_rows<E, V, U>(x + W - 1, xp, p.x.s0, t, end, r.have);
+            load_rows<E, V, U>(d + W - 1, dyp, p.dy.s0, t, end, r.have);
+            if (STARTS) starts |= start_bits<U>(p, r.b, t, end) << (W - 1);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) x[q][j] = 0.0f;
-            }
-            input_row<E, W, V>(x[i], p, r, t);
-            joined |= 1u << i;
-        }
-    }
-    const E* dyp = (const E*)p.dy.data + r.b * p.dy.s1 + r.n;
-    E* dxp = (E*)p.dx.data + r.b * p.dx.s1 + r.n;
-    // the run's own steps, and W - 1 more that finish their gradients
-    for (int t = r.t0; t < te + W - 1; ++t) {
-        if (t < len) {
-            if (starts_at(p, r.b, t)) {
-                joined = 0;
+            for (int u = 0; u < U; ++u) {
+                float pre[V], own[V];
 #pragma unroll
-                for (int i = 0; i < W - 1; ++i)
-#pragma unroll
-                    for (int j = 0; j < V; ++j) x[i][j] = 0.0f;
-            }
-            joined |= 1u << (W - 1);
-            float dy[V];
-            input_row<E, W, V>(x[W - 1], p, r, t);
-            load_part<E, V>(dy, dyp + t * p.dy.s0, r.have);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float pre = bias[j], d = dy[j];
-#pragma unroll
-                for (int i = 0; i < W; ++i) pre = fmaf(w[i][j], x[i][j], pre);
-                if (p.silu) {
-                    const float s = gate_in(-pre);
-                    d *= fmaf(pre * s, 1.0f - s, s);
-                }
-                const float own = t < te ? d : 0.0f;
-                db[j] += own;
+                for (int j = 0; j < V; ++j) pre[j] = bias[j];
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
-                    dw[i][j] = fmaf(own, x[i][j], dw[i][j]);
-                    dx[i][j] = fmaf(joined >> i & 1 ? w[i][j] : 0.0f, d, dx[i][j]);
+                    const bool cut = STARTS && i < W - 1 && starts & between(u + i, W - 1 - i);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) pre[j] = fmaf(w[i][j], cut ? 0.0f : x[u + i][j], pre[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float g = d[W - 1 + u][j];
+                    if (p.silu) {
+                        const float s = gate_in(-pre[j]);
+                        g *= fmaf(pre[j] * s, 1.0f - s, s);
+                    }
+                    // (nothing comes of a padded step, whatever the weights)
+                    g = t + u < end ? g : 0.0f;
+                    d[W - 1 + u][j] = g;
+                    own[j] = t + u < r.te ? g : 0.0f;
+                    db[j] += own[j];
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const bool cut = STARTS && i < W - 1 && starts & between(u + i, W - 1 - i);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) dw[i][j] = fmaf(own[j], cut ? 0.0f : x[u + i][j], dw[i][j]);
                 }
             }
-        }
-        // step s is finished
-        const int s = t - (W - 1), k = s - (len - (W - 1));
-        if (s >= r.t0 || r.t0 == 0) {
-            if (p.dstate_out && k >= 0 && s < len && joined & 1) {
-                float d[V];
-                load_part<E, V>(d, (const E*)p.dstate_out + ((size_t)r.b * (W - 1) + k) * p.N + r.n, r.have);
+            // steps t - (W - 1) .. t + U - W are finished
 #pragma unroll
-                for (int j = 0; j < V; ++j) dx[0][j] += d[j];
+            for (int q = 0; q < U; ++q) {
+                const int s = t - (W - 1) + q, k = s - (len - (W - 1));
+                if (s < r.te && (s >= r.t0 || r.t0 == 0)) {
+                    float g[V];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) g[j] = w[W - 1][j] * d[q][j];
+#pragma unroll
+                    for (int m = 1; m < W; ++m) {
+                        const bool cut = STARTS && starts & between(q, m);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[j] = fmaf(w[W - 1 - m][j], cut ? 0.0f : d[q + m][j], g[j]);
+                    }
+                    if (p.dstate_out && k >= 0 && s < len && !(STARTS && starts & between(q, W - 1))) {
+                        float more[V];
+                        load_part<E, V>(more, (const E*)p.dstate_out + ((size_t)r.b * (W - 1) + k) * p.N + r.n, r.have);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) g[j] += more[j];
+                    }
+                    if (s >= 0) store_part<E, V>(dxp + s * p.dx.s0, g, r.have);
+                    else if (p.dstate) store_part<E, V>((E*)p.dstate + ((size_t)r.b * (W - 1) + s + W - 1) * p.N + r.n, g, r.have);
+                }
             }
-            if (s >= 0) store_part<E, V>(dxp + s * p.dx.s0, dx[0], r.have);
-            else if (p.dstate) store_part<E, V>((E*)p.dstate + ((size_t)r.b * (W - 1) + s + W - 1) * p.N + r.n, dx[0], r.have);
-        }
-        joined >>= 1;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+            for (int i = 0; i < W - 1; ++i)
 #pragma unroll
-            for (int i = 0; i < W - 1; ++i) x[i][j] = x[i + 1][j], dx[i][j] = dx[i + 1][j];
-            dx[W - 1][j] = x[W - 1][j] = 0.0f;
+                for (int j = 0; j < V; ++j) x[i][j] = x[U + i][j], d[i][j] = d[U + i][j];
+            starts >>= U;
         }
     }
-    float* part = p.part + ((size_t)r.run * p.B + r.b) * p.N * (W + 1);
+    // over the workgroup's runs: of channel c the values c (W + 1) .. are those of its dw, then its db
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-        if (j < r.have) {
+    for (int j = 0; j < V; ++j) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) part[(size_t)(r.n + j) * W + i] = dw[i][j];
-            part[(size_t)p.N * W + r.n + j] = db[j];
-        }
+        for (int i = 0; i < W; ++i) red[threadIdx.x][j * (W + 1) + i] = dw[i][j];
+        red[threadIdx.x][j * (W + 1) + W] = db[j];
+    }
+    __syncthreads();
+    const int values = p.lanes * V * (W + 1), runs = 256 / p.lanes;
+    const long long block = p.first + blockIdx.x, tb = block / p.lane_blocks;
+    const int n0 = (int)(block - tb * p.lane_blocks) * p.lanes * V;
+    float* part = p.part + (size_t)tb * p.N * (W + 1);
+    for (int v = threadIdx.x; v < values; v += 256) {
+        const int lane = v / (V * (W + 1)), e = v % (V * (W + 1)), n = n0 + lane * V + e / (W + 1), i = e % (W + 1);
+        float s = 0.0f;
+        for (int q = 0; q < runs; ++q) s += red[q * p.lanes + lane][e];
+        if (n < p.N) part[i < W ? (size_t)n * W + i : (size_t)p.N * W + n] = s;
+    }
 }
 
-// dw and dbias from the runs' sums: columns by 64, the runs over 16 waves
-__global__ void __launch_bounds__(1024) conv_sums_kernel(const float* part, long long rows, long long cols, long long first, float* dw,
+// dw and dbias from the workgroups' sums: columns by 64, the workgroups over 16 waves
+__global__ void __launch_bounds__(1024) conv_sums_kernel(const float* part, unsigned rows, long long cols, long long first, float* dw,
                                                          long long nw, float* db) {
     __shared__ float red[16][64];
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     const long long c = (first + blockIdx.x) * 64 + lane;
-    float s = 0.0f;
-    if (c < cols)
-        for (long long r = wv; r < rows; r += 16) s += part[r * cols + c];
+    const float* at = part + min(c, cols - 1);
+    float s4[4] = {};
+    // four rows' loads in flight at a time (past the end the last row again, left out)
+    for (unsigned r = wv; r < rows; r += 64) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = at[(size_t)min(r + 16 * q, rows - 1) * cols];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s4[q] += r + 16 * q < rows ? v[q] : 0.0f;
+    }
+    float s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
     red[wv][lane] = s;
     __syncthreads();
     if (wv || c >= cols) return;
@@ -255,52 +333,67 @@ __global__ void __launch_bounds__(1024) conv_sums_kernel(const float* part, long
 
 namespace {
 
-template <class E>
-constexpr int kVec = 4;
-
-int conv_run_steps(int T, int B, int N) {
-    (void)B; (void)N;
-    return std::min(T, 32);
+struct Plan {
+    int lanes, lane_blocks, steps, runs;
+    long long task_blocks;
+};
+// 32 lanes of neighbouring channels, fewer where a row has fewer. Runs of 32 steps, backwards with the
+// W - 1 steps past their end, in blocks of U without a rest.
+Plan conv_plan(int T, int B, int N, int W, int V, bool fwd) {
+    Plan q;
+    const int groups = (N + V - 1) / V;
+    q.lanes = 1;
+    while (q.lanes < 32 && q.lanes < groups) q.lanes *= 2;
+    q.lane_blocks = (groups + q.lanes - 1) / q.lanes;
+    q.steps = std::min(T, fwd ? 32 : 32 - (W - 1));
+    q.runs = (T + q.steps - 1) / q.steps;
+    const int per = 256 / q.lanes;
+    q.task_blocks = ((long long)q.runs * B + per - 1) / per;
+    return q;
 }
 
-template <class E, int W>
+template <class E, int W, bool STARTS>
 void run_conv(CausalConv p, bool fwd, hipStream_t stream) {
-    constexpr int V = kVec<E>;
-    p.groups = (p.N + V - 1) / V;
-    p.steps = conv_run_steps(p.T, p.B, p.N);
-    p.runs = (p.T + p.steps - 1) / p.steps;
-    const long long blocks = ((long long)p.runs * p.B * p.groups + 255) / 256;
+    constexpr int V = kVec;
+    const Plan q = conv_plan(p.T, p.B, p.N, W, V, fwd);
+    p.lanes = q.lanes;
+    p.lane_blocks = q.lane_blocks;
+    p.steps = q.steps;
+    p.runs = q.runs;
+    const long long blocks = q.task_blocks * q.lane_blocks;
     for (p.first = 0; p.first < blocks; p.first += kMostBlocks) {
         const dim3 grid((unsigned)std::min<long long>(blocks - p.first, kMostBlocks));
-        if (fwd) hipLaunchKernelGGL((conv_fwd_kernel<E, V, W>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((conv_bwd_kernel<E, V, W>), grid, dim3(256), 0, stream, p);
+        if (fwd) hipLaunchKernelGGL((conv_fwd_kernel<E, V, W, STARTS>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((conv_bwd_kernel<E, V, W, STARTS>), grid, dim3(256), 0, stream, p);
     }
     if (fwd) return;
     const long long cols = (long long)p.N * (W + 1), cblocks = (cols + 63) / 64;
     for (long long first = 0; first < cblocks; first += kMostBlocks)
         hipLaunchKernelGGL(conv_sums_kernel, dim3((unsigned)std::min<long long>(cblocks - first, kMostBlocks)), dim3(1024), 0, stream, p.part,
-                           (long long)p.runs * p.B, cols, first, p.dw, (long long)p.N * W, p.db);
+                           (unsigned)q.task_blocks, cols, first, p.dw, (long long)p.N * W, p.db);
+}
+
+template <class E, int W>
+void run_conv_s(const CausalConv& p, bool fwd, hipStream_t stream) {
+    p.starts ? run_conv<E, W, true>(p, fwd, stream) : run_conv<E, W, false>(p, fwd, stream);
 }
 
 template <class E>
 void run_conv_w(const CausalConv& p, bool fwd, hipStream_t stream) {
     switch (p.W) {
-        case 2: return run_conv<E, 2>(p, fwd, stream);
-        case 3: return run_conv<E, 3>(p, fwd, stream);
-        case 4: return run_conv<E, 4>(p, fwd, stream);
-        case 5: return run_conv<E, 5>(p, fwd, stream);
-        case 6: return run_conv<E, 6>(p, fwd, stream);
-        case 7: return run_conv<E, 7>(p, fwd, stream);
-        default: return run_conv<E, 8>(p, fwd, stream);
+        case 2: return run_conv_s<E, 2>(p, fwd, stream);
+        case 3: return run_conv_s<E, 3>(p, fwd, stream);
+        case 4: return run_conv_s<E, 4>(p, fwd, stream);
+        case 5: return run_conv_s<E, 5>(p, fwd, stream);
+        case 6: return run_conv_s<E, 6>(p, fwd, stream);
+        case 7: return run_conv_s<E, 7>(p, fwd, stream);
+        default: return run_conv_s<E, 8>(p, fwd, stream);
     }
 }
 
 }  // namespace
 
-size_t conv_bwd_ws(int T, int B, int N, int W) {
-    const int steps = conv_run_steps(T, B, N);
-    return (size_t)((T + steps - 1) / steps) * B * N * (W + 1);
-}
+size_t conv_bwd_ws(int T, int B, int N, int W) { return (size_t)conv_plan(T, B, N, W, kVec, false).task_blocks * N * (W + 1); }
 
 void launch_conv(const CausalConv& p, bool fwd, hipStream_t stream) {
     if (p.bf16) run_conv_w<__bf16>(p, fwd, stream);

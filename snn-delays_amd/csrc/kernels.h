@@ -703,7 +703,8 @@ struct CausalConv {
     float* dw;
     float* db;
     float* part;                 // workspace of the backward, conv_bwd_ws floats
-    int groups, steps, runs;     // set by the launcher: lanes a row, steps of a run, runs,
+    int lanes, lane_blocks;      // set by the launcher: lanes of a workgroup's channels, workgroups a row,
+    int steps, runs;             // steps of a run, runs,
     long long first;             // the launch's first workgroup
 };
 size_t conv_bwd_ws(int T, int B, int N, int W);   // floats
