@@ -20,7 +20,7 @@ namespace delrec {
 namespace {
 
 constexpr int kVec = 4;          // channels of a lane
-constexpr int kBwdBlock = 4;     // steps of a block, backwards (of the 32 that a run and its rest take)
+constexpr int kBlock = 4;        // steps of a block
 
 __device__ __forceinline__ int conv_steps(const CausalConv& p, int b) {
     if (!p.lengths) return p.T;
@@ -75,12 +75,22 @@ struct Run {
 
 template <int V, int W>
 __device__ __forceinline__ void load_weights(float (&w)[W][V], float* bias, const CausalConv& p, const Run& r) {
+    if (r.have == V) {
+        // V channels' weights lie together
+        const float* at = p.w + (size_t)r.n * W;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        bias[j] = p.bias && j < r.have ? p.bias[r.n + j] : 0.0f;
+        for (int q = 0; q < W; ++q) {
+            const auto t = vload<float, V>(at + q * V);
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i][j] = j < r.have ? p.w[(size_t)(r.n + j) * W + i] : 0.0f;
+            for (int e = 0; e < V; ++e) w[(q * V + e) % W][(q * V + e) / W] = t.get(e);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < W; ++i) w[i][j] = j < r.have ? p.w[(size_t)(r.n + j) * W + i] : 0.0f;
     }
+    load_part<float, V>(bias, p.bias + r.n, p.bias ? r.have : 0);
 }
 
 // the state's row of step t < 0
@@ -94,21 +104,40 @@ __device__ __forceinline__ void state_row(float* v, const CausalConv& p, const R
     }
 }
 
-// Steps of a (T, B, N) tensor as a lane reads them, rows t .. t + C - 1 below `end` (the others 0)
+// Steps of a (T, B, N) tensor as a lane reads them: rows t .. t + C - 1 below `end` (the others 0), fetched
+// a block ahead of their use
 template <class E, int V, int C>
-__device__ __forceinline__ void load_rows(float (*v)[V], const E* at, long long pitch, int t, int end, int have) {
-    if (t + C <= end && have == V) {
-        Vec<E, V> x[C];
+struct Rows {
+    Vec<E, V> v[C];
+    __device__ __forceinline__ void fetch(const E* at, long long pitch, int t, int end, int have) {
+        if (t >= end) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) x[c] = vload<E, V>(at + (t + c) * pitch);
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[c].v[j] = (E)0.0f;
+        } else if (t + C <= end && have == V) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) v[c] = vload<E, V>(at + (t + c) * pitch);
+        } else {
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[c].v[j] = t + c < end && j < have ? at[(t + c) * pitch + j] : (E)0.0f;
+        }
+    }
+    __device__ __forceinline__ void get(float (*x)[V]) const {
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[c][j] = x[c].get(j);
-    } else {
-#pragma unroll
-        for (int c = 0; c < C; ++c) load_part<E, V>(v[c], at + (t + c) * pitch, t + c < end ? have : 0);
+            for (int j = 0; j < V; ++j) x[c][j] = v[c].get(j);
     }
+};
+
+// rows t .. te - 1 of an output are padding
+template <class E, int V>
+__device__ __forceinline__ void clear_rows(E* at, long long pitch, int t, int te, int have) {
+    const float none[V] = {};
+    for (; t < te; ++t) store_part<E, V>(at + t * pitch, none, have);
 }
 
 // bit c: a sequence starts at step t + c, of those below `end`
@@ -138,7 +167,7 @@ __device__ __forceinline__ void load_before(float (*x)[V], const CausalConv& p, 
 
 template <class E, int V, int W, bool STARTS>
 __global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
-    constexpr int U = 8;
+    constexpr int U = kBlock;
     const Run r(p, V);
     if (!r.on) return;
     const int len = conv_steps(p, r.b), end = min(len, r.te);
@@ -148,8 +177,12 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
     load_weights<V, W>(w, bias, p, r);
     load_before<E, V, W>(x, p, r, xp, len);
     uint32_t starts = STARTS ? start_bits<W - 1>(p, r.b, r.t0 - (W - 1), len) : 0;
-    for (int t = r.t0; t < r.te; t += U) {
-        load_rows<E, V, U>(x + W - 1, xp, p.x.s0, t, end, r.have);
+    Rows<E, V, U> xn;
+    xn.fetch(xp, p.x.s0, r.t0, end, r.have);
+    int t = r.t0;
+    for (; t < end; t += U) {
+        xn.get(x + W - 1);
+        xn.fetch(xp, p.x.s0, t + U, end, r.have);
         if (STARTS) starts |= start_bits<U>(p, r.b, t, end) << (W - 1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -175,6 +208,7 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
             for (int j = 0; j < V; ++j) x[i][j] = x[U + i][j];
         starts >>= U;
     }
+    clear_rows<E, V>(yp, p.y.s0, t, r.te, r.have);
     // The rows that the next call starts from, by the first run's lanes. All are read before the first is
     // written: with one step they may lie where the state does.
     if (!p.state_out || r.t0) return;
@@ -192,9 +226,12 @@ __global__ void __launch_bounds__(256) conv_fwd_kernel(CausalConv p) {
     for (int i = 0; i < W - 1; ++i) store_part<E, V>((E*)p.state_out + ((size_t)r.b * (W - 1) + i) * p.N + r.n, x[i], r.have);
 }
 
+// (with the tests for starts there are no registers left to fetch a block ahead: 64 us instead of 44 for
+// T1000 B50 N333 W3 fp32)
 template <class E, int V, int W, bool STARTS>
 __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
-    constexpr int U = kBwdBlock;
+    constexpr int U = kBlock;
+    constexpr bool AHEAD = !STARTS;
     __shared__ float red[256][V * (W + 1) + 1];
     const Run r(p, V);
     const int len = r.on ? conv_steps(p, r.b) : 0;
@@ -220,9 +257,20 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
         const int end = min(len, r.te + W - 1);
         // the run's own steps, and W - 1 more that finish their gradients; row i of the windows is step
         // t - (W - 1) + i
-        for (int t = r.t0; t < r.te + W - 1; t += U) {
-            load_rows<E, V, U>(x + W - 1, xp, p.x.s0, t, end, r.have);
-            load_rows<E, V, U>(d + W - 1, dyp, p.dy.s0, t, end, r.have);
+        Rows<E, V, U> xn, dn;
+        auto fetch = [&](int t) {
+            xn.fetch(xp, p.x.s0, t, end, r.have);
+            dn.fetch(dyp, p.dy.s0, t, end, r.have);
+        };
+        if (AHEAD) fetch(r.t0);
+        // (past the last step that is no padding, W - 1 more finish what it began)
+        const int stop = r.te + W - 1, live = min(stop, max(end, r.t0) + W - 1);
+        int t = r.t0;
+        for (; t < live; t += U) {
+            if (!AHEAD) fetch(t);
+            xn.get(x + W - 1);
+            dn.get(d + W - 1);
+            if (AHEAD) fetch(t + U);
             if (STARTS) starts |= start_bits<U>(p, r.b, t, end) << (W - 1);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
@@ -285,6 +333,7 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
                 for (int j = 0; j < V; ++j) x[i][j] = x[U + i][j], d[i][j] = d[U + i][j];
             starts >>= U;
         }
+        clear_rows<E, V>(dxp, p.dx.s0, max(t - (W - 1), 0), r.te, r.have);
     }
     // over the workgroup's runs: of channel c the values c (W + 1) .. are those of its dw, then its db
 #pragma unroll
@@ -304,6 +353,29 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
         for (int q = 0; q < runs; ++q) s += red[q * p.lanes + lane][e];
         if (n < p.N) part[i < W ? (size_t)n * W + i : (size_t)p.N * W + n] = s;
     }
+}
+
+// one time step without masks; the state's rows are read before the first is written
+template <class E, int V, int W>
+__global__ void __launch_bounds__(256) conv_step_kernel(CausalConv p) {
+    const Run r(p, V);
+    if (!r.on) return;
+    float w[W][V], bias[V], x[W][V], y[V];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) state_row<E, W, V>(x[i], p, r, i - (W - 1));
+    load_part<E, V>(x[W - 1], (const E*)p.x.data + r.b * p.x.s1 + r.n, r.have);
+    load_weights<V, W>(w, bias, p, r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        y[j] = bias[j];
+#pragma unroll
+        for (int i = 0; i < W; ++i) y[j] = fmaf(w[i][j], x[i][j], y[j]);
+        if (p.silu) y[j] *= gate_in(-y[j]);
+    }
+    store_part<E, V>((E*)p.y.data + r.b * p.y.s1 + r.n, y, r.have);
+    if (!p.state_out) return;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) store_part<E, V>((E*)p.state_out + ((size_t)r.b * (W - 1) + i) * p.N + r.n, x[i + 1], r.have);
 }
 
 // dw and dbias from the workgroups' sums: columns by 64, the workgroups over 16 waves
@@ -339,9 +411,9 @@ struct Plan {
 };
 // 32 lanes of neighbouring channels, fewer where a row has fewer. Runs of 32 steps, backwards with the
 // W - 1 steps past their end, in blocks of U without a rest.
-Plan conv_plan(int T, int B, int N, int W, int V, bool fwd) {
+Plan conv_plan(int T, int B, int N, int W, bool fwd) {
     Plan q;
-    const int groups = (N + V - 1) / V;
+    const int groups = (N + kVec - 1) / kVec;
     q.lanes = 1;
     while (q.lanes < 32 && q.lanes < groups) q.lanes *= 2;
     q.lane_blocks = (groups + q.lanes - 1) / q.lanes;
@@ -354,8 +426,7 @@ Plan conv_plan(int T, int B, int N, int W, int V, bool fwd) {
 
 template <class E, int W, bool STARTS>
 void run_conv(CausalConv p, bool fwd, hipStream_t stream) {
-    constexpr int V = kVec;
-    const Plan q = conv_plan(p.T, p.B, p.N, W, V, fwd);
+    const Plan q = conv_plan(p.T, p.B, p.N, W, fwd);
     p.lanes = q.lanes;
     p.lane_blocks = q.lane_blocks;
     p.steps = q.steps;
@@ -363,8 +434,9 @@ void run_conv(CausalConv p, bool fwd, hipStream_t stream) {
     const long long blocks = q.task_blocks * q.lane_blocks;
     for (p.first = 0; p.first < blocks; p.first += kMostBlocks) {
         const dim3 grid((unsigned)std::min<long long>(blocks - p.first, kMostBlocks));
-        if (fwd) hipLaunchKernelGGL((conv_fwd_kernel<E, V, W, STARTS>), grid, dim3(256), 0, stream, p);
-        else hipLaunchKernelGGL((conv_bwd_kernel<E, V, W, STARTS>), grid, dim3(256), 0, stream, p);
+        if (fwd && p.T == 1 && !p.starts && !p.lengths) hipLaunchKernelGGL((conv_step_kernel<E, kVec, W>), grid, dim3(256), 0, stream, p);
+        else if (fwd) hipLaunchKernelGGL((conv_fwd_kernel<E, kVec, W, STARTS>), grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL((conv_bwd_kernel<E, kVec, W, STARTS>), grid, dim3(256), 0, stream, p);
     }
     if (fwd) return;
     const long long cols = (long long)p.N * (W + 1), cblocks = (cols + 63) / 64;
@@ -393,7 +465,7 @@ void run_conv_w(const CausalConv& p, bool fwd, hipStream_t stream) {
 
 }  // namespace
 
-size_t conv_bwd_ws(int T, int B, int N, int W) { return (size_t)conv_plan(T, B, N, W, kVec, false).task_blocks * N * (W + 1); }
+size_t conv_bwd_ws(int T, int B, int N, int W) { return (size_t)conv_plan(T, B, N, W, false).task_blocks * N * (W + 1); }
 
 void launch_conv(const CausalConv& p, bool fwd, hipStream_t stream) {
     if (p.bf16) run_conv_w<__bf16>(p, fwd, stream);

@@ -677,33 +677,59 @@ __global__ void __launch_bounds__(1024) selective_sums_kernel(Selective p, unsig
     }
 }
 
-// one time step
-template <class E, int Q, int K>
-__global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
-    const Place<Q, K> at(p);
-    const int b = at.b, n = at.n, S = p.S;
-    const size_t row = ((size_t)b * p.N + n) * S;
-    float A[K], h[K], slope, y = 0.0f;
-    load_states<K>(A, p.A + (size_t)n * S, at.s0, S, true);
-    load_states<K>(h, p.h0 + row, at.s0, S, at.on);
-    const float x = (float)row_of<E>(p.x, b)[n];
-    const float delta = softplus((float)row_of<E>(p.dt, b)[n] + (p.dt_bias ? p.dt_bias[n] : 0.0f), &slope);
-    const E *Bv = row_of<E>(p.Bm, b), *Cv = row_of<E>(p.C, b);
+// K of a row's S values from column s0 on, as fp32; 0 past S
+template <class E, int K>
+__device__ __forceinline__ void load_low(float* v, const E* row, int s0, int S) {
+    if (s0 + K <= S) {
+        const auto t = vload<E, K>(row + s0);
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        const bool in = at.s0 + k < S;
-        h[k] = fmaf(__builtin_amdgcn_exp2f(delta * (A[k] * kLog2e)), h[k], in ? delta * x * (float)Bv[at.s0 + k] : 0.0f);
-        y += in ? h[k] * (float)Cv[at.s0 + k] : 0.0f;
+        for (int k = 0; k < K; ++k) v[k] = t.get(k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = s0 + k < S ? (float)row[s0 + k] : 0.0f;
     }
-    store_states<K>(p.h_last + row, h, at.s0, S, at.on);
-    y = lanes_total<Q>(y);
-    if (!at.on || at.j) return;
-    if (p.D) y = fmaf(p.D[n], x, y);
-    if (p.g.data) {
-        const float g = (float)row_of<E>(p.g, b)[n];
-        y *= g * sigmoid(g);
-    }
-    row_of<E>(p.y, b)[n] = (E)y;
+}
+
+// One time step of R rows (p.B of them counts rows, p.tiles workgroups of channels). Bound by the states'
+// memory: a lane's states of R rows are under way together, and A is read once for them. What a channel
+// needs once a row its lanes take in turn, a row each, as the scan's lanes their steps. All states are
+// read before the first is written: they may be written where they were read.
+template <class E, int Q, int K, int R>
+__global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
+    const Place<Q, K> at(p);                      // (b counts groups of R rows)
+    const int n = at.n, j = at.j, S = p.S, b0 = at.b * R;
+    const size_t plane = (size_t)p.N * S, chan = (size_t)n * S;
+    float A2[K], h[R][K], ys[Q];
+    auto row_at = [&](int i) { return min(b0 + i, p.B - 1); };
+#pragma unroll
+    for (int i = 0; i < R; ++i) load_states<K>(h[i], p.h0 + row_at(i) * plane + chan, at.s0, S, at.on);
+    load_states<K>(A2, p.A + chan, at.s0, S, true);
+#pragma unroll
+    for (int k = 0; k < K; ++k) A2[k] *= kLog2e;
+    const int mine = row_at(j % R);
+    const float x = (float)row_of<E>(p.x, mine)[n];
+    const Gate gate(p.g.data ? (float)row_of<E>(p.g, mine)[n] : 0.0f, p.g.data);
+    float slope;
+    const float delta = softplus((float)row_of<E>(p.dt, mine)[n] + (p.dt_bias ? p.dt_bias[n] : 0.0f), &slope), u = delta * x;
+    each<R>([&](auto row) {
+        constexpr int i = decltype(row)::value;
+        float Bv[K], Cv[K];
+        load_low<E, K>(Bv, row_of<E>(p.Bm, row_at(i)), at.s0, S);
+        load_low<E, K>(Cv, row_of<E>(p.C, row_at(i)), at.s0, S);
+        const float di = from_lane<Q, i>(delta), ui = from_lane<Q, i>(u);
+        ys[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            h[i][k] = fmaf(__builtin_amdgcn_exp2f(di * A2[k]), h[i][k], ui * Bv[k]);
+            ys[i] = fmaf(h[i][k], Cv[k], ys[i]);
+        }
+    });
+#pragma unroll
+    for (int i = R; i < Q; ++i) ys[i] = 0.0f;
+    const float y = fmaf(p.D ? p.D[n] : 0.0f, x, sums_by_lane<Q>(ys, j)) * gate.value;
+#pragma unroll
+    for (int i = 0; i < R; ++i) store_states<K>(p.h_last + row_at(i) * plane + chan, h[i], at.s0, S, at.on && b0 + i < p.B);
+    if (at.on && j < R && b0 + j < p.B) row_of<E>(p.y, b0 + j)[n] = (E)y;
 }
 
 namespace {
@@ -728,16 +754,17 @@ Plan selective_plan(int T, int B, int N, int S, bool fwd, bool mask) {
 }
 
 enum { kFwd, kBwd, kStep };
+constexpr int kStepRows = 4;
 
 template <class E, int Q, int K, bool STARTS>
 void run_selective(Selective p, const Plan& q, int what, hipStream_t stream) {
-    const long long groups = (long long)p.B * p.tiles;
+    const long long groups = (long long)(what == kStep ? (p.B + kStepRows - 1) / kStepRows : p.B) * p.tiles;
     for (int pass = what != kStep && q.ranges > 1 ? 0 : 1; pass < 2; ++pass)
         for (long long first = 0; first < groups; first += kMostBlocks) {
             p.first = first;
             const unsigned wgs = (unsigned)std::min<long long>(groups - first, kMostBlocks);
             const dim3 grid(wgs, q.ranges), inner(wgs, q.ranges - 1), block(64 * kWavesWg);
-            if (what == kStep) hipLaunchKernelGGL((selective_step_kernel<E, Q, K>), dim3(wgs), block, 0, stream, p);
+            if (what == kStep) hipLaunchKernelGGL((selective_step_kernel<E, Q, K, kStepRows>), dim3(wgs), block, 0, stream, p);
             else if (pass == 0 && what == kFwd) hipLaunchKernelGGL((selective_range_kernel<E, Q, K, STARTS, false>), inner, block, 0, stream, p);
             else if (pass == 0) hipLaunchKernelGGL((selective_range_kernel<E, Q, K, STARTS, true>), inner, block, 0, stream, p);
             else if (what == kFwd) hipLaunchKernelGGL((selective_fwd_kernel<E, Q, K, STARTS>), grid, block, 0, stream, p);
