@@ -479,7 +479,14 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
         };
         whole && t0 + kStepsB <= tend ? four(std::true_type()) : four(std::false_type());
     };
+    // the state kept before step t, a half ahead of its use (0 where the eight steps are padding: an
+    // infinite state times their step size of 0)
+    float hn[K];
+    auto fetch_kept = [&](int t) {
+        load_states<K>(hn, p.states + (size_t)(t / kKept) * plane + row, at.s0, S, at.on && t < tend);
+    };
     if (tend > ts) {
+        fetch_kept(last + kKept);
         bcv.load(last, tend, -kStepsB);
         load(last, std::integral_constant<int, 1>());
         if (OWN > 1) load(last, std::integral_constant<int, 0>());
@@ -497,8 +504,9 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
         each_back<2>([&](auto half) {
             constexpr int hf = decltype(half)::value, s0 = hf * kKept;
             float hk[K], a[kKept][K], h[kKept][K];
-            // (0 where all eight steps are padding: an infinite state times their step size of 0)
-            load_states<K>(hk, p.states + (size_t)((t0 + s0) / kKept) * plane + row, at.s0, S, at.on && t0 + s0 < tend);
+#pragma unroll
+            for (int k = 0; k < K; ++k) hk[k] = hn[k];
+            if (t0 + s0 > ts) fetch_kept(t0 + s0 - kKept);
             if constexpr (OWN > 1 || hf == 1) {
                 each<HALF>([&](auto own) {
                     constexpr int o = decltype(own)::value, c = (OWN > 1 ? hf * HALF : 0) + o;
