@@ -745,6 +745,19 @@ namespace {
 struct Plan {
     int Q, K, tiles, range, ranges;
 };
+// Four lanes a channel up to 16 states, 16 lanes beyond (their sums over lanes cost more, but 16 states a
+// lane would leave the backward no registers).
+//
+// Time over the grid where rows and channels give too few workgroups. A first launch over all ranges but
+// one then composes the ranges' maps, without outputs, half to two thirds of a pass' work. A SIMD runs a
+// vector instruction every ten cycles for one wave and every four for four, so that one workgroup a CU
+// pays for it in the backward only (bf16, N 2048, S 16, T 1024; whole and in ranges, us: B 4 forward 128 and
+// 74, backward 313 and 160; B 8 126 and 124, 320 and 290; B 12 171 and 178, 470 and 425; B 16 182 and
+// 220, 475 and 535). Padded ranges end early and leave room for others: with masks more of them, and up
+// to more workgroups (T1000 B50 N333 S8: forward 127 us whole, 86 with 12, 93 with 32; backward 290, 215
+// with 8, 256 with 24; T300 B100 N512 S16, 800 workgroups: backward 224 and 203 with 3, forward 78 and
+// 103). At least two blocks a range, at most 32 ranges (T2048 B1: backward 101 us with 32, 134 with 64,
+// each of which composes the maps of those before it).
 Plan selective_plan(int T, int B, int N, int S, bool fwd, bool mask) {
     Plan q;
     q.Q = S <= 16 ? 4 : 16;
@@ -752,9 +765,9 @@ Plan selective_plan(int T, int B, int N, int S, bool fwd, bool mask) {
     const int channels = 64 / q.Q * kWavesWg;
     q.tiles = (N + channels - 1) / channels;
     const long long groups = (long long)B * q.tiles;
-    const int blocks = (T + kStepsB - 1) / kStepsB;
-    int want = groups >= (fwd && !mask ? 256 : 512) ? 1 : (int)std::min<long long>(64, (fwd && mask ? 4096 : 1024) / groups);
-    want = std::max(1, std::min(want, blocks / 4));
+    const int blocks = (T + kStepsB - 1) / kStepsB, few = (fwd ? 256 : 512) * (mask ? 2 : 1);
+    const int wanted = fwd ? (mask ? 4096 : 1024) : (mask ? 2400 : 1536);
+    const int want = groups >= few ? 1 : std::max(1, std::min({(int)(wanted / groups), 32, blocks / 2}));
     const int per = (blocks + want - 1) / want;
     q.range = per * kStepsB;
     q.ranges = (blocks + per - 1) / per;
