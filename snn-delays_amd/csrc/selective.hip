@@ -14,10 +14,19 @@
 // in 32 bits. The sums over states that end a step (y; backwards also <l, B> and <A, q>) are taken for
 // Q steps together, half of them handed over in each exchange, and land in the lane of their step.
 //
-// The forward keeps the state before every 16th step; the backward runs 16 steps from there, holds
-// their decays and states in registers and walks back. The sums over channels (dB, dC) go through
-// the wave's lanes, the workgroup's LDS and one set of sums for each workgroup of channels in memory,
-// added up in a second launch in a fixed order, as dA, dD and the bias' over the rows.
+// The forward keeps the state before every 8th step in 32 bits (S / 2 bytes a value and step); the
+// backward runs eight steps from there, holds their decays and states in registers and walks back (16
+// steps took a second wave's registers: 397 us instead of 277 at the sizes below). The sums over
+// channels (dB, dC) go through the wave's lanes, the workgroup's LDS and one set of sums for each
+// workgroup of channels in memory, added up in a second launch in a fixed order, as dA, dD and the
+// bias' over the rows.
+//
+// Bound by vector issue: forward 8.8 and backward 25.6 instructions a state and step, the exponential at
+// less than half the rate, with the vector units busy 83 % of the time. At T250 B128 N512 S16 bf16 (262
+// million states and steps) forward 87 us, with the kept states 100; backward 250 us, the sums 8. (The
+// bytes take 26 and 65 us.) Exchanging lanes for dB and dC costs a sixth of the backward; as fp32
+// matrix products with a selector, which do not run beside the vector instructions, they took it to
+// 357 us, and through LDS to 272 (252 then).
 #include <algorithm>
 #include <utility>
 
@@ -117,11 +126,13 @@ __device__ __forceinline__ float lanes_total(float v) {
     return group_sum_t<Q>(v);
 }
 
+// halves of the wave exchanged: a keeps its lower and takes b's lower, b its upper and takes a's upper
 __device__ __forceinline__ void swap32(float& a, float& b) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     a = __uint_as_float(r[0]);
     b = __uint_as_float(r[1]);
 }
+// the same with the odd rows of 16 lanes of a and the even ones of b
 __device__ __forceinline__ void swap16(float& a, float& b) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
     a = __uint_as_float(r[0]);
@@ -194,7 +205,6 @@ __device__ __forceinline__ E* row_of(const delrec_rows& x, int b) { return (E*)x
 
 // bit i: a sequence starts at step t0 + i
 __device__ __forceinline__ uint32_t start_bits(const Selective& p, int b, int t0, int tend, int lane) {
-    if (!p.starts) return 0;
     const int t = t0 + lane;
     return (uint32_t)__ballot(lane < kStepsB && t < tend && p.starts[(size_t)min(t, p.T - 1) * p.B + b] != 0);
 }
@@ -701,7 +711,8 @@ __device__ __forceinline__ void load_low(float* v, const E* row, int s0, int S) 
 // One time step of R rows (p.B of them counts rows, p.tiles workgroups of channels). Bound by the states'
 // memory: a lane's states of R rows are under way together, and A is read once for them. What a channel
 // needs once a row its lanes take in turn, a row each, as the scan's lanes their steps. All states are
-// read before the first is written: they may be written where they were read.
+// read before the first is written: they may be written where they were read. 29.5 us at B512 N2048 S16
+// bf16 (134 MB of states, 4.6 TB/s); one row a lane, each with its own A, took 40.
 template <class E, int Q, int K, int R>
 __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     const Place<Q, K> at(p);                      // (b counts groups of R rows)

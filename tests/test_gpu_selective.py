@@ -86,7 +86,7 @@ def check_scan(c, dev):
 
 
 SCAN_SIZES = [(1, 1, 1, 1), (1, 3, 65, 16), (2, 2, 3, 5), (15, 2, 5, 3), (16, 1, 64, 16), (17, 3, 70, 8), (33, 2, 130, 17),
-              (50, 2, 20, 33), (40, 1, 17, 64), (300, 2, 96, 16), (130, 5, 33, 4), (31, 33, 16, 2)]
+              (50, 2, 20, 33), (40, 1, 17, 64), (300, 2, 96, 16), (130, 5, 33, 4), (31, 33, 16, 2), (40, 530, 8, 4)]
 
 
 @pytest.mark.gpu
@@ -264,6 +264,89 @@ def test_scan_offsets_past_32_bits(dev):
     y, last = selective_scan(*[leaves[k] for k in LEAVES])
     (dx,) = torch.autograd.grad((y, last), (leaves['x'],), (d['dy'], d['dlast']))
     assert torch.equal(y, want['y']) and torch.equal(last, want['last']) and torch.equal(dx, want['x'])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('S', [2, 40])
+def test_scan_ranges_of_time(dev, S):
+    """Long sequences of few channels are cut into ranges of time: starts and row ends anywhere, in the
+    first and last steps of a range too, rows that end before a range begins."""
+    T, B, N = 513, 6, 20
+    c = scan_case(T, B, N, S, FP32, True, rate=0.3)
+    c['lengths'] = torch.tensor([T, 0, 1, 255, 256, 257])
+    c['starts'] = torch.zeros(T, B, dtype=torch.bool)
+    for t in (31, 32, 33, 255, 256, 512):
+        c['starts'][t] = True
+    c['starts'][:, 0] = False
+    check_scan(c, dev)
+    c['starts'] = c['lengths'] = None
+    check_scan(c, dev)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_one_launch_holds(dev):
+    """Past 2^20 workgroups the launches are repeated: the last rows are computed as the first."""
+    from delrec.selective import causal_conv, conv_step, selective_scan, selective_step
+    B, N, S = (1 << 20) + 70, 1, 2
+    c = put(scan_case(1, 3, N, S, FP32, False), dev)
+    wide = {k: c[k].repeat(*([1] * (c[k].dim() - 2)), (B + 2) // 3, 1)[:, :B] if k in ('x', 'dt', 'B', 'C', 'g', 'dy') else c[k] for k in c}
+    for k in ('h0', 'dlast'):
+        wide[k] = c[k].repeat((B + 2) // 3, 1, 1)[:B]
+    want = run_scan({k: v if v is None else v.cpu() for k, v in c.items()}, dev)
+    leaves = {k: wide[k].contiguous().requires_grad_(True) for k in LEAVES}
+    y, last = selective_scan(*[leaves[k] for k in LEAVES])
+    dx, dB, dh = torch.autograd.grad((y, last), (leaves['x'], leaves['B'], leaves['h0']), (wide['dy'], wide['dlast']))
+    for got, k in ((y, 'y'), (dx, 'x'), (dB, 'B')):
+        assert torch.equal(got[:, :3], want[k]) and torch.equal(got[:, B - 1], want[k][:, (B - 1) % 3])
+    assert torch.equal(last[B - 1], want['last'][(B - 1) % 3]) and torch.equal(dh[B - 1], want['h0'][(B - 1) % 3])
+    with torch.no_grad():
+        ys, hs = selective_step(*[wide[k][0] if k in ('x', 'dt', 'B', 'C') else wide[k] for k in ('x', 'dt', 'A', 'B', 'C')], wide['h0'],
+                                wide['D'], wide['g'][0], wide['dt_bias'])
+        close(ys, y[0].double().cpu(), ROW_TOL, 'step')
+        close(hs, last.double().cpu(), ROW_TOL, 'state')
+    e = put(conv_case(1, 3, 125, 4, BF16, False), dev)
+    B = (1 << 23) + 9                    # eight rows a workgroup
+    x, state = (e[k].repeat(1, (B + 2) // 3, 1)[:, :B] if k == 'x' else e[k].repeat((B + 2) // 3, 1, 1)[:B] for k in ('x', 'state'))
+    with torch.no_grad():
+        y0, s0 = causal_conv(e['x'], e['weight'], e['bias'], e['state'])
+        y, s = causal_conv(x, e['weight'], e['bias'], state)
+        assert torch.equal(y[0, B - 3:], y0[0, [(B - 3 + i) % 3 for i in range(3)]]) and torch.equal(s[B - 1], s0[(B - 1) % 3])
+        y, s = conv_step(x[0], state, e['weight'], e['bias'])
+        assert torch.equal(y[B - 1], y0[0, (B - 1) % 3]) and torch.equal(s[B - 1], s0[(B - 1) % 3])
+
+
+@pytest.mark.gpu
+def test_parameters_of_other_types_and_saved_tensor_hooks(dev):
+    """Parameters in bf16 count as their fp32 values and get their gradients in bf16; what the graph
+    keeps may go through the host."""
+    from delrec.gated import add_norm
+    from delrec.selective import causal_conv, selective_scan
+    c = put(scan_case(30, 2, 24, 16, FP32, False), dev)
+    half = {k: c[k].bfloat16() for k in ('A', 'D', 'dt_bias')}
+    outs = []
+    for cast in (lambda t: t, lambda t: t.float()):
+        p = {k: cast(v).detach().requires_grad_(True) for k, v in half.items()}
+        y, last = selective_scan(c['x'], c['dt'], p['A'], c['B'], c['C'], p['D'], c['g'], p['dt_bias'], c['h0'])
+        outs.append((y, *torch.autograd.grad((y, last), list(p.values()), (c['dy'], c['dlast']))))
+    assert torch.equal(outs[0][0], outs[1][0])
+    for a, b in zip(outs[0][1:], outs[1][1:]):
+        assert a.dtype == BF16 and torch.equal(a, b.bfloat16())
+    e = put(conv_case(30, 2, 24, 4, BF16, True), dev)
+    n = put(add_case((6, 5, 24), BF16, FP32), dev)
+
+    def grads():
+        d = {k: c[k].detach().requires_grad_(True) for k in LEAVES}
+        y, last = selective_scan(*[d[k] for k in LEAVES])
+        f = {k: e[k].detach().requires_grad_(True) for k in CONV_LEAVES}
+        yc, after = causal_conv(*[f[k] for k in CONV_LEAVES], starts=e['starts'], lengths=e['lengths'])
+        v = [n[k].detach().requires_grad_(True) for k in ('x', 'y', 'w')]
+        x, u = add_norm(*v)
+        return lambda: torch.autograd.grad((y, last, yc, after, x, u), [*d.values(), *f.values(), *v],
+                                           (c['dy'], c['dlast'], e['dy'], e['dstate'], n['dx'], n['du']))
+    plain = grads()()
+    with torch.autograd.graph.save_on_cpu():
+        later = grads()
+    assert all(torch.equal(a, b) for a, b in zip(plain, later()))
 
 
 @pytest.mark.gpu
