@@ -412,29 +412,34 @@ struct Plan {
     long long task_blocks;
 };
 // 32 lanes of neighbouring channels, fewer where a row has fewer. Forward runs of 16 steps (T250 B128 N512
-// bf16 W4 16.0 us, 17.8 with 32, 24.5 with 64; T1000 B50 N333 with masks 26, 33 and 53). Backward runs take
-// 32 steps with the W - 1 past their end, in blocks without a rest (the same cases 32.5 and 45 us; with
-// 16 34.5 and 47, and W8 67 instead of 56), but 16 where the launch is small (T32 B64 N64 12.4 us
-// instead of 20).
-Plan conv_plan(int T, int B, int N, int W, bool fwd) {
-    Plan q;
+// bf16 W4 16.0 us, 17.8 with 32, 24.5 with 64; T1000 B50 N333 with masks 26, 33 and 53). Backward runs
+// take whole blocks with the W - 1 steps past their end, as many as make the least work for the CU that
+// has the most workgroups (32 steps and this many, us: the first case 32.4 and 29.0, T8192 B1 N2048 32.4
+// and 31.0, T1000 B16 N1024 W8 55 and 41, fp32 W4 49 and 45). With masks some runs end early, and up to
+// 32 steps are better (T1000 B50 N333 W3 50 us with 40 steps, 45 with 32).
+Plan conv_plan(int T, int B, int N, int W, bool fwd, bool mask) {
+    Plan best{};
     const int groups = (N + kVec - 1) / kVec;
-    q.lanes = 1;
-    while (q.lanes < 32 && q.lanes < groups) q.lanes *= 2;
-    q.lane_blocks = (groups + q.lanes - 1) / q.lanes;
-    const int per = 256 / q.lanes;
-    for (const int steps : {fwd ? 16 : 32 - (W - 1), 16 - (W - 1)}) {
-        q.steps = std::min(T, steps);
+    best.lanes = 1;
+    while (best.lanes < 32 && best.lanes < groups) best.lanes *= 2;
+    best.lane_blocks = (groups + best.lanes - 1) / best.lanes;
+    const int per = 256 / best.lanes;
+    double least = 0.0;
+    for (int m = 4; m <= (mask ? 8 : 16); ++m) {
+        Plan q = best;
+        q.steps = std::min(T, m * kBlock - (fwd ? 0 : W - 1));
         q.runs = (T + q.steps - 1) / q.steps;
         q.task_blocks = ((long long)q.runs * B + per - 1) / per;
-        if (fwd || q.task_blocks * q.lane_blocks >= 256) break;
+        const double work = (double)((q.task_blocks * q.lane_blocks + 255) / 256) * (m * kBlock);
+        if (m == 4 || work < least) best = q, least = work;
+        if (fwd || q.steps == T) break;
     }
-    return q;
+    return best;
 }
 
 template <class E, int W, bool STARTS>
 void run_conv(CausalConv p, bool fwd, hipStream_t stream) {
-    const Plan q = conv_plan(p.T, p.B, p.N, W, fwd);
+    const Plan q = conv_plan(p.T, p.B, p.N, W, fwd, p.starts || p.lengths);
     p.lanes = q.lanes;
     p.lane_blocks = q.lane_blocks;
     p.steps = q.steps;
@@ -473,7 +478,9 @@ void run_conv_w(const CausalConv& p, bool fwd, hipStream_t stream) {
 
 }  // namespace
 
-size_t conv_bwd_ws(int T, int B, int N, int W) { return (size_t)conv_plan(T, B, N, W, false).task_blocks * N * (W + 1); }
+size_t conv_bwd_ws(int T, int B, int N, int W) {
+    return (size_t)std::max(conv_plan(T, B, N, W, false, false).task_blocks, conv_plan(T, B, N, W, false, true).task_blocks) * N * (W + 1);
+}
 
 void launch_conv(const CausalConv& p, bool fwd, hipStream_t stream) {
     if (p.bf16) run_conv_w<__bf16>(p, fwd, stream);
