@@ -23,7 +23,7 @@
 //
 // Bound by vector issue: forward 8.8 and backward 25.6 instructions a state and step, the exponential at
 // less than half the rate, with the vector units busy 83 % of the time. At T250 B128 N512 S16 bf16 (262
-// million states and steps) forward 87 us, with the kept states 100; backward 250 us, the sums 8. (The
+// million states and steps) forward 87 us, with the kept states 100; backward 248 us, the sums 8. (The
 // bytes take 26 and 65 us.) Exchanging lanes for dB and dC costs a sixth of the backward; as fp32
 // matrix products with a selector, which do not run beside the vector instructions, they took it to
 // 357 us, and through LDS to 272 (252 then).
@@ -272,16 +272,16 @@ struct Column {
         return r;
     }
 };
-// COUNT own steps from FROM on, the last one first where DIR < 0; zeros past the row's end and in lanes
+// COUNT own steps from t0 + j on, the last one first where DIR < 0; zeros past the row's end and in lanes
 // without a channel
-template <class E, int Q, int DIR>
+template <class E, int Q, int DIR, int COUNT = Shape<Q>::own>
 struct Own {
-    E v[Shape<Q>::own];
-    template <bool FULL, int FROM = 0, int COUNT = Shape<Q>::own>
+    E v[COUNT];
+    template <bool FULL>
     __device__ __forceinline__ void load(Column<E, Q, DIR>& x, int t0, int j, int tend, bool on) {
 #pragma unroll
         for (int k = 0; k < COUNT; ++k) {
-            const int i = DIR > 0 ? FROM + k : FROM + COUNT - 1 - k;
+            const int i = DIR > 0 ? k : COUNT - 1 - k;
             const E* from = x.next();
             if (FULL) {
                 v[i] = *from;
@@ -467,8 +467,10 @@ __global__ void __launch_bounds__(256) selective_range_kernel(Selective p) {
     if (at.on && j == 0) p.mapsums[(size_t)y * p.B * p.N + chan] = cut ? -1.0f : total;
 }
 
+// Two waves a SIMD, and three where 168 registers nearly do (S 17 to 32, T250 B64 N512: 250 us, 285 with two;
+// S 8: 13 registers would not fit, 202 us instead of 172).
 template <class E, int Q, int K, bool STARTS>
-__global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
+__global__ void __launch_bounds__(256, Q == 16 && K == 2 ? 3 : 2) selective_bwd_kernel(Selective p) {
     constexpr int SP = Q * K, OWN = Shape<Q>::own;
     constexpr int HALF = OWN > 1 ? OWN / 2 : 1;       // own steps of a kept state's eight
     __shared__ __align__(16) float bc[2][kStepsB][2][SP];
@@ -489,18 +491,17 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
     Column<E, Q, -1> xc(p.x, b, n, t1), dc(p.dt, b, n, t1), gc(gated ? p.g : p.x, b, n, t1), yc(p.dy, b, n, t1);
     Column<E, Q, -1> dxc(p.dx, b, n, t1), ddc(p.ddt, b, n, t1), dgc(gated ? p.dg : p.dx, b, n, t1);
     Stage<E, SP> bcv(p, b, last);
-    Own<E, Q, -1> xv, dv, gv, yv;
-    // a half's own steps of a block (Q 16: the one, with the upper half)
-    auto load = [&](int t0, auto half) {
-        constexpr int from = OWN > 1 ? decltype(half)::value * HALF : 0;
+    // the own steps of the half block (Q 16: block) from t on, a half (block) ahead of their use
+    Own<E, Q, -1, HALF> xv, dv, gv, yv;
+    auto load = [&](int t) {
         auto four = [&](auto full) {
             constexpr bool F = decltype(full)::value;
-            dv.template load<F, from, HALF>(dc, t0, j, tend, at.on);
-            xv.template load<F, from, HALF>(xc, t0, j, tend, at.on);
-            gv.template load<F, from, HALF>(gc, t0, j, tend, at.on);
-            yv.template load<F, from, HALF>(yc, t0, j, tend, at.on);
+            dv.template load<F>(dc, t, j, tend, at.on);
+            xv.template load<F>(xc, t, j, tend, at.on);
+            gv.template load<F>(gc, t, j, tend, at.on);
+            yv.template load<F>(yc, t, j, tend, at.on);
         };
-        whole && t0 + kStepsB <= tend ? four(std::true_type()) : four(std::false_type());
+        whole && t + HALF * Q <= tend ? four(std::true_type()) : four(std::false_type());
     };
     // the state kept before step t, a half ahead of its use (0 where the eight steps are padding: an
     // infinite state times their step size of 0)
@@ -511,8 +512,7 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
     if (tend > ts) {
         fetch_kept(last + kKept);
         bcv.load(last, tend, -kStepsB);
-        load(last, std::integral_constant<int, 1>());
-        if (OWN > 1) load(last, std::integral_constant<int, 0>());
+        load(last + kStepsB - HALF * Q);
     }
     int buf = 0;
     for (int t0 = last; tend > ts && t0 >= ts; t0 -= kStepsB, buf ^= 1) {
@@ -534,15 +534,16 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
                 each<HALF>([&](auto own) {
                     constexpr int o = decltype(own)::value, c = (OWN > 1 ? hf * HALF : 0) + o;
                     const bool valid = at.on && t0 + c * Q + j < tend;
-                    const float soft = softplus((float)dv.v[c] + bias, &slope[o]);
+                    const float soft = softplus((float)dv.v[o] + bias, &slope[o]);
                     delta[o] = valid ? soft : 0.0f;
-                    xs[o] = (float)xv.v[c];
+                    xs[o] = (float)xv.v[o];
                     u[o] = delta[o] * xs[o];
-                    const Gate gate((float)gv.v[c], gated);
-                    w[o] = (float)yv.v[c] * gate.value;
-                    ga[o] = (float)yv.v[c] * gate.slope;
+                    const Gate gate((float)gv.v[o], gated);
+                    w[o] = (float)yv.v[o] * gate.value;
+                    ga[o] = (float)yv.v[o] * gate.slope;
                 });
-                if (t0 > ts) load(t0 - kStepsB, half);
+                constexpr int before = (OWN > 1 ? hf * kKept : 0) - HALF * Q;
+                if (t0 + before >= ts) load(t0 + before);
             }
             each<kKept>([&](auto step) {
                 constexpr int e = decltype(step)::value, s = s0 + e, o = OWN > 1 ? e / Q : 0, i = s % Q;
@@ -557,31 +558,38 @@ __global__ void __launch_bounds__(256, 2) selective_bwd_kernel(Selective p) {
             });
             fence();
             float left[Q == 4 ? 4 : 1][K / 2];
+            // B and C of a step, read a step ahead
+            Vec<float, K> Bn, Cn;
+            auto read_maps = [&](int s) {
+                Bn = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
+                Cn = *(const Vec<float, K>*)&bc[buf][s][1][at.s0];
+            };
+            read_maps(s0 + kKept - 1);
             each_back<kKept>([&](auto step) {
                 constexpr int e = decltype(step)::value, s = s0 + e, o = OWN > 1 ? e / Q : 0, i = s % Q;
-                const auto Bv = *(const Vec<float, K>*)&bc[buf][s][0][at.s0];
-                const auto Cv = *(const Vec<float, K>*)&bc[buf][s][1][at.s0];
+                const Vec<float, K> Bv = Bn, Cv = Cn;
+                if constexpr (e > 0) read_maps(s - 1);
                 const float di = from_lane<Q, i>(delta[o]), ui = from_lane<Q, i>(u[o]), wi = from_lane<Q, i>(w[o]);
                 const bool fresh = STARTS && (starts >> s & 1);
-                float db[K], dc[K], sy = 0.0f, sl = 0.0f, sq = 0.0f;
+                float ls[K], sy = 0.0f, sl = 0.0f, sq = 0.0f;
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
                     const float before = fresh ? 0.0f : e ? h[e ? e - 1 : 0][k] : hk[k];
-                    const float l = fmaf(wi, Cv.get(k), kc[k]);
+                    ls[k] = fmaf(wi, Cv.get(k), kc[k]);
                     sy = fmaf(h[e][k], Cv.get(k), sy);
-                    sl = fmaf(l, Bv.get(k), sl);
-                    db[k] = l * ui;
-                    dc[k] = wi * h[e][k];
-                    kc[k] = fresh ? 0.0f : a[e][k] * l;
+                    sl = fmaf(ls[k], Bv.get(k), sl);
+                    kc[k] = fresh ? 0.0f : a[e][k] * ls[k];
                     const float q = kc[k] * before;
                     sq = fmaf(A2[k], q, sq);
                     dA[k] = fmaf(di, q, dA[k]);
                 }
                 ys.template add<i>(sy, j), lb.template add<i>(sl, j), aq.template add<i>(sq, j);
-                // over the wave's rows of lanes: lanes below 32 go on with dB, the others with dC; odd
-                // rows with the upper half of the states
+                // over the wave's rows of lanes: lanes below 32 go on with dB, the others with dC (their
+                // factors change places, not the products); odd rows with the upper half of the states
+                float us = ui, ws = wi, db[K];
+                swap32(us, ws);
 #pragma unroll
-                for (int k = 0; k < K; ++k) swap32(db[k], dc[k]), db[k] += dc[k];
+                for (int k = 0; k < K; ++k) swap32(ls[k], h[e][k]), db[k] = fmaf(us, ls[k], ws * h[e][k]);
                 const int kind = at.lane >> 5, part = at.s0 + (at.lane >> 4 & 1) * (K / 2);
                 constexpr int r = Q == 4 ? i : 0;
 #pragma unroll
