@@ -64,6 +64,13 @@ __device__ __forceinline__ float softplus(float x, float* slope) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return gate_in(-x); }
 
+// a decay rate for powers of 2; infinite ones as the largest numbers, so that a step size of 0 (padding)
+// still leaves the state as it is
+__device__ __forceinline__ float rate2(float A) {
+    const float r = A * kLog2e;
+    return fabsf(r) == __builtin_inff() ? copysignf(3.402823466e38f, r) : r;
+}
+
 // lane I's value in each group of Q lanes
 template <int Q, int I>
 __device__ __forceinline__ float from_lane(float v) {
@@ -335,7 +342,7 @@ __global__ void __launch_bounds__(256) selective_fwd_kernel(Selective p) {
     load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
     load_states<K>(h, p.h0 + row, at.s0, S, p.h0 && at.on);
 #pragma unroll
-    for (int k = 0; k < K; ++k) A2[k] *= kLog2e;
+    for (int k = 0; k < K; ++k) A2[k] = rate2(A2[k]);
     if (blockIdx.y) enter_range<K>(h, p, A2, row, chan, at.s0, at.on, 0, 1, blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
     Column<E, Q, 1> xc(p.x, b, n, ts + j), dc(p.dt, b, n, ts + j), gc(gated ? p.g : p.x, b, n, ts + j), yc(p.y, b, n, ts + j);
@@ -410,7 +417,7 @@ __global__ void __launch_bounds__(256) selective_range_kernel(Selective p) {
     float A2[K], h[K], total = 0.0f;
     load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
 #pragma unroll
-    for (int k = 0; k < K; ++k) A2[k] *= kLog2e, h[k] = 0.0f;
+    for (int k = 0; k < K; ++k) A2[k] = rate2(A2[k]), h[k] = 0.0f;
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f;
     const delrec_rows& xr = BWD ? p.dy : p.x;
     constexpr int DIR = BWD ? -1 : 1;
@@ -484,7 +491,7 @@ __global__ void __launch_bounds__(256, Q == 16 && K == 2 ? 3 : 2) selective_bwd_
     load_states<K>(A2, p.A + (size_t)n * S, at.s0, S, true);
     load_states<K>(kc, p.dlast + row, at.s0, S, p.dlast && at.on);
 #pragma unroll
-    for (int k = 0; k < K; ++k) A2[k] *= kLog2e, dA[k] = 0.0f;
+    for (int k = 0; k < K; ++k) A2[k] = rate2(A2[k]), dA[k] = 0.0f;
     enter_range<K>(kc, p, A2, row, chan, at.s0, at.on, gridDim.y - 1, -1, gridDim.y - 1 - blockIdx.y);
     const float bias = p.dt_bias ? p.dt_bias[n] : 0.0f, D = p.D ? p.D[n] : 0.0f;
     const int last = ts + (tend > ts ? (tend - ts - 1) / kStepsB * kStepsB : 0), t1 = last + (OWN - 1) * Q + j;
@@ -747,7 +754,7 @@ __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
     for (int i = 0; i < R; ++i) load_states<K>(h[i], p.h0 + row_at(i) * plane + chan, at.s0, S, at.on);
     load_states<K>(A2, p.A + chan, at.s0, S, true);
 #pragma unroll
-    for (int k = 0; k < K; ++k) A2[k] *= kLog2e;
+    for (int k = 0; k < K; ++k) A2[k] = rate2(A2[k]);
     const int mine = row_at(j % R);
     const float x = (float)row_of<E>(p.x, mine)[n];
     const Gate gate(p.g.data ? (float)row_of<E>(p.g, mine)[n] : 0.0f, p.g.data);
