@@ -10,7 +10,7 @@
 // values of r along; the W - 1 steps after a run that its last dx need are computed twice. The sums of
 // dw go over a lane's steps, then through LDS over the workgroup's runs of the same channels, then from
 // memory over the workgroups, each in a fixed order. At T250 B128 N512 W4 bf16 forward 16 us (65 MB, 4.1
-// TB/s) and backward 31 + 4 (98 MB, 3.2 TB/s; some 30 vector instructions a value come near the memory's
+// TB/s) and backward 29 + 4 (98 MB, 3.4 TB/s; some 30 vector instructions a value come near the memory's
 // time).
 #include <algorithm>
 

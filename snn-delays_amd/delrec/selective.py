@@ -52,7 +52,7 @@ def selective_scan(x, dt, A, B, C, D=None, g=None, dt_bias=None, h0=None, starts
     channel, ``D``, ``dt_bias`` (N,); ``h0`` (B, N, S) fp32, zero when absent; ``starts`` (T, B) bool:
     a sequence starts at this step, the state before it is dropped; ``lengths`` (B,) ints: from this
     step on a row is padding, its state stays, its output is 0 and its inputs are not used.
-    Differentiable in all but the masks; the backward pass keeps the state before every 16th step."""
+    Differentiable in all but the masks; the backward pass keeps the state before every 8th step."""
     return _lib.require_ext().selective_scan(x, dt, A, B, C, D, g, dt_bias, h0, starts, lengths)
 
 
