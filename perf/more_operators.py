@@ -14,7 +14,6 @@ A case is a dict of plain values; ``kind`` names the operator:
 With ``joint`` the inputs are column slices of one projection's output, as the block makes them.
 """
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -182,7 +181,6 @@ SCAN_LEAVES = ('x', 'dt', 'A', 'b', 'c', 'D', 'g', 'dt_bias', 'h0')
 ADD_LEAVES = ('x', 'y', 'weight')
 
 
-@functools.lru_cache(maxsize=None)
 def _ops():
     pkg = str(Path(__file__).resolve().parent.parent / 'snn-delays_amd')
     if pkg not in sys.path:
