@@ -34,6 +34,41 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// a sum over G lanes in 64 bits
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+    return __hiloint2double(__float_as_int(dpp<CTRL>(__int_as_float(__double2hiint(v)))), __float_as_int(dpp<CTRL>(__int_as_float(__double2loint(v)))));
+}
+template <int G>
+__device__ __forceinline__ double group_sum64(double v) {
+    static_assert(G == 16 || G == 64, "a row's lanes in a wave");
+    v += dpp64<0xB1>(v);
+    v += dpp64<0x4E>(v);
+    v += dpp64<0x141>(v);
+    v += dpp64<0x140>(v);
+    if constexpr (G == 64) {
+        v += __shfl_xor(v, 16, kWave);
+        v += __shfl_xor(v, 32, kWave);
+    }
+    return v;
+}
+__device__ __forceinline__ double row_sum64(double v, double* red) {
+    v = group_sum64<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// 1/sqrt(x), correctly rounded but for ties to 14 digits: a Newton step in 64 bits from 32 bits' root (0 and
+// infinity have none)
+__device__ __forceinline__ float inv_root(float x) {
+    const float y = rsqrtf(x);
+    if (!(y > 0.0f && y < __builtin_inff())) return y;
+    const double z = y;
+    return (float)fma(0.5 * z, fma(-(double)x * z, z, 1.0), z);
+}
+
 template <class T>
 __device__ __forceinline__ T* row_ptr(const delrec_rows& x, long long row, int R1) {
     return (T*)x.data + (row / R1) * x.s0 + (row % R1) * x.s1;
@@ -156,24 +191,29 @@ __global__ void __launch_bounds__(kNb) norm_any_bwd_kernel(NormGate p) {
 // ---- a residual's addition and its norm: x' = x + y, r = 1/sqrt(mean x'^2 + eps), u = x' r w ----
 // Backwards, with e = x' r and v = w du: dx = dy = dx' + r (v - e <v e>), dw = sum du e. The same
 // rows in registers; the forward also packs u, as rounded, to 8 bits. Kept for the backward: r, and
-// x' where it is fp32 (exact), else x and y, so that no rounding of x' reaches dw. Bound by memory:
-// 65536 x 2048 bf16 with x in fp32 and u in 8 bits forward 351 us (1.7 GB, 5.0 TB/s), backward 436 (2.1 GB,
-// 4.9 TB/s).
+// x' where it is fp32 (exact), else x and y, so that no rounding of x' reaches dw.
+//
+// The squares are summed in 64 bits and r is their mean's root to its last bit: it does not depend on how a
+// row is spread over lanes, and 8-bit codes of u in fp32, which a last bit of r moves over a border of two
+// steps now and then, are those of the elementary operations more often (65536 x 2048 values: 37 differ, by
+// one step; 144 with sums and root in 32 bits). It takes no longer: bound by memory, 65536 x 2048 bf16 with x
+// in fp32 and u in 8 bits forward 351 us (1.7 GB, 5.0 TB/s), backward 436 (2.1 GB, 4.9 TB/s).
 
 template <class S, class X>
 __global__ void __launch_bounds__(kNb) add_norm_any_fwd_kernel(AddNorm p) {
-    __shared__ float red[4];
+    __shared__ double red[4];
     const int N = p.N;
+    const float inv_n = 1.0f / (float)N;
     const long long rows = (long long)p.R0 * p.R1;
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
         const X* x = row_ptr<const X>(p.x, row, p.R1);
         const S* y = row_ptr<const S>(p.y, row, p.R1);
-        float s = 0.0f;
+        double s = 0.0;
         for (int n = threadIdx.x; n < N; n += kNb) {
             const float v = to_f32(x[n]) + to_f32(y[n]);
             s += v * v;
         }
-        const float r = 1.0f / sqrtf(row_sum(s, red) / (float)N + p.eps);
+        const float r = inv_root((float)row_sum64(s, red) * inv_n + p.eps);
         for (int n = threadIdx.x; n < N; n += kNb) {
             const float v = to_f32(x[n]) + to_f32(y[n]);
             ((X*)p.x_out)[row * N + n] = (X)v;
@@ -262,6 +302,21 @@ constexpr int kRowBlock = LPR < 256 ? 256 : LPR;
 template <int LPR>
 __device__ __forceinline__ float lanes_sum(float v, float* red, int slot) {
     v = group_sum_t<LPR < 64 ? LPR : 64>(v);
+    if constexpr (LPR > 64) {
+        constexpr int W = LPR / 64;
+        if ((threadIdx.x & 63) == 0) red[slot * W + (threadIdx.x >> 6)] = v;
+        barrier_lds();
+        v = red[slot * W];
+#pragma unroll
+        for (int q = 1; q < W; ++q) v += red[slot * W + q];
+    }
+    return v;
+}
+
+// the same in 64 bits
+template <int LPR>
+__device__ __forceinline__ double lanes_sum64(double v, double* red, int slot) {
+    v = group_sum64<LPR < 64 ? LPR : 64>(v);
     if constexpr (LPR > 64) {
         constexpr int W = LPR / 64;
         if ((threadIdx.x & 63) == 0) red[slot * W + (threadIdx.x >> 6)] = v;
@@ -613,7 +668,7 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) norm_gate_bwd_kernel(NormGate 
 
 template <class S, class X, int LPR, int NE>
 __global__ void __launch_bounds__(kRowBlock<LPR>) add_norm_fwd_kernel(AddNorm p) {
-    __shared__ float red[2 * (LPR > 64 ? LPR / 64 : 1)];
+    __shared__ double red[2 * (LPR > 64 ? LPR / 64 : 1)];
     constexpr int RPW = kRowBlock<LPR> / LPR;
     const int lane = threadIdx.x % LPR, N = p.N, ng = (N + kGroup8 - 1) / kGroup8;
     const Cols<LPR, NE> c(lane, N);
@@ -632,7 +687,8 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) add_norm_fwd_kernel(AddNorm p)
         const S* yp = row_at<const S>(p.y, row, p);
 #pragma unroll
         for (int e = 0; e < NE; ++e) xv[e] = vload<X, 4>(xp + c.n0[e]), yv[e] = vload<S, 4>(yp + c.n0[e]);
-        float x[NE][4], s = 0.0f;
+        float x[NE][4];
+        double s = 0.0;
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
 #pragma unroll
@@ -642,7 +698,7 @@ __global__ void __launch_bounds__(kRowBlock<LPR>) add_norm_fwd_kernel(AddNorm p)
             }
             if (live && c.on[e]) vstore<X, 4>((X*)p.x_out + row * N + c.n0[e], x[e]);
         }
-        const float r = 1.0f / sqrtf(lanes_sum<LPR>(s, red, slot) * inv_n + p.eps);
+        const float r = inv_root((float)lanes_sum64<LPR>(s, red, slot) * inv_n + p.eps);
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
             float u[4];
