@@ -301,7 +301,9 @@ struct Own {
 };
 
 // The states that ranges of time start from. A range's map is h -> exp(A sum d) h + L (and of the carry,
-// backwards, the same with its own L); a start in it cuts off what comes before: sum d is then -1.
+// backwards, the same with its own L); a start in it cuts off what comes before: sum d is then -1. The factor
+// comes in two halves, which leave fp32 only where the product does and of which none is 0, and a state of 0
+// needs none: as step by step it stays 0 however far its rate would grow it, and an infinite one infinite.
 template <int K>
 __device__ __forceinline__ void enter_range(float* h, const Selective& p, const float* A2, size_t row, size_t chan, int s0, bool on,
                                             int from, int dir, int count) {
@@ -312,7 +314,11 @@ __device__ __forceinline__ void enter_range(float* h, const Selective& p, const 
         load_states<K>(L, p.maps + r * plane + row, s0, p.S, on);
         const float sd = on ? p.mapsums[r * p.B * p.N + chan] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) h[k] = sd < 0.0f ? L[k] : fmaf(__builtin_amdgcn_exp2f(A2[k] * sd), h[k], L[k]);
+        for (int k = 0; k < K; ++k) {
+            const float e = __builtin_amdgcn_exp2f(fmaxf(A2[k] * (0.5f * sd), -126.0f));
+            // (without a step the state is as it was, whatever the rate)
+            h[k] = sd == 0.0f ? h[k] : sd < 0.0f || h[k] == 0.0f ? L[k] : fmaf(h[k] * e, e, L[k]);
+        }
     }
 }
 

@@ -1,10 +1,12 @@
-"""The selective block's operators where they were wrong, or untested, before: last bits of a norm's factor.
+"""The selective block's operators where they were wrong, or untested, before: last bits of a norm's factor,
+growing states in ranges of time.
 Tolerances as in test_gpu_selective.py unless a test derives its own."""
 
 import pytest
 import torch
 
-from test_gpu_selective import BF16, FP32, add_case
+from oracle import selective as osel
+from test_gpu_selective import BF16, FP32, LEAVES, SCAN_TOL, add_case, check_scan, close, put, run_scan, scan_case
 
 INF, NAN = float('inf'), float('nan')
 
@@ -51,3 +53,77 @@ def test_add_norm_of_nothing_and_of_infinities(dev):
         assert torch.isnan(u[1, 1]) and float(u[1, 2:].abs().max()) == 0.0 and torch.isnan(u[2]).all() and float(u[3].abs().max()) == 0.0
         _, u = add_norm(x, y, w, eps=0.0)
         assert torch.isnan(u[0]).all()
+
+
+# ---------------------------------------------------------------- ranges of time ------------
+
+def growing_case(S, T=96, step=3.0):
+    """Rates of about 1: a state grows by e^3 a step, over a range of 32 steps past the largest fp32 number.
+    Six blocks of 16 steps and few rows: three ranges."""
+    c = scan_case(T, 2, 20, S, FP32, False)
+    c['A'] = 0.9 + 0.1 * torch.rand(20, S, generator=torch.Generator().manual_seed(5))
+    c['dt'].fill_(step)
+    c['dt_bias'].zero_()
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('S', [2, 12, 24, 40])
+def test_silent_stretches_of_growing_states(dev, S):
+    """A state, or a carry, of 0 stays 0 over ranges whose growth leaves fp32."""
+    c = growing_case(S)
+    c['h0'] = None
+    c['x'][:84] = 0.0
+    d = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+    y, last = osel.scan(*[d[k] for k in LEAVES])
+    from delrec.selective import selective_scan
+    g = put(c, dev)
+    got, end = selective_scan(*[g[k] for k in LEAVES])
+    close(got, y, SCAN_TOL, 'y')
+    close(end, last, SCAN_TOL, 'last')
+    # the carry, from the last step to the first
+    c = growing_case(S)
+    c['h0'].zero_()
+    c['x'].zero_()
+    c['dy'][12:] = 0.0
+    c['dlast'].zero_()
+    check_scan(c, dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('S', [2, 12, 24, 40])
+def test_growing_states_in_ranges(dev, S):
+    """Growth by some e^14 in all, and of a tiny state by e^90 over one range. (An exponent is off by 5e-7 of
+    itself at most: 4.6e-5.)"""
+    c = growing_case(S, step=0.0)
+    c['A'] *= 0.2
+    check_scan(c, dev)
+    c = growing_case(S, T=64)
+    c['x'].zero_()
+    c['dt'][:32], c['dt'][32:] = 2.9, -30.0
+    c['A'] = 0.95 + 0.01 * torch.rand_like(c['A'])
+    c['h0'] = 2e-38 * (1 + torch.rand_like(c['h0']))
+    d = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+    _, last = osel.scan(*[d[k] for k in LEAVES])
+    got = run_scan(c, dev)['last'].double().cpu()
+    assert float(last.abs().max()) < 1e3 and ((got - last).abs() <= 1e-4 * last).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('S', [2, 40])
+def test_infinite_states_in_ranges(dev, S):
+    """An infinite state stays infinite however far its decay goes, as step by step; a row without steps keeps
+    any state at any rate."""
+    c = scan_case(96, 3, 20, S, FP32, False)
+    c['dt'].fill_(3.0)
+    c['A'].fill_(-1.0)
+    c['h0'][0] = INF
+    c['lengths'] = torch.tensor([96, 96, 0])
+    c['h0'][2, 4] = -INF
+    c['A'][7] = NAN
+    from delrec.selective import selective_scan
+    g = put(c, dev)
+    _, end = selective_scan(*[g[k] for k in LEAVES], lengths=g['lengths'])
+    rest = [n for n in range(20) if n != 7]
+    assert (end[0, rest] == INF).all() and torch.isfinite(end[1, rest]).all() and torch.isnan(end[:2, 7]).all()
+    assert torch.equal(end[2].cpu(), c['h0'][2])
