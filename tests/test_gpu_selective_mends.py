@@ -1,12 +1,13 @@
 """The selective block's operators where they were wrong, or untested, before: last bits of a norm's factor,
-growing states in ranges of time.
+growing states in ranges of time, every shape in ranges, long runs of the convolution's backward.
 Tolerances as in test_gpu_selective.py unless a test derives its own."""
 
 import pytest
 import torch
 
 from oracle import selective as osel
-from test_gpu_selective import BF16, FP32, LEAVES, SCAN_TOL, add_case, check_scan, close, put, run_scan, scan_case
+from test_gpu_selective import (BF16, CONV_LEAVES, FP32, LEAVES, SCAN_TOL, add_case, check_conv, check_scan, close, conv_case, masks_of, put,
+                                run_conv, run_scan, scan_case)
 
 INF, NAN = float('inf'), float('nan')
 
@@ -14,6 +15,14 @@ INF, NAN = float('inf'), float('nan')
 @pytest.fixture
 def dev():
     return torch.device('cuda')
+
+
+def workspace(kind, T, B, N, L):
+    import ctypes
+    from delrec import _lib
+    size = ctypes.c_size_t(0)
+    assert _lib.load().delrec_query_workspace(kind, T, B, N, L, 0, ctypes.byref(size)) == 0
+    return size.value
 
 
 @pytest.mark.gpu
@@ -127,3 +136,69 @@ def test_infinite_states_in_ranges(dev, S):
     rest = [n for n in range(20) if n != 7]
     assert (end[0, rest] == INF).all() and torch.isfinite(end[1, rest]).all() and torch.isnan(end[:2, 7]).all()
     assert torch.equal(end[2].cpu(), c['h0'][2])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [FP32, BF16])
+@pytest.mark.parametrize('S', [2, 12, 24, 40])
+def test_every_shape_in_ranges(dev, S, dtype):
+    """Up to 8, 16, 32 and 64 states, each with lanes and registers of its own: starts and row ends at the
+    ranges' borders, rows that end before a range begins."""
+    from delrec import _lib
+    T, B, N = 513, 6, 20
+    assert workspace(_lib.WS_SELECTIVE_FWD, T, B, N, S) > 0       # (the ranges' maps)
+    c = scan_case(T, B, N, S, dtype, True, rate=0.3)
+    c['lengths'] = torch.tensor([T, 0, 1, 255, 256, 257])
+    c['starts'] = torch.zeros(T, B, dtype=torch.bool)
+    for t in (31, 32, 33, 255, 256, 512):
+        c['starts'][t] = True
+    c['starts'][:, 0] = False
+    check_scan(c, dev)
+    c['starts'] = None
+    check_scan(c, dev)
+    c['lengths'] = None
+    check_scan(c, dev)
+
+
+# ---------------------------------------------------------------- runs of the convolution ---
+
+# steps of a run of the backward, without and with masks, each more than the shortest runs' 16 - (W - 1)
+LONG_RUNS = [(120, 60, 400, 4, 17, 17), (97, 40, 1030, 5, 20, 20), (200, 64, 300, 7, 22, 22), (150, 50, 700, 8, 25, 25), (350, 32, 1000, 4, 45, 25),
+             (300, 40, 1024, 2, 51, 27)]
+
+
+def check_runs(T, B, N, W, steps, masked):
+    """The workspace holds a set of sums for each workgroup of 256 lanes (32 of them side by side): as many
+    as the stated runs make."""
+    from delrec import _lib
+    blocks = max(-(-(-(-T // s) * B) // 8) for s in (steps, masked))
+    assert N >= 125 and workspace(_lib.WS_CAUSAL_CONV_BWD, T, B, N, W) // (4 * N * (W + 1)) == blocks
+    assert min(steps, masked) > 16 - (W - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('masks', [False, True])
+@pytest.mark.parametrize('dtype', [FP32, BF16])
+@pytest.mark.parametrize('T,B,N,W,steps,masked', LONG_RUNS)
+def test_conv_long_runs_to_the_last_bit(dev, T, B, N, W, steps, masked, dtype, masks):
+    """Small whole numbers and no activation: every product and sum is exact (gradients of weights are below
+    2 * 3 * 13000 < 2^24, outputs below 2^8 in bf16), in any order."""
+    check_runs(T, B, N, W, steps, masked)
+    g = torch.Generator().manual_seed(T)
+    whole = lambda most, *shape: torch.randint(-most, most + 1, shape, generator=g)  # noqa: E731
+    c = dict(x=whole(3, T, B, N).to(dtype), weight=whole(2, N, W).float(), bias=whole(2, N).float(), state=whole(3, B, W - 1, N).to(dtype),
+             dy=whole(2, T, B, N).to(dtype), dstate=whole(2, B, W - 1, N).to(dtype), **masks_of(g, T, B, masks))
+    got = run_conv(c, dev, silu=False)
+    d = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+    leaves = {k: d[k].clone().requires_grad_(True) for k in CONV_LEAVES}
+    y, state = osel.conv(*[leaves[k] for k in CONV_LEAVES], d['starts'], d['lengths'], False)
+    ref = dict(zip(leaves, torch.autograd.grad((y, state), list(leaves.values()), (d['dy'], d['dstate']))), y=y.detach(), after=state.detach())
+    for k, v in ref.items():
+        assert torch.equal(got[k].double().cpu(), v), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('masks', [False, True])
+@pytest.mark.parametrize('T,B,N,W,steps,masked', LONG_RUNS)
+def test_conv_long_runs(dev, T, B, N, W, steps, masked, masks):
+    check_conv(conv_case(T, B, N, W, FP32 if W % 2 else BF16, masks), dev)
