@@ -409,6 +409,7 @@ py::tuple gated_step(Tensor z, Tensor f, Tensor g, Tensor x, Tensor h, OptTensor
     h = dense(h);
     w = vector_arg(w, N, z, "weight"); scale = vector_arg(scale, N, z, "scale");
     w2 = vector_arg(w2, N, z, "next_weight"); bias = vector_arg(bias, N, z, "bias");
+    if (in_place) check_state_out(h_out, "h_out", h, {&z, &f, &g, &x, &w, &scale, &w2, &bias});
     const Tensor xo = at::empty({B, N}, x.options());
     Tensor u;
     if (w2.defined()) u = at::empty({B, N}, z.options());

@@ -153,6 +153,30 @@ delrec_rows dense_rows(const Tensor& t, int64_t R1, int64_t N) {
     return {t.data_ptr(), R1 * N, N};
 }
 
+// whether t has an element in [lo, hi), from dimension `dim` on at `at`
+bool touches(const char* lo, const char* hi, const Tensor& t, const char* at, int64_t dim) {
+    int64_t last = 0, count = 1;
+    for (int64_t d = dim; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d), count *= t.size(d);
+    const int64_t e = (int64_t)t.element_size();
+    if (at >= hi || at + (last + 1) * e <= lo) return false;
+    if (last + 1 <= count) return true;               // no gaps
+    for (int64_t i = 0; i < t.size(dim) && (i == 0 || t.stride(dim)); ++i)
+        if (touches(lo, hi, t, at + i * t.stride(dim) * e, dim + 1)) return true;
+    return false;
+}
+
+// A step writes a contiguous `out` while other workgroups still read: it is the state itself, element for
+// element (each is read before it is written), or shares no memory with what the step reads.
+void check_state_out(const Tensor& out, const char* what, const Tensor& state, std::initializer_list<const Tensor*> inputs) {
+    const char *lo = (const char*)out.data_ptr(), *hi = lo + out.nbytes();
+    auto one = [&](const Tensor& t) {
+        if (t.defined() && t.numel() && touches(lo, hi, t, (const char*)t.data_ptr(), 0))
+            refuse(text(what, " shares memory with an input: it must be the state itself or memory of its own"));
+    };
+    if (state.data_ptr() != out.data_ptr()) one(state);
+    for (const Tensor* t : inputs) one(*t);
+}
+
 int as_int(int64_t v) {
     if (v > INT32_MAX) refuse(text("a size of ", v, " is past 31 bits"));
     return (int)v;

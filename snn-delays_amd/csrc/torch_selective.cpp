@@ -135,6 +135,7 @@ py::tuple conv_step(Tensor x, Tensor state, OptTensor w_, OptTensor bias_, bool 
     }
     x = rows_form(x);
     state = dense(state);
+    if (in_place) check_state_out(out, "state_out", state, {&x, &w, &bias});
     const Tensor y = at::empty({B, N}, x.options());
     delrec_causal_conv_fwd_args a{};
     a.T = 1; a.B = B; a.N = N; a.W = (int)w.size(1); a.bf16 = is_bf16(x); a.silu = silu;
@@ -290,6 +291,7 @@ py::tuple selective_step(Tensor x, Tensor dt, Tensor A, Tensor Bm, Tensor C, Ten
     h = dense(h);
     D = vector_arg(D, N, x, "D");
     bias = vector_arg(bias, N, x, "dt_bias");
+    if (in_place) check_state_out(out, "h_out", h, {&x, &dt, &g, &A, &Bm, &C, &D, &bias});
     const Tensor y = at::empty({B, N}, x.options());
     delrec_selective_step_args a{};
     a.B = B; a.N = N; a.S = S; a.bf16 = is_bf16(x);

@@ -38,7 +38,7 @@ def causal_conv(x, weight, bias=None, state=None, starts=None, lengths=None, sil
 def conv_step(x, state, weight, bias=None, silu=True, state_out=None):
     """One time step of ``causal_conv``: x (B, N), the state (B, W - 1, N); ``(y, state')``.
     ``state_out``: where the state goes, ``state`` itself to update in place, or memory that no
-    input shares. Not differentiable."""
+    input shares (anything else raises ``ValueError``). Not differentiable."""
     return _lib.require_ext().conv_step(x, state, weight, bias, silu, state_out)
 
 
@@ -59,7 +59,7 @@ def selective_scan(x, dt, A, B, C, D=None, g=None, dt_bias=None, h0=None, starts
 def selective_step(x, dt, A, B, C, h, D=None, g=None, dt_bias=None, h_out=None):
     """One time step of ``selective_scan`` in one launch: x, dt, g (B, N), B, C (B, S), the state h
     (B, N, S) fp32; ``(y, h')``. ``h_out``: where h' goes, ``h`` itself to update in place, or memory
-    that no input shares. Not differentiable."""
+    that no input shares (anything else raises ``ValueError``). Not differentiable."""
     return _lib.require_ext().selective_step(x, dt, A, B, C, h, D, g, dt_bias, h_out)
 
 

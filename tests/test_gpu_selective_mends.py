@@ -1,5 +1,6 @@
 """The selective block's operators where they were wrong, or untested, before: last bits of a norm's factor,
-growing states in ranges of time, every shape in ranges, long runs of the convolution's backward.
+growing states in ranges of time, every shape in ranges, long runs of the convolution's backward,
+states that share memory with inputs.
 Tolerances as in test_gpu_selective.py unless a test derives its own."""
 
 import pytest
@@ -202,3 +203,61 @@ def test_conv_long_runs_to_the_last_bit(dev, T, B, N, W, steps, masked, dtype, m
 @pytest.mark.parametrize('T,B,N,W,steps,masked', LONG_RUNS)
 def test_conv_long_runs(dev, T, B, N, W, steps, masked, masks):
     check_conv(conv_case(T, B, N, W, FP32 if W % 2 else BF16, masks), dev)
+
+
+# ---------------------------------------------------------------- states of steps -----------
+
+def steps_of(dev, B, N, S, W):
+    """name -> (call(state, out, x=...), the state's shape)"""
+    from delrec.gated import gated_step
+    from delrec.selective import conv_step, selective_step
+    c, e = put(scan_case(1, B, N, S, FP32, False), dev), put(conv_case(1, B, N, W, FP32, False), dev)
+    ones = torch.ones(N, device=dev)
+    x0 = c['x'][0]
+    return {
+        'h_out': (lambda h, out, x=x0: selective_step(x, c['dt'][0], c['A'], c['B'][0], c['C'][0], h, c['D'], c['g'][0], c['dt_bias'], h_out=out),
+                  (B, N, S)),
+        'state_out': (lambda s, out, x=x0: conv_step(x, s, e['weight'], e['bias'], state_out=out), (B, W - 1, N)),
+        'gated h_out': (lambda h, out, x=x0: gated_step(x, c['dt'][0], c['g'][0], c['x'][0], h, ones, ones, h_out=out)[::2], (B, N)),
+    }
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('B', [5, 300])
+def test_states_written_over_what_a_step_reads_are_refused(dev, B):
+    """Views of one buffer a row apart, and a state that the step's input lies in: an error, nothing written."""
+    for name, (call, shape) in steps_of(dev, B, 64, 8, 4).items():
+        ring = torch.randn(B + 1, *shape[1:], device=dev)
+        kept = ring.clone()
+        for h, out in ((ring[:-1], ring[1:]), (ring[1:], ring[:-1])):
+            with pytest.raises(ValueError, match=name.split()[-1]):
+                call(h, out)
+        state = torch.randn(shape, device=dev)
+        for x in (ring.reshape(-1)[:B * 64].view(B, 64), ring.reshape(-1)[-B * 64:].view(B, 64), ring.reshape(-1)[5:69].expand(B, 64)):
+            with pytest.raises(ValueError, match=name.split()[-1]):
+                call(state, ring[:B] if x.data_ptr() == ring.data_ptr() or x.stride(0) == 0 else ring[1:], x)
+        assert torch.equal(ring, kept)
+
+
+@pytest.mark.gpu
+def test_states_in_memory_of_their_own_are_taken(dev):
+    """The state itself, another part of a buffer of states, memory between an input's rows, the place of a
+    state that is copied first."""
+    B = 5
+    for name, (call, shape) in steps_of(dev, B, 64, 8, 4).items():
+        first = torch.randn(shape, device=dev)
+        want = call(first.clone(), None)
+        ring = torch.empty(3, *shape, device=dev)
+        ring[1] = first
+        for place in (1, 0, 2):
+            got = call(ring[1].clone() if place == 1 else ring[1], ring[place])
+            assert got[1].data_ptr() == ring[place].data_ptr() and all(torch.equal(a, b) for a, b in zip(got, want)), name
+            ring[1] = first
+        got = call(ring[1], ring[1])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+        n = first.numel()
+        wide = torch.randn(B, 2 * 64 + n, device=dev)
+        out, x = wide[2, 64:64 + n].view(shape), wide[:, :64]
+        want = call(first, None, x)
+        got = call(first, out, x)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), name
