@@ -69,7 +69,10 @@ class SelectiveBlock(torch.nn.Module):
     add_norm(x, y)``, where u' is the next block's input. The inner width is ``expand * N``, ``S`` the
     states of an inner channel, ``W`` the convolution's steps, ``rank`` the width of ``low`` (N / 16
     by default). ``A`` starts at -1 .. -S, step sizes (by ``dt_bias``) between 1e-3 and 1e-1. With
-    ``checkpoint=True`` the first Linear's input is kept in 8 bits, as ``add_norm`` packs it."""
+    ``checkpoint=True`` the first Linear's input is kept in 8 bits, as ``add_norm`` packs it.
+    ``undecayed``: parameters that are no weights, for an optimiser that decays weights."""
+
+    undecayed = ('A_log', 'D', 'dt_bias')
 
     def __init__(self, N, S=16, W=4, expand=2, rank=None, bias=False, eps=1e-6, checkpoint=False):
         super().__init__()

@@ -19,20 +19,26 @@ from ..utils import reset_states, seed_everything
 def make_optimizer(model, config):
     """AdamW over two groups: the delay positions (and ``p_spread``) of every recurrent
     delay layer at ``lr_positions`` without weight decay, every other trainable parameter
-    at ``lr_w`` with ``weight_decay`` (reference ``mem.py:12-31``)."""
-    positions = []
+    at ``lr_w`` with ``weight_decay`` (reference ``mem.py:12-31``). Parameters that their module
+    names in ``undecayed`` (the rates and step sizes of ``delrec.selective``, which decay would
+    pull to values of its own) make a third group, at ``lr_w`` without."""
+    positions, undecayed = [], []
     for module in model.modules():
+        undecayed += [getattr(module, name) for name in getattr(module, 'undecayed', ())]
         if isinstance(module, axonal_recdel):
             positions.append(learned_delay_parameter(module, 'recurrent_delays'))
             if hasattr(module, 'p_spread'):
                 positions.append(module.p_spread)
-    taken = {id(p) for p in positions}
+    taken = {id(p) for p in positions + undecayed}
     weights = [p for p in model.parameters() if p.requires_grad and id(p) not in taken]
-    return torch.optim.AdamW([
+    groups = [
         {'params': weights, 'lr': config.lr_w, 'weight_decay': config.weight_decay},
         {'params': [p for p in positions if p.requires_grad], 'lr': config.lr_positions,
          'weight_decay': 0.0},
-    ])
+    ]
+    if undecayed:
+        groups.append({'params': [p for p in undecayed if p.requires_grad], 'lr': config.lr_w, 'weight_decay': 0.0})
+    return torch.optim.AdamW(groups)
 
 
 def set_epoch(model, config, epoch):
