@@ -325,6 +325,8 @@ __global__ void __launch_bounds__(256) conv_bwd_kernel(CausalConv p) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) g[j] += more[j];
                     }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) g[j] = s < len ? g[j] : 0.0f;      // (infinite weights times 0)
                     if (s >= 0) store_part<E, V>(dxp + s * p.dx.s0, g, r.have);
                     else if (p.dstate) store_part<E, V>((E*)p.dstate + ((size_t)r.b * (W - 1) + s + W - 1) * p.N + r.n, g, r.have);
                 }

@@ -205,6 +205,23 @@ def test_conv_long_runs(dev, T, B, N, W, steps, masked, masks):
     check_conv(conv_case(T, B, N, W, FP32 if W % 2 else BF16, masks), dev)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('silu', [False, True])
+def test_conv_padding_has_no_gradient_whatever_the_weights(dev, silu):
+    """Infinite and NaN weights: outputs and gradients of padded steps are 0, other channels unchanged."""
+    T, B, N, W = 30, 4, 12, 4
+    c = conv_case(T, B, N, W, FP32, True)
+    want = run_conv(c, dev, silu)
+    c['weight'][3], c['weight'][5] = INF, NAN
+    got = run_conv(c, dev, silu)
+    pad = (torch.arange(T)[:, None] >= c['lengths']).to(dev)
+    assert int(pad.sum()) > T and float(got['x'][pad].abs().max()) == 0.0 and float(got['y'][pad].abs().max()) == 0.0
+    rest = [n for n in range(N) if n not in (3, 5)]
+    for k in ('y', 'x', 'state', 'after'):
+        assert torch.equal(got[k][..., rest], want[k][..., rest]), k
+    assert torch.equal(got['weight'][rest], want['weight'][rest]) and torch.equal(got['bias'][rest], want['bias'][rest])
+
+
 # ---------------------------------------------------------------- states of steps -----------
 
 def steps_of(dev, B, N, S, W):
