@@ -161,6 +161,25 @@ def test_every_shape_in_ranges(dev, S, dtype):
     check_scan(c, dev)
 
 
+@pytest.mark.gpu
+def test_step_sizes_to_their_own_size(dev):
+    """softplus, as the state that a step makes of ones. The exponent -|x| log2(e) is rounded (2^-24 of itself,
+    6.0e-8 |x| in the value) and its factor is off by 1.34e-8 of itself; the hardware's power and reciprocal
+    are good to 2^-23 each, and four operations round to 2^-24. A decay exp(-e), e > 0, is off by 5e-7 e of
+    itself likewise: since e exp(-e) <= 1 / 2.7, by at most 2e-7 and a last place of 1 in all."""
+    from delrec.selective import selective_step
+    x = torch.linspace(-80.0, 60.0, 100_001)[None]
+    one = lambda *s: torch.ones(*s, device=dev)  # noqa: E731
+    N = x.shape[1]
+    _, d = selective_step(one(1, N), x.to(dev), one(N, 1), one(1, 1), one(1, 1), torch.zeros(1, N, 1, device=dev))
+    want = torch.log1p(torch.exp(-x.double().abs())) + x.double().clamp(min=0)
+    assert (((d[0, :, 0].double().cpu() - want[0]) / want[0]).abs() <= 5e-7 + 7.4e-8 * x[0].double().abs()).all()
+    _, h = selective_step(torch.zeros(1, N, device=dev), torch.full((1, N), 2.0, device=dev), -x.abs().t().contiguous().to(dev), one(1, 1),
+                          one(1, 1), one(1, N, 1))
+    e = torch.nn.functional.softplus(torch.tensor(2.0, dtype=torch.float64)) * x[0].double().abs()
+    assert ((h[0, :, 0].double().cpu() - torch.exp(-e)).abs() <= 2e-7 + 2.0 ** -23 + 1e-30).all()
+
+
 # ---------------------------------------------------------------- runs of the convolution ---
 
 # steps of a run of the backward, without and with masks, each more than the shortest runs' 16 - (W - 1)
