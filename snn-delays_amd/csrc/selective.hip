@@ -748,7 +748,7 @@ __device__ __forceinline__ void load_low(float* v, const E* row, int s0, int S) 
 // needs once a row its lanes take in turn, a row each, as the scan's lanes their steps. All states are
 // read before the first is written: they may be written where they were read. 29.5 us at B512 N2048 S16
 // bf16 (134 MB of states, 4.6 TB/s); one row a lane, each with its own A, took 40. States stored past the
-// caches: 34.8 us with the convolution's step instead of 45.8 where they come from memory, and in place 28.0
+// caches: to a second buffer 34.8 us with the convolution's step instead of 45.8, and in place 28.0
 // instead of 28.8 (B512), 9.4 instead of 10.4 (B64 N1024 S64, four layers), 15.6 instead of 15.3 (B256).
 template <class E, int Q, int K, int R>
 __global__ void __launch_bounds__(256) selective_step_kernel(Selective p) {
