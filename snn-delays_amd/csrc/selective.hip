@@ -317,8 +317,8 @@ __device__ __forceinline__ void enter_range(float* h, const Selective& p, const 
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const float e = __builtin_amdgcn_exp2f(fmaxf(A2[k] * (0.5f * sd), -126.0f));
-            // (without a step the state is as it was, whatever the rate)
-            h[k] = sd == 0.0f ? h[k] : sd < 0.0f || h[k] == 0.0f ? L[k] : fmaf(h[k] * e, e, L[k]);
+            // (without a step, or with steps of size 0, the state is as it was, whatever the rate)
+            h[k] = sd == 0.0f ? h[k] + L[k] : sd < 0.0f || h[k] == 0.0f ? L[k] : fmaf(h[k] * e, e, L[k]);
         }
     }
 }

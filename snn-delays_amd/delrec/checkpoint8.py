@@ -68,7 +68,8 @@ class Linear8Fn(torch.autograd.Function):
 
 def linear8(x, weight, bias=None, packed=None):
     """``torch.nn.functional.linear`` that keeps x in 8 bits for the weight's gradient.
-    ``packed``: x's ``Packed8``, where what made x has packed it already (``gated.add_norm``)."""
+    ``packed``: x's ``Packed8``, where what made x has packed it already (``gated.add_norm``) and x has
+    not been changed in place since."""
     if not (torch.is_grad_enabled() and weight.requires_grad):
         return torch.nn.functional.linear(x, weight, bias)
     if torch.is_autocast_enabled('cuda'):

@@ -140,6 +140,22 @@ def test_infinite_states_in_ranges(dev, S):
 
 
 @pytest.mark.gpu
+def test_steps_of_size_zero_in_ranges(dev):
+    """They leave a state as it is over a whole range, but for what 0 times infinity gives, as step by step."""
+    from delrec.selective import selective_scan
+    c = scan_case(96, 3, 20, 4, FP32, False)
+    c['dt'][:64] = -INF
+    c['B'][5, 1, 2] = INF
+    d = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+    _, last = osel.scan(*[d[k] for k in LEAVES])
+    assert int(torch.isnan(last).sum()) == 20 and torch.isnan(last[1, :, 2]).all()
+    g = put(c, dev)
+    _, got = selective_scan(*[g[k] for k in LEAVES])
+    assert torch.equal(torch.isnan(got).cpu(), torch.isnan(last))
+    close(torch.nan_to_num(got), torch.nan_to_num(last), SCAN_TOL, 'last')
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('dtype', [FP32, BF16])
 @pytest.mark.parametrize('S', [2, 12, 24, 40])
 def test_every_shape_in_ranges(dev, S, dtype):
